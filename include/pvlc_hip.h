@@ -523,6 +523,91 @@ pvlc_hip_status pvlc_hip_kv_unpack_f16(const uint16_t *key_cache, const uint16_t
                                        uint16_t *value_rows, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * The same cache in 8 bits (new: the reference keeps f32 rows).
+ *
+ * Codes of 8 bits and one power of two for each block of 16 tokens and kv head,
+ * for keys and for values: a row's element is code * 2^exponent.  A cache is
+ * two planes of bytes and their exponents,
+ *   key plane   [num_blocks][2 kv heads][4 token quads][8 dim-chunks][4 tokens][16 dims]
+ *   value plane [num_blocks][2 kv heads][128 dims][16 tokens]
+ *   exponents   [num_blocks][2 kv heads][key, value], biased by 127
+ * so key (block b, head h, token t, dim d) is byte
+ *   (b*2 + h)*2048 + (t/4)*512 + (d/16)*64 + (t%4)*16 + d%16
+ * and value byte (b*2 + h)*2048 + d*16 + t: 512 bytes a token and 4 a block, half
+ * of the fp16 planes.  What a row is rounded to is defined exactly: its fp16
+ * values x (as the fp16 cache would hold them) become the code nearest to
+ * x * 2^-e, ties to even, where e is the least exponent, at least -32, with
+ * |x| <= L * 2^e for every x of the block's rows (L = 448 for e4m3, 127 for
+ * int8).  A row appended to a block that holds some may raise its exponent; the
+ * rows before are then rounded again, from their codes.  Infinite values are
+ * taken as 65504 with their sign; NaN sets no exponent and becomes an e4m3 NaN,
+ * 0 in int8.  Codes behind a sequence's last row are never used and never
+ * changed.
+ * A row may be appended only to a block that no other sequence reads (see the
+ * fork of pages below).
+ * ------------------------------------------------------------------------- */
+
+/* Codes: OCP e4m3 (sign, 4 exponent and 3 fraction bits, largest 448), or
+ * int8 -127..127.  int8 rounds to 1/254 of a block's power at most, e4m3 to
+ * 1/16 of each value: e4m3 for blocks with outlying channels. */
+enum { PVLC_HIP_KV_E4M3 = 0, PVLC_HIP_KV_INT8 = 1 };
+
+/* pvlc_hip_paged_decode_args with an 8-bit cache. */
+typedef struct pvlc_hip_paged_decode_q8_args {
+    uint32_t num_seqs;
+    uint32_t num_blocks;
+    uint32_t max_blocks_per_seq;
+    uint32_t code; /* PVLC_HIP_KV_E4M3 or PVLC_HIP_KV_INT8 */
+    const int32_t *block_tables;
+    const int32_t *cache_lens;
+    uint32_t uniform_cache_len;
+    uint32_t max_context;
+    uint8_t *key_cache;
+    uint8_t *value_cache;
+    uint8_t *exponents;
+    const uint16_t *query;
+    const uint16_t *new_key;
+    const uint16_t *new_value;
+    uint16_t *out;
+    const float *rope_cos;
+    const float *rope_sin;
+    uint32_t rope_rows;
+    const int32_t *positions;
+    uint32_t rotate_query;
+    uint32_t partition_tokens;
+    void *workspace; /* as the fp16 decode's: pvlc_hip_paged_decode_workspace_bytes, the two may share one */
+    size_t workspace_bytes;
+} pvlc_hip_paged_decode_q8_args;
+
+/* pvlc_hip_paged_decode_f16 over an 8-bit cache: rotate the new key (and
+ * optionally the query), round the new row into the block at cache_len, attend
+ * over cache_len+1 rows as they are held.  Codes enter the matrix products
+ * exactly and their powers are applied to f32 scores and weights, so nothing is
+ * rounded that the fp16 decode does not round.  Operands, streams, workspace,
+ * device error bits and partitions as there. */
+pvlc_hip_status pvlc_hip_paged_decode_q8_f16(const pvlc_hip_paged_decode_q8_args *args, void *stream);
+/* The same with f32 query, new key and value and output, as
+ * pvlc_hip_paged_decode_f32io: the new row is rotated from its f32 values and
+ * rounded to fp16, then to the codes. */
+pvlc_hip_status pvlc_hip_paged_decode_q8_f32io(const pvlc_hip_paged_decode_q8_args *args, const float *query,
+                                               const float *new_key, const float *new_value, float *out, void *stream);
+
+/* Compact fp16 rows [tokens][2][128] into the tokens first_token ..
+ * first_token+tokens-1 of one sequence's 8-bit blocks, through its block table
+ * (NULL = blocks 0..): a prompt's rows (first_token 0), or rows appended to a
+ * sequence of first_token rows, whose last block is rounded again where its
+ * exponent grows.  Blocks whose id lies outside the planes are skipped.  Rows
+ * need 2-byte alignment, planes 16 and exponents 4. */
+pvlc_hip_status pvlc_hip_kv_pack_q8(const uint16_t *key_rows, const uint16_t *value_rows, uint32_t first_token,
+                                    uint32_t tokens, const int32_t *block_table, uint32_t num_blocks, uint32_t code,
+                                    uint8_t *key_cache, uint8_t *value_cache, uint8_t *exponents, void *stream);
+/* Rows 0..tokens-1 of a sequence as fp16 (code * 2^exponent, at most 65504 in
+ * size; 0 for a block whose id lies outside the planes). */
+pvlc_hip_status pvlc_hip_kv_unpack_q8(const uint8_t *key_cache, const uint8_t *value_cache, const uint8_t *exponents,
+                                      uint32_t tokens, const int32_t *block_table, uint32_t num_blocks, uint32_t code,
+                                      uint16_t *key_rows, uint16_t *value_rows, void *stream);
+
+/* ---------------------------------------------------------------------------
  * Decoder GEMV with fp16 weights (the next path widened from this backend).
  * ------------------------------------------------------------------------- */
 

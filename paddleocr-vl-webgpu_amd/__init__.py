@@ -33,6 +33,9 @@ QUERY_HEADS = 16
 KV_HEADS = 2
 HEAD_DIM = 128
 BLOCK_TOKENS = 16
+# Codes of the 8-bit cache
+KV_E4M3 = 0
+KV_INT8 = 1
 
 RUNTIME_ERROR_CODES = {
     1: "AdapterUnavailable", 2: "DeviceRequest", 3: "InvalidInvocation", 4: "Validation", 5: "OutOfMemory",
@@ -164,6 +167,15 @@ class PagedDecodeArgsC(ctypes.Structure):
                 ("rotate_query", _U32), ("partition_tokens", _U32), ("workspace", _VP), ("workspace_bytes", _SZ)]
 
 
+class PagedDecodeQ8ArgsC(ctypes.Structure):
+    _fields_ = [("num_seqs", _U32), ("num_blocks", _U32), ("max_blocks_per_seq", _U32), ("code", _U32),
+                ("block_tables", _VP), ("cache_lens", _VP), ("uniform_cache_len", _U32), ("max_context", _U32),
+                ("key_cache", _VP), ("value_cache", _VP), ("exponents", _VP), ("query", _VP), ("new_key", _VP),
+                ("new_value", _VP), ("out", _VP), ("rope_cos", _VP), ("rope_sin", _VP), ("rope_rows", _U32),
+                ("positions", _VP), ("rotate_query", _U32), ("partition_tokens", _U32), ("workspace", _VP),
+                ("workspace_bytes", _SZ)]
+
+
 class PagedPrefillArgsC(ctypes.Structure):
     _fields_ = [("tokens", _U32), ("num_blocks", _U32), ("block_table", _VP), ("key_cache", _VP),
                 ("value_cache", _VP), ("query", _VP), ("key", _VP), ("value", _VP), ("out", _VP),
@@ -213,6 +225,10 @@ SIGNATURES = {
     "pvlc_hip_paged_prefill_f32io": ([ctypes.POINTER(PagedPrefillArgsC), _VP, _VP, _VP, _VP, _VP], ctypes.c_int32),
     "pvlc_hip_kv_pack_f16": ([_VP, _VP, _U32, _VP, _U32, _VP, _VP, _VP], ctypes.c_int32),
     "pvlc_hip_kv_unpack_f16": ([_VP, _VP, _U32, _VP, _U32, _VP, _VP, _VP], ctypes.c_int32),
+    "pvlc_hip_paged_decode_q8_f16": ([ctypes.POINTER(PagedDecodeQ8ArgsC), _VP], ctypes.c_int32),
+    "pvlc_hip_paged_decode_q8_f32io": ([ctypes.POINTER(PagedDecodeQ8ArgsC), _VP, _VP, _VP, _VP, _VP], ctypes.c_int32),
+    "pvlc_hip_kv_pack_q8": ([_VP, _VP, _U32, _U32, _VP, _U32, _U32, _VP, _VP, _VP, _VP], ctypes.c_int32),
+    "pvlc_hip_kv_unpack_q8": ([_VP, _VP, _VP, _U32, _VP, _U32, _U32, _VP, _VP, _VP], ctypes.c_int32),
     "pvlc_hip_gemv_tiled_plan_create": ([_U32, _U32, ctypes.POINTER(GemvTiledPlanC)], ctypes.c_int32),
     "pvlc_hip_gemv_f16": ([_VP, _VP, _VP, _U32, _U32, _VP], ctypes.c_int32),
     "pvlc_hip_gemv_group_f16": ([_VP, _U32, _VP, _U32, _VP], ctypes.c_int32),
@@ -777,6 +793,44 @@ def kv_unpack_f16(key_cache, value_cache, tokens, key_rows, value_rows, num_bloc
                   stream=None) -> None:
     _check(lib.pvlc_hip_kv_unpack_f16(_ptr(key_cache), _ptr(value_cache), tokens, _ptr(block_table), num_blocks,
                                       _ptr(key_rows), _ptr(value_rows), _stream(stream)))
+
+
+def paged_decode_q8_args(*, num_seqs, num_blocks, max_blocks_per_seq, code, key_cache, value_cache, exponents, query,
+                         new_key, new_value, out, workspace, workspace_bytes, max_context, block_tables=None,
+                         cache_lens=None, uniform_cache_len=0, rope_cos=None, rope_sin=None, rope_rows=0,
+                         positions=None, rotate_query=False, partition_tokens=0) -> PagedDecodeQ8ArgsC:
+    """paged_decode_args with an 8-bit cache: planes of codes (``code``: KV_E4M3 or KV_INT8) and their exponents
+    [num_blocks][2][key, value]."""
+    return PagedDecodeQ8ArgsC(num_seqs, num_blocks, max_blocks_per_seq, code, _ptr(block_tables), _ptr(cache_lens),
+                              uniform_cache_len, max_context, _ptr(key_cache), _ptr(value_cache), _ptr(exponents),
+                              _ptr(query), _ptr(new_key), _ptr(new_value), _ptr(out), _ptr(rope_cos), _ptr(rope_sin),
+                              rope_rows, _ptr(positions), int(rotate_query), partition_tokens, _ptr(workspace),
+                              workspace_bytes)
+
+
+def paged_decode_q8_f16(args: PagedDecodeQ8ArgsC, stream=None) -> None:
+    """paged_decode_f16 over an 8-bit cache with a power of two for each block of 16 tokens and kv head."""
+    _check(lib.pvlc_hip_paged_decode_q8_f16(ctypes.byref(args), _stream(stream)))
+
+
+def paged_decode_q8_f32io(args: PagedDecodeQ8ArgsC, query, new_key, new_value, out, stream=None) -> None:
+    """paged_decode_q8_f16 with f32 query, new key and value and output (the args' fp16 ones must be None)."""
+    _check(lib.pvlc_hip_paged_decode_q8_f32io(ctypes.byref(args), _ptr(query), _ptr(new_key), _ptr(new_value),
+                                              _ptr(out), _stream(stream)))
+
+
+def kv_pack_q8(key_rows, value_rows, tokens, key_cache, value_cache, exponents, num_blocks, code, block_table=None,
+               first_token=0, stream=None) -> None:
+    """fp16 rows [tokens][2][128] into the tokens first_token.. of a sequence's 8-bit blocks."""
+    _check(lib.pvlc_hip_kv_pack_q8(_ptr(key_rows), _ptr(value_rows), first_token, tokens, _ptr(block_table), num_blocks,
+                                   code, _ptr(key_cache), _ptr(value_cache), _ptr(exponents), _stream(stream)))
+
+
+def kv_unpack_q8(key_cache, value_cache, exponents, tokens, key_rows, value_rows, num_blocks, code, block_table=None,
+                 stream=None) -> None:
+    """Rows 0..tokens-1 of a sequence's 8-bit blocks as fp16."""
+    _check(lib.pvlc_hip_kv_unpack_q8(_ptr(key_cache), _ptr(value_cache), _ptr(exponents), tokens, _ptr(block_table),
+                                     num_blocks, code, _ptr(key_rows), _ptr(value_rows), _stream(stream)))
 
 
 def key_slot(t):

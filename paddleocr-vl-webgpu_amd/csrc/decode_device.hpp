@@ -1,6 +1,6 @@
 // Device parts of the paged decode that do not depend on how the cache is
-// stored: the launch's parameters, block ids, the combination of waves and
-// partitions, and the numbering of ragged batches.
+// stored: the launch's parameters, block ids, the numbering of ragged batches
+// and the merge of their partitions.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -163,6 +163,27 @@ struct DecodeLaunch {
     const DecodeOperands32 *f32 = nullptr;
 };
 int launch_paged_decode(const DecodeLaunch &launch, void *stream);
+// Workgroups of `kernel` the current device keeps resident at once, at most
+// max_items; *units receives its compute units (kernels_decode.hip).
+uint32_t resident_workgroups(const void *kernel, int threads, uint64_t max_items, uint32_t *units, int *err);
+
+// The 8-bit cache: bytes of one (block, head) of a plane, the bias of a stored
+// exponent, and the least exponent (an fp16 value's size is at least 2^-24, so
+// its codes reach down to 2^-33; a block of zeros has the least).
+constexpr uint32_t kQ8SlabBytes = kBlockHeadElems;
+constexpr int kQ8Bias = 127;
+constexpr int kQ8LeastExponent = -32;
+struct DecodeCodes {
+    uint32_t code;        // PVLC_HIP_KV_E4M3 or PVLC_HIP_KV_INT8
+    uint8_t *exponents;   // [block][kv head][key, value]
+};
+int launch_paged_decode_q8(const DecodeLaunch &launch, const DecodeCodes &codes, void *stream);
+int launch_kv_pack_q8(const uint16_t *key_rows, const uint16_t *value_rows, uint32_t first_token, uint32_t tokens,
+                      const int32_t *table, uint32_t num_blocks, uint32_t code, uint8_t *key_cache, uint8_t *value_cache,
+                      uint8_t *exponents, void *stream);
+int launch_kv_unpack_q8(const uint8_t *key_cache, const uint8_t *value_cache, const uint8_t *exponents, uint32_t tokens,
+                        const int32_t *table, uint32_t num_blocks, uint32_t code, uint16_t *key_rows, uint16_t *value_rows,
+                        void *stream);
 int launch_fill_u32(uint32_t *dst, size_t words, uint32_t value, void *stream);
 int launch_kv_pack(const uint16_t *key_rows, const uint16_t *value_rows, uint32_t tokens, const int32_t *table,
                    uint32_t num_blocks, uint16_t *key_cache, uint16_t *value_cache, uint32_t *error_word,
@@ -442,7 +463,13 @@ pvlc_hip_status validate_decode_geometry(const pvlc_hip_paged_decode_args *a, ui
 // merge kernel).
 pvlc_hip_status launch_decode_state(const pvlc_hip_paged_decode_args *a, uint32_t partition, uint32_t max_parts,
                                     const DecodeState &state, void *stream, uint32_t *launches_out,
-                                    const DecodeOperands32 *f32 = nullptr);
+                                    const DecodeOperands32 *f32 = nullptr, const DecodeCodes *codes = nullptr);
+// The caller's workspace checked and laid out, then the launch; with codes the
+// planes are 8-bit ones (passed through args' plane pointers).
+pvlc_hip_status launch_decode_checked(const pvlc_hip_paged_decode_args *a, void *stream, uint32_t *launches_out = nullptr,
+                                      const DecodeOperands32 *f32 = nullptr, const DecodeCodes *codes = nullptr);
+// A HIP error as a status.
+pvlc_hip_status hip_status(int error, const char *what);
 // Partition rules: balanced_parts is the partition count per (sequence, kv
 // head) of the single-shot rule; single_shot_partition returns 0 when a
 // partition would exceed kSingleShotTiles; auto_partition falls back to

@@ -278,7 +278,7 @@ pvlc_hip_status validate_decode_geometry(const pvlc_hip_paged_decode_args *a, ui
 
 pvlc_hip_status launch_decode_state(const pvlc_hip_paged_decode_args *a, uint32_t partition, uint32_t max_parts,
                                     const DecodeState &state, void *stream, uint32_t *launches_out,
-                                    const DecodeOperands32 *f32) {
+                                    const DecodeOperands32 *f32, const DecodeCodes *codes) {
     // Streaming regime: partitions longer than one chunk of the largest
     // single-shot workgroup, or ragged lengths with more workgroups than two
     // rounds of one per compute unit.  A smaller ragged launch takes one
@@ -311,20 +311,18 @@ pvlc_hip_status launch_decode_state(const pvlc_hip_paged_decode_args *a, uint32_
     // partition it settled on and the compute units it assumed in the two
     // status words.
     if ((streaming || a->cache_lens) && a->partition_tokens == 0) launch.partition_word = state.status_words;
-    const int e = launch_paged_decode(launch, stream);
+    const int e = codes ? launch_paged_decode_q8(launch, *codes, stream) : launch_paged_decode(launch, stream);
     if (e != 0) return hip_fail(static_cast<hipError_t>(e), "paged decode launch");
     if (launches_out) *launches_out = streaming ? 2u : 1u;  // persistent kernel + merge kernel, or one kernel
     return PVLC_HIP_OK;
 }
 
-}  // namespace pvlc
-
-namespace {
+pvlc_hip_status hip_status(int error, const char *what) { return hip_fail(static_cast<hipError_t>(error), what); }
 
 // The caller's workspace checked and laid out (decode_workspace_layout): the
 // error word first, the two status words after it in the same 256-byte slot.
-pvlc_hip_status launch_decode_checked(const pvlc_hip_paged_decode_args *a, void *stream,
-                                      uint32_t *launches_out = nullptr, const DecodeOperands32 *f32 = nullptr) {
+pvlc_hip_status launch_decode_checked(const pvlc_hip_paged_decode_args *a, void *stream, uint32_t *launches_out,
+                                      const DecodeOperands32 *f32, const DecodeCodes *codes) {
     uint32_t partition = 0, max_parts = 0;
     if (pvlc_hip_status st = validate_decode_geometry(a, &partition, &max_parts, f32)) return st;
     if (!a->workspace) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "paged decode workspace is NULL");
@@ -339,8 +337,12 @@ pvlc_hip_status launch_decode_checked(const pvlc_hip_paged_decode_args *a, void 
                             reinterpret_cast<uint32_t *>(ws + layout.error_offset),
                             reinterpret_cast<uint32_t *>(ws + layout.error_offset) + 1,
                             layout.part_stride};
-    return launch_decode_state(a, partition, max_parts, state, stream, launches_out, f32);
+    return launch_decode_state(a, partition, max_parts, state, stream, launches_out, f32, codes);
 }
+
+}  // namespace pvlc
+
+namespace {
 
 // Session creation shared by begin_decoder_kv_session and the one-shot path.
 // The plan is already validated.
