@@ -201,19 +201,39 @@ __device__ inline void finish_item(const DecodeParams &p, uint32_t s, uint32_t g
 // A tile's 16 bytes of a load lie 256 bytes behind those of the load before.
 __device__ inline void load_chunk(const DecodeParams &p, uint32_t g, uint32_t ids, int c, int row, int kg,
                                   q8x4_t (&kr)[8], q8x4_t (&vr)[8]) {
-    uint32_t b[kTiles];
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) b[i] = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ids), c * kTiles + i));
-    auto tile = [&](int i) { return i < 2 ? (i == 0 ? b[0] : b[1]) : (i == 2 ? b[2] : b[3]); };
+    auto id = [&](int i) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ids), c * kTiles + i)); };
+    const uint32_t b0 = id(0), b1 = id(1), b2 = id(2), b3 = id(3);
+    const uint32_t kb = (row & 8) ? ((row & 4) ? b3 : b2) : ((row & 4) ? b1 : b0);  // tile row / 4
+    const uint32_t vb = (kg & 2) ? ((kg & 1) ? b3 : b2) : ((kg & 1) ? b1 : b0);
     const uint8_t *kp = reinterpret_cast<const uint8_t *>(p.key_cache) +
-                        (static_cast<size_t>(tile(row >> 2)) * kKvHeads + g) * kQ8SlabBytes + (kg * 4 + (row & 3)) * 16;
+                        (static_cast<size_t>(kb) * kKvHeads + g) * kQ8SlabBytes + (kg * 4 + (row & 3)) * 16;
     const uint8_t *vp = reinterpret_cast<const uint8_t *>(p.value_cache) +
-                        (static_cast<size_t>(tile(kg)) * kKvHeads + g) * kQ8SlabBytes + row * 16;
+                        (static_cast<size_t>(vb) * kKvHeads + g) * kQ8SlabBytes + row * 16;
 #pragma unroll
     for (int i = 0; i < 8; ++i) kr[i] = __builtin_nontemporal_load(reinterpret_cast<const q8x4_t *>(kp + i * 256));
     __builtin_amdgcn_sched_barrier(0);  // the keys ahead of the values
 #pragma unroll
     for (int i = 0; i < 8; ++i) vr[i] = __builtin_nontemporal_load(reinterpret_cast<const q8x4_t *>(vp + i * 256));
+}
+
+// The rows before `slot` of a block and head rounded again in the cache, by one
+// wave, complete when this returns.  A loop over the block's dwords in memory: it
+// runs for a few of a sequence's rows, and in the registers of the main path its
+// code, unrolled, was a third of the kernel.
+template <int CODE>
+__device__ inline void requantise_block(uint8_t *keys, uint8_t *values, int lane, int slot, int grown_k, int grown_v) {
+#pragma unroll 1
+    for (int i = lane; i < static_cast<int>(kQ8SlabBytes) / 4; i += 64) {
+        // key dword i: token (i / 128) * 4 + (i / 4) % 4; value dword i: tokens (i % 4) * 4 .. +3
+        uint32_t *k = reinterpret_cast<uint32_t *>(keys) + i, *v = reinterpret_cast<uint32_t *>(values) + i;
+        if ((i >> 7) * 4 + ((i >> 2) & 3) < slot) *k = q8_requantise<CODE>(*k, grown_k);
+        const int rows = min(max(slot - (i & 3) * 4, 0), 4);
+        if (rows > 0) {
+            const uint32_t before = rows == 4 ? ~0u : (1u << (8 * rows)) - 1u, old = *v;
+            *v = (q8_requantise<CODE>(old, grown_v) & before) | (old & ~before);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // One work item: partition `part` (P tokens) of kv head g of sequence s, as
@@ -234,6 +254,11 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
     // byte, value in the high one.
     uint32_t ex = *reinterpret_cast<const uint16_t *>(p.exponents + (static_cast<size_t>(ids) * kKvHeads + g) * 2);
 
+    // Every pointer of the small operands in one round of scalar loads, and the
+    // operands raw, on every lane and without a branch (cos and sin read the new
+    // key row where there is no rotary): arithmetic between them and the cache's
+    // loads would wait for them before those go out.
+    asm volatile("" ::"s"(p.rope_cos), "s"(p.rope_sin), "s"(p.rope_rows));
     bool rope = p.rope_cos != nullptr;
     const bool rope_bad = rope && (pos < 0 || static_cast<uint32_t>(pos) >= p.rope_rows);
     if (rope_bad) rope = false;
@@ -243,9 +268,13 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
     // .. +8.  The new row: lane t has dims t and t + 64.
     const size_t qoff = (static_cast<size_t>(s) * kQueryHeads + g * kGroup + (row & 7)) * kHeadDim + kg * 16;
     const size_t new_base = (static_cast<size_t>(s) * kKvHeads + g) * kHeadDim;
+    const float *stand_in = F32IO ? p.new_key32 + new_base : reinterpret_cast<const float *>(p.new_key + new_base);
+    const float rc_raw = (rope ? p.rope_cos + static_cast<size_t>(pos) * 64 : stand_in)[lane];
+    const float rs_raw = (rope ? p.rope_sin + static_cast<size_t>(pos) * 64 : stand_in)[lane];
     half8_t qb[4];
     float4_t q32[F32IO ? 4 : 1][2];
-    float nk_lo, nk_hi, nv_lo, nv_hi;
+    float n32[4];  // key dims lane and lane + 64, value likewise
+    uint16_t n16[4];
     if constexpr (F32IO) {
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
@@ -253,28 +282,27 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
             q32[kb][0] = *reinterpret_cast<const float4_t *>(src);
             q32[kb][1] = *reinterpret_cast<const float4_t *>(src + 4);
         }
-        nk_lo = p.new_key32[new_base + lane];
-        nk_hi = p.new_key32[new_base + lane + 64];
-        nv_lo = p.new_value32[new_base + lane];
-        nv_hi = p.new_value32[new_base + lane + 64];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n32[i] = (i < 2 ? p.new_key32 : p.new_value32)[new_base + lane + (i & 1) * 64];
     } else {
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb)
             qb[kb] = *reinterpret_cast<const half8_t *>(p.query + qoff + (kb >> 1) * 64 + (kb & 1) * 8);
-        auto h = [](uint16_t x) { return static_cast<float>(__builtin_bit_cast(_Float16, x)); };
-        nk_lo = h(p.new_key[new_base + lane]);
-        nk_hi = h(p.new_key[new_base + lane + 64]);
-        nv_lo = h(p.new_value[new_base + lane]);
-        nv_hi = h(p.new_value[new_base + lane + 64]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n16[i] = (i < 2 ? p.new_key : p.new_value)[new_base + lane + (i & 1) * 64];
     }
-    float rc = 1.f, rs = 0.f;
-    if (rope) {
-        rc = p.rope_cos[static_cast<size_t>(pos) * 64 + lane];
-        rs = p.rope_sin[static_cast<size_t>(pos) * 64 + lane];
-    }
+    __builtin_amdgcn_sched_barrier(0);
 
     q8x4_t kr[8], vr[8];
     load_chunk(p, g, ids, 0, row, kg, kr, vr);
+    __builtin_amdgcn_sched_barrier(0);
+
+    if constexpr (!F32IO) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n32[i] = static_cast<float>(__builtin_bit_cast(_Float16, n16[i]));
+    }
+    const float nk_lo = n32[0], nk_hi = n32[1], nv_lo = n32[2], nv_hi = n32[3];
+    const float rc = rope ? rc_raw : 1.f, rs = rope ? rs_raw : 0.f;
 
     if (rope && p.rotate_query) {
         // The partner of step kb is step kb ^ 2 of the same lane; cos and sin
@@ -372,22 +400,24 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
         if (chunk > 0) load_chunk(p, g, ids, chunk, row, kg, kr, vr);
 
         if (chunk == append_chunk) {  // uniform
-            // The block of the new row: rows before it are rounded again where
-            // the exponent grew, the new row goes in, and what changed goes back
-            // to the cache.  The codes behind the new row stay in the cache as
-            // they are, and become 0 here: they may be e4m3 NaN.
-            if ((row >> 2) == ti) {
+            // The block of the new row.  Where its exponent grew (seldom), the
+            // rows before are rounded again in the cache and read back; then the
+            // new row goes into the registers and the cache.  The codes behind it
+            // stay in the cache as they are, and become 0 here: they may be e4m3
+            // NaN.
+            if (append_k != nullptr && (grown_k | grown_v) != 0) {
+                requantise_block<CODE>(append_k, append_v, lane, slot, grown_k, grown_v);
+                load_chunk(p, g, ids, chunk, row, kg, kr, vr);
+            }
+            const bool key_lane = (row >> 2) == ti && (row & 3) == (slot & 3);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int token = (i >> 1) * 4 + (row & 3);
-                    if (token < slot && grown_k > 0) {
+            for (int i = 0; i < 2; ++i) {
+                const q8x4_t piece = *reinterpret_cast<const q8x4_t *>(&sm_new[0][i * 64 + kg * 16]);
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) kr[i][w] = q8_requantise<CODE>(kr[i][w], grown_k);
-                    }
-                    if (token == slot) kr[i] = *reinterpret_cast<const q8x4_t *>(&sm_new[0][(i & 1) * 64 + kg * 16]);
-                    if (append_k != nullptr && (token == slot || (token < slot && grown_k > 0)))
-                        *reinterpret_cast<q8x4_t *>(append_k + (kg * 4 + (row & 3)) * 16 + i * 256) = kr[i];
-                }
+                for (int h = 0; h < 4; ++h)
+                    if (key_lane && h == (slot >> 2)) kr[h * 2 + i] = piece;
+                if (key_lane && append_k != nullptr)
+                    *reinterpret_cast<q8x4_t *>(append_k + (kg * 4 + (row & 3)) * 16 + ((slot >> 2) * 2 + i) * 256) = piece;
             }
             if (kg == ti) {
 #pragma unroll
@@ -399,9 +429,7 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
                         const uint32_t byte = 0xFFu << ((slot & 3) * 8);
                         const uint32_t put = w == (slot >> 2) ? byte : 0u;                                       // the new row
                         const uint32_t before = w < (slot >> 2) ? ~0u : (w == (slot >> 2) ? (byte & -byte) - 1u : 0u);  // the rows before it
-                        uint32_t v = vr[i][w];
-                        if (grown_v > 0) v = (q8_requantise<CODE>(v, grown_v) & before) | (v & ~before);
-                        v = (v & ~put) | (code & put);
+                        const uint32_t v = (vr[i][w] & ~put) | (code & put);
                         back[w] = v;
                         vr[i][w] = v & (before | put);
                     }
@@ -484,8 +512,24 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
 }
 
 // Grid (partition, kv head, sequence).
+// What the first loads' addresses need comes ahead of the parameter block, as
+// scalars: the first 14 dwords of arguments are in SGPRs when a wave starts.
 template <int WAVES, bool F32IO, int CODE>
-__global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_q8_kernel(DecodeQ8Params p) {
+__global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_q8_kernel(uint16_t *key_cache, uint16_t *value_cache, uint8_t *exponents,
+                                                                        const int32_t *cache_lens, const int32_t *block_tables,
+                                                                        uint32_t uniform_cache_len, uint32_t max_blocks_per_seq,
+                                                                        uint32_t num_blocks, uint32_t partition_and_parts,
+                                                                        DecodeQ8Params p) {
+    p.key_cache = key_cache;
+    p.value_cache = value_cache;
+    p.exponents = exponents;
+    p.cache_lens = cache_lens;
+    p.block_tables = block_tables;
+    p.uniform_cache_len = uniform_cache_len;
+    p.max_blocks_per_seq = max_blocks_per_seq;
+    p.num_blocks = num_blocks;
+    p.partition_tokens = partition_and_parts & 0xffffu;
+    p.max_parts = partition_and_parts >> 16;
     const uint32_t part = blockIdx.x, g = blockIdx.y, s = blockIdx.z;
     if ((part | g | s) == 0 && p.partition_word != nullptr && threadIdx.x == 0) {
         p.partition_word[0] = p.partition_tokens;
@@ -529,7 +573,10 @@ int launch_kernels(const DecodeLaunch &launch, DecodeQ8Params &p, hipStream_t st
         return static_cast<int>(hipGetLastError());
     }
     const dim3 grid(launch.max_parts, kKvHeads, a.num_seqs);
-#define PVLC_Q8_LAUNCH(W) hipLaunchKernelGGL((paged_decode_q8_kernel<W, F32IO, CODE>), grid, dim3((W) * 64), 0, st, p)
+#define PVLC_Q8_LAUNCH(W)                                                                                                   \
+    hipLaunchKernelGGL((paged_decode_q8_kernel<W, F32IO, CODE>), grid, dim3((W) * 64), 0, st, p.key_cache, p.value_cache,   \
+                       p.exponents, p.cache_lens, p.block_tables, p.uniform_cache_len, p.max_blocks_per_seq, p.num_blocks, \
+                       p.partition_tokens | p.max_parts << 16, p)
     switch ((launch.partition_tokens + kChunkTokens - 1) / kChunkTokens) {  // a wave for each 64 tokens, up to 384
         case 1: PVLC_Q8_LAUNCH(1); break;
         case 2: PVLC_Q8_LAUNCH(2); break;
