@@ -608,6 +608,101 @@ pvlc_hip_status pvlc_hip_kv_unpack_q8(const uint8_t *key_cache, const uint8_t *v
                                       uint16_t *key_rows, uint16_t *value_rows, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Pages of a cache: sharing, copying, freeing, compacting (new: the reference
+ * has one contiguous cache).
+ *
+ * A pool is num_blocks pages.  Page id's contents are its blocks in up to four
+ * planes (keys, values, the exponents of 8-bit ones) of each layer, at
+ * base + layer * layer_stride_bytes + id * block_bytes: one block table serves
+ * all layers.  ref_counts[id] is the number of block table entries that name the
+ * page, and bit id % 32 of free_mask[id / 32] is set where that is 0; both are
+ * the caller's buffers, and pvlc_hip_kv_pages_reset makes them an empty pool's.
+ * Entries of a table that hold no page are -1.  Everything runs on the caller's
+ * stream, without allocation, synchronisation or a copy to the host, and may be
+ * captured; what a call does depends on its inputs alone, not on timing.  Calls
+ * on one pool are stream-ordered.
+ * ------------------------------------------------------------------------- */
+
+typedef struct pvlc_hip_kv_plane {
+    void *base;                  /* 4-byte aligned; 16-byte aligned planes of 16-byte multiples move fastest */
+    uint64_t block_bytes;        /* of one page: a multiple of 4 */
+    uint64_t layer_stride_bytes; /* a multiple of 4 */
+} pvlc_hip_kv_plane;
+
+typedef struct pvlc_hip_kv_pool {
+    uint32_t num_blocks;
+    uint32_t max_blocks_per_seq; /* row stride of every block table */
+    uint32_t num_planes;         /* 1..4 */
+    uint32_t num_layers;
+    pvlc_hip_kv_plane planes[4];
+    int32_t *ref_counts; /* [num_blocks] */
+    uint32_t *free_mask; /* [ceil(num_blocks/32)]; bits behind the last block are 0 */
+    void *workspace;     /* pvlc_hip_kv_pages_workspace_bytes, 256-byte aligned, zeroed once */
+    size_t workspace_bytes;
+} pvlc_hip_kv_pool;
+
+/* Device error bits, in the first word of the pool's workspace
+ * (pvlc_hip_workspace_error reads it). */
+enum {
+    PVLC_HIP_PAGES_EXHAUSTED = 1,  /* fewer free pages than a fork asks for: it changes nothing but its outputs */
+    PVLC_HIP_PAGES_BAD_LENGTH = 2, /* an input row's length is negative or beyond its table: taken as 0 */
+    PVLC_HIP_PAGES_BAD_PARENT = 4, /* a parent outside -1..rows_in-1: taken as -1 */
+    PVLC_HIP_PAGES_BAD_BLOCK = 8,  /* an entry outside the pool: not shared, copied or counted */
+    PVLC_HIP_PAGES_BAD_COUNT = 16, /* a count would fall below 0 */
+    PVLC_HIP_PAGES_NO_ROOM = 32    /* length plus reserve exceeds the table: reserved up to its end */
+};
+
+/* Workspace for calls of up to `rows` input or output rows (a reset or a copy: 0). */
+size_t pvlc_hip_kv_pages_workspace_bytes(uint32_t num_blocks, uint32_t rows);
+/* Every page free, no error. */
+pvlc_hip_status pvlc_hip_kv_pages_reset(const pvlc_hip_kv_pool *pool, void *stream);
+
+/* Output row r continues input row parents[r] (of length L = lens_in + appended),
+ * or starts empty where that is -1, and gets pages for reserve[r] tokens more:
+ *   entries 0 .. L/16 - 1   the parent's own pages, shared;
+ *   the page of a last, partly filled block: the parent's own for its first
+ *     child, if no other entry names it; a copy (all planes, all layers) for
+ *     every other child, so that each may append to it;
+ *   up to ceil((L + reserve) / 16): pages that the parent reserved, again for
+ *     its first child as far as no other entry names them, then fresh ones;
+ *   -1 behind.
+ * The output rows hold what they name, and the input rows no longer do (unless
+ * keep_inputs): pages that nothing names any more become free, for the calls
+ * after this one.  Fresh pages are the lowest free ones, rows in order.  So a
+ * step of beam search is a fork by its parents, a prompt's fan-out a fork of one
+ * row to many, freeing a fork without those rows, truncation a fork at smaller
+ * lengths, and admission a fork with -1 and a reserve.
+ * If the pool has fewer free pages than needed, the call leaves the pool and its
+ * planes as they are, and every output row is -1 with length -1. */
+typedef struct pvlc_hip_kv_fork_args {
+    uint32_t rows_in;
+    uint32_t rows_out;
+    const int32_t *tables_in; /* [rows_in][max_blocks_per_seq] */
+    const int32_t *lens_in;   /* [rows_in] */
+    const int32_t *parents;   /* [rows_out], -1..rows_in-1; NULL: row r continues row r, or is new from rows_in on */
+    const int32_t *reserve;   /* [rows_out] tokens, or NULL: reserve_tokens each */
+    int32_t *tables_out;      /* [rows_out][max_blocks_per_seq], apart from tables_in */
+    int32_t *lens_out;        /* [rows_out], apart from lens_in */
+    uint32_t reserve_tokens;
+    uint32_t appended;    /* rows appended to every input row since lens_in was written */
+    uint32_t keep_inputs; /* the input rows stay: every child's partly filled block is a copy */
+} pvlc_hip_kv_fork_args;
+pvlc_hip_status pvlc_hip_kv_pages_fork(const pvlc_hip_kv_pool *pool, const pvlc_hip_kv_fork_args *args, void *stream);
+
+/* Moves pages so that the N in use are 0..N-1: those behind move, in order, to
+ * the free ones among the first N, in order.  tables [rows][max_blocks_per_seq]
+ * follow in place; forward (optional, [num_blocks]) receives every page's id
+ * after the call, for other tables. */
+pvlc_hip_status pvlc_hip_kv_pages_compact(const pvlc_hip_kv_pool *pool, int32_t *tables, uint32_t rows, int32_t *forward,
+                                          void *stream);
+
+/* Copies page from_blocks[i] of one pool to page to_blocks[i] of another (or the
+ * same), all planes and layers; counts and tables stay.  The pools need the same
+ * planes and layers.  Pages written must be distinct and none of those read. */
+pvlc_hip_status pvlc_hip_kv_pages_copy(const pvlc_hip_kv_pool *from, const int32_t *from_blocks, const pvlc_hip_kv_pool *to,
+                                       const int32_t *to_blocks, uint32_t count, void *stream);
+
+/* ---------------------------------------------------------------------------
  * Decoder GEMV with fp16 weights (the next path widened from this backend).
  * ------------------------------------------------------------------------- */
 
@@ -688,6 +783,44 @@ pvlc_hip_status pvlc_hip_logits_top1_f32(const float *logits, uint32_t vocab, ui
 pvlc_hip_status pvlc_hip_lm_head_top1_f16(const uint16_t *weights, const float *hidden, float *logits, uint32_t rows,
                                           uint32_t columns, uint32_t *result, void *workspace, size_t workspace_bytes,
                                           void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Beam search on the device (new: the reference decodes greedily).
+ * ------------------------------------------------------------------------- */
+
+/* The best continuations of each batch entry: row r = entry*beams + beam, whose
+ * sequence has score scores[r], continues with token t at
+ *   scores[r] + logits[r][t] - log(sum over u of exp(logits[r][u])),
+ * and the `best` highest over all beams and tokens are returned, best first:
+ * score (rounded to f32), parent row and token, and whether the sequence is
+ * finished (its parent was, or the token is end_token).  The order is that of
+ * the scores in 64 bits; equal ones by beam, then by logit (as the greedy top-1
+ * orders them), then by token.  A row with finished[r] continues with end_token
+ * alone at its score; a row whose score is -inf or NaN does not continue; its
+ * logits are not read in either case.  A logit of -inf or NaN masks its token,
+ * +inf counts as the largest finite value.  Where there are fewer candidates than
+ * `best`, the rest have score -inf, parent and token -1 and are not finished.
+ * parents is what pvlc_hip_kv_pages_fork takes.  Logits are f32 rows row_stride
+ * apart (4-byte aligned); 1 <= beams <= 64, 1 <= best <= 128. */
+typedef struct pvlc_hip_beam_args {
+    uint32_t batch;
+    uint32_t beams;
+    uint32_t vocab;
+    uint32_t best;
+    uint64_t row_stride;     /* elements */
+    const float *logits;     /* [batch*beams] rows */
+    const float *scores;     /* [batch][beams] */
+    const int32_t *finished; /* [batch][beams] or NULL */
+    int32_t end_token;       /* -1: none */
+    float *next_scores;      /* [batch][best], as the outputs below; none may overlap scores or finished */
+    int32_t *parents;
+    int32_t *tokens;
+    int32_t *next_finished; /* or NULL */
+    void *workspace;        /* pvlc_hip_beam_workspace_bytes, 256-byte aligned, zeroed once; calls on it are ordered */
+    size_t workspace_bytes;
+} pvlc_hip_beam_args;
+size_t pvlc_hip_beam_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t best);
+pvlc_hip_status pvlc_hip_beam_select_f32(const pvlc_hip_beam_args *args, void *stream);
 
 /* ---------------------------------------------------------------------------
  * Prefill projections with fp16 weights (multi-token linear layers).

@@ -36,6 +36,8 @@ BLOCK_TOKENS = 16
 # Codes of the 8-bit cache
 KV_E4M3 = 0
 KV_INT8 = 1
+# Device error bits of a page pool
+PAGES_EXHAUSTED, PAGES_BAD_LENGTH, PAGES_BAD_PARENT, PAGES_BAD_BLOCK, PAGES_BAD_COUNT, PAGES_NO_ROOM = 1, 2, 4, 8, 16, 32
 
 RUNTIME_ERROR_CODES = {
     1: "AdapterUnavailable", 2: "DeviceRequest", 3: "InvalidInvocation", 4: "Validation", 5: "OutOfMemory",
@@ -176,6 +178,29 @@ class PagedDecodeQ8ArgsC(ctypes.Structure):
                 ("workspace_bytes", _SZ)]
 
 
+class KvPlaneC(ctypes.Structure):
+    _fields_ = [("base", _VP), ("block_bytes", ctypes.c_uint64), ("layer_stride_bytes", ctypes.c_uint64)]
+
+
+class KvPoolC(ctypes.Structure):
+    _fields_ = [("num_blocks", _U32), ("max_blocks_per_seq", _U32), ("num_planes", _U32), ("num_layers", _U32),
+                ("planes", KvPlaneC * 4), ("ref_counts", _VP), ("free_mask", _VP), ("workspace", _VP),
+                ("workspace_bytes", _SZ)]
+
+
+class KvForkArgsC(ctypes.Structure):
+    _fields_ = [("rows_in", _U32), ("rows_out", _U32), ("tables_in", _VP), ("lens_in", _VP), ("parents", _VP),
+                ("reserve", _VP), ("tables_out", _VP), ("lens_out", _VP), ("reserve_tokens", _U32), ("appended", _U32),
+                ("keep_inputs", _U32)]
+
+
+class BeamArgsC(ctypes.Structure):
+    _fields_ = [("batch", _U32), ("beams", _U32), ("vocab", _U32), ("best", _U32), ("row_stride", ctypes.c_uint64),
+                ("logits", _VP), ("scores", _VP), ("finished", _VP), ("end_token", ctypes.c_int32),
+                ("next_scores", _VP), ("parents", _VP), ("tokens", _VP), ("next_finished", _VP), ("workspace", _VP),
+                ("workspace_bytes", _SZ)]
+
+
 class PagedPrefillArgsC(ctypes.Structure):
     _fields_ = [("tokens", _U32), ("num_blocks", _U32), ("block_table", _VP), ("key_cache", _VP),
                 ("value_cache", _VP), ("query", _VP), ("key", _VP), ("value", _VP), ("out", _VP),
@@ -229,6 +254,13 @@ SIGNATURES = {
     "pvlc_hip_paged_decode_q8_f32io": ([ctypes.POINTER(PagedDecodeQ8ArgsC), _VP, _VP, _VP, _VP, _VP], ctypes.c_int32),
     "pvlc_hip_kv_pack_q8": ([_VP, _VP, _U32, _U32, _VP, _U32, _U32, _VP, _VP, _VP, _VP], ctypes.c_int32),
     "pvlc_hip_kv_unpack_q8": ([_VP, _VP, _VP, _U32, _VP, _U32, _U32, _VP, _VP, _VP], ctypes.c_int32),
+    "pvlc_hip_kv_pages_workspace_bytes": ([_U32, _U32], _SZ),
+    "pvlc_hip_kv_pages_reset": ([ctypes.POINTER(KvPoolC), _VP], ctypes.c_int32),
+    "pvlc_hip_kv_pages_fork": ([ctypes.POINTER(KvPoolC), ctypes.POINTER(KvForkArgsC), _VP], ctypes.c_int32),
+    "pvlc_hip_kv_pages_compact": ([ctypes.POINTER(KvPoolC), _VP, _U32, _VP, _VP], ctypes.c_int32),
+    "pvlc_hip_kv_pages_copy": ([ctypes.POINTER(KvPoolC), _VP, ctypes.POINTER(KvPoolC), _VP, _U32, _VP], ctypes.c_int32),
+    "pvlc_hip_beam_workspace_bytes": ([_U32, _U32, _U32, _U32], _SZ),
+    "pvlc_hip_beam_select_f32": ([ctypes.POINTER(BeamArgsC), _VP], ctypes.c_int32),
     "pvlc_hip_gemv_tiled_plan_create": ([_U32, _U32, ctypes.POINTER(GemvTiledPlanC)], ctypes.c_int32),
     "pvlc_hip_gemv_f16": ([_VP, _VP, _VP, _U32, _U32, _VP], ctypes.c_int32),
     "pvlc_hip_gemv_group_f16": ([_VP, _U32, _VP, _U32, _VP], ctypes.c_int32),
@@ -831,6 +863,72 @@ def kv_unpack_q8(key_cache, value_cache, exponents, tokens, key_rows, value_rows
     """Rows 0..tokens-1 of a sequence's 8-bit blocks as fp16."""
     _check(lib.pvlc_hip_kv_unpack_q8(_ptr(key_cache), _ptr(value_cache), _ptr(exponents), tokens, _ptr(block_table),
                                      num_blocks, code, _ptr(key_rows), _ptr(value_rows), _stream(stream)))
+
+
+def kv_pages_workspace_bytes(num_blocks: int, rows: int) -> int:
+    return lib.pvlc_hip_kv_pages_workspace_bytes(num_blocks, rows)
+
+
+def kv_page_pool(*, num_blocks, max_blocks_per_seq, num_layers, planes, ref_counts, free_mask, workspace,
+                 workspace_bytes) -> KvPoolC:
+    """A pool of pages over planes [layers][num_blocks][elements of a block] (tensors, layers at any stride), or given
+    as (pointer, block bytes, layer stride bytes)."""
+    if not 1 <= len(planes) <= 4:
+        raise PvlcHipError(0x300 | 8, "a page pool has 1 to 4 planes")
+    c = KvPoolC(num_blocks, max_blocks_per_seq, len(planes), num_layers)
+    for i, p in enumerate(planes):
+        if isinstance(p, tuple):
+            base, block, stride = p
+        else:
+            if p.dim() != 3 or p.shape[0] != num_layers or p.shape[1] != num_blocks or not p[0].is_contiguous():
+                raise PvlcHipError(0x300 | 13, "a page plane is [layers][num_blocks][elements], contiguous but for layers")
+            size = p.element_size()
+            base, block, stride = p.data_ptr(), p.shape[2] * size, p.stride(0) * size
+        c.planes[i] = KvPlaneC(base, block, stride)
+    c.ref_counts, c.free_mask, c.workspace = _ptr(ref_counts), _ptr(free_mask), _ptr(workspace)
+    c.workspace_bytes = workspace_bytes
+    return c
+
+
+def kv_pages_reset(pool: KvPoolC, stream=None) -> None:
+    """Every page of the pool free."""
+    _check(lib.pvlc_hip_kv_pages_reset(ctypes.byref(pool), _stream(stream)))
+
+
+def kv_pages_fork(pool: KvPoolC, *, rows_in, rows_out, tables_in=None, lens_in=None, tables_out=None, lens_out=None,
+                  parents=None, reserve=None, reserve_tokens=0, appended=0, keep_inputs=False, stream=None) -> None:
+    """Rows of a block table taken over by others: filled blocks shared, the one that is written next copied, blocks
+    that no row names any more freed, and room reserved."""
+    a = KvForkArgsC(rows_in, rows_out, _ptr(tables_in), _ptr(lens_in), _ptr(parents), _ptr(reserve), _ptr(tables_out),
+                    _ptr(lens_out), reserve_tokens, appended, int(keep_inputs))
+    _check(lib.pvlc_hip_kv_pages_fork(ctypes.byref(pool), ctypes.byref(a), _stream(stream)))
+
+
+def kv_pages_compact(pool: KvPoolC, *, rows=0, tables=None, forward=None, stream=None) -> None:
+    """The pages in use moved to the lowest ids, block tables and all."""
+    _check(lib.pvlc_hip_kv_pages_compact(ctypes.byref(pool), _ptr(tables), rows, _ptr(forward), _stream(stream)))
+
+
+def kv_pages_copy(source: KvPoolC, source_blocks, target: KvPoolC, target_blocks, count: int, stream=None) -> None:
+    """Pages of one pool copied to pages of another, or of the same."""
+    _check(lib.pvlc_hip_kv_pages_copy(ctypes.byref(source), _ptr(source_blocks), ctypes.byref(target),
+                                      _ptr(target_blocks), count, _stream(stream)))
+
+
+def beam_workspace_bytes(batch: int, beams: int, vocab: int, best: int) -> int:
+    return lib.pvlc_hip_beam_workspace_bytes(batch, beams, vocab, best)
+
+
+def beam_select_args(*, batch, beams, vocab, best, logits, scores, next_scores, parents, tokens, workspace,
+                     workspace_bytes, row_stride=None, finished=None, next_finished=None, end_token=-1) -> BeamArgsC:
+    return BeamArgsC(batch, beams, vocab, best, vocab if row_stride is None else row_stride, _ptr(logits), _ptr(scores),
+                     _ptr(finished), end_token, _ptr(next_scores), _ptr(parents), _ptr(tokens), _ptr(next_finished),
+                     _ptr(workspace), workspace_bytes)
+
+
+def beam_select(args: BeamArgsC, stream=None) -> None:
+    """The best continuations of each batch entry over its beams and the vocabulary."""
+    _check(lib.pvlc_hip_beam_select_f32(ctypes.byref(args), _stream(stream)))
 
 
 def key_slot(t):

@@ -426,6 +426,104 @@ int launch_gemv_top1_f16(const uint16_t *weights, const float *vector, float *lo
                          uint32_t columns, Top1Slot *slots, uint32_t *result, void *stream);
 int launch_logits_top1_f32(const float *logits, uint32_t vocab, Top1Slot *slots, uint32_t *result, void *stream);
 
+// Pages of a cache (kernels_pages.hip).  A page's part of a plane: block_bytes
+// (a multiple of 4) at base + layer * layer_stride + id * block_bytes; `from`,
+// where not null, is the other pool's plane that a copy reads.  wide: 16-byte
+// accesses fit.
+constexpr uint32_t kMaxPagePlanes = 4;
+struct PagePlane {
+    uint8_t *base;
+    const uint8_t *from;
+    uint64_t block_bytes, layer_stride;
+    bool wide;
+    uint64_t from_stride;
+};
+struct PagePlanes {
+    PagePlane plane[kMaxPagePlanes];
+    uint32_t count, layers;
+};
+struct PagesFork {
+    uint32_t num_blocks, max_blocks, rows_in, rows_out, appended, reserve_tokens, keep_inputs;
+    const int32_t *tables_in, *lens_in, *parents, *reserve;
+    int32_t *tables_out, *lens_out, *ref_counts;
+    uint32_t *free_mask;
+    struct {
+        uint32_t *first, *children, *kept, *base;  // by row
+        int32_t *fresh;                            // the pages taken, in order
+        uint32_t *enough, *error_word;
+    } plan;
+};
+struct PagesCompact {
+    uint32_t num_blocks, max_blocks, rows;
+    int32_t *tables, *forward, *ref_counts;
+    uint32_t *free_mask;
+    struct {
+        uint32_t *used_before;     // by word of 32 pages, and the number in use behind them
+        int32_t *from, *to, *rank;  // moves; a page's number among them, or -1
+        uint32_t *moves;
+    } plan;
+};
+// Workspace: 256 bytes of words (0 the error word, 1 whether a fork found its
+// pages, 2 the moves of a compaction), then the plans' arrays; a fork's and a
+// compaction's share theirs.
+struct PagesWorkspace {
+    size_t rows_offset, first_offset, second_offset, third_offset, words_offset, total;
+};
+inline PagesWorkspace pages_workspace_layout(uint32_t num_blocks, uint32_t rows) {
+    auto align = [](size_t v) { return (v + 255) / 256 * 256; };
+    const size_t list = align(static_cast<size_t>(num_blocks) * 4);
+    PagesWorkspace w{};
+    w.rows_offset = 256;  // first, children, kept, base: 4 arrays of `rows`
+    w.first_offset = w.rows_offset + align(static_cast<size_t>(rows) * 16);
+    w.second_offset = w.first_offset + list;
+    w.third_offset = w.second_offset + list;
+    w.words_offset = w.third_offset + list;
+    w.total = w.words_offset + align((static_cast<size_t>(num_blocks) / 32 + 2) * 4);
+    return w;
+}
+int launch_pages_reset(int32_t *refs, uint32_t *mask, uint32_t num_blocks, uint32_t *error_word, void *stream);
+int launch_pages_fork(const PagesFork &f, const PagePlanes &planes, void *stream);
+int launch_pages_compact(const PagesCompact &c, const PagePlanes &planes, void *stream);
+int launch_pages_copy(const int32_t *src, const int32_t *dst, uint32_t count, uint32_t src_blocks, uint32_t dst_blocks, const PagePlanes &planes,
+                      uint32_t *error_word, void *stream);
+
+// Beam selection (kernels_beam.hip).  A row of logits is cut into segments of
+// kBeamThreads * kBeamEach; each leaves its best as keys (value and token in one
+// number, see there), its largest logit and its sum of exponentials.
+constexpr uint32_t kBeamThreads = 256, kBeamEach = 8, kBeamSegment = kBeamThreads * kBeamEach;
+constexpr uint32_t kBeamMaxBeams = 64, kBeamMaxBest = 128;
+struct BeamSelect {
+    uint32_t batch, beams, vocab, best, segments;
+    uint64_t row_stride;
+    const float *logits, *scores;
+    const int32_t *finished;
+    int32_t end_token;
+    float *next_scores;
+    int32_t *parents, *tokens, *next_finished;
+    uint32_t *arrived;    // by batch entry; 0 before and after a launch
+    uint64_t *keys;       // [row][segment][best]
+    double *sums;         // [row][segment]
+    float *largest;       // [row][segment]
+    uint64_t *row_keys;   // [row][best]
+    double *row_scores;   // [row][best]
+};
+struct BeamWorkspace {
+    size_t keys_offset, sums_offset, largest_offset, row_keys_offset, row_scores_offset, total;
+};
+inline BeamWorkspace beam_workspace_layout(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t best) {
+    auto align = [](size_t v) { return (v + 255) / 256 * 256; };
+    const size_t rows = static_cast<size_t>(batch) * beams, parts = rows * ((static_cast<size_t>(vocab) + kBeamSegment - 1) / kBeamSegment);
+    BeamWorkspace w{};
+    w.keys_offset = align(static_cast<size_t>(batch) * 4);
+    w.sums_offset = w.keys_offset + align(parts * best * 8);
+    w.largest_offset = w.sums_offset + align(parts * 8);
+    w.row_keys_offset = w.largest_offset + align(parts * 4);
+    w.row_scores_offset = w.row_keys_offset + align(rows * best * 8);
+    w.total = w.row_scores_offset + align(rows * best * 8);
+    return w;
+}
+int launch_beam_select(const BeamSelect &b, void *stream);
+
 // VisionPatchProjectionBytesDescriptor::plan (runtime-core lib.rs:1768-1840);
 // returns a pvlc_hip_projection_error.
 int32_t plan_projection(uint32_t patch_count, uint32_t input_width, uint32_t output_width, uint32_t weight_storage,

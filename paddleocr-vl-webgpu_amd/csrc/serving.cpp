@@ -62,6 +62,48 @@ pvlc_hip_status check_rows(const void *keys, const void *values, uint64_t end, u
     return PVLC_HIP_OK;
 }
 
+// The pool's description checked, its planes and workspace laid out.
+pvlc_hip_status check_pool(const pvlc_hip_kv_pool *pool, uint32_t rows, PagePlanes *planes, PagesWorkspace *layout) {
+    if (!pool) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "page pool is NULL");
+    if (pool->num_blocks == 0 || pool->max_blocks_per_seq == 0 || pool->num_planes == 0 || pool->num_layers == 0)
+        return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "blocks, table width, planes and layers of a page pool must be nonzero");
+    if (pool->num_blocks > 0x7FFFFFFFu || pool->num_planes > kMaxPagePlanes || pool->num_layers > 65535u)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "a page pool holds below 2^31 blocks, at most 4 planes and 65535 layers");
+    if (rows > 65535u || static_cast<uint64_t>(rows) * pool->max_blocks_per_seq > 0x7FFFFFFFull)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "at most 65535 table rows and 2^31 - 1 entries");
+    if (pool->max_blocks_per_seq > 0x7FFFFFFFu / kBlockTokens)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "a table row's tokens exceed 2^31 - 1");
+    if (!pool->ref_counts || !pool->free_mask || !pool->workspace)
+        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "page pool counts, mask or workspace pointer is NULL");
+    if (!aligned(pool->ref_counts, 4) || !aligned(pool->free_mask, 4) || !aligned(pool->workspace, 256))
+        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "page pool counts and mask must be 4-byte aligned, the workspace 256-byte aligned");
+    *planes = {};
+    planes->count = pool->num_planes;
+    planes->layers = pool->num_layers;
+    for (uint32_t i = 0; i < pool->num_planes; ++i) {
+        const pvlc_hip_kv_plane &p = pool->planes[i];
+        if (!p.base) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "page plane " + std::to_string(i) + " is NULL");
+        if (p.block_bytes == 0 || p.block_bytes % 4 != 0 || !aligned(p.base, 4) || p.layer_stride_bytes % 4 != 0)
+            return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT,
+                           "page plane " + std::to_string(i) + " must be 4-byte aligned, with blocks and layers of a multiple of 4 bytes");
+        if (p.block_bytes > 0x7FFFFFFFull) return invalid(PVLC_HIP_INV_ARITHMETIC_OVERFLOW, "a page's part of a plane exceeds 2^31 - 1 bytes");
+        if (pool->num_layers > 1 && p.layer_stride_bytes < p.block_bytes * pool->num_blocks)
+            return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "layers of page plane " + std::to_string(i) + " overlap");
+        const bool wide = aligned(p.base, 16) && p.block_bytes % 16 == 0 && p.layer_stride_bytes % 16 == 0;
+        planes->plane[i] = {static_cast<uint8_t *>(p.base), nullptr, p.block_bytes, p.layer_stride_bytes, wide, 0};
+    }
+    *layout = pages_workspace_layout(pool->num_blocks, rows);
+    if (pool->workspace_bytes < layout->total)
+        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "page workspace holds " + std::to_string(pool->workspace_bytes) +
+                                                         " bytes but the call needs " + std::to_string(layout->total));
+    return PVLC_HIP_OK;
+}
+
+bool overlap(const void *a, uint64_t a_bytes, const void *b, uint64_t b_bytes) {
+    const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+
 }  // namespace
 
 extern "C" {
@@ -95,6 +137,168 @@ pvlc_hip_status pvlc_hip_kv_unpack_q8(const uint8_t *key_cache, const uint8_t *v
     if (pvlc_hip_status st = check_rows(key_rows, value_rows, tokens, tokens, block_table, num_blocks)) return st;
     const int e = launch_kv_unpack_q8(key_cache, value_cache, exponents, tokens, block_table, num_blocks, code, key_rows, value_rows, stream);
     if (e != 0) return hip_status(e, "8-bit kv unpack launch");
+    return ok();
+}
+
+size_t pvlc_hip_kv_pages_workspace_bytes(uint32_t num_blocks, uint32_t rows) {
+    return num_blocks == 0 ? 0 : pages_workspace_layout(num_blocks, rows).total;
+}
+
+pvlc_hip_status pvlc_hip_kv_pages_reset(const pvlc_hip_kv_pool *pool, void *stream) {
+    PagePlanes planes;
+    PagesWorkspace ws;
+    if (pvlc_hip_status st = check_pool(pool, 0, &planes, &ws)) return st;
+    const int e = launch_pages_reset(pool->ref_counts, pool->free_mask, pool->num_blocks, static_cast<uint32_t *>(pool->workspace), stream);
+    if (e != 0) return hip_status(e, "page pool reset launch");
+    return ok();
+}
+
+pvlc_hip_status pvlc_hip_kv_pages_fork(const pvlc_hip_kv_pool *pool, const pvlc_hip_kv_fork_args *args, void *stream) {
+    if (!args) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "fork args are NULL");
+    const uint32_t rows = args->rows_in > args->rows_out ? args->rows_in : args->rows_out;
+    PagePlanes planes;
+    PagesWorkspace ws;
+    if (pvlc_hip_status st = check_pool(pool, rows, &planes, &ws)) return st;
+    if (rows == 0) return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "a fork needs input or output rows");
+    if (args->rows_in && (!args->tables_in || !args->lens_in)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "fork input pointer is NULL");
+    if (args->rows_out && (!args->tables_out || !args->lens_out)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "fork output pointer is NULL");
+    for (const void *p : {static_cast<const void *>(args->tables_in), static_cast<const void *>(args->lens_in), static_cast<const void *>(args->parents),
+                          static_cast<const void *>(args->reserve), static_cast<const void *>(args->tables_out), static_cast<const void *>(args->lens_out)})
+        if (!aligned(p, 4)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "fork tables, lengths, parents and reserve must be 4-byte aligned");
+    const uint64_t width = static_cast<uint64_t>(pool->max_blocks_per_seq) * 4;
+    if (overlap(args->tables_in, args->rows_in * width, args->tables_out, args->rows_out * width) ||
+        overlap(args->lens_in, args->rows_in * 4ull, args->lens_out, args->rows_out * 4ull))
+        return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "a fork's output tables and lengths may not overlap its input's");
+    // A workgroup of 256 threads for each row and for each (row, layer).
+    if (static_cast<uint64_t>(args->rows_out) * pool->num_layers + args->rows_in + args->rows_out >= 1u << 24)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows times layers of a fork exceed the grid");
+    auto *base = static_cast<unsigned char *>(pool->workspace);
+    PagesFork f{};
+    f.num_blocks = pool->num_blocks;
+    f.max_blocks = pool->max_blocks_per_seq;
+    f.rows_in = args->rows_in;
+    f.rows_out = args->rows_out;
+    f.appended = args->appended;
+    f.reserve_tokens = args->reserve_tokens;
+    f.keep_inputs = args->keep_inputs != 0;
+    f.tables_in = args->tables_in;
+    f.lens_in = args->lens_in;
+    f.parents = args->parents;
+    f.reserve = args->reserve;
+    f.tables_out = args->tables_out;
+    f.lens_out = args->lens_out;
+    f.ref_counts = pool->ref_counts;
+    f.free_mask = pool->free_mask;
+    auto *by_row = reinterpret_cast<uint32_t *>(base + ws.rows_offset);
+    f.plan = {by_row, by_row + rows, by_row + 2 * static_cast<size_t>(rows), by_row + 3 * static_cast<size_t>(rows),
+              reinterpret_cast<int32_t *>(base + ws.first_offset), reinterpret_cast<uint32_t *>(base) + 1, reinterpret_cast<uint32_t *>(base)};
+    const int e = launch_pages_fork(f, planes, stream);
+    if (e != 0) return hip_status(e, "page fork launch");
+    return ok();
+}
+
+pvlc_hip_status pvlc_hip_kv_pages_compact(const pvlc_hip_kv_pool *pool, int32_t *tables, uint32_t rows, int32_t *forward, void *stream) {
+    PagePlanes planes;
+    PagesWorkspace ws;
+    if (pvlc_hip_status st = check_pool(pool, rows, &planes, &ws)) return st;
+    if (rows && !tables) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "compaction tables pointer is NULL");
+    if (!aligned(tables, 4) || !aligned(forward, 4)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "compaction tables and map must be 4-byte aligned");
+    auto *base = static_cast<unsigned char *>(pool->workspace);
+    PagesCompact c{};
+    c.num_blocks = pool->num_blocks;
+    c.max_blocks = pool->max_blocks_per_seq;
+    c.rows = rows;
+    c.tables = tables;
+    c.forward = forward;
+    c.ref_counts = pool->ref_counts;
+    c.free_mask = pool->free_mask;
+    c.plan = {reinterpret_cast<uint32_t *>(base + ws.words_offset), reinterpret_cast<int32_t *>(base + ws.first_offset),
+              reinterpret_cast<int32_t *>(base + ws.second_offset), reinterpret_cast<int32_t *>(base + ws.third_offset),
+              reinterpret_cast<uint32_t *>(base) + 2};
+    const int e = launch_pages_compact(c, planes, stream);
+    if (e != 0) return hip_status(e, "page compaction launch");
+    return ok();
+}
+
+pvlc_hip_status pvlc_hip_kv_pages_copy(const pvlc_hip_kv_pool *from, const int32_t *from_blocks, const pvlc_hip_kv_pool *to, const int32_t *to_blocks,
+                                       uint32_t count, void *stream) {
+    PagePlanes source, planes;
+    PagesWorkspace ws;
+    if (pvlc_hip_status st = check_pool(from, 0, &source, &ws)) return st;
+    if (pvlc_hip_status st = check_pool(to, 0, &planes, &ws)) return st;
+    if (count == 0) return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "a copy of pages needs pairs");
+    if (count >= 1u << 24) return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "a copy of pages takes below 2^24 pairs");
+    if (!from_blocks || !to_blocks || !aligned(from_blocks, 4) || !aligned(to_blocks, 4))
+        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "page lists must be given and 4-byte aligned");
+    if (source.count != planes.count || source.layers != planes.layers)
+        return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "both pools of a copy need the same planes and layers");
+    for (uint32_t i = 0; i < planes.count; ++i) {
+        if (source.plane[i].block_bytes != planes.plane[i].block_bytes)
+            return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "plane " + std::to_string(i) + " has blocks of another size in the other pool");
+        planes.plane[i].from = source.plane[i].base;
+        planes.plane[i].from_stride = source.plane[i].layer_stride;
+        planes.plane[i].wide = planes.plane[i].wide && source.plane[i].wide;
+    }
+    const int e = launch_pages_copy(from_blocks, to_blocks, count, from->num_blocks, to->num_blocks, planes, static_cast<uint32_t *>(to->workspace), stream);
+    if (e != 0) return hip_status(e, "page copy launch");
+    return ok();
+}
+
+size_t pvlc_hip_beam_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t best) {
+    return batch == 0 || beams == 0 || vocab == 0 || best == 0 ? 0 : beam_workspace_layout(batch, beams, vocab, best).total;
+}
+
+pvlc_hip_status pvlc_hip_beam_select_f32(const pvlc_hip_beam_args *args, void *stream) {
+    if (!args) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "beam args are NULL");
+    if (args->batch == 0 || args->beams == 0 || args->vocab == 0 || args->best == 0)
+        return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "batch, beams, vocab and best must be nonzero");
+    if (args->beams > kBeamMaxBeams || args->best > kBeamMaxBest)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "at most 64 beams and 128 candidates");
+    if (args->vocab > 0x7FFFFFFFu || static_cast<uint64_t>(args->batch) * args->beams > 65535u)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "below 2^31 logits a row and at most 65535 rows");
+    if ((static_cast<uint64_t>(args->vocab) + kBeamSegment - 1) / kBeamSegment * args->batch * args->beams >= 1u << 24)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows times vocab of a beam selection exceed the grid");
+    if (args->row_stride < args->vocab) return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "rows of logits overlap");
+    if (!args->logits || !args->scores || !args->next_scores || !args->parents || !args->tokens || !args->workspace)
+        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "beam buffer pointer is NULL");
+    for (const void *p : {static_cast<const void *>(args->logits), static_cast<const void *>(args->scores), static_cast<const void *>(args->finished),
+                          static_cast<const void *>(args->next_scores), static_cast<const void *>(args->parents), static_cast<const void *>(args->tokens),
+                          static_cast<const void *>(args->next_finished)})
+        if (!aligned(p, 4)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "beam buffers must be 4-byte aligned");
+    const uint64_t in = static_cast<uint64_t>(args->batch) * args->beams * 4, out = static_cast<uint64_t>(args->batch) * args->best * 4;
+    for (const void *p : {static_cast<const void *>(args->next_scores), static_cast<const void *>(args->parents), static_cast<const void *>(args->tokens),
+                          static_cast<const void *>(args->next_finished)})
+        if (overlap(p, p ? out : 0, args->scores, in) || overlap(p, p ? out : 0, args->finished, args->finished ? in : 0))
+            return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "the selection's outputs may not overlap its scores or finished flags");
+    const BeamWorkspace ws = beam_workspace_layout(args->batch, args->beams, args->vocab, args->best);
+    if (args->workspace_bytes < ws.total)
+        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "beam workspace holds " + std::to_string(args->workspace_bytes) + " bytes but the call needs " +
+                                                         std::to_string(ws.total));
+    if (!aligned(args->workspace, 256)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "beam workspace must be 256-byte aligned");
+    auto *base = static_cast<unsigned char *>(args->workspace);
+    BeamSelect b{};
+    b.batch = args->batch;
+    b.beams = args->beams;
+    b.vocab = args->vocab;
+    b.best = args->best;
+    b.segments = (args->vocab + kBeamSegment - 1) / kBeamSegment;
+    b.row_stride = args->row_stride;
+    b.logits = args->logits;
+    b.scores = args->scores;
+    b.finished = args->finished;
+    b.end_token = args->end_token;
+    b.next_scores = args->next_scores;
+    b.parents = args->parents;
+    b.tokens = args->tokens;
+    b.next_finished = args->next_finished;
+    b.arrived = reinterpret_cast<uint32_t *>(base);
+    b.keys = reinterpret_cast<uint64_t *>(base + ws.keys_offset);
+    b.sums = reinterpret_cast<double *>(base + ws.sums_offset);
+    b.largest = reinterpret_cast<float *>(base + ws.largest_offset);
+    b.row_keys = reinterpret_cast<uint64_t *>(base + ws.row_keys_offset);
+    b.row_scores = reinterpret_cast<double *>(base + ws.row_scores_offset);
+    const int e = launch_beam_select(b, stream);
+    if (e != 0) return hip_status(e, "beam selection launch");
     return ok();
 }
 
