@@ -794,11 +794,11 @@ pvlc_hip_status pvlc_hip_lm_head_top1_f16(const uint16_t *weights, const float *
  * and the `best` highest over all beams and tokens are returned, best first:
  * score (rounded to f32), parent row and token, and whether the sequence is
  * finished (its parent was, or the token is end_token).  The order is that of
- * the scores in 64 bits; equal ones by beam, then by logit (as the greedy top-1
- * orders them), then by token.  A row with finished[r] continues with end_token
+ * the scores in 64 bits, of which it takes 39 of the fraction; equal ones go by
+ * beam, then by logit (as the greedy top-1 orders them), then by token.  A row with finished[r] continues with end_token
  * alone at its score; a row whose score is -inf or NaN does not continue; its
- * logits are not read in either case.  A logit of -inf or NaN masks its token,
- * +inf counts as the largest finite value.  Where there are fewer candidates than
+ * logits are not read in either case.  A logit below -2^127 (-inf and the type's
+ * lowest value among them) or NaN masks its token, one above 2^127 counts as 2^127.  Where there are fewer candidates than
  * `best`, the rest have score -inf, parent and token -1 and are not finished.
  * parents is what pvlc_hip_kv_pages_fork takes.  Logits are f32 rows row_stride
  * apart (4-byte aligned); 1 <= beams <= 64, 1 <= best <= 128. */

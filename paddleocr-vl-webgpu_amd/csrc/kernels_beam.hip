@@ -8,14 +8,16 @@
 //
 // Order.  Within a row candidates are ordered by logit, then by token: one
 // 64-bit key, (the logit's bits, made monotone) * 2^32 + (2^32 - 1 - token), so no
-// two are equal and the larger is the better.  Across rows by score, in 64 bits
-// (scores of two beams may lie closer than f32 tells apart, and the order of
-// what is returned must not depend on it), then by beam, then by key.
+// two are equal and the larger is the better.  Across rows by score, in 64 bits:
+// scores of two beams may lie closer than f32 tells apart, and the order of what
+// is returned must not depend on it.  Again one key: the score's bits, made
+// monotone, with the lowest 13 given to the candidate's number (beam, then rank
+// in its row), so that scores equal to 2^-39 go by beam and rank.
 //
-// The best n of many without sorting them: with the values dealt to threads, the
-// n-th largest of the threads' own largest is a bound that at least n values
-// reach, and only values of n threads can reach it, so a short list remains,
-// whose ranks are counted.
+// The best n of many without sorting them: with the values dealt to groups of
+// threads, the n-th largest of the groups' own largest is a bound that at least n
+// values reach, and only values of n groups can reach it, so a short list
+// remains, whose ranks are counted.
 
 #include <hip/hip_runtime.h>
 
@@ -29,29 +31,41 @@ namespace {
 
 typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 
-constexpr float kLargestFloat = 3.402823466e38f;
+// Logits above 2^127 (and +inf) count as 2^127 and those below -2^127 as masked,
+// like -inf and NaN: so masks of the type's lowest value are masks.
+constexpr float kMostLogit = 1.7014118346046923e38f;
+__device__ inline float clean(float x) { return x != x ? -INFINITY : fminf(x, kMostLogit); }
 
-// NaN counts as masked (-inf), +inf as the largest finite value.
-__device__ inline float clean(float x) { return x != x ? -INFINITY : fminf(x, kLargestFloat); }
-
-__device__ inline uint64_t key_of(float x, uint32_t token) {
+// A logit's bits as a whole number in its order (-0 below +0), and back.
+__device__ inline int32_t order_of(float x) {
     const int32_t bits = __float_as_int(x);
-    const uint32_t order = static_cast<uint32_t>(bits ^ ((bits >> 31) & 0x7FFFFFFF)) ^ 0x80000000u;
-    return static_cast<uint64_t>(order) << 32 | (0xFFFFFFFFu - token);
+    return bits ^ ((bits >> 31) & 0x7FFFFFFF);
 }
-__device__ inline float logit_of(uint64_t key) {
-    const int32_t order = static_cast<int32_t>(static_cast<uint32_t>(key >> 32) ^ 0x80000000u);
-    return __int_as_float(order ^ ((order >> 31) & 0x7FFFFFFF));
-}
-__device__ inline uint32_t token_of(uint64_t key) { return 0xFFFFFFFFu - static_cast<uint32_t>(key); }
-constexpr uint64_t kNoKey = 0;  // below every logit's key (a NaN's, which none has)
+__device__ inline float value_of(int32_t order) { return __int_as_float(order ^ ((order >> 31) & 0x7FFFFFFF)); }
+constexpr int32_t kMaskedOrder = static_cast<int32_t>((0xFF000000u ^ 0x7FFFFFFFu) - 1u);  // just below that of -2^127
 
-// exp(x) for x <= 0.  The product with log2(e) in two parts: the rounded
-// constant alone shifts a term by 1.3e-8 of its exponent.
-__device__ inline float exp_of(float x) {
-    const float y = fmaxf(x, -200.f);  // 0 below, -inf among it
-    const float hi = y * 1.44269502f;
-    return __builtin_amdgcn_exp2f(hi + (__builtin_fmaf(y, 1.44269502f, -hi) + y * 1.92596299e-8f));
+__device__ inline uint64_t key_of(int32_t order, uint32_t token) {
+    return static_cast<uint64_t>(static_cast<uint32_t>(order) ^ 0x80000000u) << 32 | (0xFFFFFFFFu - token);
+}
+__device__ inline int32_t order_in(uint64_t key) { return static_cast<int32_t>(static_cast<uint32_t>(key >> 32) ^ 0x80000000u); }
+__device__ inline uint32_t token_in(uint64_t key) { return 0xFFFFFFFFu - static_cast<uint32_t>(key); }
+constexpr uint64_t kNoKey = 0;  // below every candidate's key
+
+// A score's key, and the score to 2^-39 and the candidate's number back.
+constexpr uint32_t kNumbers = 8192;
+static_assert(kBeamMaxBeams * kBeamMaxBest <= kNumbers, "a candidate's number fits a score's key");
+__device__ inline uint64_t score_key(double score, uint32_t number) {
+    const int64_t bits = __double_as_longlong(score);
+    const uint64_t order = static_cast<uint64_t>(bits ^ ((bits >> 63) & 0x7FFFFFFFFFFFFFFFll)) ^ 0x8000000000000000ull;
+    return (order & ~static_cast<uint64_t>(kNumbers - 1)) | (kNumbers - 1 - number);
+}
+__device__ inline uint32_t number_in(uint64_t key) { return kNumbers - 1 - (static_cast<uint32_t>(key) & (kNumbers - 1)); }
+
+// exp(x - reference), x <= reference.  log2(e) in two parts: the rounded constant
+// alone shifts a term by 1.3e-8 of its exponent.
+__device__ inline float exp_term(float x, float reference) {
+    const float d = x - reference;
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(d, 1.44269502f, d * 1.92596299e-8f));
 }
 
 // A beam goes on if its score is above -inf (not NaN), a row of logits is read
@@ -59,189 +73,248 @@ __device__ inline float exp_of(float x) {
 __device__ inline bool row_finished(const BeamSelect &b, uint32_t row) { return b.finished != nullptr && b.finished[row] != 0; }
 __device__ inline bool row_alive(const BeamSelect &b, uint32_t row) { return b.scores[row] > -INFINITY; }
 
-// Order of a row's candidates: the key; of a batch entry's: score, then the lower
-// number (beam, and rank in its row).
-struct Scored {
-    double score;  // -inf: none
-    uint32_t number;
-    uint32_t pad;
-};
-__device__ inline bool better(uint64_t a, uint64_t b) { return a > b; }
-__device__ inline bool better(const Scored &a, const Scored &b) { return a.score > b.score || (a.score == b.score && a.number < b.number); }
-__device__ inline bool is_any(uint64_t a) { return a != kNoKey; }
-__device__ inline bool is_any(const Scored &a) { return a.score > -INFINITY; }
-
-// LDS of best_of: the threads' own largest, the short list, the bound.
-template <class Item, int kEach>
+// LDS of best_of, ahead of its short list.
 struct BestLds {
-    Item most[kBeamThreads];
-    Item list[kBeamMaxBest * kEach];
-    Item bound;
-    uint32_t count;
+    uint64_t most[kBeamThreads];
+    uint32_t count, pad;
 };
+// Groups whose largest bound the selection: 64 of four threads, or the threads
+// themselves where more than 64 are wanted.  Items that can reach the bound:
+constexpr uint32_t best_list(uint32_t best, uint32_t each) { return best * each * (best <= 64 ? 4 : 1); }
 
-// The `best` best of the workgroup's items, kEach a thread, in order: put(rank,
-// item) for each of them, as many as there are.  No two items are equal.  Every
-// thread calls it; what put writes to LDS is seen after the next barrier.
-template <int kEach, class Item, class Put>
-__device__ inline void best_of(const Item (&item)[kEach], const Item &none, uint32_t best, BestLds<Item, kEach> &lds, Put put) {
+__device__ inline uint64_t larger_key(uint64_t a, uint64_t b) { return a > b ? a : b; }
+template <int CTRL>
+__device__ inline uint64_t dpp_key(uint64_t k) {
+    const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(k), CTRL, 0xF, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(k >> 32), CTRL, 0xF, 0xF, false);
+    return static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo);
+}
+__device__ inline uint64_t lane_key(uint64_t k, int lane) {
+    const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k), lane));
+    const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k >> 32), lane));
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+// The `best` largest keys of the workgroup: own is the thread's largest (kNoKey:
+// none), push(bound, list) adds those of the thread's keys that reach a bound to
+// the list, and put(rank, key) receives the best, in order.  Returns how many
+// there are.  No two keys are equal.  Every thread calls it; LDS is free for the
+// next call after a barrier.
+template <class Push, class Put>
+__device__ inline uint32_t best_of(uint64_t own, uint32_t best, BestLds &lds, uint64_t *list, Push push, Put put) {
     const uint32_t i = threadIdx.x;
-    Item own = none;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e)
-        if (better(item[e], own)) own = item[e];
-    lds.most[i] = own;
-    if (i == 0) {
-        lds.bound = none;
-        lds.count = 0;
+    const int lane = i & 63;
+    if (i == 0) lds.count = 0;
+    uint64_t bound = 1;  // every key
+    if (best <= 64) {
+        own = larger_key(own, dpp_key<0xB1>(own));
+        own = larger_key(own, dpp_key<0x4E>(own));
+        if ((i & 3) == 0) lds.most[i >> 2] = own;
+        __syncthreads();
+        // every wave ranks the 64 groups, one a lane
+        const uint64_t mine = lds.most[lane];
+        uint32_t above = 0;
+#pragma unroll 16
+        for (int j = 0; j < 64; ++j) above += lds.most[j] > mine;
+        const uint64_t at = __ballot(mine != kNoKey && above == best - 1);
+        if (at != 0) bound = lane_key(mine, __ffsll(static_cast<unsigned long long>(at)) - 1);
+    } else {
+        lds.most[i] = own;
+        __syncthreads();
+        // every wave ranks all 256, four a lane
+#pragma unroll 1
+        for (uint32_t q = 0; q < kBeamThreads / 64; ++q) {
+            const uint64_t mine = lds.most[q * 64 + lane];
+            uint32_t above = 0;
+#pragma unroll 16
+            for (uint32_t j = 0; j < kBeamThreads; ++j) above += lds.most[j] > mine;
+            const uint64_t at = __ballot(mine != kNoKey && above == best - 1);
+            if (at != 0) bound = lane_key(mine, __ffsll(static_cast<unsigned long long>(at)) - 1);
+        }
     }
-    __syncthreads();
-    uint32_t above = 0;
-#pragma unroll 8
-    for (uint32_t j = 0; j < kBeamThreads; ++j) above += better(lds.most[j], own);
-    const bool in = is_any(own) && above < best;
-    if (in && above == best - 1) lds.bound = own;  // one thread at most; without it all items of fewer than `best` threads are listed
-    __syncthreads();
-    if (in) {
-        const Item bound = lds.bound;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e)
-            if (is_any(item[e]) && !better(bound, item[e])) lds.list[atomicAdd(&lds.count, 1u)] = item[e];
-    }
+    push(bound, [&](uint64_t key) { list[atomicAdd(&lds.count, 1u)] = key; });
     __syncthreads();
     const uint32_t n = lds.count;
     for (uint32_t c = i; c < n; c += kBeamThreads) {
-        const Item mine = lds.list[c];
+        const uint64_t mine = list[c];
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; ++j) rank += better(lds.list[j], mine);
+        for (uint32_t j = 0; j < n; ++j) rank += list[j] > mine;
         if (rank < best) put(rank, mine);
     }
+    return min(n, best);
 }
 
 template <class T, class Op>
 __device__ inline T workgroup_reduce(T v, T *sm, Op op) {
-    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o));
-    __syncthreads();  // sm's readers before are done
-    if (lane == 0) sm[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
     __syncthreads();
     T r = sm[0];
 #pragma unroll
     for (uint32_t w = 1; w < kBeamThreads / 64; ++w) r = op(r, sm[w]);
     return r;
 }
-__device__ inline float larger(float a, float b) { return fmaxf(a, b); }
 __device__ inline double plus(double a, double b) { return a + b; }
 
-// Grid (segment, row).
+// Grid (segment, row): kEach * kBeamThreads logits each.
+template <uint32_t kEach>
 __global__ __launch_bounds__(kBeamThreads) void beam_segment_kernel(BeamSelect b) {
-    __shared__ BestLds<uint64_t, kBeamEach> lds;
+    extern __shared__ uint64_t list[];
+    __shared__ BestLds lds;
     __shared__ float sm_f[kBeamThreads / 64];
     __shared__ double sm_d[kBeamThreads / 64];
     const uint32_t segment = blockIdx.x, row = blockIdx.y, i = threadIdx.x;
+    constexpr uint32_t kSegment = kEach * kBeamThreads;
     if (!row_alive(b, row) || row_finished(b, row)) return;  // uniform; the row's join reads nothing then
     const float *x = b.logits + static_cast<uint64_t>(row) * b.row_stride;
-    const uint32_t first = segment * kBeamSegment;
-    float v[kBeamEach];
+    const uint32_t first = segment * kSegment;
+    float v[kEach];
+    if (b.vocab - first >= kSegment) {  // uniform
 #pragma unroll
-    for (uint32_t c = 0; c < kBeamEach / 4; ++c) {
-        const uint32_t at = first + (c * kBeamThreads + i) * 4;
-        if (b.vocab - first >= kBeamSegment) {  // uniform
-            const f32x4_any q = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any *>(x + at));
+        for (uint32_t c = 0; c < kEach / 4; ++c) {
+            const f32x4_any q = __builtin_nontemporal_load(reinterpret_cast<const f32x4_any *>(x + first + (c * kBeamThreads + i) * 4));
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[c * 4 + e] = q[e];
-        } else {
+        }
+    } else {
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) v[c * 4 + e] = at + e < b.vocab ? x[at + e] : -INFINITY;
+        for (uint32_t e = 0; e < kEach; ++e) {
+            const uint32_t at = first + ((e >> 2) * kBeamThreads + i) * 4 + (e & 3);
+            v[e] = at < b.vocab ? x[at] : -INFINITY;
         }
     }
-    float most = -INFINITY;
-    uint64_t key[kBeamEach];
+    // Largest logit and sum of exponentials of the thread, relative to its own
+    // reference.  Logits that need cleaning show in one or the other.
+    int32_t order[kEach], most;
+    float reference, sum;
+    auto scan = [&]() {
+        most = order[0] = order_of(v[0]);
 #pragma unroll
-    for (uint32_t e = 0; e < kBeamEach; ++e) {
-        v[e] = clean(v[e]);
-        most = fmaxf(most, v[e]);
-        key[e] = v[e] > -INFINITY ? key_of(v[e], first + ((e >> 2) * kBeamThreads + i) * 4 + (e & 3)) : kNoKey;
+        for (uint32_t e = 1; e < kEach; ++e) {
+            order[e] = order_of(v[e]);
+            most = max(most, order[e]);
+        }
+        reference = most > kMaskedOrder ? value_of(most) : 0.f;
+        sum = 0.f;
+#pragma unroll
+        for (uint32_t e = 0; e < kEach; ++e) sum += exp_term(v[e], reference);
+    };
+    scan();
+    if (__any(most > __float_as_int(kMostLogit) || sum != sum)) {
+#pragma unroll
+        for (uint32_t e = 0; e < kEach; ++e) v[e] = clean(v[e]);
+        scan();
     }
-    most = workgroup_reduce(most, sm_f, larger);
-    float sum = 0.f;
-#pragma unroll
-    for (uint32_t e = 0; e < kBeamEach; ++e) sum += exp_of(v[e] - most);  // (NaN where all are masked: not used)
-    const double total = workgroup_reduce(static_cast<double>(sum), sm_d, plus);
+    const bool any = most > kMaskedOrder;
+    const float top = workgroup_reduce(any ? reference : -INFINITY, sm_f, [](float x, float y) { return fmaxf(x, y); });
+    const double total = workgroup_reduce(any ? static_cast<double>(sum * exp_term(reference, top)) : 0.0, sm_d, plus);
     const size_t part = static_cast<size_t>(row) * b.segments + segment;
     if (i == 0) {
-        b.largest[part] = most;
-        b.sums[part] = most > -INFINITY ? total : 0.0;
+        b.references[part] = top;
+        b.sums[part] = total;
     }
+    auto token = [&](uint32_t e) { return first + ((e >> 2) * kBeamThreads + i) * 4 + (e & 3); };
+    uint64_t own = kNoKey;
+#pragma unroll
+    for (uint32_t e = kEach; e-- > 0;)
+        if (any && order[e] == most) own = key_of(most, token(e));  // the lowest token of the largest
     uint64_t *out = b.keys + part * b.best;
-    best_of(key, kNoKey, b.best, lds, [&](uint32_t rank, uint64_t k) { out[rank] = k; });
-    for (uint32_t k = min(lds.count, b.best) + i; k < b.best; k += kBeamThreads) out[k] = kNoKey;
+    const uint32_t found = best_of(
+        own, b.best, lds, list,
+        [&](uint64_t bound, auto add) {
+            const int32_t least = max(order_in(bound), kMaskedOrder + 1);
+            if (most < least) return;
+#pragma unroll
+            for (uint32_t e = 0; e < kEach; ++e) {
+                if (order[e] < least) continue;
+                const uint64_t key = key_of(order[e], token(e));
+                if (key >= bound) add(key);
+            }
+        },
+        [&](uint32_t rank, uint64_t key) { out[rank] = key; });
+    for (uint32_t k = found + i; k < b.best; k += kBeamThreads) out[k] = kNoKey;
 }
 
 __device__ inline void store_agent(uint64_t *p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ inline uint64_t load_agent(const uint64_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
+// Keys a thread takes at a time in the join, beside one of the best so far.
+constexpr uint32_t kJoinEach = 4;
+
+// The `best` largest of keys(0) .. keys(count - 1) into run, in order, kNoKey
+// behind.  Every thread calls it; run is complete after a barrier.
+template <class Keys>
+__device__ inline void join_keys(uint64_t count, uint32_t best, BestLds &lds, uint64_t *list, uint64_t *run, Keys keys) {
+    const uint32_t i = threadIdx.x;
+    for (uint32_t k = i; k < best; k += kBeamThreads) run[k] = kNoKey;
+    __syncthreads();
+    for (uint64_t at = 0; at < count; at += kJoinEach * kBeamThreads) {
+        uint64_t key[kJoinEach + 1], own = kNoKey;
+#pragma unroll
+        for (uint32_t e = 0; e < kJoinEach; ++e) {
+            const uint64_t k = at + e * kBeamThreads + i;
+            key[e] = k < count ? keys(k) : kNoKey;
+        }
+        key[kJoinEach] = i < best ? run[i] : kNoKey;
+#pragma unroll
+        for (uint32_t e = 0; e <= kJoinEach; ++e) own = larger_key(own, key[e]);
+        best_of(
+            own, best, lds, list,
+            [&](uint64_t bound, auto add) {
+#pragma unroll
+                for (uint32_t e = 0; e <= kJoinEach; ++e)
+                    if (key[e] >= bound) add(key[e]);
+            },
+            [&](uint32_t rank, uint64_t k) { run[rank] = k; });
+        __syncthreads();
+    }
+}
+
 // A workgroup joins the segments of a row; the last row of a batch entry joins
 // its rows (relaxed agent-scope stores, their acknowledgement, a counter, and
 // agent-scope loads, as the split decode's partitions).
 __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
-    constexpr int kEach = kBeamEach + 1;  // a round's items, and one of the best so far
-    __shared__ union {
-        BestLds<uint64_t, kEach> keys;
-        BestLds<Scored, kEach> scored;
-    } lds;
-    __shared__ uint64_t run[kBeamMaxBest];
-    __shared__ Scored run_scored[kBeamMaxBest];
-    __shared__ float sm_f[kBeamThreads / 64];
-    __shared__ double sm_d[kBeamThreads / 64];
+    extern __shared__ uint64_t list[];
+    __shared__ BestLds lds;
+    __shared__ uint64_t run[kBeamMaxBest], run_scores[kBeamMaxBest];
+    __shared__ double sm_m[kBeamThreads / 64], sm_d[kBeamThreads / 64];
     __shared__ int sm_last;
     const uint32_t row = blockIdx.x, i = threadIdx.x, entry = row / b.beams;
     const float start = b.scores[row];
-    const bool finished = row_finished(b, row);
-    for (uint32_t k = i; k < b.best; k += kBeamThreads) run[k] = kNoKey;
-    __syncthreads();
-    double lse = 0.0;
-    if (start > -INFINITY && finished) {
-        if (i == 0) run[0] = 0x8000000000000000ull | (0xFFFFFFFFu - static_cast<uint32_t>(b.end_token));
-    } else if (start > -INFINITY) {
+    const bool finished = row_finished(b, row), alive = start > -INFINITY;
+    double top = -INFINITY, log_sum = 0.0;
+    if (alive && !finished) {
         const size_t part = static_cast<size_t>(row) * b.segments;
-        float most = -INFINITY;
-        for (uint32_t s = i; s < b.segments; s += kBeamThreads) most = fmaxf(most, b.largest[part + s]);
-        most = workgroup_reduce(most, sm_f, larger);
+        for (uint32_t s = i; s < b.segments; s += kBeamThreads) top = fmax(top, static_cast<double>(b.references[part + s]));
+        top = workgroup_reduce(top, sm_m, [](double x, double y) { return fmax(x, y); });
         double sum = 0.0;
-        if (most > -INFINITY)  // uniform
-            for (uint32_t s = i; s < b.segments; s += kBeamThreads) sum += b.sums[part + s] * exp(static_cast<double>(b.largest[part + s]) - most);
+        if (top > -INFINITY)  // uniform
+            for (uint32_t s = i; s < b.segments; s += kBeamThreads) sum += b.sums[part + s] * exp(static_cast<double>(b.references[part + s]) - top);
         sum = workgroup_reduce(sum, sm_d, plus);
-        lse = most + log(sum);
-        if (most > -INFINITY) {
-            const uint64_t *keys = b.keys + part * b.best;
-            const uint64_t items = static_cast<uint64_t>(b.segments) * b.best;
-            for (uint64_t at = 0; at < items; at += kBeamSegment) {
-                uint64_t key[kEach];
-#pragma unroll
-                for (uint32_t e = 0; e < kBeamEach; ++e) {
-                    const uint64_t k = at + e * kBeamThreads + i;
-                    key[e] = k < items ? keys[k] : kNoKey;
-                }
-                key[kBeamEach] = i < b.best ? run[i] : kNoKey;
-                best_of(key, kNoKey, b.best, lds.keys, [&](uint32_t rank, uint64_t k) { run[rank] = k; });
-                __syncthreads();
-            }
-        }
+        log_sum = log(sum);  // (not used where all is masked)
+        const uint64_t *keys = b.keys + part * b.best;
+        join_keys(static_cast<uint64_t>(b.segments) * b.best, b.best, lds, list, run, [&](uint64_t k) { return keys[k]; });
+    } else {
+        for (uint32_t k = i; k < b.best; k += kBeamThreads)
+            run[k] = alive && k == 0 ? key_of(0, static_cast<uint32_t>(b.end_token)) : kNoKey;
+        __syncthreads();
     }
-    __syncthreads();
-    // (thread i holds rank i of the row)
-    auto score_of = [&](uint64_t key) {
-        return finished ? static_cast<double>(start) : start + (static_cast<double>(logit_of(key)) - lse);
-    };
+    // Thread i holds rank i of the row: its token, and its score's key.
+    const uint32_t beam = row - entry * b.beams;
+    uint64_t key = kNoKey, scored = kNoKey;
+    double score = 0.0;
+    if (i < b.best) {
+        key = run[i];
+        score = finished ? static_cast<double>(start) : start + ((static_cast<double>(value_of(order_in(key))) - top) - log_sum);
+        if (key != kNoKey) scored = score_key(score, beam * b.best + i);
+    }
+    const size_t at = static_cast<size_t>(row) * b.best + i, rows_at = static_cast<size_t>(entry) * b.beams * b.best;
     if (b.beams > 1) {
         if (i < b.best) {
-            const size_t at = static_cast<size_t>(row) * b.best + i;
-            const uint64_t key = run[i];
-            store_agent(b.row_keys + at, key);
+            store_agent(b.row_keys + at, scored);
             store_agent(reinterpret_cast<uint64_t *>(b.row_scores) + at,
-                        static_cast<uint64_t>(__double_as_longlong(key != kNoKey ? score_of(key) : -INFINITY)));
+                        static_cast<uint64_t>(token_in(key)) << 32 | __float_as_uint(static_cast<float>(score)));
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -249,49 +322,46 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
         __syncthreads();
         if (!sm_last) return;
         if (i == 0) __hip_atomic_store(b.arrived + entry, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        join_keys(static_cast<uint64_t>(b.beams) * b.best, b.best, lds, list, run_scores, [&](uint64_t k) { return load_agent(b.row_keys + rows_at + k); });
+        if (i >= b.best) return;
+        scored = run_scores[i];
     }
-    const Scored none{-INFINITY, UINT32_MAX, 0};
-    for (uint32_t k = i; k < b.best; k += kBeamThreads) run_scored[k] = none;
-    __syncthreads();
-    const size_t rows_at = static_cast<size_t>(entry) * b.beams * b.best;
-    if (b.beams > 1) {
-        const uint32_t items = b.beams * b.best;
-        for (uint32_t at = 0; at < items; at += kBeamSegment) {
-            Scored s[kEach];
-#pragma unroll
-            for (uint32_t e = 0; e < kBeamEach; ++e) {
-                const uint32_t k = at + e * kBeamThreads + i;
-                s[e] = none;
-                if (k < items)
-                    s[e] = Scored{__longlong_as_double(static_cast<long long>(load_agent(reinterpret_cast<const uint64_t *>(b.row_scores) + rows_at + k))), k, 0};
-            }
-            s[kBeamEach] = i < b.best ? run_scored[i] : none;
-            best_of(s, none, b.best, lds.scored, [&](uint32_t rank, const Scored &c) { run_scored[rank] = c; });
-            __syncthreads();
-        }
-    } else if (i < b.best && run[i] != kNoKey) {
-        run_scored[i] = Scored{score_of(run[i]), i, 0};
-    }
-    __syncthreads();
     if (i >= b.best) return;
-    const Scored c = run_scored[i];
-    const bool any = c.score > -INFINITY;
-    const uint32_t parent = entry * b.beams + c.number / b.best;
-    int32_t token = -1;
-    if (any) token = static_cast<int32_t>(token_of(b.beams > 1 ? load_agent(b.row_keys + rows_at + c.number) : run[c.number]));
     const size_t o = static_cast<size_t>(entry) * b.best + i;
-    b.next_scores[o] = any ? static_cast<float>(c.score) : -INFINITY;
-    b.parents[o] = any ? static_cast<int32_t>(parent) : -1;
+    int32_t parent = -1, token = -1, ended = 0;
+    float value = -INFINITY;
+    if (scored != kNoKey) {
+        const uint32_t number = number_in(scored);
+        parent = static_cast<int32_t>(entry * b.beams + number / b.best);
+        if (b.beams > 1) {
+            const uint64_t held = load_agent(reinterpret_cast<const uint64_t *>(b.row_scores) + rows_at + number);
+            token = static_cast<int32_t>(held >> 32);
+            value = __uint_as_float(static_cast<uint32_t>(held));
+        } else {
+            token = static_cast<int32_t>(token_in(key));
+            value = static_cast<float>(score);
+        }
+        ended = token == b.end_token || row_finished(b, static_cast<uint32_t>(parent));
+    }
+    b.next_scores[o] = value;
+    b.parents[o] = parent;
     b.tokens[o] = token;
-    if (b.next_finished) b.next_finished[o] = any && (token == b.end_token || row_finished(b, parent));
+    if (b.next_finished) b.next_finished[o] = ended;
 }
 
 }  // namespace
 
 int launch_beam_select(const BeamSelect &b, void *stream) {
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(beam_segment_kernel, dim3(b.segments, b.batch * b.beams), dim3(kBeamThreads), 0, st, b);
-    hipLaunchKernelGGL(beam_join_kernel, dim3(b.batch * b.beams), dim3(kBeamThreads), 0, st, b);
+    const dim3 grid(b.segments, b.batch * b.beams);
+#define PVLC_BEAM_LAUNCH(E) hipLaunchKernelGGL(beam_segment_kernel<E>, grid, dim3(kBeamThreads), best_list(b.best, E) * 8, st, b)
+    switch (b.each) {
+        case 4: PVLC_BEAM_LAUNCH(4); break;
+        case 8: PVLC_BEAM_LAUNCH(8); break;
+        default: PVLC_BEAM_LAUNCH(16); break;
+    }
+#undef PVLC_BEAM_LAUNCH
+    hipLaunchKernelGGL(beam_join_kernel, dim3(b.batch * b.beams), dim3(kBeamThreads), best_list(b.best, kJoinEach + 1) * 8, st, b);
     return static_cast<int>(hipGetLastError());
 }
 

@@ -488,12 +488,19 @@ int launch_pages_copy(const int32_t *src, const int32_t *dst, uint32_t count, ui
                       uint32_t *error_word, void *stream);
 
 // Beam selection (kernels_beam.hip).  A row of logits is cut into segments of
-// kBeamThreads * kBeamEach; each leaves its best as keys (value and token in one
-// number, see there), its largest logit and its sum of exponentials.
-constexpr uint32_t kBeamThreads = 256, kBeamEach = 8, kBeamSegment = kBeamThreads * kBeamEach;
+// kBeamThreads * each; each leaves its best candidates as keys (logit and token in
+// one number, see there) and its sum of exponentials.
+constexpr uint32_t kBeamThreads = 256;
 constexpr uint32_t kBeamMaxBeams = 64, kBeamMaxBest = 128;
+// Logits a thread takes: 16 where that makes enough workgroups to fill the
+// device twice, fewer for few rows.
+inline uint32_t beam_each(uint64_t rows, uint32_t vocab) {
+    for (uint32_t each : {16u, 8u})
+        if (rows * ((static_cast<uint64_t>(vocab) + each * kBeamThreads - 1) / (each * kBeamThreads)) >= 2 * kTargetWorkgroups) return each;
+    return 4;
+}
 struct BeamSelect {
-    uint32_t batch, beams, vocab, best, segments;
+    uint32_t batch, beams, vocab, best, segments, each;
     uint64_t row_stride;
     const float *logits, *scores;
     const int32_t *finished;
@@ -502,22 +509,23 @@ struct BeamSelect {
     int32_t *parents, *tokens, *next_finished;
     uint32_t *arrived;    // by batch entry; 0 before and after a launch
     uint64_t *keys;       // [row][segment][best]
-    double *sums;         // [row][segment]
-    float *largest;       // [row][segment]
-    uint64_t *row_keys;   // [row][best]
-    double *row_scores;   // [row][best]
+    double *sums;         // [row][segment], relative to exp(reference)
+    float *references;    // [row][segment]
+    uint64_t *row_keys;   // [row][best]: the scores' keys
+    double *row_scores;   // [row][best]: token and f32 score
 };
 struct BeamWorkspace {
-    size_t keys_offset, sums_offset, largest_offset, row_keys_offset, row_scores_offset, total;
+    size_t keys_offset, sums_offset, references_offset, row_keys_offset, row_scores_offset, total;
 };
 inline BeamWorkspace beam_workspace_layout(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t best) {
     auto align = [](size_t v) { return (v + 255) / 256 * 256; };
-    const size_t rows = static_cast<size_t>(batch) * beams, parts = rows * ((static_cast<size_t>(vocab) + kBeamSegment - 1) / kBeamSegment);
+    const size_t rows = static_cast<size_t>(batch) * beams, segment = static_cast<size_t>(beam_each(rows, vocab)) * kBeamThreads;
+    const size_t parts = rows * ((vocab + segment - 1) / segment);
     BeamWorkspace w{};
     w.keys_offset = align(static_cast<size_t>(batch) * 4);
     w.sums_offset = w.keys_offset + align(parts * best * 8);
-    w.largest_offset = w.sums_offset + align(parts * 8);
-    w.row_keys_offset = w.largest_offset + align(parts * 4);
+    w.references_offset = w.sums_offset + align(parts * 8);
+    w.row_keys_offset = w.references_offset + align(parts * 4);
     w.row_scores_offset = w.row_keys_offset + align(rows * best * 8);
     w.total = w.row_scores_offset + align(rows * best * 8);
     return w;

@@ -256,7 +256,9 @@ pvlc_hip_status pvlc_hip_beam_select_f32(const pvlc_hip_beam_args *args, void *s
         return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "at most 64 beams and 128 candidates");
     if (args->vocab > 0x7FFFFFFFu || static_cast<uint64_t>(args->batch) * args->beams > 65535u)
         return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "below 2^31 logits a row and at most 65535 rows");
-    if ((static_cast<uint64_t>(args->vocab) + kBeamSegment - 1) / kBeamSegment * args->batch * args->beams >= 1u << 24)
+    const uint64_t rows = static_cast<uint64_t>(args->batch) * args->beams;
+    const uint32_t each = beam_each(rows, args->vocab), segments = (args->vocab - 1) / (each * kBeamThreads) + 1;
+    if (segments * rows >= 1u << 24)
         return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows times vocab of a beam selection exceed the grid");
     if (args->row_stride < args->vocab) return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "rows of logits overlap");
     if (!args->logits || !args->scores || !args->next_scores || !args->parents || !args->tokens || !args->workspace)
@@ -281,7 +283,8 @@ pvlc_hip_status pvlc_hip_beam_select_f32(const pvlc_hip_beam_args *args, void *s
     b.beams = args->beams;
     b.vocab = args->vocab;
     b.best = args->best;
-    b.segments = (args->vocab + kBeamSegment - 1) / kBeamSegment;
+    b.segments = segments;
+    b.each = each;
     b.row_stride = args->row_stride;
     b.logits = args->logits;
     b.scores = args->scores;
@@ -294,7 +297,7 @@ pvlc_hip_status pvlc_hip_beam_select_f32(const pvlc_hip_beam_args *args, void *s
     b.arrived = reinterpret_cast<uint32_t *>(base);
     b.keys = reinterpret_cast<uint64_t *>(base + ws.keys_offset);
     b.sums = reinterpret_cast<double *>(base + ws.sums_offset);
-    b.largest = reinterpret_cast<float *>(base + ws.largest_offset);
+    b.references = reinterpret_cast<float *>(base + ws.references_offset);
     b.row_keys = reinterpret_cast<uint64_t *>(base + ws.row_keys_offset);
     b.row_scores = reinterpret_cast<double *>(base + ws.row_scores_offset);
     const int e = launch_beam_select(b, stream);

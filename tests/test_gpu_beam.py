@@ -28,14 +28,14 @@ def plain(logits, scores, best, finished=None, end=-1):
             if finished is not None and finished[b, w]:
                 cand.append((s, w, 0, end, 1))
                 continue
-            x = np.where(np.isnan(logits[r]), np.float32(-np.inf), np.minimum(logits[r], np.finfo(np.float32).max))
+            x = np.where(np.isnan(logits[r]) | (logits[r] < -2.0 ** 127), np.float32(-np.inf), np.minimum(logits[r], np.float32(2.0 ** 127)))
             if not (x > -np.inf).any():
                 continue
             m = x.max().astype(np.float64)
-            lse = m + np.log(np.exp(x.astype(np.float64) - m).sum())
+            log_sum = np.log(np.exp(x.astype(np.float64) - m).sum())
             k = order_key(x)
             top = np.lexsort((np.arange(x.size), -k))[:best]
-            cand += [(s + (float(x[t]) - lse), w, i, int(t), int(t == end)) for i, t in enumerate(top) if x[t] > -np.inf]
+            cand += [(s + ((float(x[t]) - m) - log_sum), w, i, int(t), int(t == end)) for i, t in enumerate(top) if x[t] > -np.inf]
         cand.sort(key=lambda c: (-c[0], c[1], c[2]))
         for a, c in zip(cand[:best], cand[1:]):
             if a[1] != c[1] and a[0] != c[0]:
