@@ -138,7 +138,13 @@ __device__ inline uint32_t best_of(uint64_t own, uint32_t best, BestLds &lds, ui
     for (uint32_t c = i; c < n; c += kBeamThreads) {
         const uint64_t mine = list[c];
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; ++j) rank += list[j] > mine;
+        for (uint32_t j = 0; j < n; j += 8) {  // eight reads at a time, the last ones past the end
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) {
+                const uint64_t other = list[j + u];
+                rank += j + u < n && other > mine;
+            }
+        }
         if (rank < best) put(rank, mine);
     }
     return min(n, best);
@@ -243,23 +249,25 @@ __device__ inline uint64_t load_agent(const uint64_t *p) { return __hip_atomic_l
 constexpr uint32_t kJoinEach = 4;
 
 // The `best` largest of keys(0) .. keys(count - 1) into run, in order, kNoKey
-// behind.  Every thread calls it; run is complete after a barrier.
+// behind.  Every thread calls it, with its first keys, thread i's key e being
+// keys(e * kBeamThreads + i); run is complete when it returns.
 template <class Keys>
-__device__ inline void join_keys(uint64_t count, uint32_t best, BestLds &lds, uint64_t *list, uint64_t *run, Keys keys) {
+__device__ inline void join_keys(uint64_t (&key)[kJoinEach + 1], uint64_t count, uint32_t best, BestLds &lds, uint64_t *list, uint64_t *run, Keys keys) {
     const uint32_t i = threadIdx.x;
-    for (uint32_t k = i; k < best; k += kBeamThreads) run[k] = kNoKey;
-    __syncthreads();
     for (uint64_t at = 0; at < count; at += kJoinEach * kBeamThreads) {
-        uint64_t key[kJoinEach + 1], own = kNoKey;
+        uint64_t own = kNoKey;
+        key[kJoinEach] = kNoKey;
+        if (at > 0) {
 #pragma unroll
-        for (uint32_t e = 0; e < kJoinEach; ++e) {
-            const uint64_t k = at + e * kBeamThreads + i;
-            key[e] = k < count ? keys(k) : kNoKey;
+            for (uint32_t e = 0; e < kJoinEach; ++e) {
+                const uint64_t k = at + e * kBeamThreads + i;
+                key[e] = k < count ? keys(k) : kNoKey;
+            }
+            if (i < best) key[kJoinEach] = run[i];
         }
-        key[kJoinEach] = i < best ? run[i] : kNoKey;
 #pragma unroll
         for (uint32_t e = 0; e <= kJoinEach; ++e) own = larger_key(own, key[e]);
-        best_of(
+        const uint32_t found = best_of(
             own, best, lds, list,
             [&](uint64_t bound, auto add) {
 #pragma unroll
@@ -267,6 +275,7 @@ __device__ inline void join_keys(uint64_t count, uint32_t best, BestLds &lds, ui
                     if (key[e] >= bound) add(key[e]);
             },
             [&](uint32_t rank, uint64_t k) { run[rank] = k; });
+        for (uint32_t k = found + i; k < best; k += kBeamThreads) run[k] = kNoKey;
         __syncthreads();
     }
 }
@@ -281,20 +290,32 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
     __shared__ double sm_m[kBeamThreads / 64], sm_d[kBeamThreads / 64];
     __shared__ int sm_last;
     const uint32_t row = blockIdx.x, i = threadIdx.x, entry = row / b.beams;
+    const size_t part = static_cast<size_t>(row) * b.segments;
+    const uint64_t *keys = b.keys + part * b.best;
+    const uint64_t count = static_cast<uint64_t>(b.segments) * b.best;
+    // All first loads together (of a row that was not read, whatever is there).
+    uint64_t key_in[kJoinEach + 1];
+#pragma unroll
+    for (uint32_t e = 0; e < kJoinEach; ++e) key_in[e] = keys[min(static_cast<uint64_t>(e * kBeamThreads + i), count - 1)];
+    const uint32_t s0 = min(i, b.segments - 1);
+    const float reference0 = b.references[part + s0];
+    const double sum0 = b.sums[part + s0];
     const float start = b.scores[row];
     const bool finished = row_finished(b, row), alive = start > -INFINITY;
     double top = -INFINITY, log_sum = 0.0;
-    if (alive && !finished) {
-        const size_t part = static_cast<size_t>(row) * b.segments;
-        for (uint32_t s = i; s < b.segments; s += kBeamThreads) top = fmax(top, static_cast<double>(b.references[part + s]));
+    if (alive && !finished) {  // uniform
+#pragma unroll
+        for (uint32_t e = 0; e < kJoinEach; ++e)
+            if (e * kBeamThreads + i >= count) key_in[e] = kNoKey;
+        for (uint32_t s = i; s < b.segments; s += kBeamThreads) top = fmax(top, static_cast<double>(s == i ? reference0 : b.references[part + s]));
         top = workgroup_reduce(top, sm_m, [](double x, double y) { return fmax(x, y); });
         double sum = 0.0;
         if (top > -INFINITY)  // uniform
-            for (uint32_t s = i; s < b.segments; s += kBeamThreads) sum += b.sums[part + s] * exp(static_cast<double>(b.references[part + s]) - top);
+            for (uint32_t s = i; s < b.segments; s += kBeamThreads)
+                sum += (s == i ? sum0 : b.sums[part + s]) * exp(static_cast<double>(s == i ? reference0 : b.references[part + s]) - top);
         sum = workgroup_reduce(sum, sm_d, plus);
         log_sum = log(sum);  // (not used where all is masked)
-        const uint64_t *keys = b.keys + part * b.best;
-        join_keys(static_cast<uint64_t>(b.segments) * b.best, b.best, lds, list, run, [&](uint64_t k) { return keys[k]; });
+        join_keys(key_in, count, b.best, lds, list, run, [&](uint64_t k) { return keys[k]; });
     } else {
         for (uint32_t k = i; k < b.best; k += kBeamThreads)
             run[k] = alive && k == 0 ? key_of(0, static_cast<uint32_t>(b.end_token)) : kNoKey;
@@ -322,7 +343,11 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
         __syncthreads();
         if (!sm_last) return;
         if (i == 0) __hip_atomic_store(b.arrived + entry, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        join_keys(static_cast<uint64_t>(b.beams) * b.best, b.best, lds, list, run_scores, [&](uint64_t k) { return load_agent(b.row_keys + rows_at + k); });
+        const uint64_t all = static_cast<uint64_t>(b.beams) * b.best;
+        auto scores = [&](uint64_t k) { return load_agent(b.row_keys + rows_at + k); };
+#pragma unroll
+        for (uint32_t e = 0; e < kJoinEach; ++e) key_in[e] = e * kBeamThreads + i < all ? scores(e * kBeamThreads + i) : kNoKey;
+        join_keys(key_in, all, b.best, lds, list, run_scores, scores);
         if (i >= b.best) return;
         scored = run_scores[i];
     }
