@@ -673,7 +673,8 @@ pvlc_hip_status pvlc_hip_kv_pages_reset(const pvlc_hip_kv_pool *pool, void *stre
  * row to many, freeing a fork without those rows, truncation a fork at smaller
  * lengths, and admission a fork with -1 and a reserve.
  * If the pool has fewer free pages than needed, the call leaves the pool and its
- * planes as they are, and every output row is -1 with length -1. */
+ * planes as they are, and every output row is -1 with length -1.  At most 4096
+ * input and 4096 output rows. */
 typedef struct pvlc_hip_kv_fork_args {
     uint32_t rows_in;
     uint32_t rows_out;

@@ -24,7 +24,8 @@ constexpr int kPlanThreads = 1024;
 constexpr int kWideThreads = 256;
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-// Exclusive prefix sum over a workgroup of kPlanThreads; *total receives the sum.
+// Exclusive prefix sum over a workgroup of kThreads; *total receives the sum.
+template <int kThreads>
 __device__ inline uint32_t plan_scan(uint32_t v, uint32_t *sm, uint32_t *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t x = v;
@@ -38,7 +39,7 @@ __device__ inline uint32_t plan_scan(uint32_t v, uint32_t *sm, uint32_t *total) 
     __syncthreads();
     uint32_t before = 0, sum = 0;
 #pragma unroll
-    for (int w = 0; w < kPlanThreads / 64; ++w) {
+    for (int w = 0; w < kThreads / 64; ++w) {
         const uint32_t t = sm[w];
         before += w < wave ? t : 0u;
         sum += t;
@@ -49,11 +50,11 @@ __device__ inline uint32_t plan_scan(uint32_t v, uint32_t *sm, uint32_t *total) 
 
 __device__ inline bool valid_block(int32_t id, uint32_t num_blocks) { return id >= 0 && static_cast<uint32_t>(id) < num_blocks; }
 
-// Length of row r of the input, and whether it is one (a bad one counts as 0).
-__device__ inline uint32_t in_length(const PagesFork &f, uint32_t r, bool *bad) {
+// Length of row r of the input (a bad one counts as 0).
+__device__ inline uint32_t in_length(const PagesFork &f, uint32_t r, uint32_t *errors) {
     const int64_t len = static_cast<int64_t>(f.lens_in[r]) + f.appended;
     if (len < 0 || len > static_cast<int64_t>(f.max_blocks) * kBlockTokens) {
-        *bad = true;
+        *errors |= PVLC_HIP_PAGES_BAD_LENGTH;
         return 0;
     }
     return static_cast<uint32_t>(len);
@@ -67,16 +68,12 @@ struct RowWant {
 };
 __device__ inline RowWant want_of(const PagesFork &f, uint32_t r, uint32_t *errors) {
     RowWant w{f.parents ? f.parents[r] : (r < f.rows_in ? static_cast<int32_t>(r) : -1), 0, 0};
+    int64_t reserve = f.reserve ? f.reserve[r] : static_cast<int64_t>(f.reserve_tokens);
     if (w.parent < -1 || w.parent >= static_cast<int64_t>(f.rows_in)) {
         *errors |= PVLC_HIP_PAGES_BAD_PARENT;
         w.parent = -1;
     }
-    if (w.parent >= 0) {
-        bool bad = false;
-        w.length = in_length(f, static_cast<uint32_t>(w.parent), &bad);
-        if (bad) *errors |= PVLC_HIP_PAGES_BAD_LENGTH;
-    }
-    int64_t reserve = f.reserve ? f.reserve[r] : static_cast<int64_t>(f.reserve_tokens);
+    if (w.parent >= 0) w.length = in_length(f, static_cast<uint32_t>(w.parent), errors);
     if (reserve < 0) reserve = 0;
     int64_t end = w.length + reserve;
     if (end > static_cast<int64_t>(f.max_blocks) * kBlockTokens) {
@@ -87,84 +84,129 @@ __device__ inline RowWant want_of(const PagesFork &f, uint32_t r, uint32_t *erro
     return w;
 }
 
-// The plan of a fork.  kept[r]: entries of row r taken over from its parent (the
-// filled blocks, and behind them what the parent's first child may write itself:
-// pages that nobody else names); fresh[base[r]..]: its others.  first[p]: the
-// lowest row with parent p; children[p]: how many there are.
-__global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PagesFork f) {
-    __shared__ uint32_t sm[kPlanThreads / 64];
+// The plan of a fork, all that the execution needs of each row in one record.
+// An output row keeps the first `kept` of its parent's entries: the filled blocks
+// and, for the parent's first child, what follows as far as no other entry names
+// it; fresh[base ..] are its others.  Everything of a row stays in LDS and
+// registers: a round through memory costs more than all the arithmetic (four
+// beams 5.3 us through memory, three rounds more).
+template <int kThreads, uint32_t kWords>
+__global__ __launch_bounds__(kThreads) void pages_fork_plan_kernel(PagesFork f) {
+    extern __shared__ uint32_t by_row[];  // first[rows_in], children[rows_in], kept[rows_in]
+    __shared__ uint32_t sm[kThreads / 64];
     __shared__ uint32_t sm_errors;
+    constexpr uint32_t kTile = kThreads * kWords;  // words of the mask at a time
+    // Every pointer in one round of scalar loads.
+    asm volatile("" ::"s"(f.parents), "s"(f.reserve), "s"(f.lens_in), "s"(f.tables_in), "s"(f.ref_counts), "s"(f.free_mask), "s"(f.plan.rows),
+                 "s"(f.plan.fresh), "s"(f.lens_out));
+    uint32_t *first = by_row, *children = first + f.rows_in, *taken = children + f.rows_in;
     const uint32_t i = threadIdx.x;
     if (i == 0) sm_errors = 0;
-    for (uint32_t p = i; p < f.rows_in; p += kPlanThreads) {
-        f.plan.first[p] = UINT32_MAX;
-        f.plan.children[p] = 0;
+    for (uint32_t p = i; p < f.rows_in; p += kThreads) {
+        first[p] = UINT32_MAX;
+        children[p] = 0;
+        taken[p] = 0;
     }
-    __threadfence_block();
+    const uint32_t words = (f.num_blocks + 31) / 32;
+    const uint32_t last_word = (f.num_blocks & 31) ? (1u << (f.num_blocks & 31)) - 1u : ~0u;
+    auto load_mask = [&](uint32_t w0, uint32_t (&bits)[kWords]) {
+        const uint32_t w = w0 + i * kWords;
+#pragma unroll
+        for (uint32_t k = 0; k < kWords; ++k) bits[k] = w + k < words ? f.free_mask[w + k] : 0u;
+#pragma unroll
+        for (uint32_t k = 0; k < kWords; ++k)
+            if (w + k == words - 1) bits[k] &= last_word;
+    };
+    uint32_t bits[kWords];
+    load_mask(0, bits);  // its use is rounds away
     __syncthreads();
     uint32_t errors = 0;
-    for (uint32_t r = i; r < f.rows_out; r += kPlanThreads) {
+    for (uint32_t r = i; r < f.rows_out; r += kThreads) {
         const RowWant w = want_of(f, r, &errors);
         if (w.parent >= 0) {
-            atomicMin(&f.plan.first[w.parent], r);
-            atomicAdd(&f.plan.children[w.parent], 1u);
+            atomicMin(&first[w.parent], r);
+            atomicAdd(&children[w.parent], 1u);
         }
     }
-    __threadfence_block();
     __syncthreads();
-    uint32_t total = 0;
-    for (uint32_t r0 = 0; r0 < f.rows_out; r0 += kPlanThreads) {
+    uint32_t total = 0, length = 0;
+    for (uint32_t r0 = 0; r0 < f.rows_out; r0 += kThreads) {
         const uint32_t r = r0 + i;
         uint32_t fresh = 0;
+        ForkRow row{-1, 0, 0, 0, -1, 0};
         if (r < f.rows_out) {
             uint32_t none = 0;
             const RowWant w = want_of(f, r, &none);
-            uint32_t kept = 0;
-            if (w.parent >= 0) {
-                kept = w.length / kBlockTokens;  // filled blocks are shared
-                if (!f.keep_inputs && __hip_atomic_load(&f.plan.first[w.parent], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == r) {
-                    const int32_t *row = f.tables_in + static_cast<size_t>(w.parent) * f.max_blocks;
-                    while (kept < w.need) {
-                        const int32_t id = row[kept];
-                        if (!valid_block(id, f.num_blocks) || f.ref_counts[id] != 1) break;
-                        ++kept;
-                    }
+            row.parent = w.parent;
+            row.need = w.need;
+            row.length = length = w.length;
+            const uint32_t filled = w.length / kBlockTokens;
+            row.kept = filled;
+            if (w.parent >= 0 && w.need > filled) {
+                const int32_t *entries = f.tables_in + static_cast<size_t>(w.parent) * f.max_blocks;
+                int32_t id = entries[filled];
+                if (w.length % kBlockTokens != 0) {
+                    row.source = id;
+                    if (!valid_block(id, f.num_blocks)) errors |= PVLC_HIP_PAGES_BAD_BLOCK;
                 }
+                if (!f.keep_inputs && first[w.parent] == r) {
+                    while (valid_block(id, f.num_blocks) && f.ref_counts[id] == 1) {
+                        if (++row.kept == w.need) break;
+                        id = entries[row.kept];
+                    }
+                    if (row.kept > filled) row.source = -1;
+                    taken[w.parent] = row.kept;
+                }
+                if (!valid_block(row.source, f.num_blocks)) row.source = -1;
             }
-            kept = min(kept, w.need);
-            fresh = w.need - kept;
-            f.plan.kept[r] = kept;
+            fresh = w.need - row.kept;
         }
         uint32_t sum;
-        const uint32_t base = total + plan_scan(fresh, sm, &sum);
-        if (r < f.rows_out) f.plan.base[r] = base;
+        row.base = total + plan_scan<kThreads>(fresh, sm, &sum);
+        if (r < f.rows_out) f.plan.rows[r] = row;
         total += sum;
     }
-    // The lowest `total` free pages.
-    const uint32_t words = (f.num_blocks + 31) / 32;
-    uint32_t found = 0;
-    for (uint32_t w0 = 0; w0 < words && found < total; w0 += kPlanThreads) {
-        const uint32_t w = w0 + i;
-        uint32_t bits = w < words ? f.free_mask[w] : 0u;
-        if (w == words - 1 && (f.num_blocks & 31)) bits &= (1u << (f.num_blocks & 31)) - 1u;
-        uint32_t sum;
-        uint32_t at = found + plan_scan(static_cast<uint32_t>(__popc(bits)), sm, &sum);
-        for (; bits && at < total; ++at) {
-            f.plan.fresh[at] = static_cast<int32_t>(w * 32 + static_cast<uint32_t>(__ffs(bits) - 1));
-            bits &= bits - 1;
-        }
+    // The lowest `total` free pages.  All free pages up to the last one taken are
+    // taken, so the mask's words are 0 up to the tile that has it; whether there
+    // are enough is known when that tile's are counted, before its pages are
+    // named.
+    uint32_t found = 0, before = 0, w0 = 0;
+    bool enough = total == 0;
+    while (!enough && w0 < words) {
+        if (w0 > 0) load_mask(w0, bits);
+        uint32_t here = 0, sum;
+#pragma unroll
+        for (uint32_t k = 0; k < kWords; ++k) here += static_cast<uint32_t>(__popc(bits[k]));
+        uint32_t at = found + plan_scan<kThreads>(here, sm, &sum);
+        before = found;
         found += sum;
+        enough = found >= total;
+#pragma unroll
+        for (uint32_t k = 0; k < kWords; ++k) {
+            uint32_t left = bits[k];
+            const uint32_t w = w0 + i * kWords + k;
+            for (; left && at < total; ++at) {
+                const int32_t id = static_cast<int32_t>(w * 32 + static_cast<uint32_t>(__ffs(static_cast<int>(left)) - 1));
+                left &= left - 1;
+                f.plan.fresh[at] = id;
+                if (enough) f.ref_counts[id] = 1;
+            }
+            if (enough && left != bits[k]) f.free_mask[w] = left;
+        }
+        if (!enough) w0 += kTile;
     }
     if (errors) atomicOr(&sm_errors, errors);
-    __threadfence_block();
     __syncthreads();
-    const bool enough = found >= total;  // uniform
-    if (enough)
-        for (uint32_t k = i; k < total; k += kPlanThreads) {
-            const int32_t id = f.plan.fresh[k];
-            f.ref_counts[id] = 1;
-            atomicAnd(&f.free_mask[id >> 5], ~(1u << (id & 31)));
-        }
+    if (enough && before > 0) {  // pages of the tiles before
+        for (uint32_t k = i; k < before; k += kThreads) f.ref_counts[f.plan.fresh[k]] = 1;
+        for (uint32_t w = i; w < w0; w += kThreads) f.free_mask[w] = 0;
+    }
+    for (uint32_t p = i; p < f.rows_in; p += kThreads) {
+        uint32_t none = 0;
+        f.plan.inputs[p] = {children[p], in_length(f, p, &none) / kBlockTokens, taken[p], 0};
+    }
+    for (uint32_t r = i; r < f.rows_out; r += kThreads)
+        f.lens_out[r] = enough ? static_cast<int32_t>(f.rows_out <= kThreads ? length : f.plan.rows[r].length) : -1;
     if (i == 0) {
         *f.plan.enough = enough;
         const uint32_t e = sm_errors | (enough ? 0u : PVLC_HIP_PAGES_EXHAUSTED);
@@ -172,26 +214,52 @@ __global__ __launch_bounds__(kPlanThreads) void pages_fork_plan_kernel(PagesFork
     }
 }
 
-// Copies bytes of one page of a plane (a multiple of 4 bytes; 16-byte pieces
-// where size and planes allow it).
-__device__ inline void copy_page(const uint8_t *src, uint8_t *dst, uint64_t bytes, bool wide, uint32_t thread, uint32_t threads) {
-    if (wide) {
-        for (uint64_t at = thread; at < bytes / 16; at += threads)
-            reinterpret_cast<u32x4_t *>(dst)[at] = reinterpret_cast<const u32x4_t *>(src)[at];
-    } else {
-        for (uint64_t at = thread; at < bytes / 4; at += threads)
-            reinterpret_cast<uint32_t *>(dst)[at] = reinterpret_cast<const uint32_t *>(src)[at];
-    }
-}
-
+// Copies a page of one layer, all planes: the first 8 KiB of each plane (16 bytes
+// a thread at a time, 4 where the plane is not made for more) are loaded before
+// anything is stored, what is left of larger blocks in a loop.  (Plane by plane
+// and piece by piece, each store behind its load, 64 sequences' compaction took
+// 297 us.)
 __device__ inline void copy_pages(const PagePlanes &planes, uint32_t layer, uint32_t src, uint32_t dst) {
+    const uint32_t i = threadIdx.x;
+    u32x4_t v[kMaxPagePlanes][2];
+    const uint8_t *from[kMaxPagePlanes];
+    uint8_t *to[kMaxPagePlanes];
 #pragma unroll
     for (uint32_t p = 0; p < kMaxPagePlanes; ++p) {
-        if (p >= planes.count) break;
-        uint8_t *base = planes.plane[p].base + planes.plane[p].layer_stride * layer;
-        const uint8_t *from = planes.plane[p].from ? planes.plane[p].from + planes.plane[p].from_stride * layer : base;
-        copy_page(from + planes.plane[p].block_bytes * src, base + planes.plane[p].block_bytes * dst, planes.plane[p].block_bytes,
-                  planes.plane[p].wide, threadIdx.x, kWideThreads);
+        if (p >= planes.count) continue;
+        const PagePlane &q = planes.plane[p];
+        to[p] = q.base + q.layer_stride * layer + q.block_bytes * dst;
+        from[p] = (q.from ? q.from + q.from_stride * layer : q.base + q.layer_stride * layer) + q.block_bytes * src;
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            const uint32_t at = i + u * kWideThreads;
+            if (q.wide) {
+                if (at * 16ull < q.block_bytes) v[p][u] = reinterpret_cast<const u32x4_t *>(from[p])[at];
+            } else if (at * 4ull < q.block_bytes) {
+                v[p][u][0] = reinterpret_cast<const uint32_t *>(from[p])[at];
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t p = 0; p < kMaxPagePlanes; ++p) {
+        if (p >= planes.count) continue;
+        const PagePlane &q = planes.plane[p];
+#pragma unroll
+        for (uint32_t u = 0; u < 2; ++u) {
+            const uint32_t at = i + u * kWideThreads;
+            if (q.wide) {
+                if (at * 16ull < q.block_bytes) reinterpret_cast<u32x4_t *>(to[p])[at] = v[p][u];
+            } else if (at * 4ull < q.block_bytes) {
+                reinterpret_cast<uint32_t *>(to[p])[at] = v[p][u][0];
+            }
+        }
+        if (q.wide) {
+            for (uint64_t at = i + 2 * kWideThreads; at < q.block_bytes / 16; at += kWideThreads)
+                reinterpret_cast<u32x4_t *>(to[p])[at] = reinterpret_cast<const u32x4_t *>(from[p])[at];
+        } else {
+            for (uint64_t at = i + 2 * kWideThreads; at < q.block_bytes / 4; at += kWideThreads)
+                reinterpret_cast<uint32_t *>(to[p])[at] = reinterpret_cast<const uint32_t *>(from[p])[at];
+        }
     }
 }
 
@@ -202,22 +270,18 @@ __global__ __launch_bounds__(kWideThreads) void pages_fork_kernel(PagesFork f, P
     const bool enough = *f.plan.enough;
     uint32_t b = blockIdx.x;
     if (b < f.rows_in) {
-        if (!enough) return;
-        const uint32_t children = f.plan.children[b];
-        if (f.keep_inputs && children == 0) return;
-        bool bad = false;
-        const uint32_t filled = in_length(f, b, &bad) / kBlockTokens, first = f.plan.first[b];
-        const uint32_t kept = !f.keep_inputs && first != UINT32_MAX ? f.plan.kept[first] : 0u;
+        const ForkInput in = f.plan.inputs[b];
+        if (!enough || (f.keep_inputs && in.children == 0)) return;
         const int32_t *row = f.tables_in + static_cast<size_t>(b) * f.max_blocks;
         uint32_t errors = 0;
         for (uint32_t j = threadIdx.x; j < f.max_blocks; j += kWideThreads) {
             const int32_t id = row[j];
             if (!valid_block(id, f.num_blocks)) {
-                if (id != -1 || (children && j < filled)) errors |= PVLC_HIP_PAGES_BAD_BLOCK;
+                if (id != -1 || (in.children && j < in.filled)) errors |= PVLC_HIP_PAGES_BAD_BLOCK;
                 continue;
             }
             // an entry is held once by each child that takes it over, and no longer by this row
-            uint32_t held = j < filled ? children : (j < kept ? 1u : 0u);
+            const uint32_t held = j < in.filled ? in.children : (j < in.kept ? 1u : 0u);
             const int32_t delta = static_cast<int32_t>(held) - (f.keep_inputs ? 0 : 1);
             if (delta == 0) continue;
             const int32_t old = atomicAdd(&f.ref_counts[id], delta);
@@ -228,37 +292,26 @@ __global__ __launch_bounds__(kWideThreads) void pages_fork_kernel(PagesFork f, P
         return;
     }
     b -= f.rows_in;
-    uint32_t none = 0;
     if (b < f.rows_out) {
-        const RowWant w = want_of(f, b, &none);
-        const uint32_t kept = f.plan.kept[b], base = f.plan.base[b];
-        const int32_t *row = f.tables_in + static_cast<size_t>(w.parent < 0 ? 0 : w.parent) * f.max_blocks;
+        const ForkRow r = f.plan.rows[b];
+        const int32_t *row = f.tables_in + static_cast<size_t>(r.parent < 0 ? 0 : r.parent) * f.max_blocks;
         int32_t *out = f.tables_out + static_cast<size_t>(b) * f.max_blocks;
         for (uint32_t j = threadIdx.x; j < f.max_blocks; j += kWideThreads) {
             int32_t id = -1;
-            if (enough && j < kept) {
+            if (enough && j < r.kept) {
                 id = row[j];
                 if (!valid_block(id, f.num_blocks)) id = -1;
-            } else if (enough && j < w.need) {
-                id = f.plan.fresh[base + j - kept];
+            } else if (enough && j < r.need) {
+                id = f.plan.fresh[r.base + j - r.kept];
             }
             out[j] = id;
         }
-        if (threadIdx.x == 0) f.lens_out[b] = enough ? static_cast<int32_t>(w.length) : -1;
         return;
     }
     b -= f.rows_out;
-    if (!enough) return;
-    const uint32_t r = b / planes.layers, layer = b % planes.layers;
-    const RowWant w = want_of(f, r, &none);
-    const uint32_t filled = w.length / kBlockTokens;
-    if (w.parent < 0 || w.length % kBlockTokens == 0 || f.plan.kept[r] > filled) return;  // (kept >= filled)
-    const int32_t src = f.tables_in[static_cast<size_t>(w.parent) * f.max_blocks + filled];
-    if (!valid_block(src, f.num_blocks)) {
-        if (threadIdx.x == 0) atomicOr(f.plan.error_word, static_cast<uint32_t>(PVLC_HIP_PAGES_BAD_BLOCK));
-        return;
-    }
-    copy_pages(planes, layer, static_cast<uint32_t>(src), static_cast<uint32_t>(f.plan.fresh[f.plan.base[r]]));
+    const ForkRow r = f.plan.rows[b / planes.layers];
+    if (!enough || r.source < 0) return;
+    copy_pages(planes, b % planes.layers, static_cast<uint32_t>(r.source), static_cast<uint32_t>(f.plan.fresh[r.base]));
 }
 
 // Compaction.  With L pages in use, those behind the first L move, in order, to
@@ -275,7 +328,7 @@ __global__ __launch_bounds__(kPlanThreads) void pages_count_kernel(PagesCompact 
         uint32_t bits = w < words ? c.free_mask[w] : 0u;
         if (in_word < 32) bits &= (1u << in_word) - 1u;
         uint32_t sum;
-        const uint32_t before = plan_scan(in_word - static_cast<uint32_t>(__popc(bits)), sm, &sum);
+        const uint32_t before = plan_scan<kPlanThreads>(in_word - static_cast<uint32_t>(__popc(bits)), sm, &sum);
         if (w < words) c.plan.used_before[w] = used + before;
         used += sum;
     }
@@ -376,7 +429,15 @@ int launch_pages_reset(int32_t *refs, uint32_t *mask, uint32_t num_blocks, uint3
 
 int launch_pages_fork(const PagesFork &f, const PagePlanes &planes, void *stream) {
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(pages_fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, f);
+    const uint32_t lds = f.rows_in * 12;
+    // A thread for each row and each word of 32 pages, as far as 1024 go; more
+    // words a thread only for pools that take several turns otherwise.
+    if (f.rows_in <= 256 && f.rows_out <= 256 && f.num_blocks <= 256 * 32)
+        hipLaunchKernelGGL((pages_fork_plan_kernel<256, 1>), dim3(1), dim3(256), lds, st, f);
+    else if (f.num_blocks <= 4 * kPlanThreads * 32)
+        hipLaunchKernelGGL((pages_fork_plan_kernel<kPlanThreads, 1>), dim3(1), dim3(kPlanThreads), lds, st, f);
+    else
+        hipLaunchKernelGGL((pages_fork_plan_kernel<kPlanThreads, 4>), dim3(1), dim3(kPlanThreads), lds, st, f);
     const uint32_t groups = f.rows_in + f.rows_out + f.rows_out * planes.layers;
     hipLaunchKernelGGL(pages_fork_kernel, dim3(groups), dim3(kWideThreads), 0, st, f, planes);
     return static_cast<int>(hipGetLastError());

@@ -442,14 +442,26 @@ struct PagePlanes {
     PagePlane plane[kMaxPagePlanes];
     uint32_t count, layers;
 };
+// Rows of a fork (their plan is made in LDS).
+constexpr uint32_t kMaxForkRows = 4096;
+struct ForkRow {  // of the output: entries kept of the parent's, needed in all, its first fresh page, the page to copy to that (-1: none)
+    int32_t parent;
+    uint32_t kept, need, base;
+    int32_t source;
+    uint32_t length;
+};
+struct ForkInput {  // of the input: how many take it over, its filled blocks (shared by them), the end of what the first keeps
+    uint32_t children, filled, kept, pad;
+};
 struct PagesFork {
     uint32_t num_blocks, max_blocks, rows_in, rows_out, appended, reserve_tokens, keep_inputs;
     const int32_t *tables_in, *lens_in, *parents, *reserve;
     int32_t *tables_out, *lens_out, *ref_counts;
     uint32_t *free_mask;
     struct {
-        uint32_t *first, *children, *kept, *base;  // by row
-        int32_t *fresh;                            // the pages taken, in order
+        ForkRow *rows;
+        ForkInput *inputs;
+        int32_t *fresh;  // the pages taken, in order
         uint32_t *enough, *error_word;
     } plan;
 };
@@ -467,14 +479,15 @@ struct PagesCompact {
 // pages, 2 the moves of a compaction), then the plans' arrays; a fork's and a
 // compaction's share theirs.
 struct PagesWorkspace {
-    size_t rows_offset, first_offset, second_offset, third_offset, words_offset, total;
+    size_t rows_offset, inputs_offset, first_offset, second_offset, third_offset, words_offset, total;
 };
 inline PagesWorkspace pages_workspace_layout(uint32_t num_blocks, uint32_t rows) {
     auto align = [](size_t v) { return (v + 255) / 256 * 256; };
     const size_t list = align(static_cast<size_t>(num_blocks) * 4);
     PagesWorkspace w{};
-    w.rows_offset = 256;  // first, children, kept, base: 4 arrays of `rows`
-    w.first_offset = w.rows_offset + align(static_cast<size_t>(rows) * 16);
+    w.rows_offset = 256;
+    w.inputs_offset = w.rows_offset + align(static_cast<size_t>(rows) * sizeof(ForkRow));
+    w.first_offset = w.inputs_offset + align(static_cast<size_t>(rows) * sizeof(ForkInput));
     w.second_offset = w.first_offset + list;
     w.third_offset = w.second_offset + list;
     w.words_offset = w.third_offset + list;

@@ -160,6 +160,7 @@ pvlc_hip_status pvlc_hip_kv_pages_fork(const pvlc_hip_kv_pool *pool, const pvlc_
     PagesWorkspace ws;
     if (pvlc_hip_status st = check_pool(pool, rows, &planes, &ws)) return st;
     if (rows == 0) return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "a fork needs input or output rows");
+    if (rows > kMaxForkRows) return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "a fork takes at most 4096 rows");
     if (args->rows_in && (!args->tables_in || !args->lens_in)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "fork input pointer is NULL");
     if (args->rows_out && (!args->tables_out || !args->lens_out)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "fork output pointer is NULL");
     for (const void *p : {static_cast<const void *>(args->tables_in), static_cast<const void *>(args->lens_in), static_cast<const void *>(args->parents),
@@ -189,8 +190,7 @@ pvlc_hip_status pvlc_hip_kv_pages_fork(const pvlc_hip_kv_pool *pool, const pvlc_
     f.lens_out = args->lens_out;
     f.ref_counts = pool->ref_counts;
     f.free_mask = pool->free_mask;
-    auto *by_row = reinterpret_cast<uint32_t *>(base + ws.rows_offset);
-    f.plan = {by_row, by_row + rows, by_row + 2 * static_cast<size_t>(rows), by_row + 3 * static_cast<size_t>(rows),
+    f.plan = {reinterpret_cast<ForkRow *>(base + ws.rows_offset), reinterpret_cast<ForkInput *>(base + ws.inputs_offset),
               reinterpret_cast<int32_t *>(base + ws.first_offset), reinterpret_cast<uint32_t *>(base) + 1, reinterpret_cast<uint32_t *>(base)};
     const int e = launch_pages_fork(f, planes, stream);
     if (e != 0) return hip_status(e, "page fork launch");
