@@ -21,9 +21,9 @@
 // The key slab [token/4][dim/16][token%4][dim%16] makes each load of a tile 256
 // contiguous bytes; the value slab [dim][token] does as it is.
 //
-// The weights go to P.V as exact pairs of fp16 values (hi + lo, ~22 bits) in
-// both operand widths: the launch is bound by memory, and the second MFMA was
-// not measurable.
+// With f32 operands the weights go to P.V as exact pairs of fp16 values (hi + lo,
+// ~22 bits), with fp16 operands, whose output rounds as coarsely, as single ones
+// (the pair costs 0.2-0.3 us of a launch's 8 to 10, 5 of 260).
 
 #include <hip/hip_runtime.h>
 
@@ -339,17 +339,16 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
 
     // Append: the wave whose tiles hold the new row's block rotates the row,
     // rounds it to fp16 as the fp16 cache would hold it, finds the block's
-    // exponents with it, and leaves the codes in LDS.  Only that wave reads the
-    // block, so no barrier is needed, and it writes the block back from its own
-    // registers below.
+    // exponents with it, writes the row's codes and leaves them in LDS to stand
+    // in for that row of its own loads.  Only that wave reads the block, so no
+    // barrier is needed.  Where an exponent grows (seldom), the rows before are
+    // rounded again in the cache first, and read again.
     const int append_tile = cache_len >> 4, slot = cache_len & 15;
     const int rel = append_tile - (part_start >> 4);
     const bool appends = rel >= 0 && append_tile * 16 < part_end && wave == (rel / kTiles) % WAVES;
     const int append_chunk = appends ? rel / (kTiles * WAVES) : -1;
     const int ti = rel & (kTiles - 1);
     __shared__ __align__(16) uint8_t sm_new[2][kHeadDim];
-    int grown_k = 0, grown_v = 0;
-    uint8_t *append_k = nullptr, *append_v = nullptr;
     if (appends) {
         float k_lo = nk_lo, k_hi = nk_hi;
         if (rope) {
@@ -369,8 +368,6 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
         if (slot > 0) {
             e_k = max(e_k, old_k);
             e_v = max(e_v, old_v);
-            grown_k = __builtin_amdgcn_readfirstlane(e_k - old_k);
-            grown_v = __builtin_amdgcn_readfirstlane(e_v - old_v);
         }
         const float pk = exp2_whole(-e_k), pv = exp2_whole(-e_v);
         const uint32_t codes = q8_encode<CODE>(k_lo * pk, k_hi * pk, v_lo * pv, v_hi * pv);
@@ -380,11 +377,21 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
         sm_new[1][lane + 64] = static_cast<uint8_t>(codes >> 24);
         const uint32_t now = static_cast<uint32_t>(e_k + kQ8Bias) | static_cast<uint32_t>(e_v + kQ8Bias) << 8;
         if (lane == at) ex = now;
-        // (a bad id reads block 0 and writes nothing)
-        if (!__builtin_amdgcn_readlane(static_cast<int>(ids_bad), at)) {
-            const size_t slab = (static_cast<size_t>(blk) * kKvHeads + g);
-            append_k = reinterpret_cast<uint8_t *>(p.key_cache) + slab * kQ8SlabBytes;
-            append_v = reinterpret_cast<uint8_t *>(p.value_cache) + slab * kQ8SlabBytes;
+        if (!__builtin_amdgcn_readlane(static_cast<int>(ids_bad), at)) {  // (a bad id reads block 0 and writes nothing)
+            const size_t slab = static_cast<size_t>(blk) * kKvHeads + g;
+            uint8_t *ks = reinterpret_cast<uint8_t *>(p.key_cache) + slab * kQ8SlabBytes;
+            uint8_t *vs = reinterpret_cast<uint8_t *>(p.value_cache) + slab * kQ8SlabBytes;
+            const int grown = __builtin_amdgcn_readfirstlane(slot > 0 ? (e_k - old_k) | (e_v - old_v) << 16 : 0);
+            if (grown != 0) {
+                requantise_block<CODE>(ks, vs, lane, slot, grown & 0xFFFF, grown >> 16);
+                if (append_chunk == 0) load_chunk(p, g, ids, 0, row, kg, kr, vr);
+            }
+            // key (slot, d) at (slot/4)*512 + (d/16)*64 + (slot%4)*16 + d%16, value at d*16 + slot
+            uint8_t *kd = ks + (slot >> 2) * 512 + (slot & 3) * 16 + (lane >> 4) * 64 + (lane & 15), *vd = vs + lane * 16 + slot;
+            kd[0] = static_cast<uint8_t>(codes);
+            kd[256] = static_cast<uint8_t>(codes >> 8);
+            vd[0] = static_cast<uint8_t>(codes >> 16);
+            vd[1024] = static_cast<uint8_t>(codes >> 24);
             if (lane == 0) *reinterpret_cast<uint16_t *>(p.exponents + slab * 2) = static_cast<uint16_t>(now);
         }
     }
@@ -400,41 +407,25 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
         if (chunk > 0) load_chunk(p, g, ids, chunk, row, kg, kr, vr);
 
         if (chunk == append_chunk) {  // uniform
-            // The block of the new row.  Where its exponent grew (seldom), the
-            // rows before are rounded again in the cache and read back; then the
-            // new row goes into the registers and the cache.  The codes behind it
-            // stay in the cache as they are, and become 0 here: they may be e4m3
-            // NaN.
-            if (append_k != nullptr && (grown_k | grown_v) != 0) {
-                requantise_block<CODE>(append_k, append_v, lane, slot, grown_k, grown_v);
-                load_chunk(p, g, ids, chunk, row, kg, kr, vr);
-            }
+            // The new row's codes into the block's registers; the codes behind it
+            // become 0 (they may be e4m3 NaN).  All from LDS before any is used.
+            q8x4_t piece[2];
+            uint32_t code[8];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) piece[i] = *reinterpret_cast<const q8x4_t *>(&sm_new[0][i * 64 + kg * 16]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) code[i] = sm_new[1][i * 16 + row];
             const bool key_lane = (row >> 2) == ti && (row & 3) == (slot & 3);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const q8x4_t piece = *reinterpret_cast<const q8x4_t *>(&sm_new[0][i * 64 + kg * 16]);
+            for (int i = 0; i < 8; ++i)
+                if (key_lane && (i >> 1) == (slot >> 2)) kr[i] = piece[i & 1];
+            const int shift = (slot & 3) * 8;
 #pragma unroll
-                for (int h = 0; h < 4; ++h)
-                    if (key_lane && h == (slot >> 2)) kr[h * 2 + i] = piece;
-                if (key_lane && append_k != nullptr)
-                    *reinterpret_cast<q8x4_t *>(append_k + (kg * 4 + (row & 3)) * 16 + ((slot >> 2) * 2 + i) * 256) = piece;
-            }
-            if (kg == ti) {
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t before = w < (slot >> 2) ? ~0u : (w == (slot >> 2) ? (1u << shift) - 1u : 0u);
+                const uint32_t keep = kg == ti ? before : ~0u, put = kg == ti && w == (slot >> 2) ? 0xFFu << shift : 0u;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const uint32_t code = sm_new[1][i * 16 + row] * 0x01010101u;
-                    q8x4_t back;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t byte = 0xFFu << ((slot & 3) * 8);
-                        const uint32_t put = w == (slot >> 2) ? byte : 0u;                                       // the new row
-                        const uint32_t before = w < (slot >> 2) ? ~0u : (w == (slot >> 2) ? (byte & -byte) - 1u : 0u);  // the rows before it
-                        const uint32_t v = (vr[i][w] & ~put) | (code & put);
-                        back[w] = v;
-                        vr[i][w] = v & (before | put);
-                    }
-                    if (append_v != nullptr) *reinterpret_cast<q8x4_t *>(append_v + row * 16 + i * 256) = back;
-                }
+                for (int i = 0; i < 8; ++i) vr[i][w] = (vr[i][w] & keep) | ((code[i] << shift) & put);
             }
         }
         // Tiles past the end repeat the last one, whose codes behind the new row
@@ -490,15 +481,20 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
             l_run += pf;
             const float w = pf * pv;
             hi[t >> 3][t & 7] = to_h(w);
-            lo[t >> 3][t & 7] = to_h(w - static_cast<float>(hi[t >> 3][t & 7]));  // the difference is exact in f32
+            if constexpr (F32IO) lo[t >> 3][t & 7] = to_h(w - static_cast<float>(hi[t >> 3][t & 7]));  // the difference is exact in f32
         }
+        // (the eight independent products of a step side by side)
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int u = 0; u < 2; ++u) {
+            half8_t v[8];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const half8_t v = q8_half8<CODE>(vr[c][u * 2], vr[c][u * 2 + 1]);
-                o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[u], v, o[c], 0, 0, 0);
-                o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[u], v, o[c], 0, 0, 0);
+            for (int c = 0; c < 8; ++c) {
+                v[c] = q8_half8<CODE>(vr[c][u * 2], vr[c][u * 2 + 1]);
+                o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[u], v[c], o[c], 0, 0, 0);
+            }
+            if constexpr (F32IO) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[u], v[c], o[c], 0, 0, 0);
             }
         }
     }
@@ -577,13 +573,14 @@ int launch_kernels(const DecodeLaunch &launch, DecodeQ8Params &p, hipStream_t st
     hipLaunchKernelGGL((paged_decode_q8_kernel<W, F32IO, CODE>), grid, dim3((W) * 64), 0, st, p.key_cache, p.value_cache,   \
                        p.exponents, p.cache_lens, p.block_tables, p.uniform_cache_len, p.max_blocks_per_seq, p.num_blocks, \
                        p.partition_tokens | p.max_parts << 16, p)
-    switch ((launch.partition_tokens + kChunkTokens - 1) / kChunkTokens) {  // a wave for each 64 tokens, up to 384
+    switch (q8_waves(launch.partition_tokens)) {
         case 1: PVLC_Q8_LAUNCH(1); break;
         case 2: PVLC_Q8_LAUNCH(2); break;
         case 3: PVLC_Q8_LAUNCH(3); break;
         case 4: PVLC_Q8_LAUNCH(4); break;
-        case 5: PVLC_Q8_LAUNCH(5); break;
-        default: PVLC_Q8_LAUNCH(6); break;
+        case 6: PVLC_Q8_LAUNCH(6); break;
+        case 8: PVLC_Q8_LAUNCH(8); break;
+        default: PVLC_Q8_LAUNCH(12); break;
     }
 #undef PVLC_Q8_LAUNCH
     return static_cast<int>(hipGetLastError());

@@ -523,6 +523,43 @@ uint32_t auto_partition(uint32_t num_seqs, uint32_t context) {
     return p;
 }
 
+bool q8_streams(uint32_t partition_tokens, uint64_t parts, uint32_t num_seqs, bool ragged) {
+    // One round of workgroups covers the launch, one a compute unit, or the
+    // persistent kernel takes it.  Ragged launches, where many workgroups leave at
+    // once, may take two rounds of up to four waves, or of any with one partition
+    // a sequence; else they lose to it (64 sequences up to 2010 rows 17.7 us
+    // against 13.1, 16 up to 8192 18.6 against 13.3, 256 up to 300, one partition
+    // each, 13.0 against 16).  Uniform lengths stream only where one round of the
+    // largest shape does not hold them.
+    if (partition_tokens > kQ8SingleShotTiles * kBlockTokens) return true;
+    const uint64_t workgroups = parts * num_seqs * kKvHeads;
+    if (!ragged) return false;
+    return workgroups > (q8_waves(partition_tokens) <= 4 || parts == 1 ? 2 : 1) * kTargetWorkgroups;
+}
+
+uint32_t q8_auto_partition(uint32_t num_seqs, uint32_t rows, bool ragged, uint32_t workspace_parts) {
+    // The fewest waves a workgroup for which the partitions of a (sequence, kv
+    // head) merge in one batch of loads (4, 8 or 16 by the elements a thread
+    // owns) and the launch does not stream.  The fp16 rule, of more and smaller
+    // partitions, took one sequence of 1157 rows 7.6 us against 7.3, four
+    // of 2048 8.7 against 7.5, 18 of 3000 13.1 against 10.4.
+    for (uint32_t w : kQ8Shapes) {
+        const uint64_t parts = (static_cast<uint64_t>(rows) + w * 64 - 1) / (w * 64);
+        const uint32_t batch = w >= 4 ? 16 : (w >= 2 ? 8 : 4);
+        if (parts <= batch && parts <= workspace_parts && (ragged ? !q8_streams(w * 64, parts, num_seqs, true) : parts * num_seqs * kKvHeads <= kTargetWorkgroups))
+            return w * 64;
+    }
+    // Streaming: a few partitions for each compute unit, if every sequence is as
+    // long as the longest, between 512 and 1536 tokens; the kernel may double it.
+    // (64 sequences up to 8192 rows, 512 / 768 / 1024: 21.9 / 21.1 / 22.2 us; 256 up
+    // to 8192 101 / 96 / 95; 256 up to 32768 257 / 242 / 233.)
+    const uint64_t unit = static_cast<uint64_t>(num_seqs) * rows * kKvHeads / kTargetWorkgroups;
+    uint64_t p = unit * 3 / 16 / 64 * 64;
+    p = p < 512 ? 512 : (p > 1536 ? 1536 : p);
+    while ((rows + p - 1) / p > (kMaxMergeParts < workspace_parts ? kMaxMergeParts : workspace_parts) && p < 4096) p *= 2;
+    return static_cast<uint32_t>(p < 4096 ? p : 4096);
+}
+
 uint32_t auto_workspace_parts(uint32_t num_seqs, uint32_t max_context) {
     // Any automatic launch with cache lengths up to max_context fits: a
     // single-shot launch uses at most balanced_parts partitions, a streaming

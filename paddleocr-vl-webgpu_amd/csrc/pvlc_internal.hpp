@@ -177,6 +177,20 @@ struct DecodeCodes {
     uint32_t code;        // PVLC_HIP_KV_E4M3 or PVLC_HIP_KV_INT8
     uint8_t *exponents;   // [block][kv head][key, value]
 };
+// Single-shot shapes of the 8-bit decode: a wave for each 64 tokens of a
+// partition, up to 768 (the fp16 cache's largest shape in bytes).
+constexpr uint32_t kQ8Shapes[] = {1, 2, 3, 4, 6, 8, 12};
+constexpr uint32_t kQ8SingleShotTiles = 48;
+constexpr uint32_t q8_waves(uint32_t partition_tokens) {
+    for (uint32_t w : kQ8Shapes)
+        if (partition_tokens <= w * 64) return w;
+    return kQ8Shapes[6];
+}
+// Whether a launch of these partitions a sequence takes the persistent kernel.
+bool q8_streams(uint32_t partition_tokens, uint64_t parts, uint32_t num_seqs, bool ragged);
+// Partition of an automatic 8-bit decode of `rows` tokens a sequence (an upper
+// bound of them when ragged), with at most workspace_parts partitions.
+uint32_t q8_auto_partition(uint32_t num_seqs, uint32_t rows, bool ragged, uint32_t workspace_parts);
 int launch_paged_decode_q8(const DecodeLaunch &launch, const DecodeCodes &codes, void *stream);
 int launch_kv_pack_q8(const uint16_t *key_rows, const uint16_t *value_rows, uint32_t first_token, uint32_t tokens,
                       const int32_t *table, uint32_t num_blocks, uint32_t code, uint8_t *key_cache, uint8_t *value_cache,
@@ -576,7 +590,8 @@ struct DecodeState {
 // f32 operands (pvlc_hip_paged_decode_f32io) args' fp16 query, new key and
 // value and output must be NULL and the f32 ones given.
 pvlc_hip_status validate_decode_geometry(const pvlc_hip_paged_decode_args *a, uint32_t *partition_out,
-                                         uint32_t *max_parts_out, const DecodeOperands32 *f32 = nullptr);
+                                         uint32_t *max_parts_out, const DecodeOperands32 *f32 = nullptr,
+                                         bool codes = false);
 // Launch a validated decode with its split-K state at `state`; launches_out
 // receives the kernels launched (1, or 2 for the persistent kernel and its
 // merge kernel).

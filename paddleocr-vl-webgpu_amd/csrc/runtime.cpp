@@ -209,7 +209,7 @@ namespace pvlc {
 // partitions per (sequence, kv head) the launch runs.  Returns a status
 // (0 = ok) without touching the GPU.
 pvlc_hip_status validate_decode_geometry(const pvlc_hip_paged_decode_args *a, uint32_t *partition_out,
-                                         uint32_t *max_parts_out, const DecodeOperands32 *f32) {
+                                         uint32_t *max_parts_out, const DecodeOperands32 *f32, bool codes) {
     if (!a) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "paged decode args are NULL");
     if (a->num_seqs == 0 || a->num_blocks == 0 || a->max_blocks_per_seq == 0 || a->max_context == 0)
         return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "all paged decode dimensions must be nonzero");
@@ -244,6 +244,9 @@ pvlc_hip_status validate_decode_geometry(const pvlc_hip_paged_decode_args *a, ui
         if ((a->max_context + partition - 1) / partition > kMaxMergeParts)
             return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY,
                            "max_context / partition_tokens exceeds the 64 partitions one merge combines");
+    } else if (codes) {
+        partition = q8_auto_partition(a->num_seqs, a->cache_lens ? a->max_context : a->uniform_cache_len + 1, a->cache_lens != nullptr,
+                                      auto_workspace_parts(a->num_seqs, a->max_context));
     } else {
         partition = auto_partition(a->num_seqs, a->max_context);
         // A uniform cache length is known here: balance the partitions for
@@ -292,7 +295,8 @@ pvlc_hip_status launch_decode_state(const pvlc_hip_paged_decode_args *a, uint32_
     const uint32_t part_tiles = (partition + kBlockTokens - 1) / kBlockTokens;
     const uint64_t workgroups = static_cast<uint64_t>(max_parts) * kKvHeads * a->num_seqs;
     const bool streaming = a->num_seqs <= kMaxRaggedSeqs &&
-                           (part_tiles > kSingleShotTiles || (a->cache_lens != nullptr && workgroups > 2 * kTargetWorkgroups));
+                           (codes ? q8_streams(partition, max_parts, a->num_seqs, a->cache_lens != nullptr)
+                                  : part_tiles > kSingleShotTiles || (a->cache_lens != nullptr && workgroups > 2 * kTargetWorkgroups));
     const DecodeShape shape = decode_shape(partition, streaming);
     DecodeLaunch launch{a,
                         partition,
@@ -324,7 +328,7 @@ pvlc_hip_status hip_status(int error, const char *what) { return hip_fail(static
 pvlc_hip_status launch_decode_checked(const pvlc_hip_paged_decode_args *a, void *stream, uint32_t *launches_out,
                                       const DecodeOperands32 *f32, const DecodeCodes *codes) {
     uint32_t partition = 0, max_parts = 0;
-    if (pvlc_hip_status st = validate_decode_geometry(a, &partition, &max_parts, f32)) return st;
+    if (pvlc_hip_status st = validate_decode_geometry(a, &partition, &max_parts, f32, codes != nullptr)) return st;
     if (!a->workspace) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "paged decode workspace is NULL");
     const DecodeWorkspace layout = decode_workspace_layout(a->num_seqs, max_parts);
     if (a->workspace_bytes < layout.total)
