@@ -16,8 +16,7 @@
 //
 // The best n of many without sorting them: with the values dealt to groups of
 // threads, the n-th largest of the groups' own largest is a bound that at least n
-// values reach, and only values of n groups can reach it, so a short list
-// remains, whose ranks are counted.
+// values reach and few others, so a short list remains, whose ranks are counted.
 
 #include <hip/hip_runtime.h>
 
@@ -75,67 +74,62 @@ __device__ inline bool row_alive(const BeamSelect &b, uint32_t row) { return b.s
 
 // LDS of best_of, ahead of its short list.
 struct BestLds {
-    uint64_t most[kBeamThreads];
+    union {
+        uint64_t key[kBeamThreads];
+        int32_t order[kBeamThreads];
+    } most;
     uint32_t count, pad;
 };
-// Groups whose largest bound the selection: 64 of four threads, or the threads
-// themselves where more than 64 are wanted.  Items that can reach the bound:
-constexpr uint32_t best_list(uint32_t best, uint32_t each) { return best * each * (best <= 64 ? 4 : 1); }
+// Items that the exact selection may list (of four threads for each one wanted,
+// or one where more than 64 are), and room for what is read past the last.
+constexpr uint32_t best_list(uint32_t best, uint32_t each) { return best * each * (best <= 64 ? 4 : 1) + 8; }
+constexpr int32_t kNoOrder = INT32_MIN;  // of kNoKey
 
 __device__ inline uint64_t larger_key(uint64_t a, uint64_t b) { return a > b ? a : b; }
 template <int CTRL>
+__device__ inline int32_t dpp_i32(int32_t x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, 0xF, 0xF, false); }
+template <int CTRL>
 __device__ inline uint64_t dpp_key(uint64_t k) {
-    const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(k), CTRL, 0xF, 0xF, false);
-    const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(k >> 32), CTRL, 0xF, 0xF, false);
-    return static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo);
+    return static_cast<uint64_t>(static_cast<uint32_t>(dpp_i32<CTRL>(static_cast<int32_t>(k >> 32)))) << 32 |
+           static_cast<uint32_t>(dpp_i32<CTRL>(static_cast<int32_t>(k)));
 }
+template <int CTRL>
+__device__ inline double dpp_f64(double x) { return __longlong_as_double(static_cast<long long>(dpp_key<CTRL>(static_cast<uint64_t>(__double_as_longlong(x))))); }
 __device__ inline uint64_t lane_key(uint64_t k, int lane) {
     const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k), lane));
     const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(k >> 32), lane));
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
+// The least, and the sum, over the 64 lanes, in every lane (see wave_sum).
+__device__ inline int32_t wave_least(int32_t v) {
+    v = min(v, dpp_i32<0xB1>(v));
+    v = min(v, dpp_i32<0x4E>(v));
+    v = min(v, dpp_i32<0x124>(v));
+    v = min(v, dpp_i32<0x128>(v));
+    return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+               min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+__device__ inline float wave_largest(float v) {
+    v = fmaxf(v, dpp_f32<0xB1>(v));
+    v = fmaxf(v, dpp_f32<0x4E>(v));
+    v = fmaxf(v, dpp_f32<0x124>(v));
+    v = fmaxf(v, dpp_f32<0x128>(v));
+    auto at = [&](int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); };
+    return fmaxf(fmaxf(at(0), at(16)), fmaxf(at(32), at(48)));
+}
+__device__ inline double wave_sum(double v) {
+    v += dpp_f64<0xB1>(v);
+    v += dpp_f64<0x4E>(v);
+    v += dpp_f64<0x124>(v);
+    v += dpp_f64<0x128>(v);
+    auto at = [&](int lane) { return __longlong_as_double(static_cast<long long>(lane_key(static_cast<uint64_t>(__double_as_longlong(v)), lane))); };
+    return (at(0) + at(16)) + (at(32) + at(48));
+}
 
-// The `best` largest keys of the workgroup: own is the thread's largest (kNoKey:
-// none), push(bound, list) adds those of the thread's keys that reach a bound to
-// the list, and put(rank, key) receives the best, in order.  Returns how many
-// there are.  No two keys are equal.  Every thread calls it; LDS is free for the
-// next call after a barrier.
-template <class Push, class Put>
-__device__ inline uint32_t best_of(uint64_t own, uint32_t best, BestLds &lds, uint64_t *list, Push push, Put put) {
-    const uint32_t i = threadIdx.x;
-    const int lane = i & 63;
-    if (i == 0) lds.count = 0;
-    uint64_t bound = 1;  // every key
-    if (best <= 64) {
-        own = larger_key(own, dpp_key<0xB1>(own));
-        own = larger_key(own, dpp_key<0x4E>(own));
-        if ((i & 3) == 0) lds.most[i >> 2] = own;
-        __syncthreads();
-        // every wave ranks the 64 groups, one a lane
-        const uint64_t mine = lds.most[lane];
-        uint32_t above = 0;
-#pragma unroll 16
-        for (int j = 0; j < 64; ++j) above += lds.most[j] > mine;
-        const uint64_t at = __ballot(mine != kNoKey && above == best - 1);
-        if (at != 0) bound = lane_key(mine, __ffsll(static_cast<unsigned long long>(at)) - 1);
-    } else {
-        lds.most[i] = own;
-        __syncthreads();
-        // every wave ranks all 256, four a lane
-#pragma unroll 1
-        for (uint32_t q = 0; q < kBeamThreads / 64; ++q) {
-            const uint64_t mine = lds.most[q * 64 + lane];
-            uint32_t above = 0;
-#pragma unroll 16
-            for (uint32_t j = 0; j < kBeamThreads; ++j) above += lds.most[j] > mine;
-            const uint64_t at = __ballot(mine != kNoKey && above == best - 1);
-            if (at != 0) bound = lane_key(mine, __ffsll(static_cast<unsigned long long>(at)) - 1);
-        }
-    }
-    push(bound, [&](uint64_t key) { list[atomicAdd(&lds.count, 1u)] = key; });
-    __syncthreads();
-    const uint32_t n = lds.count;
-    for (uint32_t c = i; c < n; c += kBeamThreads) {
+// Ranks of the n listed keys: put(rank, key) for the `best` largest.
+template <class Put>
+__device__ inline void rank_list(const uint64_t *list, uint32_t n, uint32_t best, Put put) {
+    for (uint32_t c = threadIdx.x; c < n; c += kBeamThreads) {
         const uint64_t mine = list[c];
         uint32_t rank = 0;
         for (uint32_t j = 0; j < n; j += 8) {  // eight reads at a time, the last ones past the end
@@ -147,29 +141,128 @@ __device__ inline uint32_t best_of(uint64_t own, uint32_t best, BestLds &lds, ui
         }
         if (rank < best) put(rank, mine);
     }
+}
+
+// best_of where many items share the order that bounds it (a row masked by one
+// low value, say): the same selection by whole keys, of which no two are equal.
+template <uint32_t kEach, class Key, class Put>
+__device__ inline uint32_t best_exact(uint32_t best, BestLds &lds, uint64_t *list, Key key, Put put) {
+    const uint32_t i = threadIdx.x;
+    const int lane = i & 63;
+    uint64_t own = kNoKey;
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e) own = larger_key(own, key(e));
+    if (i == 0) lds.count = 0;
+    uint64_t bound = 1;  // every key
+    const uint32_t groups = best <= 64 ? 64 : kBeamThreads;
+    if (best <= 64) {
+        own = larger_key(own, dpp_key<0xB1>(own));
+        own = larger_key(own, dpp_key<0x4E>(own));
+        if ((i & 3) == 0) lds.most.key[i >> 2] = own;
+    } else {
+        lds.most.key[i] = own;
+    }
+    __syncthreads();
+    for (uint32_t q = 0; q < groups; q += 64) {  // every wave ranks them all, one a lane
+        const uint64_t mine = lds.most.key[q + lane];
+        uint32_t above = 0;
+#pragma unroll 8
+        for (uint32_t j = 0; j < groups; ++j) above += lds.most.key[j] > mine;
+        const uint64_t at = __ballot(mine != kNoKey && above == best - 1);
+        if (at != 0) bound = lane_key(mine, __ffsll(static_cast<unsigned long long>(at)) - 1);
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e) {
+        const uint64_t k = key(e);
+        if (k >= bound) list[atomicAdd(&lds.count, 1u)] = k;
+    }
+    __syncthreads();
+    const uint32_t n = lds.count;
+    rank_list(list, n, best, put);
     return min(n, best);
 }
 
-template <class T, class Op>
-__device__ inline T workgroup_reduce(T v, T *sm, Op op) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o));
-    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
+// The `best` largest keys of the workgroup, put(rank, key) for each: order(e) and
+// key(e) are the thread's e-th (kNoOrder and kNoKey: none), most its largest
+// order.  Returns how many there are.  Every thread calls it; LDS is free for the
+// next call after a barrier.
+//
+// The bound is the `best`-th largest of the groups' largest orders, 32 bits; what
+// reaches it is listed and ranked by whole keys.  32 groups of 8 threads for up
+// to 16 wanted, 64 of 4 for up to 64, else each thread.
+template <uint32_t kEach, class Order, class Key, class Put>
+__device__ inline uint32_t best_of(int32_t most, uint32_t best, BestLds &lds, uint64_t *list, uint32_t room, Order order, Key key, Put put) {
+    const uint32_t i = threadIdx.x;
+    const uint32_t lane = i & 63;
+    if (i == 0) lds.count = 0;
+    const uint32_t groups = best <= 16 ? 32 : (best <= 64 ? 64 : kBeamThreads);
+    if (best <= 64) {
+        most = max(most, dpp_i32<0xB1>(most));
+        most = max(most, dpp_i32<0x4E>(most));
+        if (best <= 16) {
+            most = max(most, dpp_i32<0x141>(most));  // the other four of eight
+            if ((i & 7) == 0) lds.most.order[i >> 3] = most;
+        } else if ((i & 3) == 0) {
+            lds.most.order[i >> 2] = most;
+        }
+    } else {
+        lds.most.order[i] = most;
+    }
     __syncthreads();
-    T r = sm[0];
+    // Every wave ranks the groups: those that fewer than `best` exceed are at least
+    // `best`, ties among them, and the least of them is the bound.
+    uint32_t members = 0;
+    int32_t bound = INT32_MAX;
+    for (uint32_t q = 0; q < groups; q += 64) {
+        const int32_t mine = q + lane < groups ? lds.most.order[q + lane] : kNoOrder;
+        uint32_t above = 0;
+        if (groups == 32) {
 #pragma unroll
-    for (uint32_t w = 1; w < kBeamThreads / 64; ++w) r = op(r, sm[w]);
-    return r;
+            for (uint32_t j = 0; j < 32; ++j) above += lds.most.order[j] > mine;
+        } else {
+#pragma unroll 16
+            for (uint32_t j = 0; j < groups; ++j) above += lds.most.order[j] > mine;
+        }
+        const bool in = mine != kNoOrder && above < best;
+        members += static_cast<uint32_t>(__popcll(__ballot(in)));
+        if (in) bound = min(bound, mine);
+    }
+    bound = members >= best ? wave_least(bound) : kNoOrder + 1;  // or everything
+    uint32_t here = 0;
+#pragma unroll
+    for (uint32_t e = 0; e < kEach; ++e) here += static_cast<uint32_t>(__popcll(__ballot(order(e) >= bound)));
+    if (here != 0) {  // uniform over the wave
+        uint32_t at = 0;
+        if (lane == 0) at = atomicAdd(&lds.count, here);
+        at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
+#pragma unroll
+        for (uint32_t e = 0; e < kEach; ++e) {
+            const uint64_t mask = __ballot(order(e) >= bound);
+            if (mask == 0) continue;
+            const uint32_t place = at + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
+            if (order(e) >= bound && place < room) list[place] = key(e);
+            at += static_cast<uint32_t>(__popcll(mask));
+        }
+    }
+    __syncthreads();
+    const uint32_t n = lds.count;
+    if (n > room) {  // uniform
+        __syncthreads();  // everyone has read the count
+        return best_exact<kEach>(best, lds, list, key, put);
+    }
+    rank_list(list, n, best, put);
+    return min(n, best);
 }
-__device__ inline double plus(double a, double b) { return a + b; }
+// Keys that best_of lists before it turns to the exact selection.
+constexpr uint32_t best_room(uint32_t best) { return best * 4; }
 
 // Grid (segment, row): kEach * kBeamThreads logits each.
 template <uint32_t kEach>
 __global__ __launch_bounds__(kBeamThreads) void beam_segment_kernel(BeamSelect b) {
     extern __shared__ uint64_t list[];
     __shared__ BestLds lds;
-    __shared__ float sm_f[kBeamThreads / 64];
-    __shared__ double sm_d[kBeamThreads / 64];
+    __shared__ float sm_top[kBeamThreads / 64];
+    __shared__ double sm_sum[kBeamThreads / 64];
     const uint32_t segment = blockIdx.x, row = blockIdx.y, i = threadIdx.x;
     constexpr uint32_t kSegment = kEach * kBeamThreads;
     if (!row_alive(b, row) || row_finished(b, row)) return;  // uniform; the row's join reads nothing then
@@ -212,34 +305,36 @@ __global__ __launch_bounds__(kBeamThreads) void beam_segment_kernel(BeamSelect b
         for (uint32_t e = 0; e < kEach; ++e) v[e] = clean(v[e]);
         scan();
     }
+    // Joined over the wave here, over the waves by the first thread, behind
+    // best_of's barrier.
     const bool any = most > kMaskedOrder;
-    const float top = workgroup_reduce(any ? reference : -INFINITY, sm_f, [](float x, float y) { return fmaxf(x, y); });
-    const double total = workgroup_reduce(any ? static_cast<double>(sum * exp_term(reference, top)) : 0.0, sm_d, plus);
-    const size_t part = static_cast<size_t>(row) * b.segments + segment;
-    if (i == 0) {
-        b.references[part] = top;
-        b.sums[part] = total;
+    const float top = wave_largest(any ? reference : -INFINITY);
+    const double total = wave_sum(any ? static_cast<double>(sum * exp_term(reference, top)) : 0.0);
+    if ((i & 63) == 0) {
+        sm_top[i >> 6] = top;
+        sm_sum[i >> 6] = total;
     }
-    auto token = [&](uint32_t e) { return first + ((e >> 2) * kBeamThreads + i) * 4 + (e & 3); };
-    uint64_t own = kNoKey;
-#pragma unroll
-    for (uint32_t e = kEach; e-- > 0;)
-        if (any && order[e] == most) own = key_of(most, token(e));  // the lowest token of the largest
+    const size_t part = static_cast<size_t>(row) * b.segments + segment;
     uint64_t *out = b.keys + part * b.best;
-    const uint32_t found = best_of(
-        own, b.best, lds, list,
-        [&](uint64_t bound, auto add) {
-            const int32_t least = max(order_in(bound), kMaskedOrder + 1);
-            if (most < least) return;
-#pragma unroll
-            for (uint32_t e = 0; e < kEach; ++e) {
-                if (order[e] < least) continue;
-                const uint64_t key = key_of(order[e], token(e));
-                if (key >= bound) add(key);
-            }
+    auto masked = [&](uint32_t e) { return order[e] > kMaskedOrder ? order[e] : kNoOrder; };
+    const uint32_t found = best_of<kEach>(
+        any ? most : kNoOrder, b.best, lds, list, best_room(b.best), masked,
+        [&](uint32_t e) {
+            return order[e] > kMaskedOrder ? key_of(order[e], first + ((e >> 2) * kBeamThreads + i) * 4 + (e & 3)) : kNoKey;
         },
         [&](uint32_t rank, uint64_t key) { out[rank] = key; });
     for (uint32_t k = found + i; k < b.best; k += kBeamThreads) out[k] = kNoKey;
+    if (i == 0) {
+        float all = sm_top[0];
+#pragma unroll
+        for (uint32_t w = 1; w < kBeamThreads / 64; ++w) all = fmaxf(all, sm_top[w]);
+        double s = 0.0;
+#pragma unroll
+        for (uint32_t w = 0; w < kBeamThreads / 64; ++w)
+            if (sm_top[w] > -INFINITY) s += sm_sum[w] * static_cast<double>(exp_term(sm_top[w], all));
+        b.references[part] = all;
+        b.sums[part] = s;
+    }
 }
 
 __device__ inline void store_agent(uint64_t *p, uint64_t v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -255,7 +350,6 @@ template <class Keys>
 __device__ inline void join_keys(uint64_t (&key)[kJoinEach + 1], uint64_t count, uint32_t best, BestLds &lds, uint64_t *list, uint64_t *run, Keys keys) {
     const uint32_t i = threadIdx.x;
     for (uint64_t at = 0; at < count; at += kJoinEach * kBeamThreads) {
-        uint64_t own = kNoKey;
         key[kJoinEach] = kNoKey;
         if (at > 0) {
 #pragma unroll
@@ -265,15 +359,11 @@ __device__ inline void join_keys(uint64_t (&key)[kJoinEach + 1], uint64_t count,
             }
             if (i < best) key[kJoinEach] = run[i];
         }
+        int32_t most = kNoOrder;
 #pragma unroll
-        for (uint32_t e = 0; e <= kJoinEach; ++e) own = larger_key(own, key[e]);
-        const uint32_t found = best_of(
-            own, best, lds, list,
-            [&](uint64_t bound, auto add) {
-#pragma unroll
-                for (uint32_t e = 0; e <= kJoinEach; ++e)
-                    if (key[e] >= bound) add(key[e]);
-            },
+        for (uint32_t e = 0; e <= kJoinEach; ++e) most = max(most, order_in(key[e]));
+        const uint32_t found = best_of<kJoinEach + 1>(
+            most, best, lds, list, best_room(best), [&](uint32_t e) { return order_in(key[e]); }, [&](uint32_t e) { return key[e]; },
             [&](uint32_t rank, uint64_t k) { run[rank] = k; });
         for (uint32_t k = found + i; k < best; k += kBeamThreads) run[k] = kNoKey;
         __syncthreads();
@@ -287,7 +377,6 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
     extern __shared__ uint64_t list[];
     __shared__ BestLds lds;
     __shared__ uint64_t run[kBeamMaxBest], run_scores[kBeamMaxBest];
-    __shared__ double sm_m[kBeamThreads / 64], sm_d[kBeamThreads / 64];
     __shared__ int sm_last;
     const uint32_t row = blockIdx.x, i = threadIdx.x, entry = row / b.beams;
     const size_t part = static_cast<size_t>(row) * b.segments;
@@ -297,24 +386,27 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
     uint64_t key_in[kJoinEach + 1];
 #pragma unroll
     for (uint32_t e = 0; e < kJoinEach; ++e) key_in[e] = keys[min(static_cast<uint64_t>(e * kBeamThreads + i), count - 1)];
-    const uint32_t s0 = min(i, b.segments - 1);
+    const uint32_t lane = i & 63, s0 = min(lane, b.segments - 1);
     const float reference0 = b.references[part + s0];
     const double sum0 = b.sums[part + s0];
     const float start = b.scores[row];
     const bool finished = row_finished(b, row), alive = start > -INFINITY;
-    double top = -INFINITY, log_sum = 0.0;
+    double top = 0.0, log_sum = 0.0;
     if (alive && !finished) {  // uniform
 #pragma unroll
         for (uint32_t e = 0; e < kJoinEach; ++e)
             if (e * kBeamThreads + i >= count) key_in[e] = kNoKey;
-        for (uint32_t s = i; s < b.segments; s += kBeamThreads) top = fmax(top, static_cast<double>(s == i ? reference0 : b.references[part + s]));
-        top = workgroup_reduce(top, sm_m, [](double x, double y) { return fmax(x, y); });
-        double sum = 0.0;
-        if (top > -INFINITY)  // uniform
-            for (uint32_t s = i; s < b.segments; s += kBeamThreads)
-                sum += (s == i ? sum0 : b.sums[part + s]) * exp(static_cast<double>(s == i ? reference0 : b.references[part + s]) - top);
-        sum = workgroup_reduce(sum, sm_d, plus);
-        log_sum = log(sum);  // (not used where all is masked)
+        // Every wave sums the segments by itself.
+        float most = -INFINITY;
+        for (uint32_t s = lane; s < b.segments; s += 64) most = fmaxf(most, s == lane ? reference0 : b.references[part + s]);
+        most = wave_largest(most);
+        if (most > -INFINITY) {  // uniform: something is not masked
+            top = most;
+            double sum = 0.0;
+            for (uint32_t s = lane; s < b.segments; s += 64)
+                sum += (s == lane ? sum0 : b.sums[part + s]) * exp(static_cast<double>(s == lane ? reference0 : b.references[part + s]) - top);
+            log_sum = log(wave_sum(sum));
+        }
         join_keys(key_in, count, b.best, lds, list, run, [&](uint64_t k) { return keys[k]; });
     } else {
         for (uint32_t k = i; k < b.best; k += kBeamThreads)
