@@ -315,15 +315,15 @@ __global__ __launch_bounds__(kBeamThreads) void beam_segment_kernel(BeamSelect b
         sm_sum[i >> 6] = total;
     }
     const size_t part = static_cast<size_t>(row) * b.segments + segment;
-    uint64_t *out = b.keys + part * b.best;
+    uint64_t *out = b.keys + static_cast<size_t>(row) * b.best * b.segments + segment;
     auto masked = [&](uint32_t e) { return order[e] > kMaskedOrder ? order[e] : kNoOrder; };
     const uint32_t found = best_of<kEach>(
         any ? most : kNoOrder, b.best, lds, list, best_room(b.best), masked,
         [&](uint32_t e) {
             return order[e] > kMaskedOrder ? key_of(order[e], first + ((e >> 2) * kBeamThreads + i) * 4 + (e & 3)) : kNoKey;
         },
-        [&](uint32_t rank, uint64_t key) { out[rank] = key; });
-    for (uint32_t k = found + i; k < b.best; k += kBeamThreads) out[k] = kNoKey;
+        [&](uint32_t rank, uint64_t key) { out[static_cast<size_t>(rank) * b.segments] = key; });
+    for (uint32_t k = found + i; k < b.best; k += kBeamThreads) out[static_cast<size_t>(k) * b.segments] = kNoKey;
     if (i == 0) {
         float all = sm_top[0];
 #pragma unroll
@@ -342,10 +342,15 @@ __device__ inline uint64_t load_agent(const uint64_t *p) { return __hip_atomic_l
 
 // Keys a thread takes at a time in the join, beside one of the best so far.
 constexpr uint32_t kJoinEach = 4;
+// The joined lists are sorted and lie rank by rank, the first of each list
+// first.  A thread's e-th key: consecutive ones go to different groups of best_of,
+// so that the lists' first keys do (lists left whole in a group made the bound so
+// low that the exact selection had to follow).
+__device__ inline uint32_t join_at(uint32_t e) { return e * kBeamThreads + (threadIdx.x & 7) * (kBeamThreads / 8) + (threadIdx.x >> 3); }
 
 // The `best` largest of keys(0) .. keys(count - 1) into run, in order, kNoKey
-// behind.  Every thread calls it, with its first keys, thread i's key e being
-// keys(e * kBeamThreads + i); run is complete when it returns.
+// behind.  Every thread calls it, with its first keys, keys(join_at(e)); run is
+// complete when it returns.
 template <class Keys>
 __device__ inline void join_keys(uint64_t (&key)[kJoinEach + 1], uint64_t count, uint32_t best, BestLds &lds, uint64_t *list, uint64_t *run, Keys keys) {
     const uint32_t i = threadIdx.x;
@@ -354,7 +359,7 @@ __device__ inline void join_keys(uint64_t (&key)[kJoinEach + 1], uint64_t count,
         if (at > 0) {
 #pragma unroll
             for (uint32_t e = 0; e < kJoinEach; ++e) {
-                const uint64_t k = at + e * kBeamThreads + i;
+                const uint64_t k = at + join_at(e);
                 key[e] = k < count ? keys(k) : kNoKey;
             }
             if (i < best) key[kJoinEach] = run[i];
@@ -380,12 +385,12 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
     __shared__ int sm_last;
     const uint32_t row = blockIdx.x, i = threadIdx.x, entry = row / b.beams;
     const size_t part = static_cast<size_t>(row) * b.segments;
-    const uint64_t *keys = b.keys + part * b.best;
+    const uint64_t *keys = b.keys + part * b.best;  // [rank][segment]
     const uint64_t count = static_cast<uint64_t>(b.segments) * b.best;
     // All first loads together (of a row that was not read, whatever is there).
     uint64_t key_in[kJoinEach + 1];
 #pragma unroll
-    for (uint32_t e = 0; e < kJoinEach; ++e) key_in[e] = keys[min(static_cast<uint64_t>(e * kBeamThreads + i), count - 1)];
+    for (uint32_t e = 0; e < kJoinEach; ++e) key_in[e] = keys[min(static_cast<uint64_t>(join_at(e)), count - 1)];
     const uint32_t lane = i & 63, s0 = min(lane, b.segments - 1);
     const float reference0 = b.references[part + s0];
     const double sum0 = b.sums[part + s0];
@@ -395,7 +400,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
     if (alive && !finished) {  // uniform
 #pragma unroll
         for (uint32_t e = 0; e < kJoinEach; ++e)
-            if (e * kBeamThreads + i >= count) key_in[e] = kNoKey;
+            if (join_at(e) >= count) key_in[e] = kNoKey;
         // Every wave sums the segments by itself.
         float most = -INFINITY;
         for (uint32_t s = lane; s < b.segments; s += 64) most = fmaxf(most, s == lane ? reference0 : b.references[part + s]);
@@ -422,7 +427,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
         score = finished ? static_cast<double>(start) : start + ((static_cast<double>(value_of(order_in(key))) - top) - log_sum);
         if (key != kNoKey) scored = score_key(score, beam * b.best + i);
     }
-    const size_t at = static_cast<size_t>(row) * b.best + i, rows_at = static_cast<size_t>(entry) * b.beams * b.best;
+    const size_t rows_at = static_cast<size_t>(entry) * b.beams * b.best, at = rows_at + static_cast<size_t>(i) * b.beams + beam;  // [rank][beam]
     if (b.beams > 1) {
         if (i < b.best) {
             store_agent(b.row_keys + at, scored);
@@ -438,7 +443,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
         const uint64_t all = static_cast<uint64_t>(b.beams) * b.best;
         auto scores = [&](uint64_t k) { return load_agent(b.row_keys + rows_at + k); };
 #pragma unroll
-        for (uint32_t e = 0; e < kJoinEach; ++e) key_in[e] = e * kBeamThreads + i < all ? scores(e * kBeamThreads + i) : kNoKey;
+        for (uint32_t e = 0; e < kJoinEach; ++e) key_in[e] = join_at(e) < all ? scores(join_at(e)) : kNoKey;
         join_keys(key_in, all, b.best, lds, list, run_scores, scores);
         if (i >= b.best) return;
         scored = run_scores[i];
@@ -448,10 +453,10 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
     int32_t parent = -1, token = -1, ended = 0;
     float value = -INFINITY;
     if (scored != kNoKey) {
-        const uint32_t number = number_in(scored);
-        parent = static_cast<int32_t>(entry * b.beams + number / b.best);
+        const uint32_t number = number_in(scored), from = number / b.best;
+        parent = static_cast<int32_t>(entry * b.beams + from);
         if (b.beams > 1) {
-            const uint64_t held = load_agent(reinterpret_cast<const uint64_t *>(b.row_scores) + rows_at + number);
+            const uint64_t held = load_agent(reinterpret_cast<const uint64_t *>(b.row_scores) + rows_at + static_cast<size_t>(number - from * b.best) * b.beams + from);
             token = static_cast<int32_t>(held >> 32);
             value = __uint_as_float(static_cast<uint32_t>(held));
         } else {

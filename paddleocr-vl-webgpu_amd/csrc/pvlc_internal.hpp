@@ -535,11 +535,11 @@ struct BeamSelect {
     float *next_scores;
     int32_t *parents, *tokens, *next_finished;
     uint32_t *arrived;    // by batch entry; 0 before and after a launch
-    uint64_t *keys;       // [row][segment][best]
+    uint64_t *keys;       // [row][rank][segment]
     double *sums;         // [row][segment], relative to exp(reference)
     float *references;    // [row][segment]
-    uint64_t *row_keys;   // [row][best]: the scores' keys
-    double *row_scores;   // [row][best]: token and f32 score
+    uint64_t *row_keys;   // [batch entry][rank][beam]: the scores' keys
+    double *row_scores;   // the same: token and f32 score
 };
 struct BeamWorkspace {
     size_t keys_offset, sums_offset, references_offset, row_keys_offset, row_scores_offset, total;
