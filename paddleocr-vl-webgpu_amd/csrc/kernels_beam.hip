@@ -354,6 +354,16 @@ __device__ inline uint32_t join_at(uint32_t e) { return e * kBeamThreads + (thre
 template <class Keys>
 __device__ inline void join_keys(uint64_t (&key)[kJoinEach + 1], uint64_t count, uint32_t best, BestLds &lds, uint64_t *list, uint64_t *run, Keys keys) {
     const uint32_t i = threadIdx.x;
+    if (count <= 64 && count <= best_list(best, kJoinEach + 1) - 8) {  // uniform: few enough to be ranked as they are (128 are not)
+        if (join_at(0) < count) list[join_at(0)] = key[0];
+        if (i < best) run[i] = kNoKey;
+        __syncthreads();
+        rank_list(list, static_cast<uint32_t>(count), best, [&](uint32_t rank, uint64_t k) {
+            if (k != kNoKey) run[rank] = k;
+        });
+        __syncthreads();
+        return;
+    }
     for (uint64_t at = 0; at < count; at += kJoinEach * kBeamThreads) {
         key[kJoinEach] = kNoKey;
         if (at > 0) {
@@ -478,7 +488,6 @@ int launch_beam_select(const BeamSelect &b, void *stream) {
     const dim3 grid(b.segments, b.batch * b.beams);
 #define PVLC_BEAM_LAUNCH(E) hipLaunchKernelGGL(beam_segment_kernel<E>, grid, dim3(kBeamThreads), best_list(b.best, E) * 8, st, b)
     switch (b.each) {
-        case 4: PVLC_BEAM_LAUNCH(4); break;
         case 8: PVLC_BEAM_LAUNCH(8); break;
         default: PVLC_BEAM_LAUNCH(16); break;
     }
