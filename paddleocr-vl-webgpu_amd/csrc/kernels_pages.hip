@@ -84,18 +84,36 @@ __device__ inline RowWant want_of(const PagesFork &f, uint32_t r, uint32_t *erro
     return w;
 }
 
+// What a row's plan reads: what becomes of it, the entry that it would write next
+// and that page's count.
+struct RowRead {
+    RowWant want;
+    int32_t next, count;
+};
+__device__ inline RowRead read_row(const PagesFork &f, uint32_t r, uint32_t *errors) {
+    RowRead row{want_of(f, r, errors), -1, 0};
+    const uint32_t filled = row.want.length / kBlockTokens;
+    if (row.want.parent >= 0 && row.want.need > filled) {
+        row.next = f.tables_in[static_cast<size_t>(row.want.parent) * f.max_blocks + filled];
+        if (valid_block(row.next, f.num_blocks)) row.count = f.ref_counts[row.next];
+    }
+    return row;
+}
+
 // The plan of a fork, all that the execution needs of each row in one record.
 // An output row keeps the first `kept` of its parent's entries: the filled blocks
 // and, for the parent's first child, what follows as far as no other entry names
 // it; fresh[base ..] are its others.  Everything of a row stays in LDS and
-// registers: a round through memory costs more than all the arithmetic (four
-// beams 5.3 us through memory, three rounds more).
-template <int kThreads, uint32_t kWords>
+// registers, and what it needs of the tables is read at once: the launch is a
+// chain of rounds through memory (four beams, rows through memory 5.3 us, reads
+// where they are needed 4.2).  A thread takes a Unit of the mask at a time, bytes
+// of pools that have few: it names its pages one after the other.
+template <int kThreads, class Unit, uint32_t kUnits>
 __global__ __launch_bounds__(kThreads) void pages_fork_plan_kernel(PagesFork f) {
     extern __shared__ uint32_t by_row[];  // first[rows_in], children[rows_in], kept[rows_in]
     __shared__ uint32_t sm[kThreads / 64];
     __shared__ uint32_t sm_errors;
-    constexpr uint32_t kTile = kThreads * kWords;  // words of the mask at a time
+    constexpr uint32_t kBits = sizeof(Unit) * 8, kTile = kThreads * kUnits;  // units of the mask at a time
     // Every pointer in one round of scalar loads.
     asm volatile("" ::"s"(f.parents), "s"(f.reserve), "s"(f.lens_in), "s"(f.tables_in), "s"(f.ref_counts), "s"(f.free_mask), "s"(f.plan.rows),
                  "s"(f.plan.fresh), "s"(f.lens_out));
@@ -107,52 +125,51 @@ __global__ __launch_bounds__(kThreads) void pages_fork_plan_kernel(PagesFork f) 
         children[p] = 0;
         taken[p] = 0;
     }
-    const uint32_t words = (f.num_blocks + 31) / 32;
-    const uint32_t last_word = (f.num_blocks & 31) ? (1u << (f.num_blocks & 31)) - 1u : ~0u;
-    auto load_mask = [&](uint32_t w0, uint32_t (&bits)[kWords]) {
-        const uint32_t w = w0 + i * kWords;
+    Unit *mask = reinterpret_cast<Unit *>(f.free_mask);  // (little-endian: bit b of unit u is page u * kBits + b)
+    const uint32_t units = (f.num_blocks + kBits - 1) / kBits;
+    auto load_mask = [&](uint32_t u0, uint32_t (&bits)[kUnits]) {
 #pragma unroll
-        for (uint32_t k = 0; k < kWords; ++k) bits[k] = w + k < words ? f.free_mask[w + k] : 0u;
-#pragma unroll
-        for (uint32_t k = 0; k < kWords; ++k)
-            if (w + k == words - 1) bits[k] &= last_word;
+        for (uint32_t k = 0; k < kUnits; ++k) {
+            const uint32_t u = u0 + i * kUnits + k;
+            bits[k] = u < units ? mask[u] : 0u;
+            if (u == units - 1 && f.num_blocks % kBits) bits[k] &= (1u << (f.num_blocks % kBits)) - 1u;
+        }
     };
-    uint32_t bits[kWords];
+    uint32_t bits[kUnits];
     load_mask(0, bits);  // its use is rounds away
+    uint32_t errors = 0, none = 0;
+    RowRead mine{};  // of row i, where every row has a thread
+    if (i < f.rows_out) mine = read_row(f, i, &errors);
     __syncthreads();
-    uint32_t errors = 0;
     for (uint32_t r = i; r < f.rows_out; r += kThreads) {
-        const RowWant w = want_of(f, r, &errors);
-        if (w.parent >= 0) {
-            atomicMin(&first[w.parent], r);
-            atomicAdd(&children[w.parent], 1u);
+        const int32_t parent = r == i ? mine.want.parent : want_of(f, r, &errors).parent;
+        if (parent >= 0) {
+            atomicMin(&first[parent], r);
+            atomicAdd(&children[parent], 1u);
         }
     }
     __syncthreads();
-    uint32_t total = 0, length = 0;
+    uint32_t total = 0;
     for (uint32_t r0 = 0; r0 < f.rows_out; r0 += kThreads) {
         const uint32_t r = r0 + i;
         uint32_t fresh = 0;
         ForkRow row{-1, 0, 0, 0, -1, 0};
         if (r < f.rows_out) {
-            uint32_t none = 0;
-            const RowWant w = want_of(f, r, &none);
-            row.parent = w.parent;
-            row.need = w.need;
-            row.length = length = w.length;
+            const RowRead in = r == i ? mine : read_row(f, r, &none);
+            const RowWant &w = in.want;
             const uint32_t filled = w.length / kBlockTokens;
-            row.kept = filled;
+            row = {w.parent, filled, w.need, 0, -1, w.length};
             if (w.parent >= 0 && w.need > filled) {
-                const int32_t *entries = f.tables_in + static_cast<size_t>(w.parent) * f.max_blocks;
-                int32_t id = entries[filled];
+                int32_t id = in.next, count = in.count;
                 if (w.length % kBlockTokens != 0) {
                     row.source = id;
                     if (!valid_block(id, f.num_blocks)) errors |= PVLC_HIP_PAGES_BAD_BLOCK;
                 }
                 if (!f.keep_inputs && first[w.parent] == r) {
-                    while (valid_block(id, f.num_blocks) && f.ref_counts[id] == 1) {
+                    while (valid_block(id, f.num_blocks) && count == 1) {
                         if (++row.kept == w.need) break;
-                        id = entries[row.kept];
+                        id = f.tables_in[static_cast<size_t>(w.parent) * f.max_blocks + row.kept];
+                        if (valid_block(id, f.num_blocks)) count = f.ref_counts[id];
                     }
                     if (row.kept > filled) row.source = -1;
                     taken[w.parent] = row.kept;
@@ -167,46 +184,43 @@ __global__ __launch_bounds__(kThreads) void pages_fork_plan_kernel(PagesFork f) 
         total += sum;
     }
     // The lowest `total` free pages.  All free pages up to the last one taken are
-    // taken, so the mask's words are 0 up to the tile that has it; whether there
-    // are enough is known when that tile's are counted, before its pages are
-    // named.
-    uint32_t found = 0, before = 0, w0 = 0;
+    // taken, so the mask is 0 up to the tile that has it; whether there are enough
+    // is known when that tile's are counted, before its pages are named.
+    uint32_t found = 0, before = 0, u0 = 0;
     bool enough = total == 0;
-    while (!enough && w0 < words) {
-        if (w0 > 0) load_mask(w0, bits);
+    while (!enough && u0 < units) {
+        if (u0 > 0) load_mask(u0, bits);
         uint32_t here = 0, sum;
 #pragma unroll
-        for (uint32_t k = 0; k < kWords; ++k) here += static_cast<uint32_t>(__popc(bits[k]));
+        for (uint32_t k = 0; k < kUnits; ++k) here += static_cast<uint32_t>(__popc(bits[k]));
         uint32_t at = found + plan_scan<kThreads>(here, sm, &sum);
         before = found;
         found += sum;
         enough = found >= total;
 #pragma unroll
-        for (uint32_t k = 0; k < kWords; ++k) {
+        for (uint32_t k = 0; k < kUnits; ++k) {
             uint32_t left = bits[k];
-            const uint32_t w = w0 + i * kWords + k;
+            const uint32_t u = u0 + i * kUnits + k;
             for (; left && at < total; ++at) {
-                const int32_t id = static_cast<int32_t>(w * 32 + static_cast<uint32_t>(__ffs(static_cast<int>(left)) - 1));
+                const int32_t id = static_cast<int32_t>(u * kBits + static_cast<uint32_t>(__ffs(static_cast<int>(left)) - 1));
                 left &= left - 1;
                 f.plan.fresh[at] = id;
                 if (enough) f.ref_counts[id] = 1;
             }
-            if (enough && left != bits[k]) f.free_mask[w] = left;
+            if (enough && left != bits[k]) mask[u] = static_cast<Unit>(left);
         }
-        if (!enough) w0 += kTile;
+        if (!enough) u0 += kTile;
     }
     if (errors) atomicOr(&sm_errors, errors);
     __syncthreads();
     if (enough && before > 0) {  // pages of the tiles before
         for (uint32_t k = i; k < before; k += kThreads) f.ref_counts[f.plan.fresh[k]] = 1;
-        for (uint32_t w = i; w < w0; w += kThreads) f.free_mask[w] = 0;
+        for (uint32_t u = i; u < u0; u += kThreads) mask[u] = 0;
     }
-    for (uint32_t p = i; p < f.rows_in; p += kThreads) {
-        uint32_t none = 0;
+    for (uint32_t p = i; p < f.rows_in; p += kThreads)
         f.plan.inputs[p] = {children[p], in_length(f, p, &none) / kBlockTokens, taken[p], 0};
-    }
     for (uint32_t r = i; r < f.rows_out; r += kThreads)
-        f.lens_out[r] = enough ? static_cast<int32_t>(f.rows_out <= kThreads ? length : f.plan.rows[r].length) : -1;
+        f.lens_out[r] = enough ? static_cast<int32_t>(r == i ? mine.want.length : f.plan.rows[r].length) : -1;
     if (i == 0) {
         *f.plan.enough = enough;
         const uint32_t e = sm_errors | (enough ? 0u : PVLC_HIP_PAGES_EXHAUSTED);
@@ -318,46 +332,61 @@ __global__ __launch_bounds__(kWideThreads) void pages_fork_kernel(PagesFork f, P
 // the free ones among the first L, in order: the least that moves.
 //
 // Counts of the words of 32 pages: used_before[w], and L behind the last.
-__global__ __launch_bounds__(kPlanThreads) void pages_count_kernel(PagesCompact c) {
-    __shared__ uint32_t sm[kPlanThreads / 64];
+template <int kThreads>
+__device__ inline uint32_t count_words(const PagesCompact &c, uint32_t *used_before, uint32_t *sm) {
     const uint32_t words = (c.num_blocks + 31) / 32;
     uint32_t used = 0;
-    for (uint32_t w0 = 0; w0 < words; w0 += kPlanThreads) {
+    for (uint32_t w0 = 0; w0 < words; w0 += kThreads) {
         const uint32_t w = w0 + threadIdx.x;
         const uint32_t in_word = w < words ? min(32u, c.num_blocks - w * 32) : 0u;
         uint32_t bits = w < words ? c.free_mask[w] : 0u;
         if (in_word < 32) bits &= (1u << in_word) - 1u;
         uint32_t sum;
-        const uint32_t before = plan_scan<kPlanThreads>(in_word - static_cast<uint32_t>(__popc(bits)), sm, &sum);
-        if (w < words) c.plan.used_before[w] = used + before;
+        const uint32_t before = plan_scan<kThreads>(in_word - static_cast<uint32_t>(__popc(bits)), sm, &sum);
+        if (w < words) used_before[w] = used + before;
         used += sum;
     }
-    if (threadIdx.x == 0) c.plan.used_before[words] = used;
+    return used;
+}
+__global__ __launch_bounds__(kPlanThreads) void pages_count_kernel(PagesCompact c) {
+    __shared__ uint32_t sm[kPlanThreads / 64];
+    const uint32_t used = count_words<kPlanThreads>(c, c.plan.used_before, sm);
+    if (threadIdx.x == 0) c.plan.used_before[(c.num_blocks + 31) / 32] = used;
 }
 
-// The list of moves: the k-th used page from L on, to the k-th free page.
-// forward[id]: where a page goes (its own id where it stays or is free).
+// The list of moves: the k-th used page from L on, to the k-th free page; rank[id]:
+// a page's number among them, or -1.  Workgroups of a small pool count its words
+// by themselves (a launch of its own for that took 2 us of 38 of a turnover's).
+constexpr uint32_t kCountWords = 1024;
+template <bool kCounted>
 __global__ __launch_bounds__(kWideThreads) void pages_moves_kernel(PagesCompact c) {
+    __shared__ uint32_t sm[kWideThreads / 64];
+    __shared__ uint32_t sm_before[kCounted ? 1 : kCountWords];
     const uint32_t words = (c.num_blocks + 31) / 32;
-    const uint32_t live = c.plan.used_before[words];
+    const uint32_t *used_in = kCounted ? c.plan.used_before : sm_before;
+    uint32_t live;
+    if constexpr (kCounted) {
+        live = c.plan.used_before[words];
+    } else {
+        live = count_words<kWideThreads>(c, sm_before, sm);
+        __syncthreads();
+        if (blockIdx.x == 0 && threadIdx.x == 0) c.plan.used_before[words] = live;
+    }
     const uint32_t id = blockIdx.x * kWideThreads + threadIdx.x;
     if (id >= c.num_blocks) return;
     const uint32_t bit = 1u << (id & 31), bits = c.free_mask[id >> 5];
-    const uint32_t used_before = c.plan.used_before[id >> 5] + static_cast<uint32_t>(__popc(~bits & (bit - 1)));
+    const uint32_t used_before = used_in[id >> 5] + static_cast<uint32_t>(__popc(~bits & (bit - 1)));
     const bool free_page = (bits & bit) != 0;
     if (free_page && id < live) c.plan.to[id - used_before] = static_cast<int32_t>(id);
+    int32_t rank = -1;
     if (!free_page && id >= live) {
-        // used pages before L: what is used before this one, less its rank among the movers
-        const uint32_t lw = live >> 5, below = live < c.num_blocks ? c.plan.used_before[lw] + static_cast<uint32_t>(__popc(~c.free_mask[lw] & ((1u << (live & 31)) - 1u))) : live;
-        c.plan.from[used_before - below] = static_cast<int32_t>(id);
-        c.plan.rank[id] = static_cast<int32_t>(used_before - below);
-    } else {
-        c.plan.rank[id] = -1;
+        // its rank among the used pages, less those before L
+        const uint32_t lw = live >> 5, below = used_in[lw] + static_cast<uint32_t>(__popc(~c.free_mask[lw] & ((1u << (live & 31)) - 1u)));
+        rank = static_cast<int32_t>(used_before - below);
+        c.plan.from[rank] = static_cast<int32_t>(id);
     }
-    if (id == live || (live == c.num_blocks && id == 0)) {
-        const uint32_t below = live == c.num_blocks ? live : used_before;
-        *c.plan.moves = live - below;
-    }
+    c.plan.rank[id] = rank;
+    if (id == live || (live == c.num_blocks && id == 0)) *c.plan.moves = live == c.num_blocks ? 0 : live - used_before;
 }
 
 // Copies by (move, layer), then table entries and the caller's map.
@@ -430,14 +459,16 @@ int launch_pages_reset(int32_t *refs, uint32_t *mask, uint32_t num_blocks, uint3
 int launch_pages_fork(const PagesFork &f, const PagePlanes &planes, void *stream) {
     const hipStream_t st = static_cast<hipStream_t>(stream);
     const uint32_t lds = f.rows_in * 12;
-    // A thread for each row and each word of 32 pages, as far as 1024 go; more
-    // words a thread only for pools that take several turns otherwise.
-    if (f.rows_in <= 256 && f.rows_out <= 256 && f.num_blocks <= 256 * 32)
-        hipLaunchKernelGGL((pages_fork_plan_kernel<256, 1>), dim3(1), dim3(256), lds, st, f);
+    // A thread for each row and each 8 pages, as far as 1024 go in a few turns,
+    // then 32 and 128 pages a thread.
+    if (f.rows_in <= 256 && f.rows_out <= 256 && f.num_blocks <= 256 * 8)
+        hipLaunchKernelGGL((pages_fork_plan_kernel<256, uint8_t, 1>), dim3(1), dim3(256), lds, st, f);
+    else if (f.num_blocks <= 2 * kPlanThreads * 8)
+        hipLaunchKernelGGL((pages_fork_plan_kernel<kPlanThreads, uint8_t, 1>), dim3(1), dim3(kPlanThreads), lds, st, f);
     else if (f.num_blocks <= 4 * kPlanThreads * 32)
-        hipLaunchKernelGGL((pages_fork_plan_kernel<kPlanThreads, 1>), dim3(1), dim3(kPlanThreads), lds, st, f);
+        hipLaunchKernelGGL((pages_fork_plan_kernel<kPlanThreads, uint32_t, 1>), dim3(1), dim3(kPlanThreads), lds, st, f);
     else
-        hipLaunchKernelGGL((pages_fork_plan_kernel<kPlanThreads, 4>), dim3(1), dim3(kPlanThreads), lds, st, f);
+        hipLaunchKernelGGL((pages_fork_plan_kernel<kPlanThreads, uint32_t, 4>), dim3(1), dim3(kPlanThreads), lds, st, f);
     const uint32_t groups = f.rows_in + f.rows_out + f.rows_out * planes.layers;
     hipLaunchKernelGGL(pages_fork_kernel, dim3(groups), dim3(kWideThreads), 0, st, f, planes);
     return static_cast<int>(hipGetLastError());
@@ -445,8 +476,13 @@ int launch_pages_fork(const PagesFork &f, const PagePlanes &planes, void *stream
 
 int launch_pages_compact(const PagesCompact &c, const PagePlanes &planes, void *stream) {
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(pages_count_kernel, dim3(1), dim3(kPlanThreads), 0, st, c);
-    hipLaunchKernelGGL(pages_moves_kernel, dim3((c.num_blocks + kWideThreads - 1) / kWideThreads), dim3(kWideThreads), 0, st, c);
+    const dim3 moves((c.num_blocks + kWideThreads - 1) / kWideThreads);
+    if (c.num_blocks <= kCountWords * 32) {
+        hipLaunchKernelGGL(pages_moves_kernel<false>, moves, dim3(kWideThreads), 0, st, c);
+    } else {
+        hipLaunchKernelGGL(pages_count_kernel, dim3(1), dim3(kPlanThreads), 0, st, c);
+        hipLaunchKernelGGL(pages_moves_kernel<true>, moves, dim3(kWideThreads), 0, st, c);
+    }
     const uint64_t copies = static_cast<uint64_t>(c.num_blocks / 2 + 1) * planes.layers, entries = static_cast<uint64_t>(c.rows) * c.max_blocks + c.num_blocks;
     const uint32_t copy_groups = static_cast<uint32_t>(copies < 2048 ? copies : 2048);
     const uint64_t tables = (entries + kWideThreads - 1) / kWideThreads;
