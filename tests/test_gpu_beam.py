@@ -217,3 +217,29 @@ def test_another_stream_and_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(d.out, first))
+
+
+def test_rows_beyond_32_bits_of_offset():
+    import torch
+    log("case: beam rows 4 GiB apart")
+    g = np.random.default_rng(12)
+    x, stride = logits_of(g, 2, 5000), (1 << 30) + 5
+    d = Device(1, 2, 5000, 4)
+    args = d.args(x, np.array([[-1.0, -2.0]]))
+    far = torch.empty(stride + 5000, dtype=torch.float32, device="cuda")
+    far[:5000], far[stride:] = torch.from_numpy(x[0]).cuda(), torch.from_numpy(x[1]).cuda()
+    args.logits, args.row_stride = far.data_ptr(), stride
+    pvlc.beam_select(args)
+    torch.cuda.synchronize()
+    d.check(x, np.array([[-1.0, -2.0]]), None, -1, "far rows")
+
+
+def test_rows_of_one_low_value_but_a_few():
+    """What a constrained step gives: all but a few tokens at one large negative value; every selection is exact."""
+    log("case: beam constrained rows")
+    g = np.random.default_rng(13)
+    x = np.full((4, 20011), -1e9, np.float32)
+    for r in range(4):
+        x[r, g.choice(20011, 3 + 9 * r, replace=False)] = g.standard_normal(3 + 9 * r) * 3
+    for best in (4, 16, 70):
+        Device(2, 2, 20011, best).run(x, -g.random((2, 2)), label=f"best={best}")

@@ -266,3 +266,69 @@ def test_stream_workspace_and_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(c.out.cpu().double(), first)
+
+
+@CODES
+@WIDTHS
+def test_infinite_and_nan_rows(code, f32):
+    """An appended infinity is held as 65504; a NaN as the e4m3 NaN, which its head's output shows, or as 0."""
+    import torch
+    log(f"case: q8 decode non-finite rows code={code} f32={f32}")
+    c = Case([20, 20, 20], code, f32, seed=71).upload()
+    c.nk[0, 0, 3], c.nv[0, 1, 7] = np.inf, -np.inf
+    c.nk[1, 1, 100], c.nv[1, 0, 64] = np.nan, np.nan
+    ws = workspace(3, c.width * 16)
+    c.launch(c.args(ws, rope=False, rotate_query=False))
+    torch.cuda.synchronize()
+    with np.errstate(invalid="ignore"):
+        want, bound = c.want(rope=False, rotate_query=False)
+    got = c.out.cpu().numpy().astype(np.float64)
+    nan = lambda a: np.where((a & 0x7F) == 0x7F, 0x7F, a) if code == R.E4M3 else a  # noqa: E731
+    for name, d in zip(("key", "value"), c.dev):
+        np.testing.assert_array_equal(nan(d.cpu().numpy()), nan(getattr(c.cache, name)))
+    np.testing.assert_array_equal(c.dev[2].cpu().numpy(), c.cache.exponents)
+    for s in (0, 2):
+        assert (np.abs(got[s] - want[s]) <= bound[s]).all(), s
+    if code == R.INT8:
+        assert (np.abs(got[1] - want[1]) <= bound[1]).all()
+    else:
+        assert np.isnan(got[1, 8:]).all(), "the NaN key reaches every score of its head's group"
+        assert np.isnan(got[1, :8, 64]).all() and not np.isnan(got[1, :8, :64]).any()
+
+
+def test_blocks_beyond_32_bits_of_offset():
+    """A pool whose planes exceed 4 GiB, the sequences in its last blocks."""
+    import torch
+    log("case: q8 decode in planes of more than 4 GiB")
+    c = Case([100, 37], R.E4M3, True, seed=81)
+    blocks = (1 << 20) + 5000
+    far = c.table + (blocks - c.blocks)
+    planes = [torch.zeros(blocks, 2, n, dtype=torch.uint8, device="cuda") for n in (2048, 2048, 2)]
+    for d, a in zip(planes, (c.cache.key, c.cache.value, c.cache.exponents)):
+        d[blocks - c.blocks:] = torch.from_numpy(a).cuda()
+    c.upload()
+    c.dev, c.dtable = planes, torch.from_numpy(far.astype(np.int32)).cuda()
+    ws = workspace(2, c.width * 16)
+    args = c.args(ws)
+    args.num_blocks = blocks
+    c.launch(args)
+    torch.cuda.synchronize()
+    want, bound = c.want()
+    assert (np.abs(c.out.cpu().numpy() - want) <= bound).all()
+    for d, a in zip(planes, (c.cache.key, c.cache.value, c.cache.exponents)):
+        np.testing.assert_array_equal(d[blocks - c.blocks:].cpu().numpy(), a)
+        assert not d[:blocks - c.blocks].any()
+
+
+def test_more_sequences_than_the_walk_numbers():
+    """More ragged sequences than the persistent kernel numbers: a workgroup for each partition."""
+    log("case: q8 decode 2100 sequences")
+    c = Case(np.random.default_rng(5).integers(0, 40, 2100), R.INT8, True, seed=92).upload()
+    ws = workspace(c.n, c.width * 16)
+    c.launch(c.args(ws))
+    c.check("2100 sequences")
+    c = Case([1200] + [3] * 2099, R.INT8, True, seed=93, paged=False)
+    c.upload()
+    ws = workspace(c.n, c.width * 16, 1024)
+    c.launch(c.args(ws, partition=1024))
+    c.check("2100 sequences, a long one")

@@ -268,3 +268,33 @@ def test_a_fork_and_a_compaction_replayed_from_a_graph():
         np.testing.assert_array_equal(t.cpu().numpy(), b.tables)
         b.same(f"replay {i}")
     assert b.error() == 0
+
+
+def test_pages_beyond_32_bits_of_offset_and_rows_behind_the_last():
+    """Planes of more than 4 GiB; rows of the output behind rows_out stay as they were."""
+    import torch
+    log("case: pages in planes of more than 4 GiB")
+    blocks, size = 70000, 65536
+    plane = torch.zeros(1, blocks, size, dtype=torch.uint8, device="cuda")
+    refs, mask = torch.ones(blocks, dtype=torch.int32, device="cuda"), torch.zeros(-(-blocks // 32), dtype=torch.int32, device="cuda")
+    refs[-40:] = 0
+    bits = np.zeros(-(-blocks // 32) * 32, bool)
+    bits[blocks - 40:blocks] = True
+    mask.copy_(dev(np.packbits(bits, bitorder="little").view(np.int32)))
+    nbytes = pvlc.kv_pages_workspace_bytes(blocks, 4)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    pvlc.workspace_init(ws, nbytes)
+    pool = pvlc.kv_page_pool(num_blocks=blocks, max_blocks_per_seq=3, num_layers=1, planes=[plane], ref_counts=refs, free_mask=mask,
+                             workspace=ws, workspace_bytes=nbytes)
+    last = blocks - 50
+    plane[0, last] = torch.arange(size, device="cuda").to(torch.uint8) + 3
+    t, n = dev(np.array([[5, last, -1]], np.int32)), dev(np.array([20], np.int32))
+    out, lens = torch.full((5, 3), 44, dtype=torch.int32, device="cuda"), torch.full((5,), 44, dtype=torch.int32, device="cuda")
+    pvlc.kv_pages_fork(pool, rows_in=1, rows_out=3, tables_in=t, lens_in=n, tables_out=out, lens_out=lens, parents=dev(np.zeros(3, np.int32)))
+    torch.cuda.synchronize()
+    first = blocks - 40
+    np.testing.assert_array_equal(out.cpu().numpy(), [[5, last, -1], [5, first, -1], [5, first + 1, -1], [44] * 3, [44] * 3])
+    np.testing.assert_array_equal(lens.cpu().numpy(), [20, 20, 20, 44, 44])
+    assert torch.equal(plane[0, first], plane[0, last]) and torch.equal(plane[0, first + 1], plane[0, last])
+    assert not plane[0, first + 2:].any() and not plane[0, :last].any()
+    assert pvlc.workspace_error(ws, nbytes) == 0
