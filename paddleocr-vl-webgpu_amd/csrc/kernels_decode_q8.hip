@@ -526,6 +526,10 @@ __global__ __launch_bounds__(WAVES * 64, 2) void paged_decode_q8_kernel(uint16_t
     p.num_blocks = num_blocks;
     p.partition_tokens = partition_and_parts & 0xffffu;
     p.max_parts = partition_and_parts >> 16;
+    // The pointers of the small operands in the first round of scalar loads.
+    asm volatile("" ::"s"(p.positions), "s"(p.rope_cos), "s"(p.rope_sin), "s"(p.rope_rows));
+    if constexpr (F32IO) asm volatile("" ::"s"(p.query32), "s"(p.new_key32), "s"(p.new_value32));
+    else asm volatile("" ::"s"(p.query), "s"(p.new_key), "s"(p.new_value));
     const uint32_t part = blockIdx.x, g = blockIdx.y, s = blockIdx.z;
     if ((part | g | s) == 0 && p.partition_word != nullptr && threadIdx.x == 0) {
         p.partition_word[0] = p.partition_tokens;
