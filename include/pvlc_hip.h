@@ -682,8 +682,8 @@ typedef struct pvlc_hip_kv_fork_args {
     const int32_t *lens_in;   /* [rows_in] */
     const int32_t *parents;   /* [rows_out], -1..rows_in-1; NULL: row r continues row r, or is new from rows_in on */
     const int32_t *reserve;   /* [rows_out] tokens, or NULL: reserve_tokens each */
-    int32_t *tables_out;      /* [rows_out][max_blocks_per_seq], apart from tables_in */
-    int32_t *lens_out;        /* [rows_out], apart from lens_in */
+    int32_t *tables_out;      /* [rows_out][max_blocks_per_seq], apart from every input */
+    int32_t *lens_out;        /* [rows_out], likewise */
     uint32_t reserve_tokens;
     uint32_t appended;    /* rows appended to every input row since lens_in was written */
     uint32_t keep_inputs; /* the input rows stay: every child's partly filled block is a copy */
@@ -799,8 +799,9 @@ pvlc_hip_status pvlc_hip_lm_head_top1_f16(const uint16_t *weights, const float *
  * beam, then by logit (as the greedy top-1 orders them), then by token.  A row with finished[r] continues with end_token
  * alone at its score; a row whose score is -inf or NaN does not continue; its
  * logits are not read in either case.  A logit below -2^127 (-inf and the type's
- * lowest value among them) or NaN masks its token, one above 2^127 counts as 2^127.  Where there are fewer candidates than
- * `best`, the rest have score -inf, parent and token -1 and are not finished.
+ * lowest value among them) or NaN masks its token, one above 2^127 counts as
+ * 2^127.  Where there are fewer candidates than `best`, the rest have score
+ * -inf, parent and token -1 and are not finished.
  * parents is what pvlc_hip_kv_pages_fork takes.  Logits are f32 rows row_stride
  * apart (4-byte aligned); 1 <= beams <= 64, 1 <= best <= 128. */
 typedef struct pvlc_hip_beam_args {
@@ -813,11 +814,11 @@ typedef struct pvlc_hip_beam_args {
     const float *scores;     /* [batch][beams] */
     const int32_t *finished; /* [batch][beams] or NULL */
     int32_t end_token;       /* -1: none */
-    float *next_scores;      /* [batch][best], as the outputs below; none may overlap scores or finished */
+    float *next_scores;      /* [batch][best], as the outputs below; none may overlap an input */
     int32_t *parents;
     int32_t *tokens;
     int32_t *next_finished; /* or NULL */
-    void *workspace;        /* pvlc_hip_beam_workspace_bytes, 256-byte aligned, zeroed once; calls on it are ordered */
+    void *workspace;        /* pvlc_hip_beam_workspace_bytes, 256-byte aligned, of any content; calls on it are ordered */
     size_t workspace_bytes;
 } pvlc_hip_beam_args;
 size_t pvlc_hip_beam_workspace_bytes(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t best);

@@ -265,6 +265,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_segment_kernel(BeamSelect b
     __shared__ double sm_sum[kBeamThreads / 64];
     const uint32_t segment = blockIdx.x, row = blockIdx.y, i = threadIdx.x;
     constexpr uint32_t kSegment = kEach * kBeamThreads;
+    // The join's counters, whatever the workspace held: calls of other shapes lay it out differently.
+    if (segment == 0 && row < b.batch && i == 0) b.arrived[row] = 0;
     if (!row_alive(b, row) || row_finished(b, row)) return;  // uniform; the row's join reads nothing then
     const float *x = b.logits + static_cast<uint64_t>(row) * b.row_stride;
     const uint32_t first = segment * kSegment;
@@ -449,7 +451,6 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
         if (i == 0) sm_last = __hip_atomic_fetch_add(b.arrived + entry, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == b.beams - 1;
         __syncthreads();
         if (!sm_last) return;
-        if (i == 0) __hip_atomic_store(b.arrived + entry, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         const uint64_t all = static_cast<uint64_t>(b.beams) * b.best;
         auto scores = [&](uint64_t k) { return load_agent(b.row_keys + rows_at + k); };
 #pragma unroll

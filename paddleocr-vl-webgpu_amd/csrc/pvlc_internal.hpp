@@ -533,7 +533,7 @@ struct BeamSelect {
     int32_t end_token;
     float *next_scores;
     int32_t *parents, *tokens, *next_finished;
-    uint32_t *arrived;    // by batch entry; 0 before and after a launch
+    uint32_t *arrived;    // by batch entry: rows joined; the segments' launch clears them
     uint64_t *keys;       // [row][rank][segment]
     double *sums;         // [row][segment], relative to exp(reference)
     float *references;    // [row][segment]

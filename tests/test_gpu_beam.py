@@ -76,7 +76,6 @@ class Device:
         pvlc.beam_select(args)
         torch.cuda.synchronize()
         self.check(logits, scores, finished, end, label)
-        assert not self.ws[:256 * -(-self.shape[0] // 64)].any(), "the counters come back as 0"
 
     def check(self, logits, scores, finished, end, label):
         want, gap = plain(logits, np.asarray(scores, np.float32), self.shape[3], finished, end)
@@ -243,3 +242,38 @@ def test_rows_of_one_low_value_but_a_few():
         x[r, g.choice(20011, 3 + 9 * r, replace=False)] = g.standard_normal(3 + 9 * r) * 3
     for best in (4, 16, 70):
         Device(2, 2, 20011, best).run(x, -g.random((2, 2)), label=f"best={best}")
+
+
+def test_calls_of_other_shapes_share_a_workspace():
+    """A workspace of any content, used by selections whose layouts of it differ, eagerly and from two graphs."""
+    import torch
+    log("case: beam shapes on one workspace")
+    g = np.random.default_rng(14)
+    wide, deep = Device(130, 2, 300, 4), Device(1, 8, 40000, 16)
+    ws = torch.full((max(wide.nbytes, deep.nbytes),), 0xA5, dtype=torch.uint8, device="cuda")
+    runs = []
+    for d in (wide, deep):
+        d.ws, d.nbytes = ws, ws.numel()
+        batch, beams, vocab, _ = d.shape
+        x, s = logits_of(g, batch * beams, vocab), -g.random((batch, beams))
+        args = d.args(x, s, end=7)
+        torch.cuda.synchronize()
+        runs.append((d, args, x, s, torch.cuda.CUDAGraph()))
+    for d, args, x, s, _ in runs + runs:
+        for o in d.out:
+            o.fill_(55)
+        pvlc.beam_select(args)
+        torch.cuda.synchronize()
+        d.check(x, s, None, 7, f"batch {d.shape[0]}")
+    for d, args, _, _, graph in runs:
+        with torch.cuda.graph(graph):
+            pvlc.beam_select(args, torch.cuda.current_stream())
+    for _ in range(3):
+        for d, _, _, _, graph in runs:
+            for o in d.out:
+                o.fill_(55)
+            graph.replay()
+        torch.cuda.synchronize()
+        for d, args, x, s, _ in runs:
+            d.check(x, s, None, 7, f"batch {d.shape[0]}, replayed")
+            pvlc.beam_select(args)
