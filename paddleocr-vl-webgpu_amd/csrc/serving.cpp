@@ -10,6 +10,9 @@ using namespace pvlc;
 
 namespace {
 
+// Workgroups of 256 threads that a launch may have (below 2^32 threads).
+constexpr uint64_t kMaxGroups = 1u << 24;
+
 bool aligned(const void *p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
 pvlc_hip_status check_codes(uint32_t code, const void *keys, const void *values, const void *exponents) {
@@ -57,6 +60,7 @@ pvlc_hip_status check_rows(const void *keys, const void *values, uint64_t end, u
     if (!aligned(keys, 2) || !aligned(values, 2)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "fp16 rows must be 2-byte aligned");
     if (tokens == 0 || num_blocks == 0) return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "tokens and blocks must be nonzero");
     if (end > 0xFFFFFFF0ull) return invalid(PVLC_HIP_INV_ARITHMETIC_OVERFLOW, "the last token exceeds 32 bits");
+    if (end / kBlockTokens >= kMaxGroups - 1) return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "the blocks of a move exceed the grid");
     if (!table && (end + kBlockTokens - 1) / kBlockTokens > num_blocks)
         return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "tokens exceed the contiguous blocks");
     return PVLC_HIP_OK;
@@ -89,6 +93,7 @@ pvlc_hip_status check_pool(const pvlc_hip_kv_pool *pool, uint32_t rows, PagePlan
         if (p.block_bytes > 0x7FFFFFFFull) return invalid(PVLC_HIP_INV_ARITHMETIC_OVERFLOW, "a page's part of a plane exceeds 2^31 - 1 bytes");
         if (pool->num_layers > 1 && p.layer_stride_bytes < p.block_bytes * pool->num_blocks)
             return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "layers of page plane " + std::to_string(i) + " overlap");
+        if (p.layer_stride_bytes > UINT64_MAX / 65536u) return invalid(PVLC_HIP_INV_ARITHMETIC_OVERFLOW, "the layers of a page plane exceed 64 bits");
         const bool wide = aligned(p.base, 16) && p.block_bytes % 16 == 0 && p.layer_stride_bytes % 16 == 0;
         planes->plane[i] = {static_cast<uint8_t *>(p.base), nullptr, p.block_bytes, p.layer_stride_bytes, wide, 0};
     }
@@ -166,13 +171,22 @@ pvlc_hip_status pvlc_hip_kv_pages_fork(const pvlc_hip_kv_pool *pool, const pvlc_
     for (const void *p : {static_cast<const void *>(args->tables_in), static_cast<const void *>(args->lens_in), static_cast<const void *>(args->parents),
                           static_cast<const void *>(args->reserve), static_cast<const void *>(args->tables_out), static_cast<const void *>(args->lens_out)})
         if (!aligned(p, 4)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "fork tables, lengths, parents and reserve must be 4-byte aligned");
-    const uint64_t width = static_cast<uint64_t>(pool->max_blocks_per_seq) * 4;
-    if (overlap(args->tables_in, args->rows_in * width, args->tables_out, args->rows_out * width) ||
-        overlap(args->lens_in, args->rows_in * 4ull, args->lens_out, args->rows_out * 4ull))
-        return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "a fork's output tables and lengths may not overlap its input's");
     // A workgroup of 256 threads for each row and for each (row, layer).
-    if (static_cast<uint64_t>(args->rows_out) * pool->num_layers + args->rows_in + args->rows_out >= 1u << 24)
+    if (static_cast<uint64_t>(args->rows_out) * pool->num_layers + args->rows_in + args->rows_out >= kMaxGroups)
         return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows times layers of a fork exceed the grid");
+    const uint64_t width = static_cast<uint64_t>(pool->max_blocks_per_seq) * 4;
+    const struct {
+        const void *at;
+        uint64_t bytes;
+    } in[] = {{args->tables_in, args->rows_in * width},
+              {args->lens_in, args->rows_in * 4ull},
+              {args->parents, args->parents ? args->rows_out * 4ull : 0},
+              {args->reserve, args->reserve ? args->rows_out * 4ull : 0}};
+    for (const auto &i : in)
+        if (overlap(i.at, i.bytes, args->tables_out, args->rows_out * width) || overlap(i.at, i.bytes, args->lens_out, args->rows_out * 4ull))
+            return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "a fork's output tables and lengths may not overlap its inputs");
+    if (overlap(args->tables_out, args->rows_out * width, args->lens_out, args->rows_out * 4ull))
+        return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "a fork's output tables and lengths may not overlap");
     auto *base = static_cast<unsigned char *>(pool->workspace);
     PagesFork f{};
     f.num_blocks = pool->num_blocks;
@@ -227,7 +241,7 @@ pvlc_hip_status pvlc_hip_kv_pages_copy(const pvlc_hip_kv_pool *from, const int32
     if (pvlc_hip_status st = check_pool(from, 0, &source, &ws)) return st;
     if (pvlc_hip_status st = check_pool(to, 0, &planes, &ws)) return st;
     if (count == 0) return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "a copy of pages needs pairs");
-    if (count >= 1u << 24) return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "a copy of pages takes below 2^24 pairs");
+    if (count >= kMaxGroups) return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "a copy of pages takes below 2^24 pairs");
     if (!from_blocks || !to_blocks || !aligned(from_blocks, 4) || !aligned(to_blocks, 4))
         return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "page lists must be given and 4-byte aligned");
     if (source.count != planes.count || source.layers != planes.layers)
@@ -258,7 +272,7 @@ pvlc_hip_status pvlc_hip_beam_select_f32(const pvlc_hip_beam_args *args, void *s
         return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "below 2^31 logits a row and at most 65535 rows");
     const uint64_t rows = static_cast<uint64_t>(args->batch) * args->beams;
     const uint32_t each = beam_each(rows, args->vocab), segments = (args->vocab - 1) / (each * kBeamThreads) + 1;
-    if (segments * rows >= 1u << 24)
+    if (segments * rows >= kMaxGroups)
         return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows times vocab of a beam selection exceed the grid");
     if (args->row_stride < args->vocab) return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "rows of logits overlap");
     if (!args->logits || !args->scores || !args->next_scores || !args->parents || !args->tokens || !args->workspace)
@@ -267,11 +281,13 @@ pvlc_hip_status pvlc_hip_beam_select_f32(const pvlc_hip_beam_args *args, void *s
                           static_cast<const void *>(args->next_scores), static_cast<const void *>(args->parents), static_cast<const void *>(args->tokens),
                           static_cast<const void *>(args->next_finished)})
         if (!aligned(p, 4)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "beam buffers must be 4-byte aligned");
-    const uint64_t in = static_cast<uint64_t>(args->batch) * args->beams * 4, out = static_cast<uint64_t>(args->batch) * args->best * 4;
+    if (args->row_stride > UINT64_MAX / 8 / rows) return invalid(PVLC_HIP_INV_ARITHMETIC_OVERFLOW, "the rows of logits exceed 64 bits");
+    const uint64_t in = rows * 4, out = static_cast<uint64_t>(args->batch) * args->best * 4, read = ((rows - 1) * args->row_stride + args->vocab) * 4;
     for (const void *p : {static_cast<const void *>(args->next_scores), static_cast<const void *>(args->parents), static_cast<const void *>(args->tokens),
                           static_cast<const void *>(args->next_finished)})
-        if (overlap(p, p ? out : 0, args->scores, in) || overlap(p, p ? out : 0, args->finished, args->finished ? in : 0))
-            return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "the selection's outputs may not overlap its scores or finished flags");
+        if (overlap(p, p ? out : 0, args->scores, in) || overlap(p, p ? out : 0, args->finished, args->finished ? in : 0) ||
+            overlap(p, p ? out : 0, args->logits, read))
+            return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "the selection's outputs may not overlap its logits, scores or finished flags");
     const BeamWorkspace ws = beam_workspace_layout(args->batch, args->beams, args->vocab, args->best);
     if (args->workspace_bytes < ws.total)
         return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "beam workspace holds " + std::to_string(args->workspace_bytes) + " bytes but the call needs " +

@@ -175,3 +175,25 @@ def test_null_argument_structs_refuse():
                        ("pvlc_hip_kv_pages_compact", (null, null, 0, null, null)), ("pvlc_hip_kv_pages_copy", (null, P, null, P, 1, null))):
         status = getattr(pvlc.lib, name)(*args)
         assert status == (3 << 8 | 2), name
+
+
+def test_outputs_over_any_input_refuse():
+    """What a call reads may not lie under what it writes, whichever operand it is."""
+    for change in (dict(parents=2 * P), dict(reserve=2 * P + 8), dict(lens_in=2 * P + 32), dict(tables_out=3 * P, lens_out=3 * P + 60)):
+        refused(fork(**{"tables_out": 2 * P, "lens_out": 4 * P, **change}), "InvalidActivationLayout")
+    base = dict(batch=2, beams=4, vocab=1000, best=4, logits=P * 16, scores=P * 2, next_scores=P * 5, parents=P * 6, tokens=P * 7, workspace=P * 8,
+                workspace_bytes=1 << 26)
+    for change in (dict(tokens=P * 16), dict(next_scores=P * 16 + 7 * 4000 + 3996), dict(parents=P * 17, row_stride=(P + 2000) // 4)):
+        refused(lambda: pvlc.beam_select(pvlc.beam_select_args(**{**base, **change})), "InvalidActivationLayout")
+
+
+def test_sizes_beyond_the_grid_or_64_bits_refuse():
+    move = dict(key_rows=P, value_rows=P, key_cache=P, value_cache=P, exponents=P, num_blocks=1 << 31, code=pvlc.KV_INT8)
+    for table in (None, P):
+        refused(lambda: pvlc.kv_pack_q8(tokens=1 << 28, block_table=table, **move), "InvalidDecoderGeometry")
+        refused(lambda: pvlc.kv_pack_q8(tokens=100, first_token=1 << 28, block_table=table, **move), "InvalidDecoderGeometry")
+        refused(lambda: pvlc.kv_unpack_q8(tokens=1 << 28, block_table=table, **move), "InvalidDecoderGeometry")
+    refused(lambda: pvlc.kv_pages_reset(pool(planes=[(P, 4096, 1 << 60)])), "ArithmeticOverflow")
+    refused(lambda: pvlc.beam_select(pvlc.beam_select_args(
+        batch=2, beams=4, vocab=1000, best=4, logits=P, scores=P * 2, next_scores=P * 5, parents=P * 6, tokens=P * 7, workspace=P * 8,
+        workspace_bytes=1 << 26, row_stride=1 << 60)), "ArithmeticOverflow")
