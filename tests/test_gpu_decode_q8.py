@@ -332,3 +332,55 @@ def test_more_sequences_than_the_walk_numbers():
     ws = workspace(c.n, c.width * 16, 1024)
     c.launch(c.args(ws, partition=1024))
     c.check("2100 sequences, a long one")
+
+
+@CODES
+@WIDTHS
+@pytest.mark.parametrize("partition", [400, 512, 528, 640, 768])
+def test_the_widest_workgroups(code, f32, partition):
+    """Eight and twelve waves of 64 tokens, partitions that end inside the last wave's."""
+    log(f"case: q8 decode partition={partition} code={code} f32={f32}")
+    c = Case([partition * 2 + 70, partition, partition - 1, 0], code, f32, seed=partition + code).upload()
+    ws = workspace(4, c.width * 16, partition)
+    c.launch(c.args(ws, partition=partition))
+    c.check(f"P={partition}")
+    assert pvlc.workspace_error(*ws) == 0
+
+
+@pytest.mark.parametrize("n,t", [(18, 4000), (8, 6500), (4, 6000)])
+def test_one_round_of_long_caches(n, t):
+    """Lengths at which the automatic partition of a uniform launch takes six, eight and twelve waves."""
+    log(f"case: q8 decode {n} caches of {t} rows")
+    c = Case([t] * n, R.E4M3 if n == 18 else R.INT8, n == 4, seed=t, paged=n != 18).upload()
+    ws = workspace(n, c.width * 16)
+    c.launch(c.args(ws, ragged=False))
+    c.check(f"{n} x {t}")
+
+
+def test_two_graphs_share_a_workspace():
+    """Captured launches of different shapes (single, ragged, streaming) on one workspace, replayed in turn."""
+    import torch
+    log("case: q8 decode two graphs")
+    cases = [Case([500, 33, 900], R.E4M3, True, seed=71).upload(), Case([1157], R.INT8, False, seed=72).upload(),
+             Case(np.random.default_rng(73).integers(0, 600, 70), R.INT8, True, seed=73).upload()]
+    ws = workspace(70, 37 * 16, 32)  # the largest of the three
+    runs = []
+    for c in cases:
+        partition = 32 if c.n == 70 else 0
+        assert pvlc.decode_workspace_bytes(c.n, c.width * 16, partition) <= ws[1]
+        args = c.args(ws, ragged=c.n > 1, partition=partition)
+        c.launch(args)
+        c.check(f"{c.n} sequences, eager")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c.launch(args, torch.cuda.current_stream())
+        runs.append((c, args, graph, c.out.clone()))
+    for i in range(4):
+        for c, _, graph, _ in runs:
+            c.out.zero_()
+            graph.replay()
+        torch.cuda.synchronize()
+        for c, args, _, first in runs:
+            assert torch.equal(c.out, first), f"replay {i}, {c.n} sequences"
+            c.launch(args)
+    assert pvlc.workspace_error(*ws) == 0

@@ -298,3 +298,58 @@ def test_pages_beyond_32_bits_of_offset_and_rows_behind_the_last():
     assert torch.equal(plane[0, first], plane[0, last]) and torch.equal(plane[0, first + 1], plane[0, last])
     assert not plane[0, first + 2:].any() and not plane[0, :last].any()
     assert pvlc.workspace_error(ws, nbytes) == 0
+
+
+def test_a_pool_of_more_pages_than_one_turn_names():
+    """140000 pages: four words of the mask a thread, and free pages in more than one turn of the workgroup."""
+    log("case: pages in a pool of 140000")
+    b, g = Both(140000, 70, layers=1, sizes=(4,), rows=2600), np.random.default_rng(9)
+    b.step(2000, "admission", parents=np.full(2000, -1), reserve=1100)
+    b.lens = g.integers(0, 1100, 2000).astype(np.int32)
+    b.step(1500, "reorder and truncation", parents=g.integers(-1, 2000, 1500), reserve=20)
+    b.lens = np.minimum(b.lens + 20, 70 * 16).astype(np.int32)
+    b.compact("compaction")
+    b.step(2600, "fan-out", parents=g.integers(0, 1500, 2600), reserve=1)
+    b.step(3, "most are freed")
+    b.step(3, "one new, one twice", parents=[-1, 0, 0], reserve=16)
+
+
+def test_two_graphs_share_a_pool():
+    """A fork out, and a fork back with a compaction, captured apart on one workspace and replayed in turn."""
+    import torch
+    log("case: pages two graphs")
+    b = Both(60, 4, rows=8)
+    b.step(2, "admission", parents=[-1, -1], reserve=[30, 17])
+    b.lens = np.array([30, 17], np.int32)
+    t, n = dev(b.tables), dev(b.lens)
+    t_out, n_out = torch.zeros((5, 4), dtype=torch.int32, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda")
+    parents = dev(np.array([1, 0, 1, 0, 0], np.int32))
+
+    def out(stream):
+        pvlc.kv_pages_fork(b.pool, rows_in=2, rows_out=5, tables_in=t, lens_in=n, tables_out=t_out, lens_out=n_out, parents=parents,
+                           reserve_tokens=1, keep_inputs=True, stream=stream)
+
+    def back(stream):
+        pvlc.kv_pages_fork(b.pool, rows_in=5, rows_out=0, tables_in=t_out, lens_in=n_out, stream=stream)
+        pvlc.kv_pages_compact(b.pool, rows=2, tables=t, stream=stream)
+
+    graphs = []
+    torch.cuda.synchronize()
+    for call in (out, back):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(torch.cuda.current_stream())
+        graphs.append(graph)
+    for i in range(4):
+        graphs[0].replay()
+        torch.cuda.synchronize()
+        want = b.ref.fork(b.tables, b.lens, 5, [1, 0, 1, 0, 0], 1, 0, True)
+        np.testing.assert_array_equal(t_out.cpu().numpy(), want[0])
+        b.same(f"out {i}")
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        b.ref.fork(want[0], want[1], 0)
+        b.tables, _ = b.ref.compact(b.tables)
+        np.testing.assert_array_equal(t.cpu().numpy(), b.tables)
+        b.same(f"back {i}")
+    assert b.error() == 0
