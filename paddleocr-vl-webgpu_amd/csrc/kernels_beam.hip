@@ -17,6 +17,16 @@
 // The best n of many without sorting them: with the values dealt to groups of
 // threads, the n-th largest of the groups' own largest is a bound that at least n
 // values reach and few others, so a short list remains, whose ranks are counted.
+//
+// Measured: four rows of 103424 logits, four candidates: segments 3.7-4.7 us, join
+// 5.5-6.0 (1.65 MB; both are a launch and a chain of rounds through memory and
+// barriers).  128 rows, a fifth of them finished, sixteen candidates of eight rows
+// each: segments 11.1-12.4 us (42 MB, 3.4-3.8 TB/s: a row's loads, exponentials and
+// selection follow one another in each workgroup, and little more than one round
+// of workgroups covers the other's waits), join 7.7-8.4.  One launch for both, the
+// last segment of a row joining it, took 11.7 and 32.6 us a call against 9.9 and
+// 22.9: each segment then waits for its stores and an atomic, and the join's
+// registers are every segment's.
 
 #include <hip/hip_runtime.h>
 
@@ -41,7 +51,7 @@ __device__ inline int32_t order_of(float x) {
     return bits ^ ((bits >> 31) & 0x7FFFFFFF);
 }
 __device__ inline float value_of(int32_t order) { return __int_as_float(order ^ ((order >> 31) & 0x7FFFFFFF)); }
-constexpr int32_t kMaskedOrder = static_cast<int32_t>((0xFF000000u ^ 0x7FFFFFFFu) - 1u);  // just below that of -2^127
+constexpr int32_t kLeastOrder = static_cast<int32_t>(0xFF000000u ^ 0x7FFFFFFFu);  // of -2^127
 
 __device__ inline uint64_t key_of(int32_t order, uint32_t token) {
     return static_cast<uint64_t>(static_cast<uint32_t>(order) ^ 0x80000000u) << 32 | (0xFFFFFFFFu - token);
@@ -182,16 +192,17 @@ __device__ inline uint32_t best_exact(uint32_t best, BestLds &lds, uint64_t *lis
     return min(n, best);
 }
 
-// The `best` largest keys of the workgroup, put(rank, key) for each: order(e) and
-// key(e) are the thread's e-th (kNoOrder and kNoKey: none), most its largest
-// order.  Returns how many there are.  Every thread calls it; LDS is free for the
+// The `best` largest keys of the workgroup, put(rank, key) for each: key(e) is the
+// thread's e-th (kNoKey: none), most its largest order, reaches(bound)(e) whether
+// the e-th has at least that order (kNoOrder: none; where orders are near, more may
+// be said to, and are listed).  Returns how many there are.  Every thread calls it; LDS is free for the
 // next call after a barrier.
 //
 // The bound is the `best`-th largest of the groups' largest orders, 32 bits; what
 // reaches it is listed and ranked by whole keys.  32 groups of 8 threads for up
 // to 16 wanted, 64 of 4 for up to 64, else each thread.
-template <uint32_t kEach, class Order, class Key, class Put>
-__device__ inline uint32_t best_of(int32_t most, uint32_t best, BestLds &lds, uint64_t *list, uint32_t room, Order order, Key key, Put put) {
+template <uint32_t kEach, class Reaches, class Key, class Put>
+__device__ inline uint32_t best_of(int32_t most, uint32_t best, BestLds &lds, uint64_t *list, uint32_t room, Reaches reaches, Key key, Put put) {
     const uint32_t i = threadIdx.x;
     const uint32_t lane = i & 63;
     if (i == 0) lds.count = 0;
@@ -227,20 +238,21 @@ __device__ inline uint32_t best_of(int32_t most, uint32_t best, BestLds &lds, ui
         members += static_cast<uint32_t>(__popcll(__ballot(in)));
         if (in) bound = min(bound, mine);
     }
-    bound = members >= best ? wave_least(bound) : kNoOrder + 1;  // or everything
+    const auto in_list = reaches(members >= best ? wave_least(bound) : kNoOrder + 1);  // or everything
     uint32_t here = 0;
 #pragma unroll
-    for (uint32_t e = 0; e < kEach; ++e) here += static_cast<uint32_t>(__popcll(__ballot(order(e) >= bound)));
+    for (uint32_t e = 0; e < kEach; ++e) here += static_cast<uint32_t>(__popcll(__ballot(in_list(e))));
     if (here != 0) {  // uniform over the wave
         uint32_t at = 0;
         if (lane == 0) at = atomicAdd(&lds.count, here);
         at = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(at)));
 #pragma unroll
         for (uint32_t e = 0; e < kEach; ++e) {
-            const uint64_t mask = __ballot(order(e) >= bound);
+            const bool mine = in_list(e);
+            const uint64_t mask = __ballot(mine);
             if (mask == 0) continue;
             const uint32_t place = at + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), 0));
-            if (order(e) >= bound && place < room) list[place] = key(e);
+            if (mine && place < room) list[place] = key(e);
             at += static_cast<uint32_t>(__popcll(mask));
         }
     }
@@ -256,9 +268,13 @@ __device__ inline uint32_t best_of(int32_t most, uint32_t best, BestLds &lds, ui
 // Keys that best_of lists before it turns to the exact selection.
 constexpr uint32_t best_room(uint32_t best) { return best * 4; }
 
-// Grid (segment, row): kEach * kBeamThreads logits each.
+// Grid (segment, row): kEach * kBeamThreads logits each.  The logits stay values
+// until they are listed: their maximum and what reaches the bound need no more,
+// and NaN and masked ones drop out of both.  (Made whole numbers in order first,
+// 128 rows 22.9 us a call against 22.1; with 70 registers, seven waves a SIMD, 22.1
+// against 21.6.)
 template <uint32_t kEach>
-__global__ __launch_bounds__(kBeamThreads) void beam_segment_kernel(BeamSelect b) {
+__global__ __launch_bounds__(kBeamThreads, 8) void beam_segment_kernel(BeamSelect b) {
     extern __shared__ uint64_t list[];
     __shared__ BestLds lds;
     __shared__ float sm_top[kBeamThreads / 64];
@@ -287,29 +303,25 @@ __global__ __launch_bounds__(kBeamThreads) void beam_segment_kernel(BeamSelect b
     }
     // Largest logit and sum of exponentials of the thread, relative to its own
     // reference.  Logits that need cleaning show in one or the other.
-    int32_t order[kEach], most;
-    float reference, sum;
+    float largest, reference, sum;
     auto scan = [&]() {
-        most = order[0] = order_of(v[0]);
+        largest = v[0];
 #pragma unroll
-        for (uint32_t e = 1; e < kEach; ++e) {
-            order[e] = order_of(v[e]);
-            most = max(most, order[e]);
-        }
-        reference = most > kMaskedOrder ? value_of(most) : 0.f;
+        for (uint32_t e = 1; e < kEach; ++e) largest = fmaxf(largest, v[e]);
+        reference = largest >= -kMostLogit ? largest : 0.f;
         sum = 0.f;
 #pragma unroll
         for (uint32_t e = 0; e < kEach; ++e) sum += exp_term(v[e], reference);
     };
     scan();
-    if (__any(most > __float_as_int(kMostLogit) || sum != sum)) {
+    if (__any(largest > kMostLogit || sum != sum)) {
 #pragma unroll
         for (uint32_t e = 0; e < kEach; ++e) v[e] = clean(v[e]);
         scan();
     }
     // Joined over the wave here, over the waves by the first thread, behind
     // best_of's barrier.
-    const bool any = most > kMaskedOrder;
+    const bool any = largest >= -kMostLogit;
     const float top = wave_largest(any ? reference : -INFINITY);
     const double total = wave_sum(any ? static_cast<double>(sum * exp_term(reference, top)) : 0.0);
     if ((i & 63) == 0) {
@@ -318,11 +330,14 @@ __global__ __launch_bounds__(kBeamThreads) void beam_segment_kernel(BeamSelect b
     }
     const size_t part = static_cast<size_t>(row) * b.segments + segment;
     uint64_t *out = b.keys + static_cast<size_t>(row) * b.best * b.segments + segment;
-    auto masked = [&](uint32_t e) { return order[e] > kMaskedOrder ? order[e] : kNoOrder; };
     const uint32_t found = best_of<kEach>(
-        any ? most : kNoOrder, b.best, lds, list, best_room(b.best), masked,
+        any ? order_of(largest) : kNoOrder, b.best, lds, list, best_room(b.best),
+        [&](int32_t bound) {  // as values: -0 and +0 are equal then
+            const float least = value_of(max(bound, kLeastOrder));
+            return [&v, least](uint32_t e) { return v[e] >= least; };
+        },
         [&](uint32_t e) {
-            return order[e] > kMaskedOrder ? key_of(order[e], first + ((e >> 2) * kBeamThreads + i) * 4 + (e & 3)) : kNoKey;
+            return v[e] >= -kMostLogit ? key_of(order_of(v[e]), first + ((e >> 2) * kBeamThreads + i) * 4 + (e & 3)) : kNoKey;
         },
         [&](uint32_t rank, uint64_t key) { out[static_cast<size_t>(rank) * b.segments] = key; });
     for (uint32_t k = found + i; k < b.best; k += kBeamThreads) out[static_cast<size_t>(k) * b.segments] = kNoKey;
@@ -380,7 +395,8 @@ __device__ inline void join_keys(uint64_t (&key)[kJoinEach + 1], uint64_t count,
 #pragma unroll
         for (uint32_t e = 0; e <= kJoinEach; ++e) most = max(most, order_in(key[e]));
         const uint32_t found = best_of<kJoinEach + 1>(
-            most, best, lds, list, best_room(best), [&](uint32_t e) { return order_in(key[e]); }, [&](uint32_t e) { return key[e]; },
+            most, best, lds, list, best_room(best), [&](int32_t bound) { return [&key, bound](uint32_t e) { return order_in(key[e]) >= bound; }; },
+            [&](uint32_t e) { return key[e]; },
             [&](uint32_t rank, uint64_t k) { run[rank] = k; });
         for (uint32_t k = found + i; k < best; k += kBeamThreads) run[k] = kNoKey;
         __syncthreads();
