@@ -583,8 +583,10 @@ typedef struct pvlc_hip_paged_decode_q8_args {
  * optionally the query), round the new row into the block at cache_len, attend
  * over cache_len+1 rows as they are held.  Codes enter the matrix products
  * exactly and their powers are applied to f32 scores and weights, so nothing is
- * rounded that the fp16 decode does not round.  Operands, streams, workspace,
- * device error bits and partitions as there. */
+ * rounded that the fp16 decode does not round.  Operands, streams, workspace and
+ * device error bits as there; with partition_tokens 0 the partition is this
+ * decode's own (64..768 tokens in one launch, 512..4096 where it streams) and fits
+ * the workspace that pvlc_hip_paged_decode_workspace_bytes sizes. */
 pvlc_hip_status pvlc_hip_paged_decode_q8_f16(const pvlc_hip_paged_decode_q8_args *args, void *stream);
 /* The same with f32 query, new key and value and output, as
  * pvlc_hip_paged_decode_f32io: the new row is rotated from its f32 values and

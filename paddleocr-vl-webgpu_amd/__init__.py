@@ -9,7 +9,12 @@ Python host mirror of the reference's operator surface, over the C ABI of
   ``run_decoder_cached_gqa`` and ``begin_decoder_kv_session``, and
   :class:`NativeDecoderKvSession` with ``step`` / ``finish``;
 * the device-resident hot path -- :func:`paged_decode_f16`,
-  :func:`paged_prefill_f16`, :func:`kv_pack_f16`, :func:`kv_unpack_f16`.
+  :func:`paged_prefill_f16`, :func:`kv_pack_f16`, :func:`kv_unpack_f16`;
+* serving beside it -- the cache in 8 bits (:func:`paged_decode_q8_f16`,
+  :func:`paged_decode_q8_f32io`, :func:`kv_pack_q8`, :func:`kv_unpack_q8`), its
+  pages (:func:`kv_page_pool`, :func:`kv_pages_fork`, :func:`kv_pages_compact`,
+  :func:`kv_pages_copy`) and the selection of a beam search
+  (:func:`beam_select`).
 
 Names, argument meaning and error behaviour follow the reference; failures
 raise :class:`PvlcHipError` carrying the reference's ``RuntimeErrorCode`` and,

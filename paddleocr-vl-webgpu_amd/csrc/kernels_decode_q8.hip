@@ -24,6 +24,18 @@
 // With f32 operands the weights go to P.V as exact pairs of fp16 values (hi + lo,
 // ~22 bits), with fp16 operands, whose output rounds as coarsely, as single ones
 // (the pair costs 0.2-0.3 us of a launch's 8 to 10, 5 of 260).
+//
+// What bounds it.  512 bytes a token and 8192 operations: memory, once a launch is
+// long.  256 sequences of 1024 to 32768 rows (1.20 GB): 214-220 us and the merge
+// 8-9, 5.5 TB/s, where a copy reaches 5.1; the fp16 cache's takes 453 us.  Short
+// launches are a chain of rounds: one sequence of 1157 rows 7.5 us, thirteen up to
+// 2010 7.65, 18 caches of 2048 rows (19 MB) 9.1 in e4m3 and 10.1 in int8, whose
+// conversion to fp16 takes more instructions.  Time stamps of the waves
+// put 0.75 us of that into the new row (its rounding and the LDS detour to the
+// wave's own registers), 0.8 into the hand-off and 1.3 into the merge; the rest is
+// the launch, the block ids and one round of loads.  Measured slower and not kept:
+// the merge's loads issued for every slot without a branch, and the new row's codes
+// read from LDS ahead of the loop.
 
 #include <hip/hip_runtime.h>
 

@@ -9,6 +9,14 @@
 // the bits (it needs a prefix sum over the rows and a search over the bits, a
 // few microseconds), and the execution, which every other workgroup does
 // independently: table rows, counts and page copies.
+//
+// Measured, at 18 layers: four beams of a page (2.4 MB copied): plan 3.8 us,
+// execution 3.9, both a chain of rounds; 256 rows (35 MB copied): plan 5.3,
+// execution 9.4; 64 sequences compacted, 4600 pages (up to 1.2 GB read and written):
+// 168-237 us, at the rate of a large copy.  One launch for a small fork, every
+// workgroup making the plan by itself and the last one to have it changing the
+// counts, took four beams 15.3 us in place of 17.2 for two forks from the host,
+// but as long alone, and 24 rows 55 in place of 43: not kept.
 
 #include <hip/hip_runtime.h>
 
@@ -106,7 +114,7 @@ __device__ inline RowRead read_row(const PagesFork &f, uint32_t r, uint32_t *err
 // it; fresh[base ..] are its others.  Everything of a row stays in LDS and
 // registers, and what it needs of the tables is read at once: the launch is a
 // chain of rounds through memory (four beams, rows through memory 5.3 us, reads
-// where they are needed 4.2).  A thread takes a Unit of the mask at a time, bytes
+// where they are needed 4.2, all at once 3.8).  A thread takes a Unit of the mask at a time, bytes
 // of pools that have few: it names its pages one after the other.
 template <int kThreads, class Unit, uint32_t kUnits>
 __global__ __launch_bounds__(kThreads) void pages_fork_plan_kernel(PagesFork f) {
@@ -231,8 +239,8 @@ __global__ __launch_bounds__(kThreads) void pages_fork_plan_kernel(PagesFork f) 
 // Copies a page of one layer, all planes: the first 8 KiB of each plane (16 bytes
 // a thread at a time, 4 where the plane is not made for more) are loaded before
 // anything is stored, what is left of larger blocks in a loop.  (Plane by plane
-// and piece by piece, each store behind its load, 64 sequences' compaction took
-// 297 us.)
+// and piece by piece, each store behind its load, the turnover of 64 sequences took
+// 378 us, so 328; with more workgroups, below, 276.)
 __device__ inline void copy_pages(const PagePlanes &planes, uint32_t layer, uint32_t src, uint32_t dst) {
     const uint32_t i = threadIdx.x;
     u32x4_t v[kMaxPagePlanes][2];

