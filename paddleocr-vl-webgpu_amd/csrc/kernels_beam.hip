@@ -18,15 +18,16 @@
 // threads, the n-th largest of the groups' own largest is a bound that at least n
 // values reach and few others, so a short list remains, whose ranks are counted.
 //
-// Measured: four rows of 103424 logits, four candidates: segments 3.7-4.7 us, join
-// 5.5-6.0 (1.65 MB; both are a launch and a chain of rounds through memory and
-// barriers).  128 rows, a fifth of them finished, sixteen candidates of eight rows
-// each: segments 11.1-12.4 us (42 MB, 3.4-3.8 TB/s: a row's loads, exponentials and
-// selection follow one another in each workgroup, and little more than one round
-// of workgroups covers the other's waits), join 7.7-8.4.  One launch for both, the
-// last segment of a row joining it, took 11.7 and 32.6 us a call against 9.9 and
-// 22.9: each segment then waits for its stores and an atomic, and the join's
-// registers are every segment's.
+// Measured: four rows of 103424 logits, four candidates: segments 3.7-4.6 us, join
+// 5.4-5.8 (1.65 MB; both are a launch and a chain of rounds through memory and
+// barriers: of the join's, by time stamps, loads 0.7, selection 1.6, the hand-off
+// 0.8, loads and selection among the rows 0.9, outputs 0.5).  128 rows, a fifth of
+// them finished, sixteen candidates of eight rows each: segments 11.0-12.4 us (42 MB,
+// 3.4-3.8 TB/s: a row's loads, exponentials and selection follow one another in
+// each workgroup, and little more than one round of workgroups covers the other's
+// waits), join 6.9-7.7.  One launch for both, the last segment of a row joining it,
+// took 11.7 and 32.6 us a call against 9.9 and 22.9: each segment then waits for
+// its stores and an atomic, and the join's registers are every segment's.
 
 #include <hip/hip_runtime.h>
 
@@ -78,9 +79,18 @@ __device__ inline float exp_term(float x, float reference) {
 }
 
 // A beam goes on if its score is above -inf (not NaN), a row of logits is read
-// if the beam is also not finished.
-__device__ inline bool row_finished(const BeamSelect &b, uint32_t row) { return b.finished != nullptr && b.finished[row] != 0; }
-__device__ inline bool row_alive(const BeamSelect &b, uint32_t row) { return b.scores[row] > -INFINITY; }
+// if the beam is also not finished.  Both are read at once (the score once more
+// where there are no flags).
+struct RowState {
+    float start;
+    bool alive, finished;
+};
+__device__ inline RowState row_state(const BeamSelect &b, uint32_t row) {
+    const int32_t *flags = b.finished ? b.finished : reinterpret_cast<const int32_t *>(b.scores);
+    const float start = b.scores[row];
+    const int32_t flag = flags[row];
+    return {start, start > -INFINITY, b.finished != nullptr && flag != 0};
+}
 
 // LDS of best_of, ahead of its short list.
 struct BestLds {
@@ -92,7 +102,8 @@ struct BestLds {
 };
 // Items that the exact selection may list (of four threads for each one wanted,
 // or one where more than 64 are), and room for what is read past the last.
-constexpr uint32_t best_list(uint32_t best, uint32_t each) { return best * each * (best <= 64 ? 4 : 1) + 8; }
+constexpr uint32_t kListPad = 32;
+constexpr uint32_t best_list(uint32_t best, uint32_t each) { return best * each * (best <= 64 ? 4 : 1) + kListPad; }
 constexpr int32_t kNoOrder = INT32_MIN;  // of kNoKey
 
 __device__ inline uint64_t larger_key(uint64_t a, uint64_t b) { return a > b ? a : b; }
@@ -136,13 +147,33 @@ __device__ inline double wave_sum(double v) {
     return (at(0) + at(16)) + (at(32) + at(48));
 }
 
-// Ranks of the n listed keys: put(rank, key) for the `best` largest.
+// Ranks of the n listed keys: put(rank, key) for the `best` largest.  Up to 64 are
+// ranked by four threads each (128 rows by one each: 21.5 us a call against 20.75).
 template <class Put>
 __device__ inline void rank_list(const uint64_t *list, uint32_t n, uint32_t best, Put put) {
+    constexpr uint32_t kShare = 4;
+    if (n <= kBeamThreads / kShare) {  // uniform
+        const uint32_t c = threadIdx.x / kShare, part = threadIdx.x % kShare;
+        if (c >= n) return;
+        const uint64_t mine = list[c];
+        int32_t rank = 0;
+        for (uint32_t j = 0; j < n; j += 8 * kShare) {  // eight reads at a time, the last ones past the end
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) {
+                const uint32_t at = j + u * kShare + part;
+                const uint64_t other = list[at];
+                rank += at < n && other > mine;
+            }
+        }
+        rank += dpp_i32<0xB1>(rank);
+        rank += dpp_i32<0x4E>(rank);
+        if (part == 0 && static_cast<uint32_t>(rank) < best) put(static_cast<uint32_t>(rank), mine);
+        return;
+    }
     for (uint32_t c = threadIdx.x; c < n; c += kBeamThreads) {
         const uint64_t mine = list[c];
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; j += 8) {  // eight reads at a time, the last ones past the end
+        for (uint32_t j = 0; j < n; j += 8) {
 #pragma unroll
             for (uint32_t u = 0; u < 8; ++u) {
                 const uint64_t other = list[j + u];
@@ -279,11 +310,14 @@ __global__ __launch_bounds__(kBeamThreads, 8) void beam_segment_kernel(BeamSelec
     __shared__ BestLds lds;
     __shared__ float sm_top[kBeamThreads / 64];
     __shared__ double sm_sum[kBeamThreads / 64];
+    // Every pointer in one round of scalar loads.
+    asm volatile("" ::"s"(b.logits), "s"(b.row_stride), "s"(b.scores), "s"(b.finished), "s"(b.keys), "s"(b.sums), "s"(b.references), "s"(b.arrived));
     const uint32_t segment = blockIdx.x, row = blockIdx.y, i = threadIdx.x;
     constexpr uint32_t kSegment = kEach * kBeamThreads;
     // The join's counters, whatever the workspace held: calls of other shapes lay it out differently.
     if (segment == 0 && row < b.batch && i == 0) b.arrived[row] = 0;
-    if (!row_alive(b, row) || row_finished(b, row)) return;  // uniform; the row's join reads nothing then
+    const RowState state = row_state(b, row);
+    if (!state.alive || state.finished) return;  // uniform; the row's join reads nothing then
     const float *x = b.logits + static_cast<uint64_t>(row) * b.row_stride;
     const uint32_t first = segment * kSegment;
     float v[kEach];
@@ -367,17 +401,20 @@ __device__ inline uint32_t join_at(uint32_t e) { return e * kBeamThreads + (thre
 
 // The `best` largest of keys(0) .. keys(count - 1) into run, in order, kNoKey
 // behind.  Every thread calls it, with its first keys, keys(join_at(e)); run is
-// complete when it returns.
-template <class Keys>
-__device__ inline void join_keys(uint64_t (&key)[kJoinEach + 1], uint64_t count, uint32_t best, BestLds &lds, uint64_t *list, uint64_t *run, Keys keys) {
+// complete when it returns, and meanwhile() has run once, while the first waves
+// rank a short list.
+template <class Keys, class Meanwhile>
+__device__ inline void join_keys(uint64_t (&key)[kJoinEach + 1], uint64_t count, uint32_t best, BestLds &lds, uint64_t *list, uint64_t *run, Keys keys,
+                                 Meanwhile meanwhile) {
     const uint32_t i = threadIdx.x;
-    if (count <= 64 && count <= best_list(best, kJoinEach + 1) - 8) {  // uniform: few enough to be ranked as they are (128 are not)
+    if (count <= 64 && count <= best_list(best, kJoinEach + 1) - kListPad) {  // uniform: few enough to be ranked as they are (128 are not)
         if (join_at(0) < count) list[join_at(0)] = key[0];
         if (i < best) run[i] = kNoKey;
         __syncthreads();
         rank_list(list, static_cast<uint32_t>(count), best, [&](uint32_t rank, uint64_t k) {
             if (k != kNoKey) run[rank] = k;
         });
+        meanwhile();
         __syncthreads();
         return;
     }
@@ -399,6 +436,7 @@ __device__ inline void join_keys(uint64_t (&key)[kJoinEach + 1], uint64_t count,
             [&](uint32_t e) { return key[e]; },
             [&](uint32_t rank, uint64_t k) { run[rank] = k; });
         for (uint32_t k = found + i; k < best; k += kBeamThreads) run[k] = kNoKey;
+        if (at == 0) meanwhile();
         __syncthreads();
     }
 }
@@ -411,6 +449,10 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
     __shared__ BestLds lds;
     __shared__ uint64_t run[kBeamMaxBest], run_scores[kBeamMaxBest];
     __shared__ int sm_last;
+    __shared__ float sm_most;
+    __shared__ double sm_log_sum;
+    asm volatile("" ::"s"(b.keys), "s"(b.sums), "s"(b.references), "s"(b.scores), "s"(b.finished), "s"(b.row_keys), "s"(b.row_scores), "s"(b.arrived));
+    asm volatile("" ::"s"(b.next_scores), "s"(b.parents), "s"(b.tokens), "s"(b.next_finished));
     const uint32_t row = blockIdx.x, i = threadIdx.x, entry = row / b.beams;
     const size_t part = static_cast<size_t>(row) * b.segments;
     const uint64_t *keys = b.keys + part * b.best;  // [rank][segment]
@@ -422,25 +464,31 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
     const uint32_t lane = i & 63, s0 = min(lane, b.segments - 1);
     const float reference0 = b.references[part + s0];
     const double sum0 = b.sums[part + s0];
-    const float start = b.scores[row];
-    const bool finished = row_finished(b, row), alive = start > -INFINITY;
-    double top = 0.0, log_sum = 0.0;
+    const RowState state = row_state(b, row);
+    const float start = state.start;
+    const bool finished = state.finished, alive = state.alive;
     if (alive && !finished) {  // uniform
 #pragma unroll
         for (uint32_t e = 0; e < kJoinEach; ++e)
             if (join_at(e) >= count) key_in[e] = kNoKey;
-        // Every wave sums the segments by itself.
-        float most = -INFINITY;
-        for (uint32_t s = lane; s < b.segments; s += 64) most = fmaxf(most, s == lane ? reference0 : b.references[part + s]);
-        most = wave_largest(most);
-        if (most > -INFINITY) {  // uniform: something is not masked
-            top = most;
-            double sum = 0.0;
-            for (uint32_t s = lane; s < b.segments; s += 64)
-                sum += (s == lane ? sum0 : b.sums[part + s]) * exp(static_cast<double>(s == lane ? reference0 : b.references[part + s]) - top);
-            log_sum = log(wave_sum(sum));
-        }
-        join_keys(key_in, count, b.best, lds, list, run, [&](uint64_t k) { return keys[k]; });
+        join_keys(key_in, count, b.best, lds, list, run, [&](uint64_t k) { return keys[k]; }, [&]() {
+            if (i < kBeamThreads - 64) return;
+            // The last wave sums the segments (0.65 us, of which the ranks cover a half).
+            float most = -INFINITY;
+            for (uint32_t s = lane; s < b.segments; s += 64) most = fmaxf(most, s == lane ? reference0 : b.references[part + s]);
+            most = wave_largest(most);
+            double log_sum = 0.0;
+            if (most > -INFINITY) {  // uniform: something is not masked
+                double sum = 0.0;
+                for (uint32_t s = lane; s < b.segments; s += 64)
+                    sum += (s == lane ? sum0 : b.sums[part + s]) * exp(static_cast<double>(s == lane ? reference0 : b.references[part + s]) - most);
+                log_sum = log(wave_sum(sum));
+            }
+            if (lane == 0) {
+                sm_most = most;
+                sm_log_sum = log_sum;
+            }
+        });
     } else {
         for (uint32_t k = i; k < b.best; k += kBeamThreads)
             run[k] = alive && k == 0 ? key_of(0, static_cast<uint32_t>(b.end_token)) : kNoKey;
@@ -452,7 +500,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
     double score = 0.0;
     if (i < b.best) {
         key = run[i];
-        score = finished ? static_cast<double>(start) : start + ((static_cast<double>(value_of(order_in(key))) - top) - log_sum);
+        score = finished ? static_cast<double>(start) : start + ((static_cast<double>(value_of(order_in(key))) - static_cast<double>(sm_most)) - sm_log_sum);
         if (key != kNoKey) scored = score_key(score, beam * b.best + i);
     }
     const size_t rows_at = static_cast<size_t>(entry) * b.beams * b.best, at = rows_at + static_cast<size_t>(i) * b.beams + beam;  // [rank][beam]
@@ -471,7 +519,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
         auto scores = [&](uint64_t k) { return load_agent(b.row_keys + rows_at + k); };
 #pragma unroll
         for (uint32_t e = 0; e < kJoinEach; ++e) key_in[e] = join_at(e) < all ? scores(join_at(e)) : kNoKey;
-        join_keys(key_in, all, b.best, lds, list, run_scores, scores);
+        join_keys(key_in, all, b.best, lds, list, run_scores, scores, []() {});
         if (i >= b.best) return;
         scored = run_scores[i];
     }
@@ -490,7 +538,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
             token = static_cast<int32_t>(token_in(key));
             value = static_cast<float>(score);
         }
-        ended = token == b.end_token || row_finished(b, static_cast<uint32_t>(parent));
+        ended = token == b.end_token || (b.finished != nullptr && b.finished[parent] != 0);
     }
     b.next_scores[o] = value;
     b.parents[o] = parent;
