@@ -148,3 +148,64 @@ def test_rows_at_odd_addresses_and_on_another_stream():
         for a, b in zip(dev.unpack(37, None, offset), cache.rows(np.arange(4), 37)):
             np.testing.assert_array_equal(a.astype(np.float64), b)
         del keep
+
+
+def test_an_append_replayed_from_a_graph():
+    """Rows appended behind ten others and read back, captured; each replay starts from the ten rows again."""
+    import torch
+    log("case: moves from a graph")
+    cache = R.Cache(3, R.E4M3)
+    dev = Device(cache)
+    k, v = rows(21, 40)
+    k[10:] *= 8  # the exponents of the first block grow
+    table = to_dev_i32(np.array([2, 0, 1], np.int32))
+    start = R.Cache(3, R.E4M3)
+    start.put_rows(np.array([2, 0, 1]), 0, k[:10], v[:10])
+    first = [torch.from_numpy(getattr(start, n).copy()).cuda() for n in ("key", "value", "exponents")]
+    dk, dv = torch.from_numpy(k[10:].copy()).cuda(), torch.from_numpy(v[10:].copy()).cuda()
+    back = [torch.zeros(40, 2, 128, dtype=torch.float16, device="cuda") for _ in range(2)]
+
+    def step(stream):
+        pvlc.kv_pack_q8(dk, dv, 30, dev.key, dev.value, dev.exponents, 3, R.E4M3, table, first_token=10, stream=stream)
+        pvlc.kv_unpack_q8(dev.key, dev.value, dev.exponents, 40, back[0], back[1], 3, R.E4M3, table, stream=stream)
+
+    start.put_rows(np.array([2, 0, 1]), 10, k[10:], v[10:])
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step(torch.cuda.current_stream())
+    for i in range(4):
+        for d, f in zip((dev.key, dev.value, dev.exponents), first):
+            d.copy_(f)
+        for b in back:
+            b.fill_(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        dev.same(start, f"replay {i}")
+        for a, b in zip(back, start.rows(np.array([2, 0, 1]), 40)):
+            np.testing.assert_array_equal(a.cpu().numpy().astype(np.float64), b)
+
+
+def test_moves_beyond_32_bits_of_offset():
+    import torch
+    blocks = (1 << 20) + 40
+    log(f"case: moves in planes of {blocks} blocks")
+    planes = [torch.full((blocks * 4096,), 0x5A, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    exponents = torch.full((blocks * 4,), 100, dtype=torch.uint8, device="cuda")
+    ids = np.array([blocks - 1, 3, blocks - 30], np.int32)
+    k, v = rows(22, 41)
+    dk, dv, table = torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), to_dev_i32(ids)
+    pvlc.kv_pack_q8(dk, dv, 41, planes[0], planes[1], exponents, blocks, R.INT8, table)
+    back = [torch.zeros(41, 2, 128, dtype=torch.float16, device="cuda") for _ in range(2)]
+    pvlc.kv_unpack_q8(planes[0], planes[1], exponents, 41, back[0], back[1], blocks, R.INT8, table)
+    want = R.Cache(3, R.INT8)
+    want.put_rows(np.arange(3), 0, k, v)
+    torch.cuda.synchronize()
+    for a, b in zip(back, want.rows(np.arange(3), 41)):
+        np.testing.assert_array_equal(a.cpu().numpy().astype(np.float64), b)
+    for p in planes:
+        p = p.view(blocks, 4096)
+        p[torch.from_numpy(ids).long().cuda()] = 0x5A
+        assert bool((p[:8] == 0x5A).all()) and bool((p[-64:] == 0x5A).all())
+    exponents.view(blocks, 4)[torch.from_numpy(ids).long().cuda()] = 100
+    assert bool((exponents == 100).all())

@@ -353,3 +353,24 @@ def test_two_graphs_share_a_pool():
         np.testing.assert_array_equal(t.cpu().numpy(), b.tables)
         b.same(f"back {i}")
     assert b.error() == 0
+
+
+def test_copies_replayed_from_a_graph():
+    """Pages swapped through a third one, captured: after two replays they are where they were."""
+    import torch
+    log("case: pages copied from a graph")
+    b = Both(12, 2, seed=8)
+    one, two, three = (dev(np.array(x, np.int32)) for x in ([4, 7], [9, 2], [1, 0]))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        for s, d in ((one, three), (two, one), (three, two)):
+            pvlc.kv_pages_copy(b.pool, s, b.pool, d, 2, torch.cuda.current_stream())
+    for i in range(4):
+        graph.replay()
+        for y in b.ref.planes:
+            y[:, [1, 0]] = y[:, [4, 7]]
+            y[:, [4, 7]] = y[:, [9, 2]]
+            y[:, [9, 2]] = y[:, [1, 0]]
+        b.same(f"replay {i}")
+    assert b.error() == 0
