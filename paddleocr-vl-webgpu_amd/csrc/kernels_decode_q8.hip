@@ -21,9 +21,9 @@
 // The key slab [token/4][dim/16][token%4][dim%16] makes each load of a tile 256
 // contiguous bytes; the value slab [dim][token] does as it is.
 //
-// With f32 operands the weights go to P.V as exact pairs of fp16 values (hi + lo,
-// ~22 bits), with fp16 operands, whose output rounds as coarsely, as single ones
-// (the pair costs 0.2-0.3 us of a launch's 8 to 10, 5 of 260).
+// The weights go to P.V as pairs of fp16 values (hi + lo, ~22 bits): single ones
+// are rounded as coarsely as an fp16 output, which then is off by two roundings in
+// place of one (the pair costs 0.2-0.3 us of a launch's 8 to 10, 5 of 260).
 //
 // What bounds it.  512 bytes a token and 8192 operations: memory, once a launch is
 // long.  256 sequences of 1024 to 32768 rows (1.20 GB): 214-220 us and the merge
@@ -493,7 +493,7 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
             l_run += pf;
             const float w = pf * pv;
             hi[t >> 3][t & 7] = to_h(w);
-            if constexpr (F32IO) lo[t >> 3][t & 7] = to_h(w - static_cast<float>(hi[t >> 3][t & 7]));  // the difference is exact in f32
+            lo[t >> 3][t & 7] = to_h(w - static_cast<float>(hi[t >> 3][t & 7]));  // the difference is exact in f32
         }
         // (the eight independent products of a step side by side)
 #pragma unroll
@@ -504,10 +504,8 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
                 v[c] = q8_half8<CODE>(vr[c][u * 2], vr[c][u * 2 + 1]);
                 o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[u], v[c], o[c], 0, 0, 0);
             }
-            if constexpr (F32IO) {
 #pragma unroll
-                for (int c = 0; c < 8; ++c) o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[u], v[c], o[c], 0, 0, 0);
-            }
+            for (int c = 0; c < 8; ++c) o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[u], v[c], o[c], 0, 0, 0);
         }
     }
     l_run += __shfl_xor(l_run, 16);
