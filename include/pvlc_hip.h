@@ -582,8 +582,10 @@ typedef struct pvlc_hip_paged_decode_q8_args {
 /* pvlc_hip_paged_decode_f16 over an 8-bit cache: rotate the new key (and
  * optionally the query), round the new row into the block at cache_len, attend
  * over cache_len+1 rows as they are held.  Codes enter the matrix products
- * exactly and their powers are applied to f32 scores and weights, so nothing is
- * rounded that the fp16 decode does not round.  Operands, streams, workspace and
+ * exactly, their powers are applied to f32 scores and weights, and the weights
+ * that multiply the values keep 16 bits (24 with f32 operands) and f32's range of
+ * exponents: a dim's error is relative to its own sum of weight * |value|, however
+ * large other dims or blocks are.  Operands, streams, workspace and
  * device error bits as there; with partition_tokens 0 the partition is this
  * decode's own (64..768 tokens in one launch, 512..4096 where it streams) and fits
  * the workspace that pvlc_hip_paged_decode_workspace_bytes sizes. */

@@ -8,9 +8,9 @@
 // 2^(s_t - M) 2^ev that multiply the codes are at most 1, and the terms
 // 2^(s_t - M) of the denominator at most 2^-ev <= 2^32.
 //
-// The codes become fp16 in registers, exactly, and the products are those of the
-// fp16 cache: v_mfma_f32_16x16x32_f16 for scores and for P.V.  A wave takes 64
-// tokens (four blocks) of one head at a time, all in 16-byte loads:
+// The codes become fp16 in registers for the scores (v_mfma_f32_16x16x32_f16) and
+// bf16 for P.V (v_mfma_f32_16x16x32_bf16), both exactly.  A wave takes 64 tokens
+// (four blocks) of one head at a time, all in 16-byte loads:
 //   keys    load (h, half): lane (row, kg) the dims half*64 + kg*16 .. +16 of
 //           token h*4 + row%4 of tile row/4; its low and high eight codes are
 //           the operands of two score MFMAs, and score MFMA chain h leaves lane
@@ -21,16 +21,22 @@
 // The key slab [token/4][dim/16][token%4][dim%16] makes each load of a tile 256
 // contiguous bytes; the value slab [dim][token] does as it is.
 //
-// The weights go to P.V as pairs of fp16 values (hi + lo, ~22 bits): single ones
-// are rounded as coarsely as an fp16 output, which then is off by two roundings in
-// place of one (the pair costs 0.2-0.3 us of a launch's 8 to 10, 5 of 260).
+// The weights go to P.V as sums of bf16 terms, three for f32 operands (all 24
+// bits) and two for fp16 ones (16 bits, so that the output is rounded once: with one fp16
+// term it was off by two roundings).  bf16 has the exponents of f32, which a weight
+// needs: a block whose values are 2^k times larger than another's pushes that one's
+// weights 2^k below the reference, up to 2^40, while in the dims where it is not
+// larger they count as much as its own.  (fp16 terms lost them: with one value of
+// 30000 among others of 1 those dims were off by 6e-4, of 0.05 by 1.3e-2.)  The third
+// term costs 0.2 us of a launch's 8 with f32 operands, the pair 0.2-0.4 of a single
+// one's 7.2-9.1 with fp16 ones.
 //
 // What bounds it.  512 bytes a token and 8192 operations: memory, once a launch is
 // long.  256 sequences of 1024 to 32768 rows (1.20 GB): 214-220 us and the merge
 // 8-9, 5.5 TB/s, where a copy reaches 5.1; the fp16 cache's takes 453 us.  Short
-// launches are a chain of rounds: one sequence of 1157 rows 7.5 us, thirteen up to
-// 2010 7.65, 18 caches of 2048 rows (19 MB) 9.1 in e4m3 and 10.1 in int8, whose
-// conversion to fp16 takes more instructions.  Time stamps of the waves
+// launches are a chain of rounds: one sequence of 1157 rows 7.9 us, thirteen up to
+// 2010 8.0, 18 caches of 2048 rows (19 MB) 9.5 in e4m3 and 10.1 in int8, whose
+// conversion takes more instructions.  Time stamps of the waves
 // put 0.75 us of that into the new row (its rounding and the LDS detour to the
 // wave's own registers), 0.8 into the hand-off and 1.3 into the merge; the rest is
 // the launch, the block ids and one round of loads.  Measured slower and not kept:
@@ -40,6 +46,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "decode_device.hpp"
 #include "pvlc_q8.hpp"
@@ -414,10 +421,10 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
 #pragma unroll
     for (int c = 0; c < 8; ++c) o[c] = float4_t{0.f, 0.f, 0.f, 0.f};
 
-    int ws = part_start + wave * kChunkTokens;
-    for (int chunk = 0; ws < part_end; ++chunk, ws += WAVES * kChunkTokens) {
-        if (chunk > 0) load_chunk(p, g, ids, chunk, row, kg, kr, vr);
-
+    // One chunk.  The first is code of its own, with nothing to rescale: as a turn
+    // of the loop it took one sequence of 1157 rows 8.5 us against 7.9.
+    auto attend = [&](auto first, int chunk, int ws) {
+        constexpr bool kFirst = decltype(first)::value;
         if (chunk == append_chunk) {  // uniform
             // The new row's codes into the block's registers; the codes behind it
             // become 0 (they may be e4m3 NaN).  All from LDS before any is used.
@@ -473,10 +480,9 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
         cmax = fmaxf(cmax, __shfl_xor(cmax, 16));
         cmax = fmaxf(cmax, __shfl_xor(cmax, 32));
         const float m_new = fmaxf(m_run, cmax);
-        const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-        l_run *= alpha;
-        m_run = m_new;
-        if (chunk > 0) {
+        if constexpr (!kFirst) {
+            const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+            l_run *= alpha;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float a = __shfl(alpha, kg * 4 + r);
@@ -484,29 +490,53 @@ __device__ inline void decode_q8_item(const DecodeQ8Params &p, int P, uint32_t s
                 for (int c = 0; c < 8; ++c) o[c][r] *= a;
             }
         }
+        m_run = m_new;
 
         const float pv = past ? 0.f : exp2_whole(ev);
-        half8_t hi[2], lo[2];
-#pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            const float pf = __builtin_amdgcn_exp2f(x[t] - m_new);
-            l_run += pf;
-            const float w = pf * pv;
-            hi[t >> 3][t & 7] = to_h(w);
-            lo[t >> 3][t & 7] = to_h(w - static_cast<float>(hi[t >> 3][t & 7]));  // the difference is exact in f32
-        }
-        // (the eight independent products of a step side by side)
+        // Eight tokens' terms at a time and, side by side, the products of four times
+        // 16 dims.  In the widest workgroups, whose waves have 168 registers, the dims
+        // follow one another in the schedule too: else the compiler converts all of them
+        // first, and spills (18 caches of 4000 rows, int8 and f32 operands, 14.2 us
+        // against 17.3; the others are 0.05-0.1 us faster as they are).
+        constexpr int kTerms = F32IO ? 3 : 2, kSide = 4;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            half8_t v[8];
+            q8x4_t terms[kTerms];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                v[c] = q8_half8<CODE>(vr[c][u * 2], vr[c][u * 2 + 1]);
-                o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[u], v[c], o[c], 0, 0, 0);
+            for (int i = 0; i < 4; ++i) {
+                float2_t w;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float pf = __builtin_amdgcn_exp2f(x[u * 8 + i * 2 + j] - m_new);
+                    l_run += pf;
+                    w[j] = pf * pv;
+                }
+#pragma unroll
+                for (int k = 0; k < kTerms; ++k) {
+                    const uint32_t r = __builtin_bit_cast(uint32_t, __builtin_convertvector(w, bf16x2_t));
+                    terms[k][i] = r;
+                    w -= float2_t{__uint_as_float(r << 16), __uint_as_float(r & 0xFFFF0000u)};  // exact in f32
+                }
             }
 #pragma unroll
-            for (int c = 0; c < 8; ++c) o[c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[u], v[c], o[c], 0, 0, 0);
+            for (int c0 = 0; c0 < 8; c0 += kSide) {
+                if constexpr (WAVES > 8) __builtin_amdgcn_sched_barrier(0);
+                bf16x8_t v[kSide];
+#pragma unroll
+                for (int c = 0; c < kSide; ++c) v[c] = q8_bf16x8<CODE>(vr[c0 + c][u * 2], vr[c0 + c][u * 2 + 1]);
+#pragma unroll
+                for (int k = 0; k < kTerms; ++k)
+#pragma unroll
+                    for (int c = 0; c < kSide; ++c)
+                        o[c0 + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, terms[k]), v[c], o[c0 + c], 0, 0, 0);
+            }
         }
+    };
+    int ws = part_start + wave * kChunkTokens;
+    if (ws < part_end) attend(std::true_type{}, 0, ws);
+    for (int chunk = 1; (ws += WAVES * kChunkTokens) < part_end; ++chunk) {
+        load_chunk(p, g, ids, chunk, row, kg, kr, vr);
+        attend(std::false_type{}, chunk, ws);
     }
     l_run += __shfl_xor(l_run, 16);
     l_run += __shfl_xor(l_run, 32);

@@ -27,6 +27,8 @@ namespace pvlc {
 typedef uint32_t q8x4_t __attribute__((ext_vector_type(4)));  // 16 codes
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 // 2^e, -126 <= e <= 127.
 __device__ inline float exp2_whole(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
@@ -106,6 +108,30 @@ __device__ inline half8_t q8_half8(uint32_t lo, uint32_t hi) {
         r = half8_t{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
     }
     return r;
+}
+
+// Eight codes as bf16, exactly (at most 8 significant bits): an MFMA operand.  int8
+// by way of f32, whose low half is 0 then.
+template <int CODE>
+__device__ inline bf16x8_t q8_bf16x8(uint32_t lo, uint32_t hi) {
+    q8x4_t r;
+    if constexpr (CODE == PVLC_HIP_KV_E4M3) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t w = i ? hi : lo;
+            r[i * 2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
+            r[i * 2 + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float4_t x = q8_decode<CODE>(i ? hi : lo);
+            // the high halves of two
+            r[i * 2] = __builtin_amdgcn_perm(__float_as_uint(x[1]), __float_as_uint(x[0]), 0x07060302u);
+            r[i * 2 + 1] = __builtin_amdgcn_perm(__float_as_uint(x[3]), __float_as_uint(x[2]), 0x07060302u);
+        }
+    }
+    return __builtin_bit_cast(bf16x8_t, r);
 }
 
 // The largest of the 64 lanes, in every lane (see wave_sum).

@@ -75,3 +75,37 @@ def test_fp16_outputs_are_rounded_once(code):
     c.q = (c.q * 0.03).astype(np.float16)
     c.upload()
     check(c, workspace(c.n, c.width * 16), "short sequences")
+
+
+def outlying(tokens, code, f32, size, others, score, seed):
+    """Sequences with one large value: `size` in one dim of one row of each kv head, values of scale `others` elsewhere,
+    and a score of about `score` for that row."""
+    c = Case(tokens, code, f32, seed=seed)
+    for i, t in enumerate(c.lens):
+        t = int(t)
+        k, v = c.rows(t)
+        v = (v.astype(np.float64) * others).astype(np.float16)
+        q = c.q[i].astype(np.float64).reshape(2, 8, 128) * 0.2 + c.g.standard_normal((2, 1, 128))
+        c.q[i] = q.reshape(16, 128).astype(c.q.dtype)
+        row = t // 3
+        for h in range(2):
+            mean = q[h].mean(0)
+            k[row, h] = (mean * (score * np.sqrt(128.0) / (mean @ mean))).astype(np.float16)
+            v[row, h, 5 + 60 * h] = size
+        c.cache.put_rows(c.table[i], 0, k, v)
+        c.nv[i] = (c.nv[i] * others).astype(c.nv.dtype)
+    return c
+
+
+@CODES
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("size,others,score", [(3, 1, 0), (3000, 1, 6), (30000, 1, 0), (60000, 1, 6), (30000, 0.05, 0), (60000, 0.002, -3)])
+def test_one_large_value(code, f32, size, others, score):
+    """A value far larger than the rest leaves the other dims as exact as they are without it."""
+    log(f"case: q8 decode one large value {size} among {others}, score {score}, code={code} f32={f32}")
+    c = outlying([40, 75, 130, 300], code, f32, size, others, score, seed=int(size) + code).upload()
+    check(c, workspace(c.n, c.width * 16), "short")
+    c = outlying([1200, 700], code, f32, size, others, score, seed=int(size) + 7 + code).upload()
+    check(c, workspace(c.n, c.width * 16, 64), "partitions of 64", partition=64)
+    c = outlying([900] * 3, code, f32, size, others, score, seed=int(size) + 9 + code).upload()
+    check(c, workspace(c.n, c.width * 16, 1024), "streaming", partition=1024)
