@@ -649,7 +649,8 @@ typedef struct pvlc_hip_kv_pool {
  * (pvlc_hip_workspace_error reads it). */
 enum {
     PVLC_HIP_PAGES_EXHAUSTED = 1,  /* fewer free pages than a fork asks for: it changes nothing but its outputs */
-    PVLC_HIP_PAGES_BAD_LENGTH = 2, /* an input row's length is negative or beyond its table: taken as 0 */
+    PVLC_HIP_PAGES_BAD_LENGTH = 2, /* a parent's lens_in is negative (as a fork that found too few pages leaves it), or its
+                                      length with the appended rows is beyond its table: taken as 0 */
     PVLC_HIP_PAGES_BAD_PARENT = 4, /* a parent outside -1..rows_in-1: taken as -1 */
     PVLC_HIP_PAGES_BAD_BLOCK = 8,  /* an entry outside the pool: not shared, copied or counted */
     PVLC_HIP_PAGES_BAD_COUNT = 16, /* a count would fall below 0 */

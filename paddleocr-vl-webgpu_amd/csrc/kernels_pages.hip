@@ -58,10 +58,13 @@ __device__ inline uint32_t plan_scan(uint32_t v, uint32_t *sm, uint32_t *total) 
 
 __device__ inline bool valid_block(int32_t id, uint32_t num_blocks) { return id >= 0 && static_cast<uint32_t>(id) < num_blocks; }
 
-// Length of row r of the input (a bad one counts as 0).
+// Length of row r of the input (a bad one counts as 0).  The sign is looked at
+// before the appended rows are added: a fork that found too few pages leaves
+// lengths of -1, which one more row does not make an empty sequence.
 __device__ inline uint32_t in_length(const PagesFork &f, uint32_t r, uint32_t *errors) {
-    const int64_t len = static_cast<int64_t>(f.lens_in[r]) + f.appended;
-    if (len < 0 || len > static_cast<int64_t>(f.max_blocks) * kBlockTokens) {
+    const int32_t held = f.lens_in[r];
+    const int64_t len = static_cast<int64_t>(held) + f.appended;
+    if (held < 0 || len > static_cast<int64_t>(f.max_blocks) * kBlockTokens) {
         *errors |= PVLC_HIP_PAGES_BAD_LENGTH;
         return 0;
     }
