@@ -801,7 +801,10 @@ pvlc_hip_status pvlc_hip_lm_head_top1_f16(const uint16_t *weights, const float *
  * score (rounded to f32), parent row and token, and whether the sequence is
  * finished (its parent was, or the token is end_token).  The order is that of
  * the scores in 64 bits, of which it takes 39 of the fraction; equal ones go by
- * beam, then by logit (as the greedy top-1 orders them), then by token.  A row with finished[r] continues with end_token
+ * beam, then by logit (as the greedy top-1 orders them), then by token.  The
+ * exponentials are f32 (a score is off by about 5e-8, a few 1e-6 at worst, and two
+ * beams' candidates closer than that may come in either order); a row's scores depend on its own
+ * operands alone, not on the batch.  A row with finished[r] continues with end_token
  * alone at its score; a row whose score is -inf or NaN does not continue; its
  * logits are not read in either case.  A logit below -2^127 (-inf and the type's
  * lowest value among them) or NaN masks its token, one above 2^127 counts as

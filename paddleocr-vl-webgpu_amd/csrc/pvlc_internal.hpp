@@ -515,18 +515,17 @@ int launch_pages_copy(const int32_t *src, const int32_t *dst, uint32_t count, ui
                       uint32_t *error_word, void *stream);
 
 // Beam selection (kernels_beam.hip).  A row of logits is cut into segments of
-// kBeamThreads * each; each leaves its best candidates as keys (logit and token in
+// kBeamSegment; each leaves its best candidates as keys (logit and token in
 // one number, see there) and its sum of exponentials.
 constexpr uint32_t kBeamThreads = 256;
 constexpr uint32_t kBeamMaxBeams = 64, kBeamMaxBest = 128;
-// Logits a thread takes: 16 where that makes enough workgroups to fill the
-// device twice, else 8 (four rows of 103424 logits, with 4 / 8 / 16: 10.8 / 10.3 /
-// 10.4 us; fewer make more segments to join).
-inline uint32_t beam_each(uint64_t rows, uint32_t vocab) {
-    return rows * ((static_cast<uint64_t>(vocab) + 16 * kBeamThreads - 1) / (16 * kBeamThreads)) >= 2 * kTargetWorkgroups ? 16 : 8;
-}
+// Logits a thread takes.  The same for any number of rows: what is summed
+// together in f32 decides how a row's sum of exponentials is rounded, and a row's scores
+// must not depend on what it is batched with.  (8 / 16 logits: four rows of 103424
+// 10.5 / 10.5 us, one 9.0 / 8.7, four of 32000 10.7 / 10.2, 128 of 103424 27.7 / 22.4.)
+constexpr uint32_t kBeamEach = 16, kBeamSegment = kBeamEach * kBeamThreads;
 struct BeamSelect {
-    uint32_t batch, beams, vocab, best, segments, each;
+    uint32_t batch, beams, vocab, best, segments;
     uint64_t row_stride;
     const float *logits, *scores;
     const int32_t *finished;
@@ -545,8 +544,7 @@ struct BeamWorkspace {
 };
 inline BeamWorkspace beam_workspace_layout(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t best) {
     auto align = [](size_t v) { return (v + 255) / 256 * 256; };
-    const size_t rows = static_cast<size_t>(batch) * beams, segment = static_cast<size_t>(beam_each(rows, vocab)) * kBeamThreads;
-    const size_t parts = rows * ((vocab + segment - 1) / segment);
+    const size_t rows = static_cast<size_t>(batch) * beams, parts = rows * ((static_cast<size_t>(vocab) + kBeamSegment - 1) / kBeamSegment);
     BeamWorkspace w{};
     w.keys_offset = align(static_cast<size_t>(batch) * 4);
     w.sums_offset = w.keys_offset + align(parts * best * 8);

@@ -271,7 +271,7 @@ pvlc_hip_status pvlc_hip_beam_select_f32(const pvlc_hip_beam_args *args, void *s
     if (args->vocab > 0x7FFFFFFFu || static_cast<uint64_t>(args->batch) * args->beams > 65535u)
         return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "below 2^31 logits a row and at most 65535 rows");
     const uint64_t rows = static_cast<uint64_t>(args->batch) * args->beams;
-    const uint32_t each = beam_each(rows, args->vocab), segments = (args->vocab - 1) / (each * kBeamThreads) + 1;
+    const uint32_t segments = (args->vocab - 1) / kBeamSegment + 1;
     if (segments * rows >= kMaxGroups)
         return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows times vocab of a beam selection exceed the grid");
     if (args->row_stride < args->vocab) return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "rows of logits overlap");
@@ -300,7 +300,6 @@ pvlc_hip_status pvlc_hip_beam_select_f32(const pvlc_hip_beam_args *args, void *s
     b.vocab = args->vocab;
     b.best = args->best;
     b.segments = segments;
-    b.each = each;
     b.row_stride = args->row_stride;
     b.logits = args->logits;
     b.scores = args->scores;
