@@ -71,12 +71,59 @@ __device__ inline uint32_t wave_tile_ids(const DecodeParams &p, uint32_t s, int 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 constexpr int kSc1 = 16;  // cache-policy operand of the buffer intrinsics: sc1 (agent scope)
 
-// An 8-byte agent-scope (sc1) load of two floats.
+// The hand-off of a partition's partial to the workgroup that merges: without L2
+// maintenance.  Partials, the arrival counter and the merge reads are relaxed
+// agent-scope accesses (sc1), which are coherent across the XCDs' L2s by
+// themselves; every store of the workgroup completes before its arrival is
+// counted.  (A C++ release/acquire fence at agent scope would instead write back
+// and invalidate the whole L2 of the XCD in every workgroup.)
+//
+// 8 bytes: two floats, as atomics.  16 bytes: elements of a unit's partials (a
+// sequence's kv head), through the compiler's buffer intrinsics so that its waits
+// cover them.
+__device__ inline void store_pair_sc1(float *q, float lo, float hi) {
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(q),
+                       static_cast<uint64_t>(__float_as_uint(lo)) | (static_cast<uint64_t>(__float_as_uint(hi)) << 32),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 __device__ inline void load_pair_sc1(const float *q, float *lo, float *hi) {
     const uint64_t v =
         __hip_atomic_load(reinterpret_cast<const uint64_t *>(q), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     *lo = __uint_as_float(static_cast<uint32_t>(v));
     *hi = __uint_as_float(static_cast<uint32_t>(v >> 32));
+}
+// Raw buffer over the unit's partials: stride 0, 2^31 - 1 bytes, and the fourth
+// descriptor word of a raw 32-bit-element buffer on gfx9-family parts (data
+// format 32 in bits 15-18).
+__device__ inline __amdgpu_buffer_rsrc_t partials_buffer(const DecodeParams &p, size_t unit) {
+    return __builtin_amdgcn_make_buffer_rsrc(p.part_o + unit * (kGroup * kHeadDim), 0, 0x7fffffff, 0x00020000);
+}
+__device__ inline void store_partial_sc1(__amdgpu_buffer_rsrc_t rsrc, uint32_t element, u32x4_t v) {
+    __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, static_cast<int>(element * 4), 0, kSc1);
+}
+__device__ inline u32x4_t load_partial_sc1(__amdgpu_buffer_rsrc_t rsrc, uint32_t element) {
+    return __builtin_amdgcn_raw_buffer_load_b128(rsrc, static_cast<int>(element * 4), 0, kSc1);
+}
+// Counts the workgroup's partition as arrived; whether it is the last of its
+// unit, the same for every thread (sm_last is LDS).  Every thread calls it.
+__device__ inline bool last_to_arrive(const DecodeParams &p, uint32_t s, uint32_t g, uint32_t part, int num_parts, int &sm_last) {
+    // Wait for this wave's partial stores to complete (a single-wave
+    // workgroup's __syncthreads() emits no wait), then for every wave.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    // Arrival, counted in generations (kArrivalSpan): the partition with the
+    // highest index adds kArrivalSpan - (num_parts - 1), the others 1, so the
+    // arrival that completes a multiple of kArrivalSpan is the last one, and
+    // the counter is left ready for the next launch without a reset.
+    if (threadIdx.x == 0) {
+        const uint32_t inc =
+            part == static_cast<uint32_t>(num_parts - 1) ? kArrivalSpan - static_cast<uint32_t>(num_parts - 1) : 1u;
+        const uint32_t prev =
+            __hip_atomic_fetch_add(p.counters + s * kKvHeads + g, inc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        sm_last = ((prev + inc) & (kArrivalSpan - 1)) == 0;
+    }
+    __syncthreads();
+    return sm_last;
 }
 // Cache length of sequence s if it is valid for this launch (one row to
 // append, inside the block table and the partitions of the workspace), else -1.

@@ -513,65 +513,30 @@ __device__ inline void decode_item(const DecodeParams &p, int P, uint32_t s, uin
         return;
     }
 
-    // Cross-workgroup hand-off without L2 maintenance: partials, the arrival
-    // counter and the merge reads are relaxed agent-scope atomics (sc1), which
-    // are coherent across the XCDs' L2s by themselves.  Every store of the
-    // workgroup completes (s_waitcnt vmcnt(0), then the barrier) before thread
-    // 0 counts the arrival, which orders the partials before the count.
-    // (A C++ release/acquire fence at agent scope would instead write back and
-    // invalidate the whole L2 of the XCD in every workgroup.)  Values move in
-    // 8-byte pairs: half the transactions of single floats.  Shapes whose
-    // threads own 4 or more elements (kWide: at most 256 combining threads,
-    // the single-sequence decodes of 16 partitions) move them as 16-byte
-    // buffer stores and loads with the same agent-scope (sc1) policy, issued
-    // through the compiler's buffer intrinsics so that its waits cover them:
-    // single-layer decode 8.48 -> 8.17 us.
+    // The hand-off (decode_device.hpp).  Values move in 8-byte pairs: half the
+    // transactions of single floats.  Shapes whose threads own 4 or more elements
+    // (kWide: at most 256 combining threads, the single-sequence decodes of 16
+    // partitions) move them as 16-byte buffer stores and loads: single-layer decode
+    // 8.48 -> 8.17 us.
     static_assert(kPer % 2 == 0, "partials move as float pairs");
     constexpr bool kWide = kPer % 4 == 0;
-    // Raw buffer over this unit's partials: stride 0, 2^31 - 1 bytes, and the
-    // fourth descriptor word of a raw 32-bit-element buffer on gfx9-family
-    // parts (data format 32 in bits 15-18).
-    const __amdgpu_buffer_rsrc_t o_rsrc =
-        __builtin_amdgcn_make_buffer_rsrc(p.part_o + unit * (kGroup * kHeadDim), 0, 0x7fffffff, 0x00020000);
-    auto pack = [](float lo, float hi) {
-        return static_cast<uint64_t>(__float_as_uint(lo)) | (static_cast<uint64_t>(__float_as_uint(hi)) << 32);
-    };
+    const __amdgpu_buffer_rsrc_t o_rsrc = partials_buffer(p, unit);
     if (active) {
         if constexpr (kWide) {
 #pragma unroll
             for (int e = 0; e < kPer; e += 4) {
                 const u32x4_t v = {__float_as_uint(po[e]), __float_as_uint(po[e + 1]), __float_as_uint(po[e + 2]),
                                    __float_as_uint(po[e + 3])};
-                __builtin_amdgcn_raw_buffer_store_b128(
-                    v, o_rsrc, static_cast<int>((part * (kGroup * kHeadDim) + e0 + e) * 4), 0, kSc1);
+                store_partial_sc1(o_rsrc, part * (kGroup * kHeadDim) + e0 + e, v);
             }
         } else {
 #pragma unroll
             for (int e = 0; e < kPer; e += 2)
-                __hip_atomic_store(reinterpret_cast<uint64_t *>(part_o + e0 + e), pack(po[e], po[e + 1]),
-                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                store_pair_sc1(part_o + e0 + e, po[e], po[e + 1]);
         }
-        if (d0 == 0)
-            __hip_atomic_store(reinterpret_cast<uint64_t *>(part_ml + 2 * h), pack(M, L), __ATOMIC_RELAXED,
-                               __HIP_MEMORY_SCOPE_AGENT);
+        if (d0 == 0) store_pair_sc1(part_ml + 2 * h, M, L);
     }
-    // Wait for this wave's partial stores to complete (a single-wave
-    // workgroup's __syncthreads() emits no wait), then for every wave.
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    // Arrival, counted in generations (kArrivalSpan): the partition with the
-    // highest index adds kArrivalSpan - (num_parts - 1), the others 1, so the
-    // arrival that completes a multiple of kArrivalSpan is the last one, and
-    // the counter is left ready for the next launch without a reset.
-    if (threadIdx.x == 0) {
-        const uint32_t inc =
-            part == static_cast<uint32_t>(num_parts - 1) ? kArrivalSpan - static_cast<uint32_t>(num_parts - 1) : 1u;
-        const uint32_t prev =
-            __hip_atomic_fetch_add(p.counters + s * kKvHeads + g, inc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        sm_last = ((prev + inc) & (kArrivalSpan - 1)) == 0;
-    }
-    __syncthreads();
-    if (!sm_last) return;
+    if (!last_to_arrive(p, s, g, part, num_parts, sm_last)) return;
 
     const float *all_ml = p.part_ml + unit * (2 * kGroup);
 
@@ -606,8 +571,7 @@ __device__ inline void decode_item(const DecodeParams &p, int P, uint32_t s, uin
                 if constexpr (kWide) {
 #pragma unroll
                     for (int e = 0; e < kPer; e += 4) {
-                        const u32x4_t v = __builtin_amdgcn_raw_buffer_load_b128(
-                            o_rsrc, static_cast<int>((q * (kGroup * kHeadDim) + e0 + e) * 4), 0, kSc1);
+                        const u32x4_t v = load_partial_sc1(o_rsrc, q * (kGroup * kHeadDim) + e0 + e);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) ov[b][e + k] = __uint_as_float(v[k]);
                     }

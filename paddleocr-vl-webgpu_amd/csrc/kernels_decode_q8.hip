@@ -65,9 +65,7 @@ constexpr int kChunkTokens = kTiles * 16;
 // partial (DEFER_MERGE, for paged_decode_merge_kernel) or, as the last
 // partition to arrive, merge them all.  m_run and l_run belong to head
 // lane % 16, o[c][r] to head (lane / 16) * 4 + r at dim c * 16 + lane % 16.
-// The hand-off is that of the fp16 kernel: agent-scope (sc1) stores, a wait for
-// their acknowledgement, a counter in generations of kArrivalSpan, agent-scope
-// loads by the last arrival.
+// The hand-off is decode_device.hpp's.
 template <int WAVES, bool DEFER_MERGE, bool F32IO>
 __device__ inline void finish_item(const DecodeParams &p, uint32_t s, uint32_t g, uint32_t part, int num_parts,
                                    float m_run, float l_run, const float4_t (&o)[8]) {
@@ -149,29 +147,13 @@ __device__ inline void finish_item(const DecodeParams &p, uint32_t s, uint32_t g
         }
         return;
     } else {
-        const __amdgpu_buffer_rsrc_t rsrc =
-            __builtin_amdgcn_make_buffer_rsrc(p.part_o + unit * (kGroup * kHeadDim), 0, 0x7fffffff, 0x00020000);
+        const __amdgpu_buffer_rsrc_t rsrc = partials_buffer(p, unit);
         if (active) {
 #pragma unroll
-            for (int e = 0; e < kPer / 4; ++e)
-                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, po[e]), rsrc,
-                                                       static_cast<int>((part * (kGroup * kHeadDim) + e0 + e * 4) * 4), 0, kSc1);
-            if (d0 == 0)
-                __hip_atomic_store(reinterpret_cast<uint64_t *>(part_ml + 2 * h),
-                                   static_cast<uint64_t>(__float_as_uint(M)) | static_cast<uint64_t>(__float_as_uint(L)) << 32,
-                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            for (int e = 0; e < kPer / 4; ++e) store_partial_sc1(rsrc, part * (kGroup * kHeadDim) + e0 + e * 4, __builtin_bit_cast(u32x4_t, po[e]));
+            if (d0 == 0) store_pair_sc1(part_ml + 2 * h, M, L);
         }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (a one-wave workgroup's barrier waits for nothing)
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const uint32_t inc =
-                part == static_cast<uint32_t>(num_parts - 1) ? kArrivalSpan - static_cast<uint32_t>(num_parts - 1) : 1u;
-            const uint32_t prev =
-                __hip_atomic_fetch_add(p.counters + s * kKvHeads + g, inc, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            sm_last = ((prev + inc) & (kArrivalSpan - 1)) == 0;
-        }
-        __syncthreads();
-        if (!sm_last) return;
+        if (!last_to_arrive(p, s, g, part, num_parts, sm_last)) return;
 
         const float *all_ml = p.part_ml + unit * (2 * kGroup);
         constexpr int kBatch = kPer >= 16 ? 4 : (kPer >= 8 ? 8 : 16);
@@ -191,8 +173,7 @@ __device__ inline void finish_item(const DecodeParams &p, uint32_t s, uint32_t g
                     load_pair_sc1(all_ml + q * (2 * kGroup) + 2 * h, &mv[b], &lv[b]);
 #pragma unroll
                     for (int e = 0; e < kPer / 4; ++e)
-                        ov[b][e] = __builtin_bit_cast(float4_t, __builtin_amdgcn_raw_buffer_load_b128(
-                            rsrc, static_cast<int>((q * (kGroup * kHeadDim) + e0 + e * 4) * 4), 0, kSc1));
+                        ov[b][e] = __builtin_bit_cast(float4_t, load_partial_sc1(rsrc, q * (kGroup * kHeadDim) + e0 + e * 4));
                 }
             }
             float Mb = Mg;
