@@ -452,7 +452,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
     __shared__ int sm_last;
     __shared__ float sm_most;
     __shared__ double sm_log_sum;
-    asm volatile("" ::"s"(b.keys), "s"(b.sums), "s"(b.references), "s"(b.scores), "s"(b.finished), "s"(b.row_keys), "s"(b.row_scores), "s"(b.arrived));
+    asm volatile("" ::"s"(b.keys), "s"(b.sums), "s"(b.references), "s"(b.scores), "s"(b.finished), "s"(b.row_keys), "s"(b.row_tokens), "s"(b.arrived));
     asm volatile("" ::"s"(b.next_scores), "s"(b.parents), "s"(b.tokens), "s"(b.next_finished));
     const uint32_t row = blockIdx.x, i = threadIdx.x, entry = row / b.beams;
     const size_t part = static_cast<size_t>(row) * b.segments;
@@ -508,7 +508,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
     if (b.beams > 1) {
         if (i < b.best) {
             store_agent(b.row_keys + at, scored);
-            store_agent(reinterpret_cast<uint64_t *>(b.row_scores) + at,
+            store_agent(b.row_tokens + at,
                         static_cast<uint64_t>(token_in(key)) << 32 | __float_as_uint(static_cast<float>(score)));
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -532,7 +532,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_join_kernel(BeamSelect b) {
         const uint32_t number = number_in(scored), from = number / b.best;
         parent = static_cast<int32_t>(entry * b.beams + from);
         if (b.beams > 1) {
-            const uint64_t held = load_agent(reinterpret_cast<const uint64_t *>(b.row_scores) + rows_at + static_cast<size_t>(number - from * b.best) * b.beams + from);
+            const uint64_t held = load_agent(b.row_tokens + rows_at + static_cast<size_t>(number - from * b.best) * b.beams + from);
             token = static_cast<int32_t>(held >> 32);
             value = __uint_as_float(static_cast<uint32_t>(held));
         } else {

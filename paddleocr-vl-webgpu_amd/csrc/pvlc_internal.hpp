@@ -537,10 +537,10 @@ struct BeamSelect {
     double *sums;         // [row][segment], relative to exp(reference)
     float *references;    // [row][segment]
     uint64_t *row_keys;   // [batch entry][rank][beam]: the scores' keys
-    double *row_scores;   // the same: token and f32 score
+    uint64_t *row_tokens;  // the same: token, and the score's f32 bits
 };
 struct BeamWorkspace {
-    size_t keys_offset, sums_offset, references_offset, row_keys_offset, row_scores_offset, total;
+    size_t keys_offset, sums_offset, references_offset, row_keys_offset, row_tokens_offset, total;
 };
 inline BeamWorkspace beam_workspace_layout(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t best) {
     auto align = [](size_t v) { return (v + 255) / 256 * 256; };
@@ -550,8 +550,8 @@ inline BeamWorkspace beam_workspace_layout(uint32_t batch, uint32_t beams, uint3
     w.sums_offset = w.keys_offset + align(parts * best * 8);
     w.references_offset = w.sums_offset + align(parts * 8);
     w.row_keys_offset = w.references_offset + align(parts * 4);
-    w.row_scores_offset = w.row_keys_offset + align(rows * best * 8);
-    w.total = w.row_scores_offset + align(rows * best * 8);
+    w.row_tokens_offset = w.row_keys_offset + align(rows * best * 8);
+    w.total = w.row_tokens_offset + align(rows * best * 8);
     return w;
 }
 int launch_beam_select(const BeamSelect &b, void *stream);

@@ -314,7 +314,7 @@ pvlc_hip_status pvlc_hip_beam_select_f32(const pvlc_hip_beam_args *args, void *s
     b.sums = reinterpret_cast<double *>(base + ws.sums_offset);
     b.references = reinterpret_cast<float *>(base + ws.references_offset);
     b.row_keys = reinterpret_cast<uint64_t *>(base + ws.row_keys_offset);
-    b.row_scores = reinterpret_cast<double *>(base + ws.row_scores_offset);
+    b.row_tokens = reinterpret_cast<uint64_t *>(base + ws.row_tokens_offset);
     const int e = launch_beam_select(b, stream);
     if (e != 0) return hip_status(e, "beam selection launch");
     return ok();
