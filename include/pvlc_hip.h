@@ -548,8 +548,10 @@ pvlc_hip_status pvlc_hip_kv_unpack_f16(const uint16_t *key_cache, const uint16_t
  * ------------------------------------------------------------------------- */
 
 /* Codes: OCP e4m3 (sign, 4 exponent and 3 fraction bits, largest 448), or
- * int8 -127..127.  int8 rounds to 1/254 of a block's power at most, e4m3 to
- * 1/16 of each value: e4m3 for blocks with outlying channels. */
+ * int8 -127..127.  With e the block's exponent, int8 is off by up to 2^(e-1),
+ * 1/254 to 1/127 of the block's largest value; e4m3 by up to 1/16 of each value,
+ * and by up to 2^(e-10) for those below 2^(e-6): e4m3 for blocks with outlying
+ * channels.  A row that is rounded again is off by up to as much once more. */
 enum { PVLC_HIP_KV_E4M3 = 0, PVLC_HIP_KV_INT8 = 1 };
 
 /* pvlc_hip_paged_decode_args with an 8-bit cache. */

@@ -10,7 +10,8 @@
 // 64-bit key, (the logit's bits, made monotone) * 2^32 + (2^32 - 1 - token), so no
 // two are equal and the larger is the better.  Across rows by score, in 64 bits:
 // scores of two beams may lie closer than f32 tells apart, and the order of what
-// is returned must not depend on it.  Again one key: the score's bits, made
+// is returned must not depend on it (nor on the batch: a row's score is the same
+// in any, though its sum's terms are f32).  Again one key: the score's bits, made
 // monotone, with the lowest 13 given to the candidate's number (beam, then rank
 // in its row), so that scores equal to 2^-39 go by beam and rank.
 //
@@ -18,12 +19,12 @@
 // threads, the n-th largest of the groups' own largest is a bound that at least n
 // values reach and few others, so a short list remains, whose ranks are counted.
 //
-// Measured: four rows of 103424 logits, four candidates: segments 3.7-4.6 us, join
-// 5.4-5.8 (1.65 MB; both are a launch and a chain of rounds through memory and
+// Measured: four rows of 103424 logits, four candidates: segments 4.9-5.1 us, join
+// 5.8-6.0 (1.65 MB; both are a launch and a chain of rounds through memory and
 // barriers: of the join's, by time stamps, loads 0.7, selection 1.6, the hand-off
 // 0.8, loads and selection among the rows 0.9, outputs 0.5).  128 rows, a fifth of
-// them finished, sixteen candidates of eight rows each: segments 11.0-12.4 us (42 MB,
-// 3.4-3.8 TB/s: a row's loads, exponentials and selection follow one another in
+// them finished, sixteen candidates of eight rows each: segments 11.4-12.4 us (42 MB,
+// 3.4-3.7 TB/s: a row's loads, exponentials and selection follow one another in
 // each workgroup, and little more than one round of workgroups covers the other's
 // waits), join 6.9-7.7.  One launch for both, the last segment of a row joining it,
 // took 11.7 and 32.6 us a call against 9.9 and 22.9: each segment then waits for

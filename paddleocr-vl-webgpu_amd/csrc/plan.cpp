@@ -542,7 +542,10 @@ uint32_t q8_auto_partition(uint32_t num_seqs, uint32_t rows, bool ragged, uint32
     // head) merge in one batch of loads (4, 8 or 16 by the elements a thread
     // owns) and the launch does not stream.  The fp16 rule, of more and smaller
     // partitions, took one sequence of 1157 rows 7.6 us against 7.3, four
-    // of 2048 8.7 against 7.5, 18 of 3000 13.1 against 10.4.
+    // of 2048 8.7 against 7.5, 18 of 3000 13.1 against 10.4.  The widest shape
+    // against 512, 384 and 1024 tokens: 18 of 4000 (e4m3) 12.7 against 18.9, 17.8 and
+    // 15.8, (int8, f32 operands) 14.2 against 20.7, 19.8 and 18.5; but one sequence of
+    // 9000, of more partitions than one batch, 12.2 against 11.75, 10.5 and 14.3.
     for (uint32_t w : kQ8Shapes) {
         const uint64_t parts = (static_cast<uint64_t>(rows) + w * 64 - 1) / (w * 64);
         const uint32_t batch = w >= 4 ? 16 : (w >= 2 ? 8 : 4);
@@ -551,8 +554,10 @@ uint32_t q8_auto_partition(uint32_t num_seqs, uint32_t rows, bool ragged, uint32
     }
     // Streaming: a few partitions for each compute unit, if every sequence is as
     // long as the longest, between 512 and 1536 tokens; the kernel may double it.
-    // (64 sequences up to 8192 rows, 512 / 768 / 1024: 21.9 / 21.1 / 22.2 us; 256 up
-    // to 8192 101 / 96 / 95; 256 up to 32768 257 / 242 / 233.)
+    // (e4m3 with fp16 operands, then int8 with f32 ones: 64 sequences of 256-8192
+    // rows, 512 / 768 / 1024 tokens: 21.9 / 21.0 / 22.8 and 24.3 / 23.8 / 26.3 us; 256
+    // of them 70.9 / 65.7 / 69.2 and 78.2 / 71.0 / 75.4; 256 of 1024-32768, 512 / 1024 /
+    // 1536 / 2048: 258 / 234 / 226 / 222 and 273 / 242 / 233 / 231.)
     const uint64_t unit = static_cast<uint64_t>(num_seqs) * rows * kKvHeads / kTargetWorkgroups;
     uint64_t p = unit * 3 / 16 / 64 * 64;
     p = p < 512 ? 512 : (p > 1536 ? 1536 : p);
