@@ -824,7 +824,7 @@ typedef struct pvlc_hip_beam_args {
     const float *scores;     /* [batch][beams] */
     const int32_t *finished; /* [batch][beams] or NULL */
     int32_t end_token;       /* -1: none */
-    float *next_scores;      /* [batch][best], as the outputs below; none may overlap an input */
+    float *next_scores;      /* [batch][best], as the outputs below; none may overlap an input or another */
     int32_t *parents;
     int32_t *tokens;
     int32_t *next_finished; /* or NULL */

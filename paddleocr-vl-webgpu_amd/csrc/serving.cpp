@@ -217,6 +217,8 @@ pvlc_hip_status pvlc_hip_kv_pages_compact(const pvlc_hip_kv_pool *pool, int32_t 
     if (pvlc_hip_status st = check_pool(pool, rows, &planes, &ws)) return st;
     if (rows && !tables) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "compaction tables pointer is NULL");
     if (!aligned(tables, 4) || !aligned(forward, 4)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "compaction tables and map must be 4-byte aligned");
+    if (overlap(tables, static_cast<uint64_t>(rows) * pool->max_blocks_per_seq * 4, forward, forward ? pool->num_blocks * 4ull : 0))
+        return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "a compaction's map may not overlap its tables");
     auto *base = static_cast<unsigned char *>(pool->workspace);
     PagesCompact c{};
     c.num_blocks = pool->num_blocks;
@@ -283,11 +285,15 @@ pvlc_hip_status pvlc_hip_beam_select_f32(const pvlc_hip_beam_args *args, void *s
         if (!aligned(p, 4)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "beam buffers must be 4-byte aligned");
     if (args->row_stride > UINT64_MAX / 8 / rows) return invalid(PVLC_HIP_INV_ARITHMETIC_OVERFLOW, "the rows of logits exceed 64 bits");
     const uint64_t in = rows * 4, out = static_cast<uint64_t>(args->batch) * args->best * 4, read = ((rows - 1) * args->row_stride + args->vocab) * 4;
-    for (const void *p : {static_cast<const void *>(args->next_scores), static_cast<const void *>(args->parents), static_cast<const void *>(args->tokens),
-                          static_cast<const void *>(args->next_finished)})
+    const void *outputs[] = {args->next_scores, args->parents, args->tokens, args->next_finished};
+    for (const void *p : outputs)
         if (overlap(p, p ? out : 0, args->scores, in) || overlap(p, p ? out : 0, args->finished, args->finished ? in : 0) ||
             overlap(p, p ? out : 0, args->logits, read))
             return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "the selection's outputs may not overlap its logits, scores or finished flags");
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(outputs[i], outputs[i] ? out : 0, outputs[j], outputs[j] ? out : 0))
+                return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "the selection's outputs may not overlap one another");
     const BeamWorkspace ws = beam_workspace_layout(args->batch, args->beams, args->vocab, args->best);
     if (args->workspace_bytes < ws.total)
         return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "beam workspace holds " + std::to_string(args->workspace_bytes) + " bytes but the call needs " +
