@@ -33,16 +33,16 @@
 //
 // What bounds it.  512 bytes a token and 8192 operations: memory, once a launch is
 // long.  256 sequences of 1024 to 32768 rows (1.20 GB): 216-222 us (int8 221-232,
-// with f32 operands 223-244) and the merge 8-9, 5.4 TB/s, where a copy reaches 5.1; the
-// fp16 cache's takes 453 us.  Short
-// launches are a chain of rounds: one sequence of 1157 rows 7.8 us, thirteen up to
-// 2010 7.9, 18 caches of 2048 rows (19 MB) 9.5 in e4m3 and 10.0 in int8, whose
-// conversion takes more instructions; f32 operands and int8 8.2, 8.9 and 10.7.  Time stamps of the waves
-// put 0.75 us of that into the new row (its rounding and the LDS detour to the
-// wave's own registers), 0.8 into the hand-off and 1.3 into the merge; the rest is
-// the launch, the block ids and one round of loads.  Measured slower and not kept:
-// the merge's loads issued for every slot without a branch, and the new row's codes
-// read from LDS ahead of the loop.
+// with f32 operands 223-244) and the merge 8-9, 5.4 TB/s, where a copy reaches 5.1;
+// the fp16 cache's takes 453 us.  Short launches are a chain of rounds: one
+// sequence of 1157 rows 7.8 us (f32 operands), thirteen up to 2010 7.9, 18 caches
+// of 2048 rows (19 MB) 9.5 in e4m3 and 10.0 in int8, whose conversion takes more
+// instructions; in int8 with f32 operands 8.2, 8.9 and 10.7.  Time stamps of the
+// waves put 0.75 us of that into the new row (its rounding and the LDS detour to
+// the wave's own registers), 0.8 into the hand-off and 1.3 into the merge; the
+// rest is the launch, the block ids and one round of loads.  Measured slower and
+// not kept: the merge's loads issued for every slot without a branch, and the new
+// row's codes read from LDS ahead of the loop.
 
 #include <hip/hip_runtime.h>
 
