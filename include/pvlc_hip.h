@@ -553,6 +553,8 @@ pvlc_hip_status pvlc_hip_kv_unpack_f16(const uint16_t *key_cache, const uint16_t
  * and by up to 2^(e-10) for those below 2^(e-6): e4m3 for blocks with outlying
  * channels.  A row that is rounded again is off by up to as much once more. */
 enum { PVLC_HIP_KV_E4M3 = 0, PVLC_HIP_KV_INT8 = 1 };
+/* The fp16 planes, in the calls that take either cache. */
+enum { PVLC_HIP_KV_F16 = 2 };
 
 /* pvlc_hip_paged_decode_args with an 8-bit cache. */
 typedef struct pvlc_hip_paged_decode_q8_args {
@@ -709,6 +711,96 @@ pvlc_hip_status pvlc_hip_kv_pages_compact(const pvlc_hip_kv_pool *pool, int32_t 
  * planes and layers.  Pages written must be distinct and none of those read. */
 pvlc_hip_status pvlc_hip_kv_pages_copy(const pvlc_hip_kv_pool *from, const int32_t *from_blocks, const pvlc_hip_kv_pool *to,
                                        const int32_t *to_blocks, uint32_t count, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Batches over paged caches: several sequences' rows in one call (new: the
+ * reference prefills one prompt at a time, into one contiguous cache).
+ *
+ * Rows are packed: sequence s has the rows row_offsets[s] .. row_offsets[s+1]-1
+ * of the call's matrices (row_offsets NULL: rows / num_seqs each), any number of
+ * them, none included.  They follow the cache_lens[s] rows that its pages hold
+ * (cache_lens NULL: none), in the blocks that its table names; the tables,
+ * lengths and offsets are device memory and are not changed.  A block that a
+ * call writes to belongs to one sequence alone (see the fork of pages); what a
+ * block holds behind a sequence's last row is neither used nor changed.
+ * Matrices and planes are 16-byte aligned.  Everything runs on the caller's
+ * stream, without allocation, synchronisation or a copy to the host, and may be
+ * captured; calls on one workspace are stream-ordered.
+ *
+ * Device error bits (of error_word, or the first word of a workspace, which
+ * pvlc_hip_workspace_error reads): 1 = offsets that descend or pass `rows`, a
+ * negative length, or rows that pass a sequence's table (the sequence is skipped;
+ * with such offsets others may be, too); 2 = a block id outside the planes (its
+ * rows are not written, block 0 is read); 4 = a rotary position outside the
+ * tables (no rotation).
+ * ------------------------------------------------------------------------- */
+
+/* Rows rotated and written into pages. */
+typedef struct pvlc_hip_kv_append_args {
+    uint32_t num_seqs;
+    uint32_t rows; /* of key and value; rows behind the last sequence's are not used */
+    uint32_t num_blocks;
+    uint32_t max_blocks_per_seq;
+    uint32_t code; /* PVLC_HIP_KV_F16, PVLC_HIP_KV_E4M3 or PVLC_HIP_KV_INT8 */
+    const int32_t *row_offsets;  /* [num_seqs+1] or NULL */
+    const int32_t *block_tables; /* [num_seqs][max_blocks_per_seq] or NULL (contiguous) */
+    const int32_t *cache_lens;   /* [num_seqs] or NULL */
+    void *key_cache;             /* planes of the code's layout */
+    void *value_cache;
+    uint8_t *exponents;    /* of 8-bit planes */
+    uint64_t key_stride;   /* elements from row to row (a multiple of 16 bytes); 0: 256, compact rows */
+    uint64_t value_stride; /* (slices of one q|k|v matrix: 2560) */
+    const float *rope_cos; /* [rope_rows][64] or NULL: no rotary */
+    const float *rope_sin;
+    uint32_t rope_rows;
+    const int32_t *positions; /* [rows] rotary positions, or NULL: the row's place in its sequence */
+    uint32_t *error_word;     /* optional, caller-zeroed */
+} pvlc_hip_kv_append_args;
+
+/* Keys are rotated in f32 (products and sum each rounded) and rounded to fp16,
+ * values rounded to fp16, as pvlc_hip_paged_decode_f16 / _f32io append theirs;
+ * 8-bit pages take them as pvlc_hip_kv_pack_q8 does.  key and value: rows of
+ * [2][128], fp16 or f32.  They may not overlap the planes. */
+pvlc_hip_status pvlc_hip_kv_append_f16(const pvlc_hip_kv_append_args *args, const uint16_t *key, const uint16_t *value,
+                                       void *stream);
+pvlc_hip_status pvlc_hip_kv_append_f32(const pvlc_hip_kv_append_args *args, const float *key, const float *value,
+                                       void *stream);
+
+/* Packed prompts, or chunks of prompts, over fp16 pages. */
+typedef struct pvlc_hip_packed_prefill_args {
+    uint32_t num_seqs;
+    uint32_t rows;
+    uint32_t num_blocks;
+    uint32_t max_blocks_per_seq;
+    uint32_t max_context; /* >= cache_len + rows of every sequence (sizes the workspace and the launch) */
+    const int32_t *row_offsets;
+    const int32_t *block_tables;
+    const int32_t *cache_lens;
+    uint16_t *key_cache;
+    uint16_t *value_cache;
+    uint64_t query_stride; /* elements; 0: 2048 */
+    uint64_t key_stride;
+    uint64_t value_stride;
+    const float *rope_cos;
+    const float *rope_sin;
+    uint32_t rope_rows;
+    const int32_t *positions;
+    void *workspace; /* pvlc_hip_packed_prefill_workspace_bytes, 256-byte aligned, zeroed once */
+    size_t workspace_bytes;
+} pvlc_hip_packed_prefill_args;
+
+size_t pvlc_hip_packed_prefill_workspace_bytes(uint32_t num_seqs, uint32_t rows, uint32_t max_context);
+/* Every sequence's rows appended (as pvlc_hip_kv_append_f16) and attended: row i
+ * of sequence s to the cache_lens[s] + i + 1 rows up to itself, its query rotated
+ * as the key is.  query: rows of [16][128]; out: [rows][16][128], compact, of
+ * which only the sequences' rows are written.  Arithmetic as
+ * pvlc_hip_paged_prefill_f16, and, with f32 operands, pvlc_hip_paged_prefill_f32io.
+ * A sequence longer than max_context is skipped (error bit 1).  The output may
+ * overlap no input and no plane. */
+pvlc_hip_status pvlc_hip_packed_prefill_f16(const pvlc_hip_packed_prefill_args *args, const uint16_t *query,
+                                            const uint16_t *key, const uint16_t *value, uint16_t *out, void *stream);
+pvlc_hip_status pvlc_hip_packed_prefill_f32io(const pvlc_hip_packed_prefill_args *args, const float *query,
+                                              const float *key, const float *value, float *out, void *stream);
 
 /* ---------------------------------------------------------------------------
  * Decoder GEMV with fp16 weights (the next path widened from this backend).

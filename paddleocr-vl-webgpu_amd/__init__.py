@@ -41,6 +41,8 @@ BLOCK_TOKENS = 16
 # Codes of the 8-bit cache
 KV_E4M3 = 0
 KV_INT8 = 1
+# The fp16 planes, in the calls that take either cache
+KV_F16 = 2
 # Device error bits of a page pool
 PAGES_EXHAUSTED, PAGES_BAD_LENGTH, PAGES_BAD_PARENT, PAGES_BAD_BLOCK, PAGES_BAD_COUNT, PAGES_NO_ROOM = 1, 2, 4, 8, 16, 32
 
@@ -206,6 +208,22 @@ class BeamArgsC(ctypes.Structure):
                 ("workspace_bytes", _SZ)]
 
 
+class KvAppendArgsC(ctypes.Structure):
+    _fields_ = [("num_seqs", _U32), ("rows", _U32), ("num_blocks", _U32), ("max_blocks_per_seq", _U32), ("code", _U32),
+                ("row_offsets", _VP), ("block_tables", _VP), ("cache_lens", _VP), ("key_cache", _VP),
+                ("value_cache", _VP), ("exponents", _VP), ("key_stride", ctypes.c_uint64),
+                ("value_stride", ctypes.c_uint64), ("rope_cos", _VP), ("rope_sin", _VP), ("rope_rows", _U32),
+                ("positions", _VP), ("error_word", _VP)]
+
+
+class PackedPrefillArgsC(ctypes.Structure):
+    _fields_ = [("num_seqs", _U32), ("rows", _U32), ("num_blocks", _U32), ("max_blocks_per_seq", _U32),
+                ("max_context", _U32), ("row_offsets", _VP), ("block_tables", _VP), ("cache_lens", _VP),
+                ("key_cache", _VP), ("value_cache", _VP), ("query_stride", ctypes.c_uint64),
+                ("key_stride", ctypes.c_uint64), ("value_stride", ctypes.c_uint64), ("rope_cos", _VP),
+                ("rope_sin", _VP), ("rope_rows", _U32), ("positions", _VP), ("workspace", _VP), ("workspace_bytes", _SZ)]
+
+
 class PagedPrefillArgsC(ctypes.Structure):
     _fields_ = [("tokens", _U32), ("num_blocks", _U32), ("block_table", _VP), ("key_cache", _VP),
                 ("value_cache", _VP), ("query", _VP), ("key", _VP), ("value", _VP), ("out", _VP),
@@ -264,6 +282,11 @@ SIGNATURES = {
     "pvlc_hip_kv_pages_fork": ([ctypes.POINTER(KvPoolC), ctypes.POINTER(KvForkArgsC), _VP], ctypes.c_int32),
     "pvlc_hip_kv_pages_compact": ([ctypes.POINTER(KvPoolC), _VP, _U32, _VP, _VP], ctypes.c_int32),
     "pvlc_hip_kv_pages_copy": ([ctypes.POINTER(KvPoolC), _VP, ctypes.POINTER(KvPoolC), _VP, _U32, _VP], ctypes.c_int32),
+    "pvlc_hip_kv_append_f16": ([ctypes.POINTER(KvAppendArgsC), _VP, _VP, _VP], ctypes.c_int32),
+    "pvlc_hip_kv_append_f32": ([ctypes.POINTER(KvAppendArgsC), _VP, _VP, _VP], ctypes.c_int32),
+    "pvlc_hip_packed_prefill_workspace_bytes": ([_U32, _U32, _U32], _SZ),
+    "pvlc_hip_packed_prefill_f16": ([ctypes.POINTER(PackedPrefillArgsC), _VP, _VP, _VP, _VP, _VP], ctypes.c_int32),
+    "pvlc_hip_packed_prefill_f32io": ([ctypes.POINTER(PackedPrefillArgsC), _VP, _VP, _VP, _VP, _VP], ctypes.c_int32),
     "pvlc_hip_beam_workspace_bytes": ([_U32, _U32, _U32, _U32], _SZ),
     "pvlc_hip_beam_select_f32": ([ctypes.POINTER(BeamArgsC), _VP], ctypes.c_int32),
     "pvlc_hip_gemv_tiled_plan_create": ([_U32, _U32, ctypes.POINTER(GemvTiledPlanC)], ctypes.c_int32),
@@ -868,6 +891,53 @@ def kv_unpack_q8(key_cache, value_cache, exponents, tokens, key_rows, value_rows
     """Rows 0..tokens-1 of a sequence's 8-bit blocks as fp16."""
     _check(lib.pvlc_hip_kv_unpack_q8(_ptr(key_cache), _ptr(value_cache), _ptr(exponents), tokens, _ptr(block_table),
                                      num_blocks, code, _ptr(key_rows), _ptr(value_rows), _stream(stream)))
+
+
+def kv_append_args(*, num_seqs, rows, num_blocks, max_blocks_per_seq, code, key_cache, value_cache, exponents=None,
+                   row_offsets=None, block_tables=None, cache_lens=None, key_stride=0, value_stride=0, rope_cos=None,
+                   rope_sin=None, rope_rows=0, positions=None, error_word=None) -> KvAppendArgsC:
+    """Rows of several sequences for their pages: those of sequence s are row_offsets[s]..row_offsets[s+1]-1 (None:
+    rows / num_seqs each), behind the cache_lens[s] rows that it has; ``code``: KV_F16, KV_E4M3 or KV_INT8."""
+    return KvAppendArgsC(num_seqs, rows, num_blocks, max_blocks_per_seq, code, _ptr(row_offsets), _ptr(block_tables),
+                         _ptr(cache_lens), _ptr(key_cache), _ptr(value_cache), _ptr(exponents), key_stride,
+                         value_stride, _ptr(rope_cos), _ptr(rope_sin), rope_rows, _ptr(positions), _ptr(error_word))
+
+
+def kv_append_f16(args: KvAppendArgsC, key, value, stream=None) -> None:
+    """fp16 rows [2][128], keys rotated on the way, into the pages of their sequences."""
+    _check(lib.pvlc_hip_kv_append_f16(ctypes.byref(args), _ptr(key), _ptr(value), _stream(stream)))
+
+
+def kv_append_f32(args: KvAppendArgsC, key, value, stream=None) -> None:
+    """kv_append_f16 with f32 rows, rounded to fp16 after the rotation."""
+    _check(lib.pvlc_hip_kv_append_f32(ctypes.byref(args), _ptr(key), _ptr(value), _stream(stream)))
+
+
+def packed_prefill_workspace_bytes(num_seqs: int, rows: int, max_context: int) -> int:
+    return lib.pvlc_hip_packed_prefill_workspace_bytes(num_seqs, rows, max_context)
+
+
+def packed_prefill_args(*, num_seqs, rows, num_blocks, max_blocks_per_seq, max_context, key_cache, value_cache,
+                        workspace, workspace_bytes, row_offsets=None, block_tables=None, cache_lens=None,
+                        query_stride=0, key_stride=0, value_stride=0, rope_cos=None, rope_sin=None, rope_rows=0,
+                        positions=None) -> PackedPrefillArgsC:
+    """Prompts of several sequences, or chunks of them, packed as kv_append_args packs rows, over fp16 pages."""
+    return PackedPrefillArgsC(num_seqs, rows, num_blocks, max_blocks_per_seq, max_context, _ptr(row_offsets),
+                              _ptr(block_tables), _ptr(cache_lens), _ptr(key_cache), _ptr(value_cache), query_stride,
+                              key_stride, value_stride, _ptr(rope_cos), _ptr(rope_sin), rope_rows, _ptr(positions),
+                              _ptr(workspace), workspace_bytes)
+
+
+def packed_prefill_f16(args: PackedPrefillArgsC, query, key, value, out, stream=None) -> None:
+    """The rows rotated, appended and attended, each causal over its own sequence: out [rows][16][128]."""
+    _check(lib.pvlc_hip_packed_prefill_f16(ctypes.byref(args), _ptr(query), _ptr(key), _ptr(value), _ptr(out),
+                                           _stream(stream)))
+
+
+def packed_prefill_f32io(args: PackedPrefillArgsC, query, key, value, out, stream=None) -> None:
+    """packed_prefill_f16 with f32 query, key, value and output."""
+    _check(lib.pvlc_hip_packed_prefill_f32io(ctypes.byref(args), _ptr(query), _ptr(key), _ptr(value), _ptr(out),
+                                             _stream(stream)))
 
 
 def kv_pages_workspace_bytes(num_blocks: int, rows: int) -> int:

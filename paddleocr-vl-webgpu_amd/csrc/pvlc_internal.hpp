@@ -213,6 +213,51 @@ struct PrefillOperands32 {
 };
 int launch_prefill(const pvlc_hip_paged_prefill_args *args, void *stream, const PrefillOperands32 *f32 = nullptr);
 
+// Rows of several sequences in one call (ragged_device.hpp): those of sequence
+// s are offsets[s] .. offsets[s + 1] - 1 (without offsets: `each` rows apiece),
+// and its pages hold lens[s] rows before them (without lens: none).
+struct RaggedRows {
+    uint32_t num_seqs, rows, each;
+    const int32_t *offsets, *lens;
+    uint32_t num_blocks, max_blocks;
+    const int32_t *tables;
+    uint32_t max_tokens;  // that a sequence may come to hold
+};
+// Rows appended to their pages (kernels_append.hip); strides in elements.
+struct AppendRows {
+    RaggedRows ragged;
+    uint32_t code;
+    bool f32;
+    const void *key, *value;
+    int64_t key_stride, value_stride;
+    const float *rope_cos, *rope_sin;
+    uint32_t rope_rows;
+    const int32_t *positions;
+    void *key_cache, *value_cache;
+    uint8_t *exponents;
+    uint32_t *error_word;
+};
+int launch_kv_append(const AppendRows &rows, void *stream);
+// Packed prompts over pages that hold their rows (kernels_packed.hip).
+struct PackedRows {
+    RaggedRows ragged;
+    bool f32;
+    const void *query;
+    void *out;
+    int64_t query_stride;
+    const float *rope_cos, *rope_sin;
+    uint32_t rope_rows;
+    const int32_t *positions;
+    const uint16_t *key_cache, *value_cache;
+    float scale_log2;
+};
+int launch_packed_prefill(const PackedRows &rows, void *stream);
+// Its workspace: 256 bytes of words (0 the error word).
+struct PackedWorkspace {
+    size_t total;
+};
+inline PackedWorkspace packed_workspace_layout(uint32_t, uint32_t, uint32_t) { return {256}; }
+
 // Prefill projection with fp16 weights: workspace of the exact hi/lo split
 // of the activations ([rows][K] fp16 each) and the per-row exponents.
 // Workspace of the projection: the hi/lo planes of the split activations in
