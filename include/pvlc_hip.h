@@ -802,6 +802,48 @@ pvlc_hip_status pvlc_hip_packed_prefill_f16(const pvlc_hip_packed_prefill_args *
 pvlc_hip_status pvlc_hip_packed_prefill_f32io(const pvlc_hip_packed_prefill_args *args, const float *query,
                                               const float *key, const float *value, float *out, void *stream);
 
+/* One decode step of groups of sequences whose first pages are the same ones: the
+ * beams of a page, answers to one prompt, requests behind one instruction. */
+typedef struct pvlc_hip_shared_decode_args {
+    uint32_t num_seqs;
+    uint32_t num_groups;
+    uint32_t num_blocks;
+    uint32_t max_blocks_per_seq;
+    uint32_t code;                /* PVLC_HIP_KV_F16, PVLC_HIP_KV_E4M3 or PVLC_HIP_KV_INT8 */
+    const int32_t *group_offsets; /* [num_groups+1]: group g is the sequences group_offsets[g] .. group_offsets[g+1]-1; NULL:
+                                     num_seqs / num_groups each */
+    const int32_t *shared_lens;   /* [num_groups] rows that a group's sequences have in common */
+    const int32_t *block_tables;  /* [num_seqs][max_blocks_per_seq] */
+    const int32_t *cache_lens;    /* [num_seqs] rows already cached */
+    uint32_t max_context;         /* >= cache_len + 1 of every sequence */
+    void *key_cache;
+    void *value_cache;
+    uint8_t *exponents;
+    const float *rope_cos;
+    const float *rope_sin;
+    uint32_t rope_rows;
+    const int32_t *positions; /* [num_seqs] or NULL: cache_len */
+    uint32_t rotate_query;
+    void *workspace; /* pvlc_hip_shared_decode_workspace_bytes, 256-byte aligned, zeroed once */
+    size_t workspace_bytes;
+} pvlc_hip_shared_decode_args;
+
+size_t pvlc_hip_shared_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context);
+/* pvlc_hip_paged_decode_f16 / _q8_f16 of every sequence (rotation, append,
+ * attention over cache_len + 1 rows, and their arithmetic), with the first
+ * shared_lens[g] rows of a group read once for all of it, through its first
+ * sequence's table, whose entries the others repeat: rows in whole blocks of 16,
+ * and no more than the group's shortest sequence has (so a prompt's length may
+ * stand there although its last block has been copied).  Any number of sequences
+ * may share any number of rows, none included; every sequence is in one group
+ * (others are appended to, and not attended).  query [num_seqs][16][128], new_key
+ * and new_value [num_seqs][2][128], out [num_seqs][16][128], compact. */
+pvlc_hip_status pvlc_hip_shared_decode_f16(const pvlc_hip_shared_decode_args *args, const uint16_t *query,
+                                           const uint16_t *new_key, const uint16_t *new_value, uint16_t *out,
+                                           void *stream);
+pvlc_hip_status pvlc_hip_shared_decode_f32io(const pvlc_hip_shared_decode_args *args, const float *query,
+                                             const float *new_key, const float *new_value, float *out, void *stream);
+
 /* ---------------------------------------------------------------------------
  * Decoder GEMV with fp16 weights (the next path widened from this backend).
  * ------------------------------------------------------------------------- */

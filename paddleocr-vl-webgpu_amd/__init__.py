@@ -224,6 +224,14 @@ class PackedPrefillArgsC(ctypes.Structure):
                 ("rope_sin", _VP), ("rope_rows", _U32), ("positions", _VP), ("workspace", _VP), ("workspace_bytes", _SZ)]
 
 
+class SharedDecodeArgsC(ctypes.Structure):
+    _fields_ = [("num_seqs", _U32), ("num_groups", _U32), ("num_blocks", _U32), ("max_blocks_per_seq", _U32),
+                ("code", _U32), ("group_offsets", _VP), ("shared_lens", _VP), ("block_tables", _VP),
+                ("cache_lens", _VP), ("max_context", _U32), ("key_cache", _VP), ("value_cache", _VP),
+                ("exponents", _VP), ("rope_cos", _VP), ("rope_sin", _VP), ("rope_rows", _U32), ("positions", _VP),
+                ("rotate_query", _U32), ("workspace", _VP), ("workspace_bytes", _SZ)]
+
+
 class PagedPrefillArgsC(ctypes.Structure):
     _fields_ = [("tokens", _U32), ("num_blocks", _U32), ("block_table", _VP), ("key_cache", _VP),
                 ("value_cache", _VP), ("query", _VP), ("key", _VP), ("value", _VP), ("out", _VP),
@@ -287,6 +295,9 @@ SIGNATURES = {
     "pvlc_hip_packed_prefill_workspace_bytes": ([_U32, _U32, _U32], _SZ),
     "pvlc_hip_packed_prefill_f16": ([ctypes.POINTER(PackedPrefillArgsC), _VP, _VP, _VP, _VP, _VP], ctypes.c_int32),
     "pvlc_hip_packed_prefill_f32io": ([ctypes.POINTER(PackedPrefillArgsC), _VP, _VP, _VP, _VP, _VP], ctypes.c_int32),
+    "pvlc_hip_shared_decode_workspace_bytes": ([_U32, _U32, _U32], _SZ),
+    "pvlc_hip_shared_decode_f16": ([ctypes.POINTER(SharedDecodeArgsC), _VP, _VP, _VP, _VP, _VP], ctypes.c_int32),
+    "pvlc_hip_shared_decode_f32io": ([ctypes.POINTER(SharedDecodeArgsC), _VP, _VP, _VP, _VP, _VP], ctypes.c_int32),
     "pvlc_hip_beam_workspace_bytes": ([_U32, _U32, _U32, _U32], _SZ),
     "pvlc_hip_beam_select_f32": ([ctypes.POINTER(BeamArgsC), _VP], ctypes.c_int32),
     "pvlc_hip_gemv_tiled_plan_create": ([_U32, _U32, ctypes.POINTER(GemvTiledPlanC)], ctypes.c_int32),
@@ -938,6 +949,34 @@ def packed_prefill_f32io(args: PackedPrefillArgsC, query, key, value, out, strea
     """packed_prefill_f16 with f32 query, key, value and output."""
     _check(lib.pvlc_hip_packed_prefill_f32io(ctypes.byref(args), _ptr(query), _ptr(key), _ptr(value), _ptr(out),
                                              _stream(stream)))
+
+
+def shared_decode_workspace_bytes(num_seqs: int, num_groups: int, max_context: int) -> int:
+    return lib.pvlc_hip_shared_decode_workspace_bytes(num_seqs, num_groups, max_context)
+
+
+def shared_decode_args(*, num_seqs, num_groups, num_blocks, max_blocks_per_seq, shared_lens, block_tables, cache_lens,
+                       max_context, key_cache, value_cache, workspace, workspace_bytes, code=KV_F16, exponents=None,
+                       group_offsets=None, rope_cos=None, rope_sin=None, rope_rows=0, positions=None,
+                       rotate_query=False) -> SharedDecodeArgsC:
+    """A decode step of groups of sequences (group g: group_offsets[g]..group_offsets[g+1]-1; None: num_seqs /
+    num_groups each) whose first shared_lens[g] rows lie in the same pages."""
+    return SharedDecodeArgsC(num_seqs, num_groups, num_blocks, max_blocks_per_seq, code, _ptr(group_offsets),
+                             _ptr(shared_lens), _ptr(block_tables), _ptr(cache_lens), max_context, _ptr(key_cache),
+                             _ptr(value_cache), _ptr(exponents), _ptr(rope_cos), _ptr(rope_sin), rope_rows,
+                             _ptr(positions), int(rotate_query), _ptr(workspace), workspace_bytes)
+
+
+def shared_decode_f16(args: SharedDecodeArgsC, query, new_key, new_value, out, stream=None) -> None:
+    """Rotation, append and attention of one token for every sequence, a group's shared rows read once for all of it."""
+    _check(lib.pvlc_hip_shared_decode_f16(ctypes.byref(args), _ptr(query), _ptr(new_key), _ptr(new_value), _ptr(out),
+                                          _stream(stream)))
+
+
+def shared_decode_f32io(args: SharedDecodeArgsC, query, new_key, new_value, out, stream=None) -> None:
+    """shared_decode_f16 with f32 query, new key and value and output."""
+    _check(lib.pvlc_hip_shared_decode_f32io(ctypes.byref(args), _ptr(query), _ptr(new_key), _ptr(new_value), _ptr(out),
+                                            _stream(stream)))
 
 
 def kv_pages_workspace_bytes(num_blocks: int, rows: int) -> int:

@@ -1,5 +1,5 @@
 // Entry points of batches over paged caches (appends of several sequences' rows,
-// packed prompts): argument checks before any GPU effect, then the launches.
+// packed prompts, decode with shared pages): argument checks before any GPU effect, then the launches.
 
 #include <cstdint>
 #include <initializer_list>
@@ -26,44 +26,6 @@ bool overlap(const Range &a, const Range &b) {
     return a.at && b.at && a.bytes && b.bytes && x < y + b.bytes && y < x + a.bytes;
 }
 
-pvlc_hip_status apart(std::initializer_list<Range> written, std::initializer_list<Range> read, const char *what) {
-    for (const Range *w = written.begin(); w != written.end(); ++w) {
-        for (const Range &r : read)
-            if (overlap(*w, r)) return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, std::string(what) + " overlap its inputs");
-        for (const Range *v = written.begin(); v != w; ++v)
-            if (overlap(*w, *v)) return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, std::string(what) + " overlap one another");
-    }
-    return PVLC_HIP_OK;
-}
-
-// What the calls of this file have in common.
-template <class Args>
-pvlc_hip_status check_rows(const Args *a, uint32_t share, uint32_t spare) {
-    if (a->num_seqs == 0 || a->rows == 0 || a->num_blocks == 0 || a->max_blocks_per_seq == 0)
-        return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "sequences, rows, blocks and table width must be nonzero");
-    if (a->rows > 0x7FFFFFFFu || a->num_blocks > 0x7FFFFFFFu || a->max_blocks_per_seq > 0x7FFFFFFFu / kBlockTokens)
-        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows, blocks and a table row's tokens must be below 2^31");
-    if (a->rows / share + static_cast<uint64_t>(spare) * a->num_seqs >= kMaxGroups)
-        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows and sequences exceed the grid");
-    if (!a->row_offsets && a->rows % a->num_seqs != 0)
-        return invalid(PVLC_HIP_INV_INVALID_SEQUENCE_BOUNDARIES, "without offsets the rows must divide among the sequences");
-    if (!a->block_tables && static_cast<uint64_t>(a->num_seqs) * a->max_blocks_per_seq > a->num_blocks)
-        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "the sequences' contiguous blocks exceed the planes");
-    for (const void *p : {static_cast<const void *>(a->row_offsets), static_cast<const void *>(a->block_tables),
-                          static_cast<const void *>(a->cache_lens), static_cast<const void *>(a->positions)})
-        if (!aligned(p, 4)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "offsets, tables, lengths and positions must be 4-byte aligned");
-    return PVLC_HIP_OK;
-}
-
-template <class Args>
-pvlc_hip_status check_rope(const Args *a) {
-    if ((a->rope_cos == nullptr) != (a->rope_sin == nullptr) || (a->rope_cos && a->rope_rows == 0))
-        return invalid(PVLC_HIP_INV_INVALID_ROTARY_DIMENSION, "rotary tables must be given together with rows");
-    if (!aligned(a->rope_cos, 16) || !aligned(a->rope_sin, 16))
-        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "rotary tables must be 16-byte aligned");
-    return PVLC_HIP_OK;
-}
-
 pvlc_hip_status check_planes(uint32_t code, const void *keys, const void *values, const void *exponents) {
     if (code != PVLC_HIP_KV_F16 && code != PVLC_HIP_KV_E4M3 && code != PVLC_HIP_KV_INT8)
         return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT,
@@ -73,10 +35,6 @@ pvlc_hip_status check_planes(uint32_t code, const void *keys, const void *values
     if (!aligned(keys, 16) || !aligned(values, 16) || (code != PVLC_HIP_KV_F16 && !aligned(exponents, 4)))
         return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "cache planes must be 16-byte aligned, exponents 4-byte aligned");
     return PVLC_HIP_OK;
-}
-
-uint64_t plane_bytes(uint32_t num_blocks, uint32_t code) {
-    return static_cast<uint64_t>(num_blocks) * kKvHeads * kBlockHeadElems * (code == PVLC_HIP_KV_F16 ? 2 : 1);
 }
 
 // A matrix of `rows` rows of `width` elements, `stride` (0: width) apart.
@@ -91,108 +49,139 @@ pvlc_hip_status check_matrix(const void *at, uint64_t *stride, uint32_t rows, ui
     return PVLC_HIP_OK;
 }
 
+// An append's arguments, the overlaps aside, as the kernels take them.
+pvlc_hip_status check_append(const pvlc_hip_kv_append_args *args, const void *key, const void *value, bool f32, AppendRows *out, Range *keys,
+                             Range *values) {
+    if (pvlc_hip_status st = check_planes(args->code, args->key_cache, args->value_cache, args->exponents)) return st;
+    if (args->num_seqs == 0 || args->rows == 0 || args->num_blocks == 0 || args->max_blocks_per_seq == 0)
+        return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "sequences, rows, blocks and table width must be nonzero");
+    if (args->rows > 0x7FFFFFFFu || args->num_blocks > 0x7FFFFFFFu || args->max_blocks_per_seq > 0x7FFFFFFFu / kBlockTokens)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows, blocks and a table row's tokens must be below 2^31");
+    if (args->rows / kBlockTokens + 2ull * args->num_seqs >= kMaxGroups)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows and sequences exceed the grid");
+    if (!args->row_offsets && args->rows % args->num_seqs != 0)
+        return invalid(PVLC_HIP_INV_INVALID_SEQUENCE_BOUNDARIES, "without offsets the rows must divide among the sequences");
+    if (!args->block_tables && static_cast<uint64_t>(args->num_seqs) * args->max_blocks_per_seq > args->num_blocks)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "the sequences' contiguous blocks exceed the planes");
+    for (const void *p : {static_cast<const void *>(args->row_offsets), static_cast<const void *>(args->block_tables),
+                          static_cast<const void *>(args->cache_lens), static_cast<const void *>(args->positions),
+                          static_cast<const void *>(args->error_word)})
+        if (!aligned(p, 4)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "offsets, tables, lengths, positions and error word must be 4-byte aligned");
+    if ((args->rope_cos == nullptr) != (args->rope_sin == nullptr) || (args->rope_cos && args->rope_rows == 0))
+        return invalid(PVLC_HIP_INV_INVALID_ROTARY_DIMENSION, "rotary tables must be given together with rows");
+    if (!aligned(args->rope_cos, 16) || !aligned(args->rope_sin, 16))
+        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "rotary tables must be 16-byte aligned");
+    const uint32_t size = f32 ? 4 : 2;
+    uint64_t key_stride = args->key_stride, value_stride = args->value_stride;
+    if (pvlc_hip_status st = check_matrix(key, &key_stride, args->rows, kRowElems, size, "key", keys)) return st;
+    if (pvlc_hip_status st = check_matrix(value, &value_stride, args->rows, kRowElems, size, "value", values)) return st;
+    *out = {};
+    out->ragged = {args->num_seqs, args->rows, args->rows / args->num_seqs, args->row_offsets, args->cache_lens, args->num_blocks,
+                   args->max_blocks_per_seq, args->block_tables, args->max_blocks_per_seq * kBlockTokens};
+    out->code = args->code;
+    out->f32 = f32;
+    out->key = key;
+    out->value = value;
+    out->key_stride = static_cast<int64_t>(key_stride);
+    out->value_stride = static_cast<int64_t>(value_stride);
+    out->rope_cos = args->rope_cos;
+    out->rope_sin = args->rope_sin;
+    out->rope_rows = args->rope_rows;
+    out->positions = args->positions;
+    out->key_cache = args->key_cache;
+    out->value_cache = args->value_cache;
+    out->exponents = args->exponents;
+    out->error_word = args->error_word;
+    return PVLC_HIP_OK;
+}
+
+// What the call writes lies apart from what it reads and from one another.
+pvlc_hip_status check_apart(const pvlc_hip_kv_append_args &a, const Range &keys, const Range &values, std::initializer_list<Range> reads,
+                            std::initializer_list<Range> writes) {
+    const uint64_t plane = static_cast<uint64_t>(a.num_blocks) * kKvHeads * kBlockHeadElems * (a.code == PVLC_HIP_KV_F16 ? 2 : 1);
+    Range read[16] = {keys, values,
+                      {a.row_offsets, 4ull * a.num_seqs + 4},
+                      {a.block_tables, 4ull * a.num_seqs * a.max_blocks_per_seq},
+                      {a.cache_lens, 4ull * a.num_seqs},
+                      {a.positions, 4ull * a.rows},
+                      {a.rope_cos, 256ull * a.rope_rows},
+                      {a.rope_sin, 256ull * a.rope_rows}};
+    Range written[8] = {{a.key_cache, plane}, {a.value_cache, plane}, {a.code == PVLC_HIP_KV_F16 ? nullptr : a.exponents, 4ull * a.num_blocks}};
+    int n = 8, m = 3;
+    for (const Range &r : reads) read[n++] = r;
+    for (const Range &r : writes) written[m++] = r;
+    for (int w = 0; w < m; ++w) {
+        for (int r = 0; r < n; ++r)
+            if (overlap(written[w], read[r]))
+                return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "planes, exponents, workspace and output may not overlap the call's inputs");
+        for (int v = 0; v < w; ++v)
+            if (overlap(written[w], written[v]))
+                return invalid(PVLC_HIP_INV_INVALID_ACTIVATION_LAYOUT, "planes, exponents, workspace and output may not overlap");
+    }
+    return PVLC_HIP_OK;
+}
+
 template <class Args>
-RaggedRows ragged_rows(const Args *a) {
-    return {a->num_seqs, a->rows, a->rows / a->num_seqs, a->row_offsets, a->cache_lens, a->num_blocks, a->max_blocks_per_seq, a->block_tables,
-            a->max_blocks_per_seq * kBlockTokens};
+pvlc_hip_status check_context(const Args *a) {
+    if (a->max_context == 0) return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "max_context must be nonzero");
+    if (a->max_context > static_cast<uint64_t>(a->max_blocks_per_seq) * kBlockTokens)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "max_context exceeds a sequence's table");
+    return PVLC_HIP_OK;
+}
+
+template <class Args>
+pvlc_hip_status check_workspace(const Args *a, size_t bytes, const char *what) {
+    if (!a->workspace || !aligned(a->workspace, 256))
+        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, std::string(what) + " workspace must be given, 256-byte aligned");
+    if (a->workspace_bytes < bytes)
+        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, std::string(what) + " workspace holds " + std::to_string(a->workspace_bytes) +
+                                                         " bytes but the call needs " + std::to_string(bytes));
+    return PVLC_HIP_OK;
 }
 
 pvlc_hip_status append(const pvlc_hip_kv_append_args *args, const void *key, const void *value, bool f32, void *stream) {
     if (!args) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "append args are NULL");
-    if (pvlc_hip_status st = check_planes(args->code, args->key_cache, args->value_cache, args->exponents)) return st;
-    if (pvlc_hip_status st = check_rows(args, kBlockTokens, 2)) return st;
-    if (pvlc_hip_status st = check_rope(args)) return st;
-    if (!aligned(args->error_word, 4)) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "the error word must be 4-byte aligned");
-    const uint32_t size = f32 ? 4 : 2;
-    uint64_t key_stride = args->key_stride, value_stride = args->value_stride;
-    Range keys, values;
-    if (pvlc_hip_status st = check_matrix(key, &key_stride, args->rows, kRowElems, size, "key", &keys)) return st;
-    if (pvlc_hip_status st = check_matrix(value, &value_stride, args->rows, kRowElems, size, "value", &values)) return st;
-    const uint64_t bytes = plane_bytes(args->num_blocks, args->code);
-    const bool codes = args->code != PVLC_HIP_KV_F16;
-    if (pvlc_hip_status st = apart({{args->key_cache, bytes},
-                                    {args->value_cache, bytes},
-                                    {codes ? args->exponents : nullptr, 4ull * args->num_blocks},
-                                    {args->error_word, 4}},
-                                   {keys, values,
-                                    {args->row_offsets, 4ull * args->num_seqs + 4},
-                                    {args->block_tables, 4ull * args->num_seqs * args->max_blocks_per_seq},
-                                    {args->cache_lens, 4ull * args->num_seqs},
-                                    {args->positions, 4ull * args->rows},
-                                    {args->rope_cos, 256ull * args->rope_rows},
-                                    {args->rope_sin, 256ull * args->rope_rows}},
-                                   "an append's planes, exponents and error word"))
-        return st;
     AppendRows a{};
-    a.ragged = ragged_rows(args);
-    a.code = args->code;
-    a.f32 = f32;
-    a.key = key;
-    a.value = value;
-    a.key_stride = static_cast<int64_t>(key_stride);
-    a.value_stride = static_cast<int64_t>(value_stride);
-    a.rope_cos = args->rope_cos;
-    a.rope_sin = args->rope_sin;
-    a.rope_rows = args->rope_rows;
-    a.positions = args->positions;
-    a.key_cache = args->key_cache;
-    a.value_cache = args->value_cache;
-    a.exponents = args->exponents;
-    a.error_word = args->error_word;
-    const int e = launch_kv_append(a, stream);
-    if (e != 0) return hip_status(e, "append launch");
+    Range keys, values;
+    if (pvlc_hip_status st = check_append(args, key, value, f32, &a, &keys, &values)) return st;
+    if (pvlc_hip_status st = check_apart(*args, keys, values, {}, {{args->error_word, 4}})) return st;
+    if (const int e = launch_kv_append(a, stream)) return hip_status(e, "append launch");
     return ok();
 }
 
 pvlc_hip_status prefill(const pvlc_hip_packed_prefill_args *args, const void *query, const void *key, const void *value, void *out, bool f32,
                         void *stream) {
     if (!args) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "packed prefill args are NULL");
-    if (pvlc_hip_status st = check_planes(PVLC_HIP_KV_F16, args->key_cache, args->value_cache, nullptr)) return st;
-    if (pvlc_hip_status st = check_rows(args, kBlockTokens, 2)) return st;
-    if (pvlc_hip_status st = check_rope(args)) return st;
-    if (args->max_context == 0) return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "max_context must be nonzero");
-    if (args->max_context > static_cast<uint64_t>(args->max_blocks_per_seq) * kBlockTokens)
-        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "max_context exceeds a sequence's table");
+    pvlc_hip_kv_append_args rows{};
+    rows.num_seqs = args->num_seqs;
+    rows.rows = args->rows;
+    rows.num_blocks = args->num_blocks;
+    rows.max_blocks_per_seq = args->max_blocks_per_seq;
+    rows.code = PVLC_HIP_KV_F16;
+    rows.row_offsets = args->row_offsets;
+    rows.block_tables = args->block_tables;
+    rows.cache_lens = args->cache_lens;
+    rows.key_cache = args->key_cache;
+    rows.value_cache = args->value_cache;
+    rows.key_stride = args->key_stride;
+    rows.value_stride = args->value_stride;
+    rows.rope_cos = args->rope_cos;
+    rows.rope_sin = args->rope_sin;
+    rows.rope_rows = args->rope_rows;
+    rows.positions = args->positions;
+    rows.error_word = static_cast<uint32_t *>(args->workspace);
+    AppendRows a{};
+    Range keys, values;
+    if (pvlc_hip_status st = check_append(&rows, key, value, f32, &a, &keys, &values)) return st;
+    if (pvlc_hip_status st = check_context(args)) return st;
     const uint32_t size = f32 ? 4 : 2;
-    uint64_t query_stride = args->query_stride, key_stride = args->key_stride, value_stride = args->value_stride, out_stride = 0;
-    Range queries, keys, values, outs;
+    uint64_t query_stride = args->query_stride, out_stride = 0;
+    Range queries, outs;
     if (pvlc_hip_status st = check_matrix(query, &query_stride, args->rows, kQueryHeads * kHeadDim, size, "query", &queries)) return st;
-    if (pvlc_hip_status st = check_matrix(key, &key_stride, args->rows, kRowElems, size, "key", &keys)) return st;
-    if (pvlc_hip_status st = check_matrix(value, &value_stride, args->rows, kRowElems, size, "value", &values)) return st;
     if (pvlc_hip_status st = check_matrix(out, &out_stride, args->rows, kQueryHeads * kHeadDim, size, "out", &outs)) return st;
     const PackedWorkspace ws = packed_workspace_layout(args->num_seqs, args->rows, args->max_context);
-    if (!args->workspace || !aligned(args->workspace, 256))
-        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "packed prefill workspace must be given, 256-byte aligned");
-    if (args->workspace_bytes < ws.total)
-        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "packed prefill workspace holds " + std::to_string(args->workspace_bytes) +
-                                                         " bytes but the call needs " + std::to_string(ws.total));
-    const uint64_t bytes = plane_bytes(args->num_blocks, PVLC_HIP_KV_F16);
-    if (pvlc_hip_status st = apart({{args->key_cache, bytes}, {args->value_cache, bytes}, {args->workspace, ws.total}, outs},
-                                   {queries, keys, values,
-                                    {args->row_offsets, 4ull * args->num_seqs + 4},
-                                    {args->block_tables, 4ull * args->num_seqs * args->max_blocks_per_seq},
-                                    {args->cache_lens, 4ull * args->num_seqs},
-                                    {args->positions, 4ull * args->rows},
-                                    {args->rope_cos, 256ull * args->rope_rows},
-                                    {args->rope_sin, 256ull * args->rope_rows}},
-                                   "a packed prefill's planes, workspace and output"))
-        return st;
-    auto *base = static_cast<unsigned char *>(args->workspace);
-    AppendRows a{};
-    a.ragged = ragged_rows(args);
-    a.code = PVLC_HIP_KV_F16;
-    a.f32 = f32;
-    a.key = key;
-    a.value = value;
-    a.key_stride = static_cast<int64_t>(key_stride);
-    a.value_stride = static_cast<int64_t>(value_stride);
-    a.rope_cos = args->rope_cos;
-    a.rope_sin = args->rope_sin;
-    a.rope_rows = args->rope_rows;
-    a.positions = args->positions;
-    a.key_cache = args->key_cache;
-    a.value_cache = args->value_cache;
-    a.error_word = reinterpret_cast<uint32_t *>(base);
+    if (pvlc_hip_status st = check_workspace(args, ws.total, "packed prefill")) return st;
+    if (pvlc_hip_status st = check_apart(rows, keys, values, {queries}, {{args->workspace, ws.total}, outs})) return st;
     a.ragged.max_tokens = args->max_context;
     PackedRows r{};
     r.ragged = a.ragged;
@@ -208,6 +197,80 @@ pvlc_hip_status prefill(const pvlc_hip_packed_prefill_args *args, const void *qu
     r.value_cache = args->value_cache;
     if (const int e = launch_kv_append(a, stream)) return hip_status(e, "packed prefill append launch");
     if (const int e = launch_packed_prefill(r, stream)) return hip_status(e, "packed prefill launch");
+    return ok();
+}
+
+pvlc_hip_status shared(const pvlc_hip_shared_decode_args *args, const void *query, const void *key, const void *value, void *out, bool f32,
+                       void *stream) {
+    if (!args) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "shared decode args are NULL");
+    if (args->num_groups == 0) return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "groups must be nonzero");
+    if (!args->block_tables || !args->cache_lens || !args->shared_lens)
+        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "shared decode tables, lengths and shared lengths must be given");
+    pvlc_hip_kv_append_args rows{};
+    rows.num_seqs = rows.rows = args->num_seqs;
+    rows.num_blocks = args->num_blocks;
+    rows.max_blocks_per_seq = args->max_blocks_per_seq;
+    rows.code = args->code;
+    rows.block_tables = args->block_tables;
+    rows.cache_lens = args->cache_lens;
+    rows.key_cache = args->key_cache;
+    rows.value_cache = args->value_cache;
+    rows.exponents = args->exponents;
+    rows.rope_cos = args->rope_cos;
+    rows.rope_sin = args->rope_sin;
+    rows.rope_rows = args->rope_rows;
+    rows.positions = args->positions;
+    rows.error_word = static_cast<uint32_t *>(args->workspace);
+    AppendRows a{};
+    Range keys, values;
+    if (pvlc_hip_status st = check_append(&rows, key, value, f32, &a, &keys, &values)) return st;
+    if (!args->group_offsets && args->num_seqs % args->num_groups != 0)
+        return invalid(PVLC_HIP_INV_INVALID_SEQUENCE_BOUNDARIES, "without offsets the sequences must divide among the groups");
+    // (a workgroup for each sequence, kv head and part of its rows, at least)
+    if (static_cast<uint64_t>(args->num_seqs) + args->num_groups > 65536u)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "sequences and groups of a shared decode exceed 65536");
+    if (!aligned(args->group_offsets, 4) || !aligned(args->shared_lens, 4))
+        return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "group offsets and shared lengths must be 4-byte aligned");
+    if (pvlc_hip_status st = check_context(args)) return st;
+    const uint32_t size = f32 ? 4 : 2;
+    uint64_t query_stride = 0, out_stride = 0;
+    Range queries, outs;
+    if (pvlc_hip_status st = check_matrix(query, &query_stride, args->num_seqs, kQueryHeads * kHeadDim, size, "query", &queries)) return st;
+    if (pvlc_hip_status st = check_matrix(out, &out_stride, args->num_seqs, kQueryHeads * kHeadDim, size, "out", &outs)) return st;
+    const SharedWorkspace ws = shared_workspace_layout(args->num_seqs, args->num_groups, args->max_context);
+    if (pvlc_hip_status st = check_workspace(args, ws.total, "shared decode")) return st;
+    const Range groups{args->group_offsets, 4ull * args->num_groups + 4}, lens{args->shared_lens, 4ull * args->num_groups};
+    if (pvlc_hip_status st = check_apart(rows, keys, values, {queries, groups, lens}, {{args->workspace, ws.total}, outs})) return st;
+    a.ragged.max_tokens = args->max_context;
+    auto *base = static_cast<unsigned char *>(args->workspace);
+    SharedRows r{};
+    r.ragged = a.ragged;
+    r.num_groups = args->num_groups;
+    r.code = args->code;
+    r.f32 = f32;
+    r.group_offsets = args->group_offsets;
+    r.shared_lens = args->shared_lens;
+    r.query = query;
+    r.out = out;
+    r.rope_cos = args->rope_cos;
+    r.rope_sin = args->rope_sin;
+    r.rope_rows = args->rope_rows;
+    r.positions = args->positions;
+    r.rotate_query = args->rotate_query;
+    r.key_cache = args->key_cache;
+    r.value_cache = args->value_cache;
+    r.exponents = args->exponents;
+    r.error_word = a.error_word;
+    r.columns = ws.columns;
+    r.shares = ws.shares;
+    r.shared_parts = ws.shared_parts;
+    r.own_parts = ws.own_parts;
+    r.part_o = reinterpret_cast<float *>(base + ws.part_o_offset);
+    r.part_ml = reinterpret_cast<float *>(base + ws.part_ml_offset);
+    r.own_o = reinterpret_cast<float *>(base + ws.own_o_offset);
+    r.own_ml = reinterpret_cast<float *>(base + ws.own_ml_offset);
+    if (const int e = launch_kv_append(a, stream)) return hip_status(e, "shared decode append launch");
+    if (const int e = launch_shared_decode(r, stream)) return hip_status(e, "shared decode launch");
     return ok();
 }
 
@@ -236,6 +299,21 @@ pvlc_hip_status pvlc_hip_packed_prefill_f16(const pvlc_hip_packed_prefill_args *
 pvlc_hip_status pvlc_hip_packed_prefill_f32io(const pvlc_hip_packed_prefill_args *args, const float *query, const float *key,
                                               const float *value, float *out, void *stream) {
     return prefill(args, query, key, value, out, true, stream);
+}
+
+size_t pvlc_hip_shared_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context) {
+    if (num_seqs == 0 || num_groups == 0 || max_context == 0) return 0;
+    return shared_workspace_layout(num_seqs, num_groups, max_context).total;
+}
+
+pvlc_hip_status pvlc_hip_shared_decode_f16(const pvlc_hip_shared_decode_args *args, const uint16_t *query, const uint16_t *new_key,
+                                           const uint16_t *new_value, uint16_t *out, void *stream) {
+    return shared(args, query, new_key, new_value, out, false, stream);
+}
+
+pvlc_hip_status pvlc_hip_shared_decode_f32io(const pvlc_hip_shared_decode_args *args, const float *query, const float *new_key,
+                                             const float *new_value, float *out, void *stream) {
+    return shared(args, query, new_key, new_value, out, true, stream);
 }
 
 }  // extern "C"
