@@ -7,6 +7,7 @@
 #include <type_traits>
 
 #include "pvlc_q8.hpp"
+#include "packed_plan.hpp"
 #include "ragged_device.hpp"
 
 namespace pvlc {
@@ -38,7 +39,18 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendRows p) {
     typedef std::conditional_t<F32, float4_t, half8_t> Raw;
     constexpr int kLoads = F32 ? 2 : 1, kElems = F32 ? 4 : 8;
     const int i = threadIdx.x;
-    const SeqRows q = find_share<16, 2>(p.ragged, blockIdx.x);
+    uint32_t share = blockIdx.x;
+    if constexpr (!kQ8) {
+        // A plan for the launch behind this one, by one workgroup more.
+        if (p.plan.items) {
+            if (share == 0) {
+                make_packed_plan(p.ragged, p.plan);
+                return;
+            }
+            --share;
+        }
+    }
+    const SeqRows q = find_share<16, 2>(p.ragged, share);
     if (!q.ok) {
         if (i == 0 && p.error_word) atomicOr(p.error_word, 1u);
         return;  // uniform, as below
@@ -228,7 +240,7 @@ void (*append_kernel(uint32_t code))(AppendRows) {
 }  // namespace
 
 int launch_kv_append(const AppendRows &p, void *stream) {
-    const uint32_t shares = p.ragged.rows / kBlockTokens + 2 * p.ragged.num_seqs;
+    const uint32_t shares = p.ragged.rows / kBlockTokens + 2 * p.ragged.num_seqs + (p.plan.items ? 1 : 0);
     hipLaunchKernelGGL(p.f32 ? append_kernel<true>(p.code) : append_kernel<false>(p.code), dim3(shares), dim3(kThreads), 0,
                        static_cast<hipStream_t>(stream), p);
     return static_cast<int>(hipGetLastError());

@@ -7,87 +7,307 @@
 #include <type_traits>
 
 #include "attend_device.hpp"
+#include "packed_plan.hpp"
 
 namespace pvlc {
 namespace {
 
-constexpr int kF16 = PVLC_HIP_KV_F16;
+typedef float float16_t __attribute__((ext_vector_type(16)));
 
-// A workgroup takes 32 tokens of a sequence and the 8 query heads of a kv head,
-// a wave two of the heads: 64 columns.
-constexpr int kWideTokens = 32, kWideWaves = 4, kWideColumns = 4;
+// A workgroup takes 16 tokens of a sequence and the 8 query heads of a kv head,
+// a wave two of the heads: 32 columns.
+constexpr int kWideWaves = 4, kWideStep = 64;
+constexpr size_t kPartFloats = kPackedPartFloats / kWideWaves;  // of a wave: outputs, references and sums
+constexpr int kStepElems = kWideStep * kHeadDim;  // fp16 elements of a step's keys (or values) of a kv head
 
 template <bool F32>
-__global__ __launch_bounds__(kWideWaves * 64, 1) void packed_wide_kernel(PackedRows p) {
+struct Wide {
     typedef std::conditional_t<F32, float, uint16_t> Element;
-    const uint32_t g = blockIdx.x & 1u;
-    const SeqRows q = find_share<kWideTokens, 1>(p.ragged, (gridDim.x >> 1) - 1 - (blockIdx.x >> 1));
-    const int t0 = q.share * kWideTokens;
-    if (!q.ok || t0 >= q.count) return;  // (the append reports it)
-    const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-    const int h0 = static_cast<int>(g) * kGroup + wave * 2;
-    const int valid = q.held + q.count;
+    const PackedRows &p;
+    const uint32_t g;
+    const int lane, col, half, wave;
+    half8_t qf[8];
+    float16_t o[4];  // dims dt * 32 + (r / 4) * 8 + half * 4 + r % 4 of the lane's query
+    float m, l;
+    int limit;
 
-    // Columns: head ct / 2 of the wave's, tokens t0 + ct % 2 * 16 + row (the last one again past the sequence).
-    half8_t qf[kWideColumns][4];
-    int limit[kWideColumns];
-#pragma unroll
-    for (int th = 0; th < 2; ++th) {
-        const int t = min(t0 + th * 16 + row, q.count - 1);
+    __device__ Wide(const PackedRows &rows, uint32_t head)
+        : p(rows), g(head), lane(threadIdx.x & 63), col(lane & 31), half(lane >> 5),
+          wave(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6))) {}
+
+    __device__ void load_queries(const PackedItem &q, int t0) {
+        const int t = min(t0 + (col & 15), q.count - 1);  // (past the sequence: its last one again, not stored)
         const int64_t at = q.begin + static_cast<int64_t>(t);
         const int64_t pos = p.positions ? p.positions[at] : q.held + static_cast<int64_t>(t);
         const bool rope = p.rope_cos != nullptr && pos >= 0 && pos < static_cast<int64_t>(p.rope_rows);
-        AttendQuery<F32> raw[2][2];
-        const Element *src = static_cast<const Element *>(p.query) + at * p.query_stride + h0 * kHeadDim;
+        const Element *src = static_cast<const Element *>(p.query) + at * p.query_stride + (g * kGroup + wave * 2 + (col >> 4)) * kHeadDim;
+        AttendQuery<F32> raw[4];
 #pragma unroll
-        for (int hp = 0; hp < 2; ++hp)
+        for (int kb = 0; kb < 4; ++kb) raw[kb].load(src, kb * 16 + half * 8);
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) raw[hp][kb].load(src + hp * kHeadDim, attend_dim<kF16>(kb, kg));
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
+        for (int kb = 0; kb < 4; ++kb) {
             float4_t cs[2]{}, sn[2]{};
             if (rope) {
 #pragma unroll
                 for (int f = 0; f < 2; ++f) {
-                    cs[f] = *reinterpret_cast<const float4_t *>(p.rope_cos + pos * 64 + attend_dim<kF16>(kb, kg) + f * 4);
-                    sn[f] = *reinterpret_cast<const float4_t *>(p.rope_sin + pos * 64 + attend_dim<kF16>(kb, kg) + f * 4);
+                    cs[f] = *reinterpret_cast<const float4_t *>(p.rope_cos + pos * 64 + kb * 16 + half * 8 + f * 4);
+                    sn[f] = *reinterpret_cast<const float4_t *>(p.rope_sin + pos * 64 + kb * 16 + half * 8 + f * 4);
                 }
             }
-#pragma unroll
-            for (int hp = 0; hp < 2; ++hp) raw[hp][kb].rotate(rope, cs, sn, &qf[hp * 2 + th][kb], &qf[hp * 2 + th][kb + 2]);
+            raw[kb].rotate(rope, cs, sn, &qf[kb], &qf[kb + 4]);
         }
+        limit = q.held + t + 1;
+        m = -INFINITY;
+        l = 0.f;
 #pragma unroll
-        for (int hp = 0; hp < 2; ++hp) limit[hp * 2 + th] = q.held + t + 1;
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
     }
-    AttendPages pages;
-    pages.keys = reinterpret_cast<const uint8_t *>(p.key_cache);
-    pages.values = reinterpret_cast<const uint8_t *>(p.value_cache);
-    pages.exponents = nullptr;
-    pages.table = p.ragged.tables ? p.ragged.tables + static_cast<size_t>(q.seq) * p.ragged.max_blocks : nullptr;
-    pages.first = static_cast<uint32_t>(q.seq) * p.ragged.max_blocks;
-    pages.num_blocks = p.ragged.num_blocks;
-    pages.head = g;
-    const int keys = min(q.held + t0 + kWideTokens, valid);
-    pages.last_tile = (keys - 1) >> 4;
-    AttendState<kWideColumns> st;
-    st.clear();
-    attend<kF16, F32, kWideColumns>(pages, qf, 0, (keys + kAttendStep - 1) / kAttendStep, 1, (q.held + t0 + 1) / kAttendStep, limit, valid,
-                                    p.scale_log2, st);
+
+    // S^T = K Q^T of 32 keys: a row of the first operand is a slot of a block, so
+    // lane (query, half) receives keys half * 8 + 0 .. 7 of each of the two
+    // blocks in order, which is its operand of the second product.
+    typedef float16_t Scores;
+    __device__ __attribute__((always_inline)) void scores(const uint16_t *kl, Scores &x) const {
 #pragma unroll
-    for (int ct = 0; ct < kWideColumns; ++ct) {
-        const float inv = 1.0f / column_sum(st.l[ct]);
-        const int t = t0 + (ct & 1) * 16 + row;
-        if (t < q.count) {
-            Element *dst = static_cast<Element *>(p.out) + ((q.begin + static_cast<int64_t>(t)) * kQueryHeads + h0 + (ct >> 1)) * kHeadDim + kg * 4;
+        for (int r = 0; r < 16; ++r) x[r] = 0.f;
+        const uint16_t *src = kl + (col >> 4) * static_cast<int>(kBlockHeadElems) + half * 128 + (col & 15) * 8;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const float4_t v = st.o[ct][c] * inv;
-                if constexpr (F32) *reinterpret_cast<float4_t *>(dst + c * 16) = v;
-                else *reinterpret_cast<half4_t *>(dst + c * 16) = half4_t{to_h(v[0]), to_h(v[1]), to_h(v[2]), to_h(v[3])};
+        for (int kb = 0; kb < 8; ++kb) {
+            const half8_t k = *reinterpret_cast<const half8_t *>(src + kb * 256);
+            x = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qf[kb], x, 0, 0, 0);
+        }
+    }
+    __device__ __attribute__((always_inline)) void mask(int key0, Scores &x) const {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int key = key0 + (r >> 3) * 16 + half * 8 + (r & 7);
+            x[r] = key < limit ? x[r] : -INFINITY;
+        }
+    }
+    // The softmax reference moves when a maximum passes it by 2^8 or more.
+    __device__ __attribute__((always_inline)) void rescale(const Scores &x) {
+        float c = m;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) c = fmaxf(c, x[r]);
+        const attend_u32x2 v = __builtin_amdgcn_permlane32_swap(__float_as_uint(c), __float_as_uint(c), false, false);
+        const float top = fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1]));
+        if (__any((top - m) * p.scale_log2 > kAttendRescaleLog2)) {  // uniform
+            const float a = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
+            m = top;
+            l *= a;
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[dt][r] *= a;
+        }
+    }
+    // The weights of 32 keys in fp16 (with f32 operands as hi + lo), their sum as
+    // rounded, and O^T += V^T P^T.
+    __device__ __attribute__((always_inline)) void product(const Scores &x, const uint16_t *vl) {
+        const half2_t ones = {static_cast<_Float16>(1.0f), static_cast<_Float16>(1.0f)};
+        half8_t hi[2], lo[2];
+        const float ms = m == -INFINITY ? 0.f : m * p.scale_log2;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b * 8 + e], p.scale_log2, -ms));
+                hi[b][e] = to_h(w);
+                if constexpr (F32) lo[b][e] = to_h(w - static_cast<float>(hi[b][e]));
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                l = __builtin_amdgcn_fdot2(half2_t{hi[b][e], hi[b][e + 1]}, ones, l, false);
+                if constexpr (F32) l = __builtin_amdgcn_fdot2(half2_t{lo[b][e], lo[b][e + 1]}, ones, l, false);
             }
         }
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int dt = 0; dt < 4; ++dt) {
+                const half8_t v = *reinterpret_cast<const half8_t *>(vl + (b * 2 + half) * (static_cast<int>(kHeadDim) * 8) + (dt * 32 + col) * 8);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, hi[b], o[dt], 0, 0, 0);
+                if constexpr (F32) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, lo[b], o[dt], 0, 0, 0);
+            }
     }
+    // 1 / the sum of the query's weights, over both halves of the wave.
+    __device__ float inverse_sum() const {
+        const attend_u32x2 v = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        return 1.0f / (__uint_as_float(v[0]) + __uint_as_float(v[1]));
+    }
+    __device__ void store(int64_t row, float inv) const {
+        Element *dst = static_cast<Element *>(p.out) + (row * kQueryHeads + g * kGroup + wave * 2 + (col >> 4)) * kHeadDim + half * 4;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float4_t f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] = o[dt][r * 4 + e] * inv;
+                if constexpr (F32) *reinterpret_cast<float4_t *>(dst + dt * 32 + r * 8) = f;
+                else *reinterpret_cast<half4_t *>(dst + dt * 32 + r * 8) = half4_t{to_h(f[0]), to_h(f[1]), to_h(f[2]), to_h(f[3])};
+            }
+    }
+};
+
+// Double-buffered LDS, filled by direct global-to-LDS loads (lane l's 16 bytes
+// land at the wave's base + 16 l): wave w fetches the step's block w, keys in
+// their own order, values as [token half][128 dims][8 tokens], so that every 16
+// lanes of an operand's read are 256 contiguous bytes.
+template <bool F32>
+__global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedRows p) {
+    typedef std::conditional_t<F32, float, uint16_t> Element;
+    // (distinct arrays, picked at compile time, so that the compiler sees that a
+    // step's loads and its reads touch different ones)
+    __shared__ __align__(16) uint16_t sk0[kStepElems], sk1[kStepElems], sv0[kStepElems], sv1[kStepElems];
+    const uint32_t g = blockIdx.x & 1u, b = blockIdx.x >> 1;
+    PackedItem q;
+    if (p.items) {
+        if (b >= load_const(p.counts, 0)) return;
+        q = load_item(p.items, b);
+    } else {
+        const SeqRows s = find_share<kPackedTokens, 1>(p.ragged, (gridDim.x >> 1) - 1 - b);
+        if (!s.ok || s.share >= (s.count + kPackedTokens - 1) / kPackedTokens) return;  // (the append reports it)
+        q = packed_item(s);
+    }
+    Wide<F32> w(p, g);
+    const int lane = w.lane, wave = w.wave, t0 = q.t0, first = q.first, end = q.end;
+    const int valid = q.held + q.count, last_tile = (min(q.held + t0 + kPackedTokens, valid) - 1) >> 4;
+    const int masked = (q.held + t0 + 1) / 32;  // pieces from this one on reach past the first query's keys
+
+    const int32_t *table = p.ragged.tables ? p.ragged.tables + static_cast<size_t>(q.seq) * p.ragged.max_blocks : nullptr;
+    const int64_t base = static_cast<int64_t>(q.seq) * p.ragged.max_blocks;
+    auto slab = [&](int tile) -> size_t {
+        tile = min(tile, last_tile);  // (tiles behind the last are never used)
+        const int64_t id = table ? load_const(table, tile) : base + tile;
+        const bool ok = id >= 0 && id < static_cast<int64_t>(p.ragged.num_blocks);
+        return (static_cast<size_t>(ok ? id : 0) * kKvHeads + g) * kBlockHeadElems;
+    };
+    typedef __attribute__((address_space(3))) void *lds_ptr;
+    // A step is pieces n and n + 1: their values, and the keys of pieces n + 1 and n + 2.
+    auto fetch_k = [&](int n, uint16_t *dst) {
+        const uint16_t *src = p.key_cache + slab(n * 2 + 2 + wave) + lane * 8;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            __builtin_amdgcn_global_load_lds(src + r * 512, (lds_ptr)(dst + wave * static_cast<int>(kBlockHeadElems) + r * 512), 16, 0, 0);
+    };
+    auto fetch_v = [&](int n, uint16_t *dst) {
+        const uint16_t *src = p.value_cache + slab(n * 2 + wave) + lane * 16;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            __builtin_amdgcn_global_load_lds(src + (r & 1) * 1024 + (r >> 1) * 8, (lds_ptr)(dst + wave * static_cast<int>(kBlockHeadElems) + r * 512), 16, 0, 0);
+    };
+    constexpr int kPiece = kStepElems / 2;
+    fetch_k(first - 1, sk1);  // (of which the first piece's are read)
+    fetch_k(first, sk0);
+    fetch_v(first, sv0);
+    w.load_queries(q, t0);
+    __syncthreads();  // (every wave waits for its loads first)
+
+    typename Wide<F32>::Scores x, y;
+    w.scores(sk1, x);
+    if (masked <= first) w.mask(first * 32, x);
+    w.rescale(x);
+    __syncthreads();
+    // The scores of a piece stand beside the weights of the one before, its
+    // maxima beside that one's product.
+    auto plain = [&](int n, const uint16_t *kc, uint16_t *kn, const uint16_t *vc, uint16_t *vn) __attribute__((always_inline)) {
+        fetch_k(n + 2, kn);
+        fetch_v(n + 2, vn);
+        w.scores(kc, y);
+        w.product(x, vc);
+        w.rescale(y);
+        w.scores(kc + kPiece, x);
+        w.product(y, vc + kPiece);
+        w.rescale(x);
+        __syncthreads();
+    };
+    auto edge = [&](int n, const uint16_t *kc, uint16_t *kn, uint16_t *vc, uint16_t *vn) __attribute__((always_inline)) {
+        fetch_k(n + 2, kn);
+        fetch_v(n + 2, vn);
+        if ((n + 2) * 32 > valid) {
+            // Values behind the sequence's rows become 0: what the pages hold there may
+            // be NaN, and a weight of 0 would not remove it.
+            for (int i = static_cast<int>(threadIdx.x); i < kStepElems; i += kWideWaves * 64)
+                if (n * 32 + (i >> 11) * 16 + ((i >> 10) & 1) * 8 + (i & 7) >= valid) vc[i] = 0;
+            __syncthreads();
+        }
+        if (n + 1 < end) {
+            w.scores(kc, y);
+            if (masked <= n + 1) w.mask((n + 1) * 32, y);
+        }
+        w.product(x, vc);
+        if (n + 1 < end) {
+            w.rescale(y);
+            if (n + 2 < end) {
+                w.scores(kc + kPiece, x);
+                if (masked <= n + 2) w.mask((n + 2) * 32, x);
+            }
+            w.product(y, vc + kPiece);
+            if (n + 2 < end) w.rescale(x);
+        }
+        __syncthreads();
+    };
+    int n = first;
+    for (; n + 4 < min(masked, end); n += 4) {
+        plain(n, sk0, sk1, sv0, sv1);
+        plain(n + 2, sk1, sk0, sv1, sv0);
+    }
+    for (; n < end; n += 4) {
+        edge(n, sk0, sk1, sv0, sv1);
+        if (n + 2 < end) edge(n + 2, sk1, sk0, sv1, sv0);
+    }
+
+    const int t = t0 + (w.col & 15);
+    if (q.slot >= 0) {
+        // A part of the keys: left as it is, for the join.
+        float *part = p.partials + ((static_cast<size_t>(q.slot) * 2 + g) * kWideWaves + wave) * kPartFloats;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                *reinterpret_cast<float4_t *>(part + ((dt * 4 + r) * 64 + lane) * 4) =
+                    float4_t{w.o[dt][r * 4], w.o[dt][r * 4 + 1], w.o[dt][r * 4 + 2], w.o[dt][r * 4 + 3]};
+        part[64 * 64 + lane] = w.m;
+        part[65 * 64 + lane] = w.l;
+    } else if (t < q.count) {
+        w.store(q.begin + static_cast<int64_t>(t), w.inverse_sum());
+    }
+}
+
+// The parts of a split item joined: wave and lane hold what they held there.
+template <bool F32>
+__global__ __launch_bounds__(kWideWaves * 64) void packed_join_kernel(PackedRows p) {
+    const uint32_t g = blockIdx.x & 1u, b = blockIdx.x >> 1;
+    if (b >= load_const(p.counts, 1)) return;
+    const PackedItem q = load_item(p.joins, b);  // first, end: its slots
+    Wide<F32> w(p, g);
+    w.m = -INFINITY;
+    w.l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w.o[dt][r] = 0.f;
+    for (int s = q.first; s < q.end; ++s) {
+        const float *part = p.partials + ((static_cast<size_t>(s) * 2 + g) * kWideWaves + w.wave) * kPartFloats;
+        float4_t o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = *reinterpret_cast<const float4_t *>(part + (i * 64 + w.lane) * 4);
+        const float m = part[64 * 64 + w.lane], l = part[65 * 64 + w.lane], top = fmaxf(w.m, m);
+        const float a = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((w.m - top) * p.scale_log2);
+        const float c = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
+        w.l = w.l * a + l * c;
+        w.m = top;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w.o[i >> 2][(i & 3) * 4 + e] = w.o[i >> 2][(i & 3) * 4 + e] * a + o[i][e] * c;
+    }
+    const int t = q.t0 + (w.col & 15);
+    const float inv = w.inverse_sum();
+    if (t < q.count) w.store(q.begin + static_cast<int64_t>(t), inv);
 }
 
 }  // namespace
@@ -95,9 +315,10 @@ __global__ __launch_bounds__(kWideWaves * 64, 1) void packed_wide_kernel(PackedR
 int launch_packed_prefill(const PackedRows &rows, void *stream) {
     PackedRows p = rows;
     p.scale_log2 = kAttendLog2e / sqrtf(static_cast<float>(kHeadDim));
-    const uint32_t shares = p.ragged.rows / kWideTokens + p.ragged.num_seqs;
-    hipLaunchKernelGGL(p.f32 ? packed_wide_kernel<true> : packed_wide_kernel<false>, dim3(2 * shares), dim3(kWideWaves * 64), 0,
-                       static_cast<hipStream_t>(stream), p);
+    const dim3 threads(kWideWaves * 64);
+    const auto st = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(p.f32 ? packed_wide_kernel<true> : packed_wide_kernel<false>, dim3(2 * p.max_items), threads, 0, st, p);
+    if (p.max_joins) hipLaunchKernelGGL(p.f32 ? packed_join_kernel<true> : packed_join_kernel<false>, dim3(2 * p.max_joins), threads, 0, st, p);
     return static_cast<int>(hipGetLastError());
 }
 

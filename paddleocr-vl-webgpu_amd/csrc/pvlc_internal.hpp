@@ -223,6 +223,19 @@ struct RaggedRows {
     const int32_t *tables;
     uint32_t max_tokens;  // that a sequence may come to hold
 };
+// Packed prompts: 16 tokens t0 .. of a sequence (its rows begin at `begin`) and
+// the pieces of 32 keys that one workgroup takes; slot: where it leaves a part
+// of them, or -1.
+constexpr int kPackedTokens = 16;
+struct PackedItem {
+    int32_t begin, count, held, seq, t0, first, end, slot;
+};
+// Where an append's launch leaves a plan of items (items null: it makes none).
+struct PackedPlan {
+    int32_t *counts;
+    PackedItem *items, *joins;
+    uint32_t max_items, max_joins, max_parts;
+};
 // Rows appended to their pages (kernels_append.hip); strides in elements.
 struct AppendRows {
     RaggedRows ragged;
@@ -236,6 +249,7 @@ struct AppendRows {
     void *key_cache, *value_cache;
     uint8_t *exponents;
     uint32_t *error_word;
+    PackedPlan plan;
 };
 int launch_kv_append(const AppendRows &rows, void *stream);
 // Packed prompts over pages that hold their rows (kernels_packed.hip).
@@ -250,13 +264,40 @@ struct PackedRows {
     const int32_t *positions;
     const uint16_t *key_cache, *value_cache;
     float scale_log2;
+    // The plan that the append's launch made (items null: none), and what
+    // bounds its items and joins.
+    const int32_t *counts;  // items, joins
+    const PackedItem *items, *joins;
+    float *partials;  // [slot][kv head][kPackedPartFloats]
+    uint32_t max_items, max_joins;
 };
 int launch_packed_prefill(const PackedRows &rows, void *stream);
-// Its workspace: 256 bytes of words (0 the error word).
+// Its workspace: 256 bytes of words (0 the error word, 1 and 2 the plan's
+// counts), then the items, the joins and the parts.  Sequences beyond
+// kPackedPlanSeqs are not planned.  An item has at most kPackedLeastPart
+// pieces, or as many as an even share of the call's (512 workgroups are
+// resident); so a call's split items have at most kPackedMaxParts parts.
+constexpr uint32_t kPackedPlanSeqs = 4096, kPackedLeastPart = 16, kPackedMaxParts = 512;
+constexpr size_t kPackedPartFloats = 4 * 66 * 64;  // 4 waves x (64 outputs, reference, sum) x 64 lanes
 struct PackedWorkspace {
-    size_t total;
+    bool plan;
+    uint32_t max_items, max_joins, max_parts;
+    size_t items_offset, joins_offset, partials_offset, total;
 };
-inline PackedWorkspace packed_workspace_layout(uint32_t, uint32_t, uint32_t) { return {256}; }
+inline PackedWorkspace packed_workspace_layout(uint32_t num_seqs, uint32_t rows, uint32_t max_context) {
+    auto align = [](size_t v) { return (v + 255) / 256 * 256; };
+    PackedWorkspace w{};
+    w.plan = num_seqs <= kPackedPlanSeqs;
+    w.max_items = rows / kPackedTokens + num_seqs;
+    if (w.plan && max_context > 32 * kPackedLeastPart) w.max_parts = kPackedMaxParts;
+    w.max_joins = w.max_parts / 2;
+    w.max_items += w.max_parts;
+    w.items_offset = 256;
+    w.joins_offset = w.items_offset + align(w.plan ? w.max_items * sizeof(PackedItem) : 0);
+    w.partials_offset = w.joins_offset + align(w.max_joins * sizeof(PackedItem));
+    w.total = w.partials_offset + static_cast<size_t>(w.max_parts) * 2 * kPackedPartFloats * 4;
+    return w;
+}
 
 // A decode step of groups with shared pages (kernels_shared.hip).  ragged: the
 // sequences, a row each.
