@@ -37,12 +37,15 @@ __device__ inline PackedItem packed_item(const SeqRows &s) {
 // atomics: it decides where results lie, not what they are.
 __device__ inline void make_packed_plan(const RaggedRows &r, const PackedPlan &plan) {
     constexpr int kThreads = 256, kLengths = 64;
-    __shared__ int32_t sm_offset[kPackedPlanSeqs + 1];
+    __shared__ int32_t sm_offset[kPackedPlanSeqs + 1], sm_held[kPackedPlanSeqs];
     __shared__ uint32_t sm_length[kLengths];
     __shared__ uint32_t sm_parts, sm_joins;
     __shared__ unsigned long long sm_pieces;
     const int i = threadIdx.x;
-    for (uint32_t s = i; s <= r.num_seqs; s += kThreads) sm_offset[s] = r.offsets ? r.offsets[s] : static_cast<int32_t>(s * r.each);
+    for (uint32_t s = i; s <= r.num_seqs; s += kThreads) {
+        sm_offset[s] = r.offsets ? r.offsets[s] : static_cast<int32_t>(s * r.each);
+        if (s < r.num_seqs) sm_held[s] = r.lens ? r.lens[s] : 0;
+    }
     if (i < kLengths) sm_length[i] = 0;
     if (i == 0) {
         sm_pieces = 0;
@@ -51,6 +54,17 @@ __device__ inline void make_packed_plan(const RaggedRows &r, const PackedPlan &p
     __syncthreads();
     auto first_share = [&](uint32_t s) { return static_cast<uint32_t>(max(sm_offset[s], 0)) / kPackedTokens + s; };
     const uint32_t shares = r.rows / kPackedTokens + r.num_seqs;
+    auto rows_of = [&](uint32_t s) {
+        SeqRows q;
+        q.seq = static_cast<int>(s);
+        q.begin = sm_offset[s];
+        const int end = sm_offset[s + 1];
+        q.held = sm_held[s];
+        q.ok = q.begin >= 0 && end >= q.begin && static_cast<uint32_t>(end) <= r.rows && q.held >= 0;
+        q.count = q.ok ? end - q.begin : 0;
+        q.ok = q.ok && static_cast<int64_t>(q.held) + q.count <= static_cast<int64_t>(r.max_tokens);
+        return q;
+    };
     // The whole item of share u, if there is one.
     auto item = [&](uint32_t u, PackedItem *q) {
         uint32_t lo = 0, n = r.num_seqs;
@@ -63,24 +77,19 @@ __device__ inline void make_packed_plan(const RaggedRows &r, const PackedPlan &p
                 n = half;
             }
         }
-        SeqRows s;
-        s.seq = static_cast<int>(lo);
-        s.begin = sm_offset[lo];
-        const int end = sm_offset[lo + 1];
-        s.held = r.lens ? r.lens[lo] : 0;
-        s.ok = s.begin >= 0 && end >= s.begin && static_cast<uint32_t>(end) <= r.rows && s.held >= 0;
-        s.count = s.ok ? end - s.begin : 0;
-        s.ok = s.ok && static_cast<int64_t>(s.held) + s.count <= static_cast<int64_t>(r.max_tokens);
+        SeqRows s = rows_of(lo);
         s.share = static_cast<int>(u - first_share(lo));
         if (!s.ok || s.share < 0 || s.share >= (s.count + kPackedTokens - 1) / kPackedTokens) return false;
         *q = packed_item(s);
         return true;
     };
     PackedItem q;
-    unsigned long long pieces = 0;
-    for (uint32_t u = i; u < shares; u += kThreads)
-        if (item(u, &q)) pieces += q.end;
-    atomicAdd(&sm_pieces, pieces);
+    // Pieces of all items, at most: (held + 16 (k + 1) + 31) / 32 for the k-th of a sequence.
+    for (uint32_t s = i; s < r.num_seqs; s += kThreads) {
+        const SeqRows w = rows_of(s);
+        const unsigned long long n = (w.count + kPackedTokens - 1) / kPackedTokens;
+        if (w.ok && n) atomicAdd(&sm_pieces, (n * (w.held + 47ull) + 8 * n * (n - 1)) / 32 + 1);
+    }
     __syncthreads();
     // An even share of both kv heads' pieces, in whole steps of two.  An item of
     // n > most pieces is cut into at most n / most + 1 <= 2 n / most parts, so all
