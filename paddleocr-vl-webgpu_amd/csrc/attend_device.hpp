@@ -168,26 +168,47 @@ struct AttendTile {
     }
 };
 
-// Steps first, first + stride, .. below end of the sequence's keys.  A column's
+// Steps first, first + stride, .. below end of a sequence's keys.  A column's
 // query sees the keys below its limit; steps below `masked` lie below every
-// limit.  `valid` keys are the sequence's (see AttendTile::keep).
+// limit.  `valid` keys are the sequence's (see AttendTile::keep).  begin() sends
+// out the first step's loads, so that the queries can be made ready under them.
 template <int CODE, bool F32, int CT>
-__device__ __attribute__((always_inline)) inline void attend(const AttendPages &p, const half8_t (&qf)[CT][4], int first, int end, int stride,
-                                                              int masked, const int (&limit)[CT], int valid, float scale, AttendState<CT> &st) {
+struct Attend {
+    AttendPages p;
+    int first, end, stride;
+    uint32_t ids;  // blocks, one per lane: lane 2 i + j holds tile j of step i0 + i (32 steps a load)
+    AttendTile<CODE> tile;
+
+    __device__ int tile_of(int i0) const {
+        const int lane = threadIdx.x & 63;
+        return min(2 * (first + (i0 + (lane >> 1)) * stride) + (lane & 1), p.last_tile);
+    }
+    __device__ uint32_t id_of(int i, int j) const {
+        return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ids), 2 * (i & 31) + j));
+    }
+    __device__ __attribute__((always_inline)) void begin(const AttendPages &pages, int from, int to, int by) {
+        p = pages;
+        first = from;
+        end = to;
+        stride = by;
+        if (first >= end) return;  // uniform
+        const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
+        ids = attend_block(p, tile_of(0));
+        tile.load_k(p, id_of(0, 0), id_of(0, 1), row, kg);
+        tile.load_v(p, id_of(0, 0), id_of(0, 1), row, kg);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    __device__ __attribute__((always_inline)) void run(const half8_t (&qf)[CT][4], int masked, const int (&limit)[CT], int valid, float scale,
+                                                       AttendState<CT> &st);
+};
+
+template <int CODE, bool F32, int CT>
+__device__ __attribute__((always_inline)) inline void Attend<CODE, F32, CT>::run(const half8_t (&qf)[CT][4], int masked, const int (&limit)[CT],
+                                                                                  int valid, float scale, AttendState<CT> &st) {
     constexpr bool kQ8 = CODE != PVLC_HIP_KV_F16;
     if (first >= end) return;  // uniform
     const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
-    // Block ids, one per lane: lane 2 i + j holds tile j of step i0 + i (32
-    // steps a load).
-    auto tile_of = [&](int i0) { return min(2 * (first + (i0 + (lane >> 1)) * stride) + (lane & 1), p.last_tile); };
-    uint32_t ids = attend_block(p, tile_of(0)), next_ids = 0;
-    auto id_of = [&](int i, int j) {
-        return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(ids), 2 * (i & 31) + j));
-    };
-    AttendTile<CODE> tile;
-    tile.load_k(p, id_of(0, 0), id_of(0, 1), row, kg);
-    tile.load_v(p, id_of(0, 0), id_of(0, 1), row, kg);
-    __builtin_amdgcn_sched_barrier(0);
+    uint32_t next_ids = 0;
 
     auto step = [&](auto mask, int s, int i) __attribute__((always_inline)) {
         if ((i & 31) == 0 && s + 32 * stride < end) next_ids = attend_block(p, tile_of(i + 32));

@@ -241,9 +241,8 @@ pvlc_hip_status shared(const pvlc_hip_shared_decode_args *args, const void *quer
     if (pvlc_hip_status st = check_append(&rows, key, value, f32, &a, &keys, &values)) return st;
     if (!args->group_offsets && args->num_seqs % args->num_groups != 0)
         return invalid(PVLC_HIP_INV_INVALID_SEQUENCE_BOUNDARIES, "without offsets the sequences must divide among the groups");
-    // (a workgroup for each sequence, kv head and part of its rows, at least)
-    if (static_cast<uint64_t>(args->num_seqs) + args->num_groups > 65536u)
-        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "sequences and groups of a shared decode exceed 65536");
+    if (static_cast<uint64_t>(args->num_seqs) + args->num_groups > kMaxSharedSets)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "sequences and groups of a shared decode exceed 16384");
     if (!aligned(args->group_offsets, 4) || !aligned(args->shared_lens, 4))
         return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "group offsets and shared lengths must be 4-byte aligned");
     if (pvlc_hip_status st = check_context(args)) return st;
@@ -252,7 +251,7 @@ pvlc_hip_status shared(const pvlc_hip_shared_decode_args *args, const void *quer
     Range queries, outs;
     if (pvlc_hip_status st = check_matrix(query, &query_stride, args->num_seqs, kQueryHeads * kHeadDim, size, "query", &queries)) return st;
     if (pvlc_hip_status st = check_matrix(out, &out_stride, args->num_seqs, kQueryHeads * kHeadDim, size, "out", &outs)) return st;
-    const SharedWorkspace ws = shared_workspace_layout(args->num_seqs, args->num_groups, args->max_context);
+    const SharedWorkspace ws = shared_workspace_layout(args->num_seqs, args->num_groups, args->max_context, args->group_offsets != nullptr);
     if (pvlc_hip_status st = check_workspace(args, ws.total, "shared decode")) return st;
     const Range groups{args->group_offsets, 4ull * args->num_groups + 4}, lens{args->shared_lens, 4ull * args->num_groups};
     if (pvlc_hip_status st = check_apart(rows, keys, values, {queries, groups, lens}, {{args->workspace, ws.total}, outs})) return st;
@@ -266,6 +265,8 @@ pvlc_hip_status shared(const pvlc_hip_shared_decode_args *args, const void *quer
     r.group_offsets = args->group_offsets;
     r.shared_lens = args->shared_lens;
     r.query = query;
+    r.new_key = key;
+    r.new_value = value;
     r.out = out;
     r.rope_cos = args->rope_cos;
     r.rope_sin = args->rope_sin;
@@ -280,11 +281,12 @@ pvlc_hip_status shared(const pvlc_hip_shared_decode_args *args, const void *quer
     r.shares = ws.shares;
     r.shared_parts = ws.shared_parts;
     r.own_parts = ws.own_parts;
+    r.unit_columns = ws.unit_columns;
     r.part_o = reinterpret_cast<float *>(base + ws.part_o_offset);
     r.part_ml = reinterpret_cast<float *>(base + ws.part_ml_offset);
-    r.own_o = reinterpret_cast<float *>(base + ws.own_o_offset);
-    r.own_ml = reinterpret_cast<float *>(base + ws.own_ml_offset);
-    if (const int e = launch_kv_append(a, stream)) return hip_status(e, "shared decode append launch");
+    // (a row added to an 8-bit block may round the others of the block again: a launch before their readers)
+    if (args->code != PVLC_HIP_KV_F16)
+        if (const int e = launch_kv_append(a, stream)) return hip_status(e, "shared decode append launch");
     if (const int e = launch_shared_decode(r, stream)) return hip_status(e, "shared decode launch");
     return ok();
 }
@@ -318,7 +320,9 @@ pvlc_hip_status pvlc_hip_packed_prefill_f32io(const pvlc_hip_packed_prefill_args
 
 size_t pvlc_hip_shared_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context) {
     if (num_seqs == 0 || num_groups == 0 || max_context == 0) return 0;
-    return shared_workspace_layout(num_seqs, num_groups, max_context).total;
+    const size_t with = shared_workspace_layout(num_seqs, num_groups, max_context, true).total;
+    const size_t without = shared_workspace_layout(num_seqs, num_groups, max_context, false).total;
+    return with > without ? with : without;
 }
 
 pvlc_hip_status pvlc_hip_shared_decode_f16(const pvlc_hip_shared_decode_args *args, const uint16_t *query, const uint16_t *new_key,

@@ -1,6 +1,6 @@
 // One decode step of groups of sequences that share their first pages: the shared
 // rows are attended once for all of a group, each sequence's own rows by
-// themselves, and the parts joined.  The new rows are in the pages by then.
+// themselves, and the parts joined by a second launch.
 
 #include <hip/hip_runtime.h>
 
@@ -14,236 +14,349 @@ namespace {
 
 constexpr int kWaves = kSharedWaves, kThreads = kWaves * 64;
 
-// A group's set of up to 2 CT sequences, a share of find_share: 16 columns are
-// the 8 heads of a kv head of 2 sequences.
-template <int CT>
+// Up to 2 CT sequences of a group: 16 columns are the 8 heads of a kv head of 2 sequences.
 struct SharedSet {
     int first, count;  // sequences
     int shared;        // rows, in whole blocks
+    int lens;          // lane i: the length of sequence i
+    __device__ int len(int i) const { return __builtin_amdgcn_readlane(lens, i); }
 };
 
 // The rows that a group shares are no more than its shortest sequence has.
-// Sequences whose length does not fit the call are left out (the append reports
-// them, and so it does offsets that are none).
+// Sequences whose length does not fit the call are left out (they are reported
+// where their row would be appended).
 template <int CT>
-__device__ inline bool find_set(const SharedRows &p, uint32_t u, SharedSet<CT> *set) {
-    RaggedRows groups = p.ragged;
-    groups.num_seqs = p.num_groups;
-    groups.rows = p.ragged.num_seqs;
-    groups.each = p.ragged.num_seqs / p.num_groups;
-    groups.offsets = p.group_offsets;
-    groups.lens = p.shared_lens;
-    groups.max_tokens = 0xFFFFFFFFu;
-    const SeqRows q = find_share<2 * CT, 1>(groups, u);
-    const int first = q.share * 2 * CT;
-    if (!q.ok || first >= q.count) {
-        if (!q.ok && threadIdx.x == 0) atomicOr(p.error_word, 1u);
-        return false;
+__device__ inline bool find_set(const SharedRows &p, uint32_t u, SharedSet *set) {
+    int begin, count, first, least;
+    if (p.group_offsets) {
+        RaggedRows groups = p.ragged;
+        groups.num_seqs = p.num_groups;
+        groups.rows = p.ragged.num_seqs;
+        groups.offsets = p.group_offsets;
+        groups.lens = p.shared_lens;
+        groups.max_tokens = 0xFFFFFFFFu;
+        const SeqRows q = find_share<2 * CT, 1>(groups, u);
+        first = q.share * 2 * CT;
+        if (!q.ok || first >= q.count) {
+            if (!q.ok && threadIdx.x == 0) atomicOr(p.error_word, 1u);
+            return false;
+        }
+        begin = q.begin;
+        count = q.count;
+        least = q.held;
+    } else {
+        count = static_cast<int>(p.ragged.num_seqs / p.num_groups);
+        const int sets = (count + 2 * CT - 1) / (2 * CT), group = static_cast<int>(u) / sets;
+        first = (static_cast<int>(u) - group * sets) * 2 * CT;
+        begin = group * count;
+        least = p.shared_lens[group];
     }
     const int lane = threadIdx.x & 63;
-    int least = q.held;
-    for (int i = lane; i < q.count; i += 64) {
-        const int len = p.ragged.lens[q.begin + i];
+    set->first = begin + first;
+    set->count = min(count - first, 2 * CT);
+    set->lens = p.ragged.lens[set->first + min(lane, set->count - 1)];
+    for (int i = lane; i < count; i += 64) {
+        const int len = p.ragged.lens[begin + i];
         if (len >= 0 && static_cast<uint32_t>(len) < p.ragged.max_tokens) least = min(least, len);
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) least = min(least, __shfl_xor(least, d));
-    set->first = q.begin + first;
-    set->count = min(q.count - first, 2 * CT);
-    set->shared = __builtin_amdgcn_readfirstlane(least) / static_cast<int>(kBlockTokens) * static_cast<int>(kBlockTokens);
+    least = __builtin_amdgcn_readfirstlane(least);
+    if (least < 0) {
+        if (threadIdx.x == 0) atomicOr(p.error_word, 1u);
+        return false;
+    }
+    set->shared = least / static_cast<int>(kBlockTokens) * static_cast<int>(kBlockTokens);
     return true;
 }
 
 __device__ inline bool fits(const SharedRows &p, int len) { return len >= 0 && static_cast<uint32_t>(len) < p.ragged.max_tokens; }
 
-// Steps of a part: the keys are cut into `parts` (fewer for few keys: a part has a step for each wave).
-__device__ inline int part_steps(int keys, int parts) {
-    const int steps = (keys + kAttendStep - 1) / kAttendStep;
-    return max((steps + parts - 1) / parts, kWaves);
+// Steps of a part: the keys are cut into `parts`, fewer for few keys (a part has a
+// step for each wave); and the parts that this makes.
+__device__ inline int part_steps(int keys, int parts) { return max(((keys + kAttendStep - 1) / kAttendStep + parts - 1) / parts, kWaves); }
+__device__ inline int parts_of(int keys, int parts) {
+    const int steps = part_steps(keys, parts);
+    return ((keys + kAttendStep - 1) / kAttendStep + steps - 1) / steps;
 }
 
-// CT * 16 columns over the part's steps, a wave every fourth step; the waves' results joined through LDS, and written unnormalised.
-template <int CODE, bool F32, int CT>
-__device__ inline void attend_part(const SharedRows &p, int seq0, int rows, int columns, uint32_t g, AttendPages pages, int keys, int first,
-                                   int end, float *part_o, float *part_ml, float (*sm_m)[64], float (*sm_l)[64], float4_t *sm_o) {
-    typedef std::conditional_t<F32, float, uint16_t> Element;
-    const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-    half8_t qf[CT][4];
-    int limit[CT];
+struct SharedLds {
+    float m[kWaves][32], l[kWaves][32];
+    float4_t o[kWaves * 4 * 64];
+};
+
+// cos and sin of the 8 dims from d0 (below 64) at a position.
+__device__ inline void load_angles(const SharedRows &p, bool rope, int64_t pos, int d0, float4_t (&cs)[2], float4_t (&sn)[2]) {
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-        const int seq = seq0 + min(ct * 2 + (row >> 3), rows - 1);
-        const int64_t pos = p.positions ? p.positions[seq] : p.ragged.lens[seq];
-        const bool rope = p.rotate_query && p.rope_cos != nullptr && pos >= 0 && pos < static_cast<int64_t>(p.rope_rows);
-        const Element *src = static_cast<const Element *>(p.query) + (static_cast<int64_t>(seq) * kQueryHeads + g * kGroup + (row & 7)) * kHeadDim;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            AttendQuery<F32> raw;
-            raw.load(src, attend_dim<CODE>(kb, kg));
-            float4_t cs[2]{}, sn[2]{};
-            if (rope) {
-#pragma unroll
-                for (int f = 0; f < 2; ++f) {
-                    cs[f] = *reinterpret_cast<const float4_t *>(p.rope_cos + pos * 64 + attend_dim<CODE>(kb, kg) + f * 4);
-                    sn[f] = *reinterpret_cast<const float4_t *>(p.rope_sin + pos * 64 + attend_dim<CODE>(kb, kg) + f * 4);
-                }
-            }
-            raw.rotate(rope, cs, sn, &qf[ct][kb], &qf[ct][kb + 2]);
-        }
-        limit[ct] = keys;
+    for (int f = 0; f < 2; ++f) {
+        cs[f] = rope ? *reinterpret_cast<const float4_t *>(p.rope_cos + pos * 64 + d0 + f * 4) : float4_t{};
+        sn[f] = rope ? *reinterpret_cast<const float4_t *>(p.rope_sin + pos * 64 + d0 + f * 4) : float4_t{};
     }
+}
+
+// The new row of a sequence, by one wave: rotated, written to its page, and one
+// more key of the wave's columns.
+template <bool F32>
+__device__ inline void append_and_attend(const SharedRows &p, int seq, int len, uint32_t g, const half8_t (&qf)[4], AttendState<1> &st) {
+    typedef std::conditional_t<F32, float, uint16_t> Element;
+    constexpr int kF16 = PVLC_HIP_KV_F16;
+    const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
+    const size_t at = (static_cast<size_t>(seq) * kKvHeads + g) * kHeadDim;
+    const Element *key = static_cast<const Element *>(p.new_key) + at, *value = static_cast<const Element *>(p.new_value) + at;
+    const int64_t pos = p.positions ? p.positions[seq] : len;
+    const bool rope = p.rope_cos != nullptr && pos >= 0 && pos < static_cast<int64_t>(p.rope_rows);
+    const int64_t id = p.ragged.tables[static_cast<size_t>(seq) * p.ragged.max_blocks + len / static_cast<int>(kBlockTokens)];
+    half8_t k[4];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        AttendQuery<F32> raw;
+        float4_t cs[2], sn[2];
+        raw.load(key, attend_dim<kF16>(kb, kg));
+        load_angles(p, rope, pos, attend_dim<kF16>(kb, kg), cs, sn);
+        raw.rotate(rope, cs, sn, &k[kb], &k[kb + 2]);
+        if constexpr (!F32) {
+            if (!rope) {  // as given, bit for bit
+                k[kb] = raw.x[0][0];
+                k[kb + 2] = raw.x[1][0];
+            }
+        }
+    }
+    auto half_value = [&](int d) { return F32 ? to_h(value[d]) : __builtin_bit_cast(_Float16, static_cast<uint16_t>(value[d])); };
+    bool ok;
+    const size_t slab = (static_cast<size_t>(checked_block(p.ragged, id, &ok)) * kKvHeads + g) * kBlockHeadElems;
+    const int slot = len % static_cast<int>(kBlockTokens);
+    if (ok) {
+        uint16_t *kc = static_cast<uint16_t *>(p.key_cache) + slab + key_slot(slot) * 8;
+        if (row == 0) {
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) *reinterpret_cast<half8_t *>(kc + attend_dim<kF16>(kb, kg) / 8 * 128) = k[kb];
+        }
+        uint16_t *vc = static_cast<uint16_t *>(p.value_cache) + slab + slot;
+#pragma unroll
+        for (int d = 0; d < 2; ++d) vc[(lane + d * 64) * kBlockTokens] = __builtin_bit_cast(uint16_t, half_value(lane + d * 64));
+    }
+    if (lane == 0 && g == 0) {
+        if (!ok) atomicOr(p.error_word, 2u);
+        if (!rope && p.rope_cos != nullptr) atomicOr(p.error_word, 4u);
+    }
+    // Key 0 of a score product whose other rows are 0.
+    float4_t acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(row == 0 ? k[kb] : half8_t{}, qf[kb], acc, 0, 0, 0);
+    const float x = __shfl(acc[0], row), top = fmaxf(st.m[0], x);
+    const float a = st.m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[0] - top) * p.scale_log2);
+    const float w = __builtin_amdgcn_exp2f((x - top) * p.scale_log2);
+    st.m[0] = top;
+    st.l[0] = st.l[0] * a + (kg == 0 ? w : 0.f);
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st.o[0][c][r] = st.o[0][c][r] * a + w * static_cast<float>(half_value(c * 16 + kg * 4 + r));
+}
+
+// CT * 16 columns over the part's steps, a wave every fourth step; the waves'
+// results joined through LDS, and written unnormalised.  new_row: the length of
+// the sequence whose new row is one more key (fp16 pages), or -1.
+template <int CODE, bool F32, int CT>
+__device__ inline void attend_part(const SharedRows &p, const SharedSet &set, int r0, int rows, uint32_t g, AttendPages pages, int keys, int first, int end, int new_row,
+                                   float *part_o, float *part_ml, SharedLds &lds) {
+    typedef std::conditional_t<F32, float, uint16_t> Element;
+    const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4, columns = rows * static_cast<int>(kGroup);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     pages.keys = static_cast<const uint8_t *>(p.key_cache);
     pages.values = static_cast<const uint8_t *>(p.value_cache);
     pages.exponents = p.exponents;
     pages.num_blocks = p.ragged.num_blocks;
     pages.head = g;
     pages.last_tile = (keys - 1) >> 4;
+    Attend<CODE, F32, CT> loop;
+    loop.begin(pages, first + wave, end, kWaves);
+    half8_t qf[CT][4];
+    int limit[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+        const int r = r0 + min(ct * 2 + (row >> 3), rows - 1), seq = set.first + r, len = __shfl(set.lens, r);
+        const int64_t pos = p.positions ? p.positions[seq] : len;
+        const bool rope = p.rotate_query && p.rope_cos != nullptr && pos >= 0 && pos < static_cast<int64_t>(p.rope_rows);
+        const Element *src = static_cast<const Element *>(p.query) + (static_cast<int64_t>(seq) * kQueryHeads + g * kGroup + (row & 7)) * kHeadDim;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            AttendQuery<F32> raw;
+            float4_t cs[2], sn[2];
+            raw.load(src, attend_dim<CODE>(kb, kg));
+            load_angles(p, rope, pos, attend_dim<CODE>(kb, kg), cs, sn);
+            raw.rotate(rope, cs, sn, &qf[ct][kb], &qf[ct][kb + 2]);
+        }
+        limit[ct] = keys;
+    }
     AttendState<CT> st;
     st.clear();
-    attend<CODE, F32, CT>(pages, qf, first + wave, end, kWaves, keys / kAttendStep, limit, keys, p.scale_log2, st);
+    loop.run(qf, keys / kAttendStep, limit, keys, p.scale_log2, st);
+    if constexpr (CODE == PVLC_HIP_KV_F16 && CT == 1) {
+        if (new_row >= 0 && wave == 0) append_and_attend<F32>(p, set.first + r0, new_row, g, qf[0], st);  // uniform
+    }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         const float l = column_sum(st.l[ct]);
         if (kg == 0) {
-            sm_m[wave][ct * 16 + row] = st.m[ct];
-            sm_l[wave][ct * 16 + row] = l;
+            lds.m[wave][ct * 16 + row] = st.m[ct];
+            lds.l[wave][ct * 16 + row] = l;
         }
     }
     __syncthreads();
     float a[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-        float m = sm_m[0][ct * 16 + row];
+        float m = lds.m[0][ct * 16 + row];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sm_m[w][ct * 16 + row]);
+        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, lds.m[w][ct * 16 + row]);
         a[ct] = st.m[ct] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[ct] - m) * p.scale_log2);
     }
-    for (int c = static_cast<int>(threadIdx.x); c < columns; c += kThreads) {
-        float m = sm_m[0][c], l = 0.f;
+    if (static_cast<int>(threadIdx.x) < columns) {
+        const int c = threadIdx.x;
+        float m = lds.m[0][c], l = 0.f;
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sm_m[w][c]);
+        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, lds.m[w][c]);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) l += sm_m[w][c] == -INFINITY ? 0.f : sm_l[w][c] * __builtin_amdgcn_exp2f((sm_m[w][c] - m) * p.scale_log2);
+        for (int w = 0; w < kWaves; ++w) l += lds.m[w][c] == -INFINITY ? 0.f : lds.l[w][c] * __builtin_amdgcn_exp2f((lds.m[w][c] - m) * p.scale_log2);
         part_ml[c * 2] = m * p.scale_log2;
         part_ml[c * 2 + 1] = l;
     }
-    // Two 16-dim tiles at a time.
+    // 4 / CT 16-dim tiles at a time.
+    constexpr int kTiles = 4 / CT;
 #pragma unroll
-    for (int c0 = 0; c0 < 8; c0 += 2) {
+    for (int c0 = 0; c0 < 8; c0 += kTiles) {
+        if (c0) __syncthreads();
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-            for (int ct = 0; ct < CT; ++ct) sm_o[((wave * 2 + c) * CT + ct) * 64 + lane] = st.o[ct][c0 + c] * a[ct];
+            for (int ct = 0; ct < CT; ++ct) lds.o[((wave * kTiles + c) * CT + ct) * 64 + lane] = st.o[ct][c0 + c] * a[ct];
         __syncthreads();
-        for (int i = static_cast<int>(threadIdx.x); i < 2 * CT * 64; i += kThreads) {
-            const int l = i & 63, ct = (i >> 6) % CT, c = (i >> 6) / CT, column = ct * 16 + (l & 15);
-            float4_t v = sm_o[i];
+        {
+            const int i = threadIdx.x, n = i & 63, ct = (i >> 6) % CT, c = (i >> 6) / CT, column = ct * 16 + (n & 15);
+            float4_t v = lds.o[i];
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) v += sm_o[w * 2 * CT * 64 + i];
-            if (column < columns) *reinterpret_cast<float4_t *>(part_o + column * kHeadDim + (c0 + c) * 16 + (l >> 4) * 4) = v;
+            for (int w = 1; w < kWaves; ++w) v += lds.o[w * 256 + i];
+            if (column < columns) *reinterpret_cast<float4_t *>(part_o + column * static_cast<int>(kHeadDim) + (c0 + c) * 16 + (n >> 4) * 4) = v;
         }
-        __syncthreads();
     }
 }
 
 // Workgroup: share u, kv head, then the parts of the shared rows and those of
 // the set's sequences.
 template <int CODE, bool F32, int CT>
-__global__ __launch_bounds__(kThreads, CT == 4 ? 1 : 2) void shared_attention_kernel(SharedRows p) {
-    __shared__ float sm_m[kWaves][64], sm_l[kWaves][64];
-    __shared__ float4_t sm_o[kWaves * 2 * CT * 64];
+__global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedRows p) {
+    __shared__ SharedLds lds;
+    constexpr bool kNewRow = CODE == PVLC_HIP_KV_F16;  // (8-bit pages hold the new rows already)
     const uint32_t g = blockIdx.x & 1u;
     uint32_t b = blockIdx.x >> 1;
-    const bool common = b < p.shares * p.shared_parts;  // uniform
+    const bool common = b < p.shares * p.shared_parts;  // uniform, as all below
     if (!common) b -= p.shares * p.shared_parts;
     const uint32_t per = common ? p.shared_parts : 2 * CT * p.own_parts;
     const uint32_t u = b / per, rest = b % per;
-    SharedSet<CT> set;
+    SharedSet set;
     if (!find_set<CT>(p, u, &set)) return;
+    const int shared_parts = static_cast<int>(p.shared_parts), own_parts = static_cast<int>(p.own_parts);
+    const size_t unit = static_cast<size_t>(u) * 2 + g;
+    float *const part_o = p.part_o + unit * p.unit_columns * kHeadDim, *const part_ml = p.part_ml + unit * p.unit_columns * 2;
+    const int own_column = shared_parts * CT * 16;
     AttendPages pages{};
     if (common) {
-        const int steps = part_steps(set.shared, static_cast<int>(p.shared_parts)), first = static_cast<int>(rest) * steps;
-        if (first * kAttendStep >= set.shared) return;
-        pages.table = p.ragged.tables + static_cast<size_t>(set.first) * p.ragged.max_blocks;
-        const size_t slot = (static_cast<size_t>(u) * 2 + g) * p.shared_parts + rest;
-        attend_part<CODE, F32, CT>(p, set.first, set.count, set.count * static_cast<int>(kGroup), g, pages, set.shared, first,
-                                   min(first + steps, (set.shared + kAttendStep - 1) / kAttendStep),
-                                   p.part_o + slot * CT * 16 * kHeadDim, p.part_ml + slot * CT * 16 * 2, sm_m, sm_l, sm_o);
+        const int part = static_cast<int>(rest), steps = part_steps(set.shared, shared_parts), first = part * steps;
+        if (part < parts_of(set.shared, shared_parts)) {
+            pages.table = p.ragged.tables + static_cast<size_t>(set.first) * p.ragged.max_blocks;
+            attend_part<CODE, F32, CT>(p, set, 0, set.count, g, pages, set.shared, first,
+                                       min(first + steps, (set.shared + kAttendStep - 1) / kAttendStep), -1, part_o + part * CT * 16 * static_cast<int>(kHeadDim),
+                                       part_ml + part * CT * 16 * 2, lds);
+        }
     } else {
-        const int r = static_cast<int>(rest / p.own_parts), part = static_cast<int>(rest % p.own_parts);
+        const int r = static_cast<int>(rest) / own_parts, part = static_cast<int>(rest) % own_parts;
         if (r >= set.count) return;
-        const int seq = set.first + r, len = p.ragged.lens[seq];
-        if (!fits(p, len)) return;
-        const int keys = len + 1 - set.shared, steps = part_steps(keys, static_cast<int>(p.own_parts)), first = part * steps;
-        if (first * kAttendStep >= keys) return;
-        pages.table = p.ragged.tables + static_cast<size_t>(seq) * p.ragged.max_blocks + set.shared / static_cast<int>(kBlockTokens);
-        const size_t slot = ((static_cast<size_t>(u) * 2 + g) * 2 * CT + r) * p.own_parts + part;
-        attend_part<CODE, F32, 1>(p, seq, 1, kGroup, g, pages, keys, first, min(first + steps, (keys + kAttendStep - 1) / kAttendStep),
-                                  p.own_o + slot * kGroup * kHeadDim, p.own_ml + slot * kGroup * 2, sm_m, sm_l, sm_o);
+        const int seq = set.first + r, len = set.len(r);
+        const int keys = len + (kNewRow ? 0 : 1) - set.shared;
+        if (!fits(p, len)) {
+            if (threadIdx.x == 0 && part == 0) atomicOr(p.error_word, 1u);
+        } else if (part < parts_of(keys, own_parts) || (kNewRow && part == 0)) {
+            const int steps = part_steps(keys, own_parts), first = part * steps;
+            pages.table = p.ragged.tables + static_cast<size_t>(seq) * p.ragged.max_blocks + set.shared / static_cast<int>(kBlockTokens);
+            const int column = own_column + (r * own_parts + part) * static_cast<int>(kGroup);
+            attend_part<CODE, F32, 1>(p, set, r, 1, g, pages, keys, first, min(first + steps, (keys + kAttendStep - 1) / kAttendStep),
+                                      part == 0 ? len : -1, part_o + column * static_cast<int>(kHeadDim), part_ml + column * 2, lds);
+        }
     }
 }
 
-// Workgroup: a sequence and kv head; thread t has head t / 32 and dims t % 32 * 4 .. + 3.
-template <bool F32, int CT>
-__global__ __launch_bounds__(256) void shared_merge_kernel(SharedRows p) {
+// Workgroup: a sequence and kv head; thread t has head t / 32 and dims t % 32 * 4
+// .. + 3.  The parts are loaded with the lengths that say which of them are there.
+template <int CODE, bool F32, int CT>
+__global__ __launch_bounds__(256) void shared_join_kernel(SharedRows p) {
+    constexpr int kNewRow = CODE == PVLC_HIP_KV_F16, kBatch = 16;
     const uint32_t g = blockIdx.x & 1u, u = (blockIdx.x >> 1) / (2 * CT);
     const int r = static_cast<int>((blockIdx.x >> 1) % (2 * CT));
-    SharedSet<CT> set;
-    if (!find_set<CT>(p, u, &set) || r >= set.count) return;
-    const int seq = set.first + r, len = p.ragged.lens[seq];
-    if (!fits(p, len)) return;
+    const int shared_parts = static_cast<int>(p.shared_parts), own_parts = static_cast<int>(p.own_parts), all = shared_parts + own_parts;
     const int head = threadIdx.x >> 5, d0 = (threadIdx.x & 31) * 4;
-    auto parts_of = [](int keys, uint32_t parts) {
-        const int steps = part_steps(keys, static_cast<int>(parts));
-        return keys <= 0 ? 0 : ((keys + kAttendStep - 1) / kAttendStep + steps - 1) / steps;
-    };
-    const int shared = parts_of(set.shared, p.shared_parts), own = parts_of(len + 1 - set.shared, p.own_parts);
     const size_t unit = static_cast<size_t>(u) * 2 + g;
+    const float *part_o = p.part_o + unit * p.unit_columns * kHeadDim, *part_ml = p.part_ml + unit * p.unit_columns * 2;
+    typedef float float2v __attribute__((ext_vector_type(2)));
+    float2v ml[kBatch];
+    float4_t v[kBatch];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int part = min(i0 + i, all - 1);
+            const int column = (part < shared_parts ? part * CT * 16 + r * static_cast<int>(kGroup)
+                                                    : shared_parts * CT * 16 + (r * own_parts + part - shared_parts) * static_cast<int>(kGroup)) + head;
+            ml[i] = *reinterpret_cast<const float2v *>(part_ml + column * 2);
+            v[i] = *reinterpret_cast<const float4_t *>(part_o + column * static_cast<int>(kHeadDim) + d0);
+        }
+    };
+    load(0);
+    __builtin_amdgcn_sched_barrier(0);
+    SharedSet set;
+    if (!find_set<CT>(p, u, &set) || r >= set.count) return;
+    const int len = set.len(r);
+    if (!fits(p, len)) return;
+    const int shared = parts_of(set.shared, shared_parts), own = max(parts_of(len + 1 - kNewRow - set.shared, own_parts), kNewRow);
     float m = -INFINITY, l = 0.f;
     float4_t o{0.f, 0.f, 0.f, 0.f};
-    auto add = [&](const float *ml, const float *po) {
-        const float pm = ml[0], pl = ml[1];
-        const float4_t v = *reinterpret_cast<const float4_t *>(po);
-        const float top = fmaxf(m, pm);
-        const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), b = pm == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(pm - top);
-        l = l * a + pl * b;
-        o = o * a + v * b;
+    for (int i0 = 0;;) {
+        float top = m;
+        auto there = [&](int i) { return i0 + i < shared_parts ? i0 + i < shared : i0 + i - shared_parts < own; };
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) top = there(i) ? fmaxf(top, ml[i][0]) : top;
+        const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        l *= a;
+        o *= a;
         m = top;
-    };
-    for (int i = 0; i < shared; ++i) {
-        const size_t column = (unit * p.shared_parts + i) * CT * 16 + r * kGroup + head;
-        add(p.part_ml + column * 2, p.part_o + column * kHeadDim + d0);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (there(i) && ml[i][0] != -INFINITY) {
+                const float w = __builtin_amdgcn_exp2f(ml[i][0] - top);
+                l += ml[i][1] * w;
+                o += v[i] * w;
+            }
+        }
+        i0 += kBatch;
+        if (i0 >= shared_parts + own) break;
+        load(i0);
     }
-    for (int i = 0; i < own; ++i) {
-        const size_t column = ((unit * 2 * CT + r) * p.own_parts + i) * kGroup + head;
-        add(p.own_ml + column * 2, p.own_o + column * kHeadDim + d0);
-    }
-    const float inv = 1.0f / l;
-    const size_t at = (static_cast<size_t>(seq) * kQueryHeads + g * kGroup + head) * kHeadDim + d0;
-    if constexpr (F32) *reinterpret_cast<float4_t *>(static_cast<float *>(p.out) + at) = o * inv;
-    else *reinterpret_cast<half4_t *>(static_cast<uint16_t *>(p.out) + at) = half4_t{to_h(o[0] * inv), to_h(o[1] * inv), to_h(o[2] * inv), to_h(o[3] * inv)};
+    const float4_t f = o * (1.0f / l);
+    const size_t at = (static_cast<size_t>(set.first + r) * kQueryHeads + g * kGroup + head) * kHeadDim + d0;
+    if constexpr (F32) *reinterpret_cast<float4_t *>(static_cast<float *>(p.out) + at) = f;
+    else *reinterpret_cast<half4_t *>(static_cast<uint16_t *>(p.out) + at) = half4_t{to_h(f[0]), to_h(f[1]), to_h(f[2]), to_h(f[3])};
 }
 
 template <int CODE, bool F32, int CT>
 void launch(const SharedRows &p, hipStream_t stream) {
-    const uint32_t groups = 2 * p.shares * (p.shared_parts + 2 * CT * p.own_parts);
-    hipLaunchKernelGGL((shared_attention_kernel<CODE, F32, CT>), dim3(groups), dim3(kThreads), 0, stream, p);
-    hipLaunchKernelGGL((shared_merge_kernel<F32, CT>), dim3(2 * p.shares * 2 * CT), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((shared_attention_kernel<CODE, F32, CT>), dim3(2 * p.shares * (p.shared_parts + 2 * CT * p.own_parts)), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((shared_join_kernel<CODE, F32, CT>), dim3(2 * p.shares * 2 * CT), dim3(256), 0, stream, p);
 }
 
-template <int CODE, bool F32>
-void launch_columns(const SharedRows &p, hipStream_t stream) {
-    if (p.columns == 1) launch<CODE, F32, 1>(p, stream);
-    else if (p.columns == 2) launch<CODE, F32, 2>(p, stream);
-    else launch<CODE, F32, 4>(p, stream);
-}
-
-template <bool F32>
+template <bool F32, int CT>
 void launch_code(const SharedRows &p, hipStream_t stream) {
-    if (p.code == PVLC_HIP_KV_F16) launch_columns<PVLC_HIP_KV_F16, F32>(p, stream);
-    else if (p.code == PVLC_HIP_KV_E4M3) launch_columns<PVLC_HIP_KV_E4M3, F32>(p, stream);
-    else launch_columns<PVLC_HIP_KV_INT8, F32>(p, stream);
+    if (p.code == PVLC_HIP_KV_F16) launch<PVLC_HIP_KV_F16, F32, CT>(p, stream);
+    else if (p.code == PVLC_HIP_KV_E4M3) launch<PVLC_HIP_KV_E4M3, F32, CT>(p, stream);
+    else launch<PVLC_HIP_KV_INT8, F32, CT>(p, stream);
 }
 
 }  // namespace
@@ -251,8 +364,9 @@ void launch_code(const SharedRows &p, hipStream_t stream) {
 int launch_shared_decode(const SharedRows &rows, void *stream) {
     SharedRows p = rows;
     p.scale_log2 = kAttendLog2e / sqrtf(static_cast<float>(kHeadDim));
-    if (p.f32) launch_code<true>(p, static_cast<hipStream_t>(stream));
-    else launch_code<false>(p, static_cast<hipStream_t>(stream));
+    const auto st = static_cast<hipStream_t>(stream);
+    if (p.columns == 1) p.f32 ? launch_code<true, 1>(p, st) : launch_code<false, 1>(p, st);
+    else p.f32 ? launch_code<true, 2>(p, st) : launch_code<false, 2>(p, st);
     return static_cast<int>(hipGetLastError());
 }
 

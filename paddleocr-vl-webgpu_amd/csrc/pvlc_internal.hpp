@@ -300,53 +300,52 @@ inline PackedWorkspace packed_workspace_layout(uint32_t num_seqs, uint32_t rows,
 }
 
 // A decode step of groups with shared pages (kernels_shared.hip).  ragged: the
-// sequences, a row each.
+// sequences, a row each (8-bit pages hold it already).
 constexpr int kSharedWaves = 4;
 struct SharedRows {
     RaggedRows ragged;
     uint32_t num_groups, code;
     bool f32;
     const int32_t *group_offsets, *shared_lens;
-    const void *query;
+    const void *query, *new_key, *new_value;
     void *out;
     const float *rope_cos, *rope_sin;
     uint32_t rope_rows;
     const int32_t *positions;
     uint32_t rotate_query;
-    const void *key_cache, *value_cache;
+    void *key_cache, *value_cache;
     const uint8_t *exponents;
     float scale_log2;
     uint32_t *error_word;
     // sets of 2 * columns sequences, the parts that their shared rows and a
-    // sequence's own are cut into, and what these leave: outputs [share][kv head]
-    // [part][column][128], (max in log2 units, sum) likewise; own ones [share][kv
-    // head][sequence of the set][part][8 heads][128]
-    uint32_t columns, shares, shared_parts, own_parts;
-    float *part_o, *part_ml, *own_o, *own_ml;
+    // sequence's own are cut into, and what these leave for each kv head: outputs
+    // [share][kv head][column][128] and (max in log2 units, sum) likewise, the
+    // columns [shared part][columns * 16], then [sequence of the set][own part][8]
+    uint32_t columns, shares, shared_parts, own_parts, unit_columns;
+    float *part_o, *part_ml;
 };
 int launch_shared_decode(const SharedRows &rows, void *stream);
-// Its workspace: 256 bytes of words (0 the error word), then the parts'.
+// Its workspace: 256 bytes of words (0 the error word), then the parts' results.
+constexpr uint32_t kMaxSharedSets = 16384;
 struct SharedWorkspace {
-    uint32_t columns, shares, shared_parts, own_parts;
-    size_t part_o_offset, part_ml_offset, own_o_offset, own_ml_offset, total;
+    uint32_t columns, shares, shared_parts, own_parts, unit_columns;
+    size_t part_o_offset, part_ml_offset, total;
 };
-inline SharedWorkspace shared_workspace_layout(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context) {
+inline SharedWorkspace shared_workspace_layout(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context, bool offsets) {
     auto align = [](size_t v) { return (v + 255) / 256 * 256; };
     auto clamp = [](uint32_t v, uint32_t hi) { return v < 1 ? 1u : v > hi ? hi : v; };
     SharedWorkspace w{};
     const uint32_t each = (num_seqs + num_groups - 1) / num_groups;
-    w.columns = each <= 2 ? 1 : each <= 4 ? 2 : 4;
-    w.shares = num_seqs / (2 * w.columns) + num_groups;
+    w.columns = each <= 2 ? 1 : 2;
+    w.shares = offsets ? num_seqs / (2 * w.columns) + num_groups : num_groups * ((each + 2 * w.columns - 1) / (2 * w.columns));
     const uint32_t most = clamp((max_context + 32 * kSharedWaves - 1) / (32 * kSharedWaves), 64);
-    w.shared_parts = clamp(512 / (2 * w.shares), most);
+    w.shared_parts = clamp((512 / (2 * w.shares) + 3) / 4 * 4, most);
     w.own_parts = clamp(512 / (2 * num_seqs), most);
-    const size_t units = static_cast<size_t>(w.shares) * 2;
-    const size_t shared = units * w.shared_parts * w.columns * 16, own = units * 2 * w.columns * w.own_parts * kGroup;
+    w.unit_columns = w.shared_parts * w.columns * 16 + 2 * w.columns * w.own_parts * kGroup;
+    const size_t columns = static_cast<size_t>(w.shares) * 2 * w.unit_columns;
     w.part_o_offset = 256;
-    w.part_ml_offset = w.part_o_offset + align(shared * kHeadDim * 4);
-    w.own_o_offset = w.part_ml_offset + align(shared * 8);
-    w.own_ml_offset = w.own_o_offset + align(own * kHeadDim * 4);
-    w.total = w.own_ml_offset + align(own * 8);
+    w.part_ml_offset = w.part_o_offset + align(columns * kHeadDim * 4);
+    w.total = w.part_ml_offset + align(columns * 8);
     return w;
 }
 
