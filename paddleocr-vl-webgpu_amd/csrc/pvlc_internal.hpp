@@ -339,8 +339,8 @@ inline SharedWorkspace shared_workspace_layout(uint32_t num_seqs, uint32_t num_g
     w.columns = each <= 2 ? 1 : 2;
     w.shares = offsets ? num_seqs / (2 * w.columns) + num_groups : num_groups * ((each + 2 * w.columns - 1) / (2 * w.columns));
     const uint32_t most = clamp((max_context + 32 * kSharedWaves - 1) / (32 * kSharedWaves), 64);
-    w.shared_parts = clamp((512 / (2 * w.shares) + 3) / 4 * 4, most);
-    w.own_parts = clamp(512 / (2 * num_seqs), most);
+    w.shared_parts = clamp((256 / (2 * w.shares) + 3) / 4 * 4, most);
+    w.own_parts = clamp(256 / (2 * num_seqs), most);
     w.unit_columns = w.shared_parts * w.columns * 16 + 2 * w.columns * w.own_parts * kGroup;
     const size_t columns = static_cast<size_t>(w.shares) * 2 * w.unit_columns;
     w.part_o_offset = 256;

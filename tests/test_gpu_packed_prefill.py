@@ -1,0 +1,169 @@
+"""Packed prompts and chunks of prompts against the plain form in 64 bits; planes bit for bit."""
+
+import numpy as np
+import pytest
+
+import batches_ref as B
+from pvlc_testlib import log, pvlc
+
+pytestmark = pytest.mark.gpu
+WIDTHS = pytest.mark.parametrize("f32", [False, True])
+
+
+def workspace(b, context):
+    import torch
+    nbytes = pvlc.packed_prefill_workspace_bytes(b.n, b.rows, context)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    pvlc.workspace_init(ws, nbytes)
+    return ws, nbytes
+
+
+def args_of(b, ws, **change):
+    b.keep = change
+    base = dict(b.packed(), max_context=b.width * 16, query_stride=b.dq.stride(0), workspace=ws[0], workspace_bytes=ws[1])
+    return pvlc.packed_prefill_args(**{**base, **change})
+
+
+def launch(b, args, stream=None):
+    (pvlc.packed_prefill_f32io if b.f32 else pvlc.packed_prefill_f16)(args, b.dq, b.dk, b.dv, b.out, stream)
+
+
+def wanted(b, some=None):
+    """Outputs of the rows (or of some of them) and their bounds, after the rows have been put into the cache."""
+    rows = np.arange(int(b.offsets[-1])) if some is None else some
+    want, limit = np.empty((len(rows), 16, 128)), np.empty((len(rows), 16, 128))
+    for s in range(b.n):
+        mine = np.flatnonzero((rows >= b.offsets[s]) & (rows < b.offsets[s + 1]))
+        if mine.size == 0:
+            continue
+        k, v = b.cache.rows(b.table[s], b.held[s] + b.counts[s])
+        limits = [b.place(int(r))[1] + 1 for r in rows[mine]]
+        q = np.stack([b.turned(b.q[r], int(r)) for r in rows[mine]])
+        out, big, most = B.attend(q, k, v, limits)
+        want[mine] = out
+        limit[mine] = B.bound(out, big, most, max(limits), b.f32)
+    return want, limit
+
+
+def check(b, label, some=None):
+    import torch
+    torch.cuda.synchronize()
+    b.put()
+    b.check_planes(label)
+    want, limit = wanted(b, some)
+    got = b.out.float().cpu().numpy()
+    rows = np.arange(int(b.offsets[-1])) if some is None else some
+    B.check(label, got[rows], want, limit)
+    assert (got[int(b.offsets[-1]):] == 9.0).all(), "rows behind the last sequence stay as they were"
+
+
+BATCHES = {
+    "one": ([1], [0]), "few": ([5, 0, 97, 16], [0, 0, 0, 0]), "behind": ([3, 33, 1, 40], [17, 100, 64, 31]), "ends": ([16, 32, 48, 64, 15, 17], [0, 16, 0, 1, 49, 15]),
+    "many": ([1 + i % 5 for i in range(70)], [i * 11 % 70 for i in range(70)]), "long": ([300], [0]), "chunk": ([20, 1], [3000, 700]),
+}
+
+
+@WIDTHS
+@pytest.mark.parametrize("name", list(BATCHES))
+def test_batches(f32, name):
+    """Planes hold NaN wherever no row is: values behind a sequence's last row carry no weight."""
+    log(f"case: packed prefill {name} f32={f32}")
+    counts, held = BATCHES[name]
+    b = B.Batch(counts, held, f32=f32, seed=len(name), paged=name != "ends", fused=name in ("few", "chunk"), spare=3, positions=name == "behind",
+                rope=name != "many").upload()
+    ws = workspace(b, b.width * 16)
+    launch(b, args_of(b, ws))
+    check(b, name)
+    assert pvlc.workspace_error(*ws) == 0
+
+
+@WIDTHS
+def test_items_are_cut_and_joined(f32):
+    """Few rows on long histories, and a long prompt beside short ones: items in parts."""
+    log(f"case: packed prefill in parts f32={f32}")
+    b = B.Batch([40, 1500, 7], [6000, 0, 2047], f32=f32, seed=31).upload()
+    ws = workspace(b, b.width * 16)
+    launch(b, args_of(b, ws))
+    some = np.unique(np.concatenate([np.arange(0, 40, 3), 40 + np.array([0, 15, 16, 31, 500, 1023, 1024, 1300, 1499]), 1540 + np.arange(7)]))
+    check(b, "parts", some)
+
+
+@WIDTHS
+def test_rising_scores_move_the_reference(f32):
+    """Scores that grow along the sequence by far more than the reference may lag."""
+    log(f"case: packed prefill, rising scores f32={f32}")
+    b = B.Batch([200], [90], f32=f32, seed=12, rope=False)
+    b.q[:] = 1.0
+    b.k[:, :, :] = (np.arange(b.rows)[:, None, None] * 0.05).astype(b.k.dtype)
+    b.upload()
+    ws = workspace(b, b.width * 16)
+    launch(b, args_of(b, ws))
+    check(b, "rising")
+
+
+def test_without_offsets_lengths_and_table():
+    log("case: packed prefill without offsets")
+    b = B.Batch([21] * 3, [0] * 3, seed=6, paged=False).upload()
+    ws = workspace(b, b.width * 16)
+    launch(b, args_of(b, ws, row_offsets=None, cache_lens=None))
+    check(b, "equal prompts")
+
+
+def test_many_sequences():
+    """More sequences than are planned, the last ones without rows."""
+    log("case: packed prefill, many sequences")
+    n = 1100
+    b = B.Batch([(i % 3) if i < 1000 else 0 for i in range(n)], [0] * n, seed=7).upload()
+    ws = workspace(b, b.width * 16)
+    launch(b, args_of(b, ws))
+    check(b, "many")
+
+
+def test_a_sequence_beyond_the_context_is_skipped():
+    import torch
+    log("case: packed prefill, beyond the context")
+    b = B.Batch([20, 8, 6], [30, 3, 0], seed=9, room=16).upload()
+    ws = workspace(b, 48)
+    launch(b, args_of(b, ws, max_context=48))
+    torch.cuda.synchronize()
+    assert pvlc.workspace_error(*ws) == 1
+    got = b.out.float().cpu().numpy()
+    assert (got[:20] == 9.0).all()
+    b.counts = [0, 8, 6]
+    b.put()
+    b.check_planes("skipped")
+    some = np.arange(20, 34)
+    want, limit = wanted(b, some)
+    B.check("the others", got[some], want, limit)
+
+
+def test_graphs_that_share_a_workspace():
+    """Two captured calls of different shapes over one workspace, replayed in turn with direct calls between."""
+    import torch
+    log("case: packed prefill from graphs")
+    one, two = (B.Batch(c, h, f32=f, seed=s).upload() for c, h, f, s in (([50, 9], [700, 0], False, 1), ([7] * 20, [40] * 20, True, 2)))
+    sizes = [pvlc.packed_prefill_workspace_bytes(b.n, b.rows, b.width * 16) for b in (one, two)]
+    ws = torch.empty(max(sizes), dtype=torch.uint8, device="cuda")
+    pvlc.workspace_init(ws, max(sizes))
+    args = [args_of(b, (ws, max(sizes))) for b in (one, two)]
+    for b, a in zip((one, two), args):
+        launch(b, a)
+    torch.cuda.synchronize()
+    want = [b.out.clone() for b in (one, two)]
+    check(one, "direct")
+    check(two, "direct")
+    stream, graphs = torch.cuda.Stream(), []
+    for b, a in zip((one, two), args):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=stream):
+            launch(b, a, stream)
+    for _ in range(3):
+        for g, b, w in zip(graphs, (one, two), want):
+            b.out.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(b.out, w)
+        launch(one, args[0])
+        torch.cuda.synchronize()
+        assert torch.equal(one.out, want[0])
+    assert pvlc.workspace_error(ws, max(sizes)) == 0

@@ -1,0 +1,182 @@
+"""Decode of groups with shared pages against the plain form in 64 bits; planes and exponents byte for byte."""
+
+import numpy as np
+import pytest
+
+import batches_ref as B
+import q8_ref as R
+from pvlc_testlib import log, pvlc
+
+pytestmark = pytest.mark.gpu
+CODES = pytest.mark.parametrize("code", [B.F16, R.E4M3, R.INT8])
+WIDTHS = pytest.mark.parametrize("f32", [False, True])
+
+
+class Groups(B.Batch):
+    """Groups of sizes whose sequences have their first `shared` rows in common (in whole blocks) and `tails` of their own."""
+
+    def __init__(self, sizes, shared, tails, code, f32, seed=0, **how):
+        self.sizes, self.shared = list(sizes), list(shared)
+        group = np.repeat(np.arange(len(sizes)), sizes)
+        held = [shared[g] + t for g, t in zip(group, tails)]
+        super().__init__([1] * len(group), held, code, f32, seed, **how)
+        firsts = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+        self.firsts = firsts
+        for i, g in enumerate(group):  # the others repeat the first one's entries
+            whole = shared[g] // 16
+            self.table[i, :whole] = self.table[firsts[g], :whole]
+
+    def shared_args(self, ws, offsets=False, **change):
+        import torch
+        self.keep = change
+        self.dshared = torch.tensor(self.shared, dtype=torch.int32, device="cuda")
+        self.dfirsts = torch.from_numpy(self.firsts).cuda() if offsets else None
+        base = dict(self.common(), num_seqs=self.n, num_groups=len(self.sizes), group_offsets=self.dfirsts, shared_lens=self.dshared,
+                    cache_lens=self.dlens, max_context=self.width * 16, code=self.code, exponents=self.exponents, rotate_query=True,
+                    workspace=ws[0], workspace_bytes=ws[1], block_tables=self.dtable)
+        return pvlc.shared_decode_args(**{**base, **change})
+
+    def workspace(self):
+        import torch
+        nbytes = pvlc.shared_decode_workspace_bytes(self.n, len(self.sizes), self.width * 16)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+        pvlc.workspace_init(ws, nbytes)
+        return ws, nbytes
+
+    def launch(self, args, stream=None):
+        (pvlc.shared_decode_f32io if self.f32 else pvlc.shared_decode_f16)(args, self.dq, self.dk, self.dv, self.out, stream)
+
+    def check(self, label, rotate_query=True, skipped=()):
+        import torch
+        torch.cuda.synchronize()
+        for i in range(self.n):
+            if i not in skipped:
+                self.cache.put_rows(self.table[i], self.held[i], self.turned(self.k[i], i)[None],
+                                    self.v[i].astype(np.float16).astype(np.float64)[None])
+        self.check_planes(label)
+        got = self.out.float().cpu().numpy()
+        for i in range(self.n):
+            if i in skipped:
+                assert (got[i] == 9.0).all(), f"{label}: sequence {i}"
+                continue
+            k, v = self.cache.rows(self.table[i], self.held[i] + 1)
+            q = self.turned(self.q[i], i) if rotate_query else self.q[i].astype(np.float16).astype(np.float64)
+            out, big, most = B.attend(q[None], k, v, [self.held[i] + 1])
+            B.check(f"{label} sequence {i}", got[i:i + 1], out, B.bound(out, big, most, self.held[i] + 1, self.f32, self.code))
+
+
+def tails_of(n, most, seed=1):
+    return np.random.default_rng(seed).integers(0, most + 1, n).tolist()
+
+
+CASES = {
+    # group sizes, shared rows, own rows
+    "one": ([1], [0], [0]), "alone": ([1], [300], [7]), "beams": ([4], [157], tails_of(4, 40)), "beams_no_tail": ([4], [160], [0] * 4),
+    "nothing_shared": ([3, 3], [0, 15], [0, 20, 130, 1, 16, 17]), "pages": ([2] * 5, [16, 33, 64, 200, 129], tails_of(10, 33)),
+    "answers": ([23], [500], tails_of(23, 60)), "long": ([5, 5], [4000, 40], tails_of(10, 300)),
+}
+
+
+@CODES
+@WIDTHS
+@pytest.mark.parametrize("name", list(CASES))
+def test_groups_of_one_size(code, f32, name):
+    log(f"case: shared decode {name} code={code} f32={f32}")
+    sizes, shared, tails = CASES[name]
+    c = Groups(sizes, shared, tails, code, f32, seed=len(name), positions=name == "pages", rope=name != "answers").upload()
+    ws = c.workspace()
+    c.launch(c.shared_args(ws, rotate_query=name != "beams"))
+    c.check(name, rotate_query=name != "beams")
+    assert pvlc.workspace_error(*ws) == 0
+
+
+@CODES
+@pytest.mark.parametrize("sizes", [[1, 7, 0, 3, 12], [3] * 70, [0, 40, 0]])
+def test_groups_of_different_sizes(code, sizes):
+    log(f"case: shared decode groups of {sizes[:6]}.. code={code}")
+    shared = [16 * (i % 5) + i % 7 for i in range(len(sizes))]
+    c = Groups(sizes, shared, tails_of(sum(sizes), 50), code, code == R.E4M3, seed=sum(sizes)).upload()
+    ws = c.workspace()
+    c.launch(c.shared_args(ws, offsets=True))
+    c.check("sizes")
+    assert pvlc.workspace_error(*ws) == 0
+
+
+@CODES
+def test_rows_that_are_not_shared_by_all(code):
+    """A shared length beyond the group's shortest sequence counts as that one's."""
+    log(f"case: shared decode, lengths beyond, code={code}")
+    c = Groups([3], [96], [0, 5, 40], code, True, seed=2).upload()
+    c.shared = [4000]
+    ws = c.workspace()
+    c.launch(c.shared_args(ws))
+    c.check("beyond")
+    assert pvlc.workspace_error(*ws) == 0
+
+
+@CODES
+def test_errors_are_reported_and_skipped(code):
+    import torch
+    log(f"case: shared decode errors, code={code}")
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    c = Groups([3, 2], [48, 16], [0, 5, 20, 3, 4], code, False, seed=3).upload()
+    ws = c.workspace()
+    lens = list(c.held)
+    lens[1], lens[3] = -1, c.width * 16
+    c.launch(c.shared_args(ws, offsets=True, cache_lens=ints(lens)))
+    c.check("lengths", skipped=(1, 3))
+    assert pvlc.workspace_error(*ws) == 1
+    c = Groups([2], [32], [5, 9], code, False, seed=4).upload()  # a position outside the tables: no rotation
+    ws = c.workspace()
+    c.launch(c.shared_args(ws, positions=ints([c.table_rows, -1])))
+    c.rope = False
+    c.check("positions")
+    assert pvlc.workspace_error(*ws) == 4
+
+
+def test_steps_from_a_graph_beside_direct_calls():
+    """A captured step replayed, and direct calls of another shape on the same workspace between the replays."""
+    import torch
+    log("case: shared decode from a graph")
+    for code in (B.F16, R.E4M3):
+        one, two = Groups([4], [700], [3, 9, 0, 40], code, True, seed=5).upload(), Groups([2] * 9, [40] * 9, tails_of(18, 20), code, True, seed=6).upload()
+        nbytes = max(pvlc.shared_decode_workspace_bytes(c.n, len(c.sizes), c.width * 16) for c in (one, two))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+        pvlc.workspace_init(ws, nbytes)
+        args = [c.shared_args((ws, nbytes)) for c in (one, two)]
+        stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            one.launch(args[0], stream)
+        start = [x.clone() for x in one.planes + ([] if one.exponents is None else [one.exponents])]
+        outs = []
+        for _ in range(3):
+            for d, s in zip(one.planes + ([] if one.exponents is None else [one.exponents]), start):
+                d.copy_(s)
+            one.out.fill_(9.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            outs.append(one.out.clone())
+            two.launch(args[1])
+            torch.cuda.synchronize()
+        assert all(torch.equal(outs[0], x) for x in outs)
+        one.check("replayed")
+        assert pvlc.workspace_error(ws, nbytes) == 0
+
+
+def test_far_blocks():
+    """Shared and own blocks whose elements lie beyond 2^31."""
+    import torch
+    log("case: shared decode, far blocks")
+    c = Groups([3], [40], [2, 20, 9], B.F16, True, seed=7).upload()
+    blocks = (1 << 31) // 4096 + 300
+    far = torch.from_numpy(np.arange(blocks - c.blocks, blocks).astype(np.int32)).cuda()
+    planes = [torch.zeros(blocks * 4096, dtype=torch.int16, device="cuda") for _ in range(2)]
+    for p, small in zip(planes, c.planes):
+        p.view(blocks, 4096)[blocks - c.blocks:] = small.view(c.blocks, 4096)
+    ws = c.workspace()
+    c.launch(c.shared_args(ws, num_blocks=blocks, key_cache=planes[0], value_cache=planes[1], block_tables=far[c.dtable.long()]))
+    torch.cuda.synchronize()
+    for p, small in zip(planes, c.planes):
+        small.copy_(p.view(blocks, 4096)[blocks - c.blocks:].view_as(small))
+    c.check("far")
