@@ -35,15 +35,21 @@ struct Wide {
         : p(rows), g(head), lane(threadIdx.x & 63), col(lane & 31), half(lane >> 5),
           wave(__builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6))) {}
 
-    __device__ void load_queries(const PackedItem &q, int t0) {
-        const int t = min(t0 + (col & 15), q.count - 1);  // (past the sequence: its last one again, not stored)
+    // The query of this lane's column (past the sequence: its last one again, not
+    // stored): sent for, then rotated.
+    AttendQuery<F32> raw[4];
+    int64_t pos;
+    __device__ __attribute__((always_inline)) void send_for_queries(const PackedItem &q) {
+        const int t = min(q.t0 + (col & 15), q.count - 1);
         const int64_t at = q.begin + static_cast<int64_t>(t);
-        const int64_t pos = p.positions ? p.positions[at] : q.held + static_cast<int64_t>(t);
-        const bool rope = p.rope_cos != nullptr && pos >= 0 && pos < static_cast<int64_t>(p.rope_rows);
+        limit = q.held + t + 1;
+        pos = p.positions ? p.positions[at] : q.held + static_cast<int64_t>(t);
         const Element *src = static_cast<const Element *>(p.query) + at * p.query_stride + (g * kGroup + wave * 2 + (col >> 4)) * kHeadDim;
-        AttendQuery<F32> raw[4];
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) raw[kb].load(src, kb * 16 + half * 8);
+    }
+    __device__ __attribute__((always_inline)) void take_queries() {
+        const bool rope = p.rope_cos != nullptr && pos >= 0 && pos < static_cast<int64_t>(p.rope_rows);
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
             float4_t cs[2]{}, sn[2]{};
@@ -56,7 +62,6 @@ struct Wide {
             }
             raw[kb].rotate(rope, cs, sn, &qf[kb], &qf[kb + 4]);
         }
-        limit = q.held + t + 1;
         m = -INFINITY;
         l = 0.f;
 #pragma unroll
@@ -137,18 +142,40 @@ struct Wide {
         const attend_u32x2 v = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
         return 1.0f / (__uint_as_float(v[0]) + __uint_as_float(v[1]));
     }
-    __device__ void store(int64_t row, float inv) const {
-        Element *dst = static_cast<Element *>(p.out) + (row * kQueryHeads + g * kGroup + wave * 2 + (col >> 4)) * kHeadDim + half * 4;
+    // The wave's outputs, turned in LDS (16 KiB of its own) so that 16 lanes store
+    // a row of 128 dims, or half of one in f32: whole lines.
+    __device__ void store(const PackedItem &q, float inv, void *own) const {
+        constexpr int kPasses = F32 ? 2 : 1, kDims = kHeadDim / kPasses, kPitch = kDims + 16 / sizeof(Element), kPer = 16 / sizeof(Element);
+        Element *lds = static_cast<Element *>(own);
+        typedef std::conditional_t<F32, float4_t, half4_t> Four;
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
+        for (int pass = 0; pass < kPasses; ++pass) {
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float4_t f;
+            for (int dt = 0; dt < 4 / kPasses; ++dt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f[e] = o[dt][r * 4 + e] * inv;
-                if constexpr (F32) *reinterpret_cast<float4_t *>(dst + dt * 32 + r * 8) = f;
-                else *reinterpret_cast<half4_t *>(dst + dt * 32 + r * 8) = half4_t{to_h(f[0]), to_h(f[1]), to_h(f[2]), to_h(f[3])};
+                for (int r = 0; r < 4; ++r) {
+                    const float16_t &from = o[pass * (4 / kPasses) + dt];
+                    Four f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (F32) f[e] = from[r * 4 + e] * inv;
+                        else f[e] = to_h(from[r * 4 + e] * inv);
+                    }
+                    *reinterpret_cast<Four *>(lds + col * kPitch + dt * 32 + r * 8 + half * 4) = f;
+                }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = i * 4 + (lane >> 4), t = q.t0 + (c & 15), d = (lane & 15) * kPer;
+                const q8x4_t v = *reinterpret_cast<const q8x4_t *>(lds + c * kPitch + d);
+                if (t < q.count)
+                    *reinterpret_cast<q8x4_t *>(static_cast<Element *>(p.out) +
+                                                ((q.begin + static_cast<int64_t>(t)) * kQueryHeads + g * kGroup + wave * 2 + (c >> 4)) * kHeadDim +
+                                                pass * kDims + d) = v;
             }
+        }
     }
 };
 
@@ -158,15 +185,15 @@ struct Wide {
 // lanes of an operand's read are 256 contiguous bytes.
 template <bool F32>
 __global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedRows p) {
-    typedef std::conditional_t<F32, float, uint16_t> Element;
     // (distinct arrays, picked at compile time, so that the compiler sees that a
     // step's loads and its reads touch different ones)
     __shared__ __align__(16) uint16_t sk0[kStepElems], sk1[kStepElems], sv0[kStepElems], sv1[kStepElems];
     const uint32_t g = blockIdx.x & 1u, b = blockIdx.x >> 1;
     PackedItem q;
     if (p.items) {
-        if (b >= load_const(p.counts, 0)) return;
-        q = load_item(p.items, b);
+        const uint32_t items = load_const(p.counts, 0);
+        q = load_item(p.items, b);  // (beside the count, in one round)
+        if (b >= items) return;
     } else {
         const SeqRows s = find_share<kPackedTokens, 1>(p.ragged, (gridDim.x >> 1) - 1 - b);
         if (!s.ok || s.share >= (s.count + kPackedTokens - 1) / kPackedTokens) return;  // (the append reports it)
@@ -200,10 +227,11 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedR
             __builtin_amdgcn_global_load_lds(src + (r & 1) * 1024 + (r >> 1) * 8, (lds_ptr)(dst + wave * static_cast<int>(kBlockHeadElems) + r * 512), 16, 0, 0);
     };
     constexpr int kPiece = kStepElems / 2;
+    w.send_for_queries(q);
     fetch_k(first - 1, sk1);  // (of which the first piece's are read)
     fetch_k(first, sk0);
     fetch_v(first, sv0);
-    w.load_queries(q, t0);
+    w.take_queries();
     __syncthreads();  // (every wave waits for its loads first)
 
     typename Wide<F32>::Scores x, y;
@@ -260,7 +288,6 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedR
         if (n + 2 < end) edge(n + 2, sk1, sk0, sv1, sv0);
     }
 
-    const int t = t0 + (w.col & 15);
     if (q.slot >= 0) {
         // A part of the keys: left as it is, for the join.
         float *part = p.partials + ((static_cast<size_t>(q.slot) * 2 + g) * kWideWaves + wave) * kPartFloats;
@@ -272,17 +299,19 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedR
                     float4_t{w.o[dt][r * 4], w.o[dt][r * 4 + 1], w.o[dt][r * 4 + 2], w.o[dt][r * 4 + 3]};
         part[64 * 64 + lane] = w.m;
         part[65 * 64 + lane] = w.l;
-    } else if (t < q.count) {
-        w.store(q.begin + static_cast<int64_t>(t), w.inverse_sum());
+    } else {
+        // (every wave is past its last read of the buffers)
+        w.store(q, w.inverse_sum(), wave < 2 ? (wave == 0 ? sk0 : sk1) : (wave == 2 ? sv0 : sv1));
     }
 }
 
 // The parts of a split item joined: wave and lane hold what they held there.
 template <bool F32>
 __global__ __launch_bounds__(kWideWaves * 64) void packed_join_kernel(PackedRows p) {
-    const uint32_t g = blockIdx.x & 1u, b = blockIdx.x >> 1;
-    if (b >= load_const(p.counts, 1)) return;
+    __shared__ __align__(16) float lds[kWideWaves][32 * 68];
+    const uint32_t g = blockIdx.x & 1u, b = blockIdx.x >> 1, joins = load_const(p.counts, 1);
     const PackedItem q = load_item(p.joins, b);  // first, end: its slots
+    if (b >= joins) return;
     Wide<F32> w(p, g);
     w.m = -INFINITY;
     w.l = 0.f;
@@ -305,9 +334,7 @@ __global__ __launch_bounds__(kWideWaves * 64) void packed_join_kernel(PackedRows
 #pragma unroll
             for (int e = 0; e < 4; ++e) w.o[i >> 2][(i & 3) * 4 + e] = w.o[i >> 2][(i & 3) * 4 + e] * a + o[i][e] * c;
     }
-    const int t = q.t0 + (w.col & 15);
-    const float inv = w.inverse_sum();
-    if (t < q.count) w.store(q.begin + static_cast<int64_t>(t), inv);
+    w.store(q, w.inverse_sum(), lds[w.wave]);
 }
 
 }  // namespace

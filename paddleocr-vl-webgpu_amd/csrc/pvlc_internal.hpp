@@ -277,7 +277,7 @@ int launch_packed_prefill(const PackedRows &rows, void *stream);
 // kPackedPlanSeqs are not planned.  An item has at most kPackedLeastPart
 // pieces, or as many as an even share of the call's (512 workgroups are
 // resident); so a call's split items have at most kPackedMaxParts parts.
-constexpr uint32_t kPackedPlanSeqs = 1024, kPackedLeastPart = 16, kPackedMaxParts = 512;
+constexpr uint32_t kPackedPlanSeqs = 1024, kPackedLeastPart = 16, kPackedMaxParts = 256;
 constexpr size_t kPackedPartFloats = 4 * 66 * 64;  // 4 waves x (64 outputs, reference, sum) x 64 lanes
 struct PackedWorkspace {
     bool plan;
