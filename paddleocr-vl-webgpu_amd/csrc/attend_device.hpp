@@ -237,10 +237,12 @@ __device__ __attribute__((always_inline)) inline void Attend<CODE, F32, CT>::run
                     for (int r = 0; r < 4; ++r) x[ct][h * 4 + r] = kQ8 ? acc[ct][h][r] * power : acc[ct][h][r];
         }
         __builtin_amdgcn_sched_barrier(0);
-        // The next step's keys (behind the last: a clamped tile, never used).
+        // The next step's keys.  (Loads behind the last step would be waited for
+        // where the results are joined: a part of one step a wave 1 us longer.)
         if (((i + 1) & 31) == 0) ids = next_ids;
         const uint32_t b0 = id_of(i + 1, 0), b1 = id_of(i + 1, 1);
-        tile.load_k(p, b0, b1, row, kg);
+        const bool more = s + stride < end;  // uniform
+        if (more) tile.load_k(p, b0, b1, row, kg);
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (mask) {
             const int key = s * kAttendStep + kg * 8;
@@ -329,7 +331,7 @@ __device__ __attribute__((always_inline)) inline void Attend<CODE, F32, CT>::run
             }
         }
         __builtin_amdgcn_sched_barrier(0);
-        tile.load_v(p, b0, b1, row, kg);
+        if (more) tile.load_v(p, b0, b1, row, kg);
         __builtin_amdgcn_sched_barrier(0);
     };
     const std::integral_constant<bool, true> yes;

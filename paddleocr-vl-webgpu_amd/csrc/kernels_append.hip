@@ -240,8 +240,9 @@ void (*append_kernel(uint32_t code))(AppendRows) {
 }  // namespace
 
 int launch_kv_append(const AppendRows &p, void *stream) {
-    const uint32_t shares = p.ragged.rows / kBlockTokens + 2 * p.ragged.num_seqs + (p.plan.items ? 1 : 0);
-    hipLaunchKernelGGL(p.f32 ? append_kernel<true>(p.code) : append_kernel<false>(p.code), dim3(shares), dim3(kThreads), 0,
+    const RaggedRows &r = p.ragged;
+    const uint32_t shares = r.offsets ? r.rows / kBlockTokens + 2 * r.num_seqs : r.num_seqs * shares_of_each<kBlockTokens, 2>(r.each);
+    hipLaunchKernelGGL(p.f32 ? append_kernel<true>(p.code) : append_kernel<false>(p.code), dim3(shares + (p.plan.items ? 1 : 0)), dim3(kThreads), 0,
                        static_cast<hipStream_t>(stream), p);
     return static_cast<int>(hipGetLastError());
 }

@@ -72,17 +72,21 @@ __device__ inline bool find_set(const SharedRows &p, uint32_t u, SharedSet *set)
 
 __device__ inline bool fits(const SharedRows &p, int len) { return len >= 0 && static_cast<uint32_t>(len) < p.ragged.max_tokens; }
 
-// Steps of a part: the keys are cut into `parts`, fewer for few keys (a part has a
-// step for each wave); and the parts that this makes.
-__device__ inline int part_steps(int keys, int parts) { return max(((keys + kAttendStep - 1) / kAttendStep + parts - 1) / parts, kWaves); }
-__device__ inline int parts_of(int keys, int parts) {
-    const int steps = part_steps(keys, parts);
+// Steps of a part: the keys are cut into `parts`, fewer for few keys (a part has
+// `least` steps: one for each wave of shared rows, two of own ones); and the
+// parts that this makes.
+constexpr int kLeastShared = kWaves, kLeastOwn = 2;
+__device__ inline int part_steps(int keys, int parts, int least) { return max(((keys + kAttendStep - 1) / kAttendStep + parts - 1) / parts, least); }
+__device__ inline int parts_of(int keys, int parts, int least) {
+    const int steps = part_steps(keys, parts, least);
     return ((keys + kAttendStep - 1) / kAttendStep + steps - 1) / steps;
 }
 
+// A wave's results: of its columns, reference, sum and outputs [16-dim tile][16 columns][lane].
+template <int CT>
 struct SharedLds {
-    float m[kWaves][32], l[kWaves][32];
-    float4_t o[kWaves * 4 * 64];
+    float m[kWaves][CT * 16], l[kWaves][CT * 16];
+    float4_t o[kWaves][8 * CT * 64];
 };
 
 // cos and sin of the 8 dims from d0 (below 64) at a position.
@@ -154,47 +158,73 @@ __device__ inline void append_and_attend(const SharedRows &p, int seq, int len, 
         for (int r = 0; r < 4; ++r) st.o[0][c][r] = st.o[0][c][r] * a + w * static_cast<float>(half_value(c * 16 + kg * 4 + r));
 }
 
-// CT * 16 columns over the part's steps, a wave every fourth step; the waves'
-// results joined through LDS, and written unnormalised.  new_row: the length of
-// the sequence whose new row is one more key (fp16 pages), or -1.
-template <int CODE, bool F32, int CT>
-__device__ inline void attend_part(const SharedRows &p, const SharedSet &set, int r0, int rows, uint32_t g, AttendPages pages, int keys, int first, int end, int new_row,
-                                   float *part_o, float *part_ml, SharedLds &lds) {
-    typedef std::conditional_t<F32, float, uint16_t> Element;
-    const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4, columns = rows * static_cast<int>(kGroup);
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+// Eight dims of a lane's column (the query of head row & 7 of sequence r of the
+// set) and their rotary partners: sent for, then rotated.
+template <int CODE, bool F32>
+struct SharedQuery {
+    AttendQuery<F32> raw;
+    float4_t cs[2], sn[2];
+    bool rope;
+    __device__ __attribute__((always_inline)) void send(const SharedRows &p, const SharedSet &set, int r, uint32_t g, int kb) {
+        const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4, seq = set.first + r, len = __shfl(set.lens, r);
+        const int64_t pos = p.positions ? p.positions[seq] : len;
+        rope = p.rotate_query && p.rope_cos != nullptr && pos >= 0 && pos < static_cast<int64_t>(p.rope_rows);
+        const auto *src = static_cast<const typename AttendQuery<F32>::Element *>(p.query) +
+                          (static_cast<int64_t>(seq) * kQueryHeads + g * kGroup + (row & 7)) * kHeadDim;
+        raw.load(src, attend_dim<CODE>(kb, kg));
+        load_angles(p, rope, pos, attend_dim<CODE>(kb, kg), cs, sn);
+    }
+    __device__ __attribute__((always_inline)) void take(half8_t *lo, half8_t *hi) const { raw.rotate(rope, cs, sn, lo, hi); }
+};
+
+__device__ inline AttendPages pages_of(const SharedRows &p, int seq, int first_row, int keys, uint32_t g) {
+    AttendPages pages;
     pages.keys = static_cast<const uint8_t *>(p.key_cache);
     pages.values = static_cast<const uint8_t *>(p.value_cache);
     pages.exponents = p.exponents;
+    pages.table = p.ragged.tables + static_cast<size_t>(seq) * p.ragged.max_blocks + first_row / static_cast<int>(kBlockTokens);
+    pages.first = 0;
     pages.num_blocks = p.ragged.num_blocks;
     pages.head = g;
     pages.last_tile = (keys - 1) >> 4;
+    return pages;
+}
+
+// A part of a set's shared rows: the columns of all its sequences, a wave every
+// fourth step; the waves' results joined through LDS, and written unnormalised.
+template <int CODE, bool F32, int CT>
+__device__ inline void attend_shared(const SharedRows &p, const SharedSet &set, uint32_t g, int first, int end, float *part_o, float *part_ml,
+                                     SharedLds<CT> &lds) {
+    const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4, columns = set.count * static_cast<int>(kGroup), keys = set.shared;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    // Wave w rotates pair w % 2 of column tile w / 2; all take the rest from LDS.
+    SharedQuery<CODE, F32> query;
+    if (wave < 2 * CT) query.send(p, set, min((wave >> 1) * 2 + (row >> 3), set.count - 1), g, wave & 1);
+    __builtin_amdgcn_sched_barrier(0);
     Attend<CODE, F32, CT> loop;
-    loop.begin(pages, first + wave, end, kWaves);
+    loop.begin(pages_of(p, set.first, 0, keys, g), first + wave, end, kWaves);
+    half8_t *const sm_q = reinterpret_cast<half8_t *>(&lds.o[0][0]);  // [column tile][kb][lane], before the join
+    if (wave < 2 * CT) {
+        half8_t lo, hi;
+        query.take(&lo, &hi);
+        sm_q[((wave >> 1) * 4 + (wave & 1)) * 64 + lane] = lo;
+        sm_q[((wave >> 1) * 4 + (wave & 1) + 2) * 64 + lane] = hi;
+    }
+    // (fences of LDS alone: the keys and values stay in flight)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
     half8_t qf[CT][4];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) qf[ct][kb] = sm_q[(ct * 4 + kb) * 64 + lane];
     int limit[CT];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
-        const int r = r0 + min(ct * 2 + (row >> 3), rows - 1), seq = set.first + r, len = __shfl(set.lens, r);
-        const int64_t pos = p.positions ? p.positions[seq] : len;
-        const bool rope = p.rotate_query && p.rope_cos != nullptr && pos >= 0 && pos < static_cast<int64_t>(p.rope_rows);
-        const Element *src = static_cast<const Element *>(p.query) + (static_cast<int64_t>(seq) * kQueryHeads + g * kGroup + (row & 7)) * kHeadDim;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            AttendQuery<F32> raw;
-            float4_t cs[2], sn[2];
-            raw.load(src, attend_dim<CODE>(kb, kg));
-            load_angles(p, rope, pos, attend_dim<CODE>(kb, kg), cs, sn);
-            raw.rotate(rope, cs, sn, &qf[ct][kb], &qf[ct][kb + 2]);
-        }
-        limit[ct] = keys;
-    }
+    for (int ct = 0; ct < CT; ++ct) limit[ct] = keys;
     AttendState<CT> st;
     st.clear();
     loop.run(qf, keys / kAttendStep, limit, keys, p.scale_log2, st);
-    if constexpr (CODE == PVLC_HIP_KV_F16 && CT == 1) {
-        if (new_row >= 0 && wave == 0) append_and_attend<F32>(p, set.first + r0, new_row, g, qf[0], st);  // uniform
-    }
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         const float l = column_sum(st.l[ct]);
@@ -204,13 +234,14 @@ __device__ inline void attend_part(const SharedRows &p, const SharedSet &set, in
         }
     }
     __syncthreads();
-    float a[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         float m = lds.m[0][ct * 16 + row];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) m = fmaxf(m, lds.m[w][ct * 16 + row]);
-        a[ct] = st.m[ct] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[ct] - m) * p.scale_log2);
+        const float a = st.m[ct] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[ct] - m) * p.scale_log2);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) lds.o[wave][(c * CT + ct) * 64 + lane] = st.o[ct][c] * a;
     }
     if (static_cast<int>(threadIdx.x) < columns) {
         const int c = threadIdx.x;
@@ -222,68 +253,86 @@ __device__ inline void attend_part(const SharedRows &p, const SharedSet &set, in
         part_ml[c * 2] = m * p.scale_log2;
         part_ml[c * 2 + 1] = l;
     }
-    // 4 / CT 16-dim tiles at a time.
-    constexpr int kTiles = 4 / CT;
+    __syncthreads();
 #pragma unroll
-    for (int c0 = 0; c0 < 8; c0 += kTiles) {
-        if (c0) __syncthreads();
+    for (int i = static_cast<int>(threadIdx.x); i < 8 * CT * 64; i += kThreads) {
+        const int n = i & 63, ct = (i >> 6) % CT, c = (i >> 6) / CT, column = ct * 16 + (n & 15);
+        float4_t v = lds.o[0][i];
 #pragma unroll
-        for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-            for (int ct = 0; ct < CT; ++ct) lds.o[((wave * kTiles + c) * CT + ct) * 64 + lane] = st.o[ct][c0 + c] * a[ct];
-        __syncthreads();
-        {
-            const int i = threadIdx.x, n = i & 63, ct = (i >> 6) % CT, c = (i >> 6) / CT, column = ct * 16 + (n & 15);
-            float4_t v = lds.o[i];
-#pragma unroll
-            for (int w = 1; w < kWaves; ++w) v += lds.o[w * 256 + i];
-            if (column < columns) *reinterpret_cast<float4_t *>(part_o + column * static_cast<int>(kHeadDim) + (c0 + c) * 16 + (n >> 4) * 4) = v;
-        }
+        for (int w = 1; w < kWaves; ++w) v += lds.o[w][i];
+        if (column < columns) *reinterpret_cast<float4_t *>(part_o + column * static_cast<int>(kHeadDim) + c * 16 + (n >> 4) * 4) = v;
     }
 }
 
-// Workgroup: share u, kv head, then the parts of the shared rows and those of
-// the set's sequences.
+// A part of a sequence's own rows, by one wave.  new_row: the sequence's length,
+// whose new row is one more key (fp16 pages), or -1.
+template <int CODE, bool F32>
+__device__ inline void attend_own(const SharedRows &p, const SharedSet &set, int r, uint32_t g, int keys, int first, int end, int new_row, float *part_o,
+                                  float *part_ml) {
+    const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
+    SharedQuery<CODE, F32> query[2];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) query[kb].send(p, set, r, g, kb);
+    __builtin_amdgcn_sched_barrier(0);
+    Attend<CODE, F32, 1> loop;
+    loop.begin(pages_of(p, set.first + r, set.shared, keys, g), first, end, 1);
+    half8_t qf[1][4];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) query[kb].take(&qf[0][kb], &qf[0][kb + 2]);
+    const int limit[1] = {keys};
+    AttendState<1> st;
+    st.clear();
+    loop.run(qf, keys / kAttendStep, limit, keys, p.scale_log2, st);
+    if constexpr (CODE == PVLC_HIP_KV_F16) {
+        if (new_row >= 0) append_and_attend<F32>(p, set.first + r, new_row, g, qf[0], st);  // uniform
+    }
+    const float l = column_sum(st.l[0]);
+    if (row < static_cast<int>(kGroup)) {
+        if (kg == 0) {
+            part_ml[row * 2] = st.m[0] * p.scale_log2;
+            part_ml[row * 2 + 1] = l;
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<float4_t *>(part_o + row * static_cast<int>(kHeadDim) + c * 16 + kg * 4) = st.o[0][c];
+    }
+}
+
+// Workgroup: share u and kv head, and a part of the shared rows, or a part of
+// every sequence's own ones, a wave each.
 template <int CODE, bool F32, int CT>
 __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedRows p) {
-    __shared__ SharedLds lds;
-    constexpr bool kNewRow = CODE == PVLC_HIP_KV_F16;  // (8-bit pages hold the new rows already)
+    __shared__ SharedLds<CT> lds;
+    constexpr int kNewRow = CODE == PVLC_HIP_KV_F16;  // (8-bit pages hold the new rows already)
     const uint32_t g = blockIdx.x & 1u;
     uint32_t b = blockIdx.x >> 1;
     const bool common = b < p.shares * p.shared_parts;  // uniform, as all below
     if (!common) b -= p.shares * p.shared_parts;
-    const uint32_t per = common ? p.shared_parts : 2 * CT * p.own_parts;
-    const uint32_t u = b / per, rest = b % per;
+    const uint32_t per = common ? p.shared_parts : p.own_parts, u = b / per;
+    const int part = static_cast<int>(b % per);
     SharedSet set;
     if (!find_set<CT>(p, u, &set)) return;
     const int shared_parts = static_cast<int>(p.shared_parts), own_parts = static_cast<int>(p.own_parts);
     const size_t unit = static_cast<size_t>(u) * 2 + g;
     float *const part_o = p.part_o + unit * p.unit_columns * kHeadDim, *const part_ml = p.part_ml + unit * p.unit_columns * 2;
-    const int own_column = shared_parts * CT * 16;
-    AttendPages pages{};
     if (common) {
-        const int part = static_cast<int>(rest), steps = part_steps(set.shared, shared_parts), first = part * steps;
-        if (part < parts_of(set.shared, shared_parts)) {
-            pages.table = p.ragged.tables + static_cast<size_t>(set.first) * p.ragged.max_blocks;
-            attend_part<CODE, F32, CT>(p, set, 0, set.count, g, pages, set.shared, first,
-                                       min(first + steps, (set.shared + kAttendStep - 1) / kAttendStep), -1, part_o + part * CT * 16 * static_cast<int>(kHeadDim),
-                                       part_ml + part * CT * 16 * 2, lds);
-        }
-    } else {
-        const int r = static_cast<int>(rest) / own_parts, part = static_cast<int>(rest) % own_parts;
-        if (r >= set.count) return;
-        const int seq = set.first + r, len = set.len(r);
-        const int keys = len + (kNewRow ? 0 : 1) - set.shared;
-        if (!fits(p, len)) {
-            if (threadIdx.x == 0 && part == 0) atomicOr(p.error_word, 1u);
-        } else if (part < parts_of(keys, own_parts) || (kNewRow && part == 0)) {
-            const int steps = part_steps(keys, own_parts), first = part * steps;
-            pages.table = p.ragged.tables + static_cast<size_t>(seq) * p.ragged.max_blocks + set.shared / static_cast<int>(kBlockTokens);
-            const int column = own_column + (r * own_parts + part) * static_cast<int>(kGroup);
-            attend_part<CODE, F32, 1>(p, set, r, 1, g, pages, keys, first, min(first + steps, (keys + kAttendStep - 1) / kAttendStep),
-                                      part == 0 ? len : -1, part_o + column * static_cast<int>(kHeadDim), part_ml + column * 2, lds);
-        }
+        const int steps = part_steps(set.shared, shared_parts, kLeastShared), first = part * steps, column = part * CT * 16;
+        if (part < parts_of(set.shared, shared_parts, kLeastShared))
+            attend_shared<CODE, F32, CT>(p, set, g, first, min(first + steps, (set.shared + kAttendStep - 1) / kAttendStep),
+                                         part_o + column * static_cast<int>(kHeadDim), part_ml + column * 2, lds);
+        return;
     }
+    const int r = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    if (r >= set.count) return;
+    const int len = set.len(r), keys = len + 1 - kNewRow - set.shared;
+    if (!fits(p, len)) {
+        if ((threadIdx.x & 63) == 0 && part == 0) atomicOr(p.error_word, 1u);
+        return;
+    }
+    if (part >= max(parts_of(keys, own_parts, kLeastOwn), kNewRow)) return;
+    const int steps = part_steps(keys, own_parts, kLeastOwn), first = part * steps;
+    const int column = shared_parts * CT * 16 + (r * own_parts + part) * static_cast<int>(kGroup);
+    attend_own<CODE, F32>(p, set, r, g, keys, first, min(first + steps, (keys + kAttendStep - 1) / kAttendStep), part == 0 ? len : -1,
+                          part_o + column * static_cast<int>(kHeadDim), part_ml + column * 2);
 }
 
 // Workgroup: a sequence and kv head; thread t has head t / 32 and dims t % 32 * 4
@@ -316,7 +365,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedRows p) {
     if (!find_set<CT>(p, u, &set) || r >= set.count) return;
     const int len = set.len(r);
     if (!fits(p, len)) return;
-    const int shared = parts_of(set.shared, shared_parts), own = max(parts_of(len + 1 - kNewRow - set.shared, own_parts), kNewRow);
+    const int shared = parts_of(set.shared, shared_parts, kLeastShared), own = max(parts_of(len + 1 - kNewRow - set.shared, own_parts, kLeastOwn), kNewRow);
     float m = -INFINITY, l = 0.f;
     float4_t o{0.f, 0.f, 0.f, 0.f};
     for (int i0 = 0;;) {
@@ -348,7 +397,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedRows p) {
 
 template <int CODE, bool F32, int CT>
 void launch(const SharedRows &p, hipStream_t stream) {
-    hipLaunchKernelGGL((shared_attention_kernel<CODE, F32, CT>), dim3(2 * p.shares * (p.shared_parts + 2 * CT * p.own_parts)), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((shared_attention_kernel<CODE, F32, CT>), dim3(2 * p.shares * (p.shared_parts + p.own_parts)), dim3(kThreads), 0, stream, p);
     hipLaunchKernelGGL((shared_join_kernel<CODE, F32, CT>), dim3(2 * p.shares * 2 * CT), dim3(256), 0, stream, p);
 }
 

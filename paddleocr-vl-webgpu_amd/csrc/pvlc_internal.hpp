@@ -223,6 +223,12 @@ struct RaggedRows {
     const int32_t *tables;
     uint32_t max_tokens;  // that a sequence may come to hold
 };
+// Shares of UNIT rows that n rows take: with SPARE 1 from their own first row
+// on, with SPARE 2 from any row of a share on.
+template <int UNIT, int SPARE>
+constexpr uint32_t shares_of_each(uint32_t n) {
+    return SPARE == 2 ? (n + UNIT - 2) / UNIT + 1 : (n + UNIT - 1) / UNIT;
+}
 // Packed prompts: 16 tokens t0 .. of a sequence (its rows begin at `begin`) and
 // the pieces of 32 keys that one workgroup takes; slot: where it leaves a part
 // of them, or -1.
@@ -340,7 +346,7 @@ inline SharedWorkspace shared_workspace_layout(uint32_t num_seqs, uint32_t num_g
     w.shares = offsets ? num_seqs / (2 * w.columns) + num_groups : num_groups * ((each + 2 * w.columns - 1) / (2 * w.columns));
     const uint32_t most = clamp((max_context + 32 * kSharedWaves - 1) / (32 * kSharedWaves), 64);
     w.shared_parts = clamp((256 / (2 * w.shares) + 3) / 4 * 4, most);
-    w.own_parts = clamp(256 / (2 * num_seqs), most);
+    w.own_parts = clamp(128 / (2 * w.shares), most);
     w.unit_columns = w.shared_parts * w.columns * 16 + 2 * w.columns * w.own_parts * kGroup;
     const size_t columns = static_cast<size_t>(w.shares) * 2 * w.unit_columns;
     w.part_o_offset = 256;

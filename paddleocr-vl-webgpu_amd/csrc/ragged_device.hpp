@@ -22,10 +22,22 @@ struct SeqRows {
 // SPARE - 1 shares, so that no workgroup has to add up the lengths before it.
 // Every wave looks 64 sequences at once: one round of loads up to 64 sequences, two
 // up to 4096.  Whatever the offsets hold, the sequence is one of the call's.
+// Without offsets every sequence has shares_of_each.
 template <int UNIT, int SPARE>
 __device__ inline SeqRows find_share(const RaggedRows &r, uint32_t u) {
+    SeqRows q;
+    if (!r.offsets) {
+        const uint32_t per = shares_of_each<UNIT, SPARE>(r.each), s = min(u / per, r.num_seqs - 1);
+        q.seq = static_cast<int>(s);
+        q.begin = static_cast<int>(s * r.each);
+        q.count = static_cast<int>(r.each);
+        q.held = r.lens ? r.lens[s] : 0;
+        q.share = static_cast<int>(u - s * per);
+        q.ok = q.held >= 0 && static_cast<int64_t>(q.held) + q.count <= static_cast<int64_t>(r.max_tokens);
+        return q;
+    }
     const uint32_t lane = threadIdx.x & 63u;
-    auto offset = [&](uint32_t s) { return r.offsets ? r.offsets[s] : static_cast<int32_t>(s * r.each); };
+    auto offset = [&](uint32_t s) { return r.offsets[s]; };
     auto first = [&](int32_t at, uint32_t s) { return static_cast<uint32_t>(max(at, 0)) / UNIT + SPARE * s; };
     uint32_t lo = 0, n = r.num_seqs;
     while (n > 64) {
@@ -39,7 +51,6 @@ __device__ inline SeqRows find_share(const RaggedRows &r, uint32_t u) {
     const int32_t a = offset(s), b = offset(s + 1), held = r.lens ? r.lens[s] : 0;
     const uint64_t before = __ballot(lane < n && first(a, s) <= u);
     const int k = before ? 63 - __builtin_clzll(before) : 0;
-    SeqRows q;
     q.seq = static_cast<int>(lo) + k;
     q.begin = __builtin_amdgcn_readlane(a, k);
     const int end = __builtin_amdgcn_readlane(b, k);
