@@ -215,6 +215,39 @@ pvlc_hip_status prefill(const pvlc_hip_packed_prefill_args *args, const void *qu
     return ok();
 }
 
+// The call as a paged decode (its checks are those of that one's arguments).
+pvlc_hip_status decode_alone(const pvlc_hip_shared_decode_args *args, const void *query, const void *key, const void *value, void *out, bool f32,
+                             void *stream) {
+    pvlc_hip_paged_decode_args d{};
+    d.num_seqs = args->num_seqs;
+    d.num_blocks = args->num_blocks;
+    d.max_blocks_per_seq = args->max_blocks_per_seq;
+    d.block_tables = args->block_tables;
+    d.cache_lens = args->cache_lens;
+    d.max_context = args->max_context;
+    d.key_cache = static_cast<uint16_t *>(args->key_cache);
+    d.value_cache = static_cast<uint16_t *>(args->value_cache);
+    d.rope_cos = args->rope_cos;
+    d.rope_sin = args->rope_sin;
+    d.rope_rows = args->rope_rows;
+    d.positions = args->positions;
+    d.rotate_query = args->rotate_query;
+    d.workspace = args->workspace;
+    d.workspace_bytes = args->workspace_bytes;
+    DecodeOperands32 o{};
+    if (f32) {
+        o = {static_cast<const float *>(query), static_cast<const float *>(key), static_cast<const float *>(value), static_cast<float *>(out)};
+    } else {
+        d.query = static_cast<const uint16_t *>(query);
+        d.new_key = static_cast<const uint16_t *>(key);
+        d.new_value = static_cast<const uint16_t *>(value);
+        d.out = static_cast<uint16_t *>(out);
+    }
+    const DecodeCodes codes{args->code, args->exponents};
+    if (pvlc_hip_status st = launch_decode_checked(&d, stream, nullptr, f32 ? &o : nullptr, args->code == PVLC_HIP_KV_F16 ? nullptr : &codes)) return st;
+    return ok();
+}
+
 pvlc_hip_status shared(const pvlc_hip_shared_decode_args *args, const void *query, const void *key, const void *value, void *out, bool f32,
                        void *stream) {
     if (!args) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "shared decode args are NULL");
@@ -251,10 +284,14 @@ pvlc_hip_status shared(const pvlc_hip_shared_decode_args *args, const void *quer
     Range queries, outs;
     if (pvlc_hip_status st = check_matrix(query, &query_stride, args->num_seqs, kQueryHeads * kHeadDim, size, "query", &queries)) return st;
     if (pvlc_hip_status st = check_matrix(out, &out_stride, args->num_seqs, kQueryHeads * kHeadDim, size, "out", &outs)) return st;
-    const SharedWorkspace ws = shared_workspace_layout(args->num_seqs, args->num_groups, args->max_context, args->group_offsets != nullptr);
-    if (pvlc_hip_status st = check_workspace(args, ws.total, "shared decode")) return st;
+    const bool offsets = args->group_offsets != nullptr;
+    const bool small = shared_is_small(args->num_seqs, args->num_groups, args->max_context, offsets, args->code);
+    const SharedWorkspace ws = shared_workspace_layout(args->num_seqs, args->num_groups, args->max_context, offsets);
+    const size_t needed = small ? pvlc_hip_paged_decode_workspace_bytes(args->num_seqs, args->max_context, 0) : ws.total;
+    if (pvlc_hip_status st = check_workspace(args, needed, "shared decode")) return st;
     const Range groups{args->group_offsets, 4ull * args->num_groups + 4}, lens{args->shared_lens, 4ull * args->num_groups};
-    if (pvlc_hip_status st = check_apart(rows, keys, values, {queries, groups, lens}, {{args->workspace, ws.total}, outs})) return st;
+    if (pvlc_hip_status st = check_apart(rows, keys, values, {queries, groups, lens}, {{args->workspace, needed}, outs})) return st;
+    if (small) return decode_alone(args, query, key, value, out, f32, stream);
     a.ragged.max_tokens = args->max_context;
     auto *base = static_cast<unsigned char *>(args->workspace);
     SharedRows r{};
@@ -322,7 +359,12 @@ size_t pvlc_hip_shared_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_gr
     if (num_seqs == 0 || num_groups == 0 || max_context == 0) return 0;
     const size_t with = shared_workspace_layout(num_seqs, num_groups, max_context, true).total;
     const size_t without = shared_workspace_layout(num_seqs, num_groups, max_context, false).total;
-    return with > without ? with : without;
+    size_t most = with > without ? with : without;
+    if (shared_is_small(num_seqs, num_groups, max_context, false, PVLC_HIP_KV_E4M3)) {
+        const size_t alone = pvlc_hip_paged_decode_workspace_bytes(num_seqs, max_context, 0);
+        most = most > alone ? most : alone;
+    }
+    return most;
 }
 
 pvlc_hip_status pvlc_hip_shared_decode_f16(const pvlc_hip_shared_decode_args *args, const uint16_t *query, const uint16_t *new_key,

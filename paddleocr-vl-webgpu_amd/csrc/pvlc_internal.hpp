@@ -331,7 +331,24 @@ struct SharedRows {
     float *part_o, *part_ml;
 };
 int launch_shared_decode(const SharedRows &rows, void *stream);
-// Its workspace: 256 bytes of words (0 the error word), then the parts' results.
+// Calls that the paged decode answers sooner, each sequence reading all of its
+// rows: those of up to so many rows (num_seqs times max_context; what is shared,
+// and how many rows there are, the host does not know), and those without a
+// group of two.  Two launches (three over 8-bit pages) take 10-20 us of any
+// call, the paged decode's one 8-12 of these: 4 sequences of 1157 rows 12.1
+// against 8.3 us (fp16) and 15.3 against 7.9 (e4m3), 16 groups of 4 (80 thousand
+// rows) 16.6 against 16.4 and 18.8 against 12.3, 16 groups of 8 (160 thousand)
+// 17.8 against 24.1 and 20.7 against 19.5, 32 groups of 8 (320 thousand) 26.8
+// against 44.4 and 30.2 against 32.4, 64 sequences with none in common 30.3
+// against 28.6 and 25.3 against 19.0.
+constexpr uint32_t kSharedLeastRows = 80000, kSharedLeastRowsQ8 = 200000;
+inline bool shared_is_small(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context, bool offsets, uint32_t code) {
+    if (num_seqs > kMaxRaggedSeqs || max_context > kMaxMergeParts * 4096) return false;
+    return (!offsets && num_seqs == num_groups) ||
+           static_cast<uint64_t>(num_seqs) * max_context <= (code == PVLC_HIP_KV_F16 ? kSharedLeastRows : kSharedLeastRowsQ8);
+}
+// Its workspace: the paged decode's words and counters (0 the error word), which
+// no call's parts lie on, then the parts' results.
 constexpr uint32_t kMaxSharedSets = 16384;
 struct SharedWorkspace {
     uint32_t columns, shares, shared_parts, own_parts, unit_columns;
@@ -349,7 +366,7 @@ inline SharedWorkspace shared_workspace_layout(uint32_t num_seqs, uint32_t num_g
     w.own_parts = clamp(128 / (2 * w.shares), most);
     w.unit_columns = w.shared_parts * w.columns * 16 + 2 * w.columns * w.own_parts * kGroup;
     const size_t columns = static_cast<size_t>(w.shares) * 2 * w.unit_columns;
-    w.part_o_offset = 256;
+    w.part_o_offset = 256 + align(kMaxRaggedSeqs * kKvHeads * 4);
     w.part_ml_offset = w.part_o_offset + align(columns * kHeadDim * 4);
     w.total = w.part_ml_offset + align(columns * 8);
     return w;

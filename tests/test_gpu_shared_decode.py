@@ -10,12 +10,14 @@ from pvlc_testlib import log, pvlc
 pytestmark = pytest.mark.gpu
 CODES = pytest.mark.parametrize("code", [B.F16, R.E4M3, R.INT8])
 WIDTHS = pytest.mark.parametrize("f32", [False, True])
+# Calls of few rows run as paged decodes: `far` makes room for more rows than those have, and the sequences as short as they were.
+FAR = pytest.mark.parametrize("far", [False, True])
 
 
 class Groups(B.Batch):
     """Groups of sizes whose sequences have their first `shared` rows in common (in whole blocks) and `tails` of their own."""
 
-    def __init__(self, sizes, shared, tails, code, f32, seed=0, **how):
+    def __init__(self, sizes, shared, tails, code, f32, seed=0, far=True, **how):
         self.sizes, self.shared = list(sizes), list(shared)
         group = np.repeat(np.arange(len(sizes)), sizes)
         held = [shared[g] + t for g, t in zip(group, tails)]
@@ -25,6 +27,9 @@ class Groups(B.Batch):
         for i, g in enumerate(group):  # the others repeat the first one's entries
             whole = shared[g] // 16
             self.table[i, :whole] = self.table[firsts[g], :whole]
+        if far:
+            self.width = max(self.width, -(-220000 // self.n // 16))
+            self.table = np.pad(self.table, ((0, 0), (0, self.width - self.table.shape[1])), constant_values=-1)
 
     def shared_args(self, ws, offsets=False, **change):
         import torch
@@ -79,11 +84,12 @@ CASES = {
 
 @CODES
 @WIDTHS
+@FAR
 @pytest.mark.parametrize("name", list(CASES))
-def test_groups_of_one_size(code, f32, name):
-    log(f"case: shared decode {name} code={code} f32={f32}")
+def test_groups_of_one_size(code, f32, far, name):
+    log(f"case: shared decode {name} code={code} f32={f32} far={far}")
     sizes, shared, tails = CASES[name]
-    c = Groups(sizes, shared, tails, code, f32, seed=len(name), positions=name == "pages", rope=name != "answers").upload()
+    c = Groups(sizes, shared, tails, code, f32, seed=len(name), far=far, positions=name == "pages", rope=name != "answers").upload()
     ws = c.workspace()
     c.launch(c.shared_args(ws, rotate_query=name != "beams"))
     c.check(name, rotate_query=name != "beams")
@@ -115,18 +121,19 @@ def test_rows_that_are_not_shared_by_all(code):
 
 
 @CODES
-def test_errors_are_reported_and_skipped(code):
+@FAR
+def test_errors_are_reported_and_skipped(code, far):
     import torch
-    log(f"case: shared decode errors, code={code}")
+    log(f"case: shared decode errors, code={code} far={far}")
     ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
-    c = Groups([3, 2], [48, 16], [0, 5, 20, 3, 4], code, False, seed=3).upload()
+    c = Groups([3, 2], [48, 16], [0, 5, 20, 3, 4], code, False, seed=3, far=far).upload()
     ws = c.workspace()
     lens = list(c.held)
     lens[1], lens[3] = -1, c.width * 16
     c.launch(c.shared_args(ws, offsets=True, cache_lens=ints(lens)))
     c.check("lengths", skipped=(1, 3))
     assert pvlc.workspace_error(*ws) == 1
-    c = Groups([2], [32], [5, 9], code, False, seed=4).upload()  # a position outside the tables: no rotation
+    c = Groups([2], [32], [5, 9], code, False, seed=4, far=far).upload()  # a position outside the tables: no rotation
     ws = c.workspace()
     c.launch(c.shared_args(ws, positions=ints([c.table_rows, -1])))
     c.rope = False
@@ -139,7 +146,8 @@ def test_steps_from_a_graph_beside_direct_calls():
     import torch
     log("case: shared decode from a graph")
     for code in (B.F16, R.E4M3):
-        one, two = Groups([4], [700], [3, 9, 0, 40], code, True, seed=5).upload(), Groups([2] * 9, [40] * 9, tails_of(18, 20), code, True, seed=6).upload()
+        one = Groups([4], [700], [3, 9, 0, 40], code, True, seed=5).upload()
+        two = Groups([2] * 9, [40] * 9, tails_of(18, 20), code, True, seed=6, far=False).upload()  # (a paged decode on the same words)
         nbytes = max(pvlc.shared_decode_workspace_bytes(c.n, len(c.sizes), c.width * 16) for c in (one, two))
         ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
         pvlc.workspace_init(ws, nbytes)
@@ -170,12 +178,12 @@ def test_far_blocks():
     log("case: shared decode, far blocks")
     c = Groups([3], [40], [2, 20, 9], B.F16, True, seed=7).upload()
     blocks = (1 << 31) // 4096 + 300
-    far = torch.from_numpy(np.arange(blocks - c.blocks, blocks).astype(np.int32)).cuda()
+    ids = torch.from_numpy(np.arange(blocks - c.blocks, blocks).astype(np.int32)).cuda()
     planes = [torch.zeros(blocks * 4096, dtype=torch.int16, device="cuda") for _ in range(2)]
     for p, small in zip(planes, c.planes):
         p.view(blocks, 4096)[blocks - c.blocks:] = small.view(c.blocks, 4096)
     ws = c.workspace()
-    c.launch(c.shared_args(ws, num_blocks=blocks, key_cache=planes[0], value_cache=planes[1], block_tables=far[c.dtable.long()]))
+    c.launch(c.shared_args(ws, num_blocks=blocks, key_cache=planes[0], value_cache=planes[1], block_tables=torch.where(c.dtable < 0, -1, ids[c.dtable.clamp_min(0).long()])))
     torch.cuda.synchronize()
     for p, small in zip(planes, c.planes):
         small.copy_(p.view(blocks, 4096)[blocks - c.blocks:].view_as(small))
