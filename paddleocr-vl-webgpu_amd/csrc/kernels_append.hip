@@ -15,17 +15,35 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kPad = 8;  // elements behind each LDS row of 256 dims, against bank conflicts
-// Key piece i (16 bytes) of a block's two 8-bit slabs: its token, and its first dim among both heads.
-__device__ inline int q8_key_token(int i) { return ((i >> 5) & 3) * 4 + (i & 3); }
-__device__ inline int q8_key_dim(int i) { return (i >> 7) * kHeadDim + ((i >> 2) & 7) * 16; }
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+constexpr uint32_t kLargestHalf = 0x7BFF;  // 65504; infinity is the next, NaN behind
+
+__device__ inline uint32_t largest(u16x8_t x) {
+    uint16_t m = x[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m = max(m, x[j]);
+    return m;
+}
+// Over the row of 16 lanes.
+__device__ inline uint32_t row_max(uint32_t x) {
+#define PVLC_ROW_MAX(CTRL) x = max(x, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), CTRL, 0xF, 0xF, false)))
+    PVLC_ROW_MAX(0xB1);
+    PVLC_ROW_MAX(0x4E);
+    PVLC_ROW_MAX(0x124);
+    PVLC_ROW_MAX(0x128);
+#undef PVLC_ROW_MAX
+    return x;
+}
 
 // A workgroup for each 16-token block that a sequence writes to, both heads.
 // Keys: every thread rotates one pair of 8-dim chunks, c and c + 8, which are
 // each other's partners (item = head, pair, token).  fp16 pages: 16 threads fill
 // a 256-byte run of the key slab, and the values are turned through LDS into
-// 32-byte rows of the value slab.  8-bit pages: both go through LDS, the block's
-// exponents come from the sizes, and rows that the block holds already are
-// rounded again where these grew.  Other tokens of a block stay as they are.
+// 32-byte rows of the value slab.  8-bit pages: the block's exponents come from
+// the sizes, and rows that the block holds already are rounded again where these
+// grew; 8 dims of a token are 8 bytes, stored from the registers (a wave's fill
+// runs of 64 bytes; with the keys in LDS too, as they had been, a compute unit held
+// six workgroups in place of eight).  Other tokens of a block stay as they are.
 //
 // Short calls are bound by the chain of dependent rounds: the sequence; its
 // table entry, positions and rows; cos and sin; (8 bits: the old block with the
@@ -33,8 +51,8 @@ __device__ inline int q8_key_dim(int i) { return (i >> 7) * kHeadDim + ((i >> 2)
 template <bool F32, int CODE>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendRows p) {
     constexpr bool kQ8 = CODE != PVLC_HIP_KV_F16;
-    __shared__ __align__(16) uint16_t sr[kQ8 ? 2 : 1][kBlockTokens][kRowElems + kPad];
-    __shared__ uint32_t sm_size[2][kKvHeads];
+    __shared__ __align__(16) uint16_t sv[kBlockTokens][kRowElems + kPad];
+    __shared__ uint32_t sm_size[2][kKvHeads], sm_special;
     typedef std::conditional_t<F32, float, uint16_t> Element;
     typedef std::conditional_t<F32, float4_t, half8_t> Raw;
     constexpr int kLoads = F32 ? 2 : 1, kElems = F32 ? 4 : 8;
@@ -67,8 +85,10 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendRows p) {
 
     const int tt = i & 15, c = (i >> 4) & 7, hh = i >> 7;
     const int64_t t = row0 + min(max(tt, lo), hi - 1);  // (tokens that are not the call's repeat one that is)
-    const int64_t id_raw = p.ragged.tables ? p.ragged.tables[entry] : entry;
-    const int64_t pos = p.positions ? p.positions[t] : t - q.begin + q.held;
+    // (Arrays that are not given are read through the key pointer, so that no load waits behind a branch.)
+    const int32_t *stand_in = static_cast<const int32_t *>(p.key);
+    const int32_t id_given = load_const(p.ragged.tables ? p.ragged.tables + entry : stand_in, 0);
+    const int32_t pos_given = *(p.positions ? p.positions + t : stand_in);
     Raw key[2][kLoads], val[2][kLoads];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -81,40 +101,58 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendRows p) {
             val[r][f] = *reinterpret_cast<const Raw *>(vs + f * kElems);
         }
     }
+    __builtin_amdgcn_sched_barrier(0);
+    const int64_t pos = p.positions ? pos_given : t - q.begin + q.held;
     const bool rope = p.rope_cos != nullptr && pos >= 0 && pos < static_cast<int64_t>(p.rope_rows);
-    float4_t cs[2]{}, sn[2]{};
-    if (rope) {
+    float4_t cs[2], sn[2];
+    {
+        const float *cr = rope ? p.rope_cos + pos * 64 + c * 8 : reinterpret_cast<const float *>(stand_in);
+        const float *sr = rope ? p.rope_sin + pos * 64 + c * 8 : reinterpret_cast<const float *>(stand_in);
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
-            cs[f] = *reinterpret_cast<const float4_t *>(p.rope_cos + pos * 64 + c * 8 + f * 4);
-            sn[f] = *reinterpret_cast<const float4_t *>(p.rope_sin + pos * 64 + c * 8 + f * 4);
+            cs[f] = *reinterpret_cast<const float4_t *>(cr + f * 4);
+            sn[f] = *reinterpret_cast<const float4_t *>(sr + f * 4);
         }
     }
+    __builtin_amdgcn_sched_barrier(0);
     bool ok;
-    const uint32_t id = checked_block(p.ragged, id_raw, &ok);  // uniform
-    q8x4_t old_k{}, old_v{};
+    const uint32_t id = checked_block(p.ragged, p.ragged.tables ? id_given : entry, &ok);  // uniform
+    u32x2_t old_k[2]{};
+    q8x4_t old_v{};
     uint32_t old_e = 0;
     const bool whole = lo == 0 && hi == static_cast<int>(kBlockTokens);  // uniform
-    const size_t slab = static_cast<size_t>(id) * kKvHeads * kQ8SlabBytes + static_cast<size_t>(i) * 16;
+    // 8 bits: the bytes of dims c * 8 .. of token tt (64 dims on: 256 bytes on), and (head, dim) i of the values.
+    const size_t slab = static_cast<size_t>(id) * kKvHeads * kQ8SlabBytes;
+    uint8_t *const key_bytes = static_cast<uint8_t *>(p.key_cache) + slab + hh * static_cast<int>(kQ8SlabBytes) + (tt >> 2) * 512 + (c >> 1) * 64 + (tt & 3) * 16 + (c & 1) * 8;
+    uint8_t *const value_bytes = static_cast<uint8_t *>(p.value_cache) + slab + i * 16;
     if (kQ8 && ok && !whole) {
-        old_k = *reinterpret_cast<const q8x4_t *>(static_cast<uint8_t *>(p.key_cache) + slab);
-        old_v = *reinterpret_cast<const q8x4_t *>(static_cast<uint8_t *>(p.value_cache) + slab);
-        old_e = *reinterpret_cast<const uint16_t *>(p.exponents + (static_cast<size_t>(id) * kKvHeads + (i >> 7)) * 2);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) old_k[r] = *reinterpret_cast<const u32x2_t *>(key_bytes + r * 256);
+        old_v = *reinterpret_cast<const q8x4_t *>(value_bytes);
+        old_e = *reinterpret_cast<const uint16_t *>(p.exponents + (static_cast<size_t>(id) * kKvHeads + hh) * 2);
     }
     if (kQ8 && i < 2 * static_cast<int>(kKvHeads)) sm_size[i >> 1][i & 1] = 0;
+    if (kQ8 && i == 0) sm_special = 0;
     half8_t out[2];
+    if (__any(rope)) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {  // as rotate_chunk rotates
-        const float x = static_cast<float>(key[0][j / kElems][j % kElems]);
-        const float y = static_cast<float>(key[1][j / kElems][j % kElems]);
-        const float co = cs[j >> 2][j & 3], si = sn[j >> 2][j & 3];
-        out[0][j] = to_h(rope ? x * co + (-y) * si : x);
-        out[1][j] = to_h(rope ? y * co + x * si : y);
+        for (int j = 0; j < 8; ++j) {  // as rotate_chunk rotates
+            const float x = static_cast<float>(key[0][j / kElems][j % kElems]);
+            const float y = static_cast<float>(key[1][j / kElems][j % kElems]);
+            const float co = cs[j >> 2][j & 3], si = sn[j >> 2][j & 3];
+            out[0][j] = to_h(x * co + (-y) * si);
+            out[1][j] = to_h(y * co + x * si);
+        }
     }
-    if constexpr (!F32) {
-        if (!rope) {  // as given, bit for bit
-            out[0] = key[0][0];
-            out[1] = key[1][0];
+    if (__any(!rope) && !rope) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            if constexpr (F32) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) out[r][j] = to_h(key[r][j / kElems][j % kElems]);
+            } else {
+                out[r] = key[r][0];  // as given, bit for bit
+            }
         }
     }
     half8_t v[2];
@@ -127,8 +165,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendRows p) {
             v[r] = val[r][0];
         }
         const int k = i + r * kThreads;
-        *reinterpret_cast<half8_t *>(&sr[kQ8 ? 1 : 0][k >> 5][(k & 31) * 8]) = v[r];
-        if constexpr (kQ8) *reinterpret_cast<half8_t *>(&sr[0][tt][hh * kHeadDim + c * 8 + r * 64]) = out[r];
+        *reinterpret_cast<half8_t *>(&sv[k >> 5][(k & 31) * 8]) = v[r];
     }
     if (p.error_word) {
         if (!ok && i == 0) atomicOr(p.error_word, 2u);
@@ -147,68 +184,80 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendRows p) {
             u16x8_t a, b;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                a[e] = sr[0][e][i];
-                b[e] = sr[0][e + 8][i];
+                a[e] = sv[e][i];
+                b[e] = sv[e + 8][i];
             }
             *reinterpret_cast<u16x8_t *>(dst) = a;
             *reinterpret_cast<u16x8_t *>(dst + 8) = b;
         } else {
-            for (int e = lo; e < hi; ++e) dst[e] = sr[0][e][i];
+            for (int e = lo; e < hi; ++e) dst[e] = sv[e][i];
         }
     } else {
         __syncthreads();  // the rows are in LDS, and sm_size is cleared
-        auto widen = [](uint16_t x) { return q8_value(static_cast<float>(__builtin_bit_cast(_Float16, x))); };
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             // A wave's key items are of one head; 16 lanes hold the values of one
-            // head.  Sizes are not negative, so their bits are in order.
-            float size = 0.f;
+            // head.  fp16 sizes are in the order of their bits.
+            const u16x8_t every = static_cast<uint16_t>(0x7FFF);
+            const u16x8_t a = __builtin_bit_cast(u16x8_t, w ? v[0] : out[0]) & every, b = __builtin_bit_cast(u16x8_t, w ? v[1] : out[1]) & every;
+            uint32_t size = largest(__builtin_elementwise_max(a, b));
+            if (size > kLargestHalf) {  // an infinity counts as the largest value, a NaN as none
+                size = 0;
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) size = q8_size(size, q8_value(static_cast<float>(w ? v[r][j] : out[r][j])));
-            size = fmaxf(size, dpp_f32<0xB1>(size));
-            size = fmaxf(size, dpp_f32<0x4E>(size));
-            size = fmaxf(size, dpp_f32<0x124>(size));
-            size = fmaxf(size, dpp_f32<0x128>(size));
-            if ((i & 15) == 0) atomicMax(&sm_size[w][w ? (i >> 4) & 1 : hh], __float_as_uint(size));
+                for (int j = 0; j < 8; ++j) {
+                    if (a[j] <= kLargestHalf + 1u) size = max(size, min(static_cast<uint32_t>(a[j]), kLargestHalf));
+                    if (b[j] <= kLargestHalf + 1u) size = max(size, min(static_cast<uint32_t>(b[j]), kLargestHalf));
+                }
+                sm_special = 1;
+            }
+            size = row_max(size);
+            if ((i & 15) == 0) atomicMax(&sm_size[w][w ? (i >> 4) & 1 : hh], size);
         }
         __syncthreads();
         if (!ok) return;
-        const int head = i >> 7;  // of key piece i and of value row i
-        int e[2], grown[2];
+        const bool special = sm_special != 0;  // uniform
+        // Four fp16 values to codes.  Without infinities and NaN nothing is clamped, and the sum of
+        // an int8 code and 1.5 2^23 has the code, rounded to even, as its low byte.
+        auto encode = [&](_Float16 x0, _Float16 x1, _Float16 x2, _Float16 x3, float inv) -> uint32_t {
+            const float f0 = static_cast<float>(x0), f1 = static_cast<float>(x1), f2 = static_cast<float>(x2), f3 = static_cast<float>(x3);
+            if (special) return q8_encode<CODE>(q8_value(f0) * inv, q8_value(f1) * inv, q8_value(f2) * inv, q8_value(f3) * inv);
+            if constexpr (CODE == PVLC_HIP_KV_E4M3) {
+                return q8_encode<CODE>(f0 * inv, f1 * inv, f2 * inv, f3 * inv);
+            } else {
+                constexpr float kWhole = 12582912.0f;
+                auto bits = [&](float f) { return __float_as_uint(__builtin_fmaf(f, inv, kWhole)); };
+                return __builtin_amdgcn_perm(bits(f1), bits(f0), 0x0C0C0400u) | __builtin_amdgcn_perm(bits(f3), bits(f2), 0x04000C0Cu);
+            }
+        };
+        int e[2], grown[2];  // of head hh: the thread's keys and its row of the values
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-            e[w] = q8_exponent<CODE>(__uint_as_float(sm_size[w][head]));
+            e[w] = q8_exponent<CODE>(static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(sm_size[w][hh]))));
             const int before = static_cast<int>((old_e >> (8 * w)) & 255) - kQ8Bias;
             if (lo > 0) e[w] = max(e[w], before);
             grown[w] = lo > 0 ? e[w] - before : 0;
         }
-        {
-            const int token = q8_key_token(i);
+        if (tt < hi && (tt >= lo || grown[0] > 0)) {
             const float inv = exp2_whole(-e[0]);
-            const uint16_t *src = &sr[0][token][q8_key_dim(i)];
-            const u16x8_t a = *reinterpret_cast<const u16x8_t *>(src), b = *reinterpret_cast<const u16x8_t *>(src + 8);
-            q8x4_t codes;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const u16x8_t &x = w < 2 ? a : b;
-                const int j = (w & 1) * 4;
-                codes[w] = q8_encode<CODE>(widen(x[j]) * inv, widen(x[j + 1]) * inv, widen(x[j + 2]) * inv, widen(x[j + 3]) * inv);
-            }
-            if (token < lo && grown[0] > 0) {
+            for (int r = 0; r < 2; ++r) {
+                const half8_t &x = out[r];
+                u32x2_t codes = {encode(x[0], x[1], x[2], x[3], inv), encode(x[4], x[5], x[6], x[7], inv)};
+                if (lo > 0) {  // uniform
 #pragma unroll
-                for (int w = 0; w < 4; ++w) codes[w] = q8_requantise<CODE>(old_k[w], grown[0]);
+                    for (int w = 0; w < 2; ++w) codes[w] = tt < lo ? q8_requantise<CODE>(old_k[r][w], grown[0]) : codes[w];
+                }
+                *reinterpret_cast<u32x2_t *>(key_bytes + r * 256) = codes;
             }
-            if (token < hi && (token >= lo || grown[0] > 0)) *reinterpret_cast<q8x4_t *>(static_cast<uint8_t *>(p.key_cache) + slab) = codes;
         }
         {
             const float inv = exp2_whole(-e[1]);
             q8x4_t codes;
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-                codes[w] = q8_encode<CODE>(widen(sr[1][w * 4][i]) * inv, widen(sr[1][w * 4 + 1][i]) * inv, widen(sr[1][w * 4 + 2][i]) * inv,
-                                           widen(sr[1][w * 4 + 3][i]) * inv);
+            for (int w = 0; w < 4; ++w) {
+                auto value = [&](int j) { return __builtin_bit_cast(_Float16, sv[w * 4 + j][i]); };
+                codes[w] = encode(value(0), value(1), value(2), value(3), inv);
+            }
             if (!whole) {
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
@@ -222,10 +271,10 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendRows p) {
                     codes[w] = x;
                 }
             }
-            *reinterpret_cast<q8x4_t *>(static_cast<uint8_t *>(p.value_cache) + slab) = codes;
+            *reinterpret_cast<q8x4_t *>(value_bytes) = codes;
         }
         if ((i & 127) == 0)
-            *reinterpret_cast<uint16_t *>(p.exponents + (static_cast<size_t>(id) * kKvHeads + head) * 2) =
+            *reinterpret_cast<uint16_t *>(p.exponents + (static_cast<size_t>(id) * kKvHeads + hh) * 2) =
                 static_cast<uint16_t>((e[0] + kQ8Bias) | (e[1] + kQ8Bias) << 8);
     }
 }
