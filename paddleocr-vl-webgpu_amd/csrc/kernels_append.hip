@@ -69,10 +69,8 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendRows p) {
         }
     }
     const SeqRows q = find_share<16, 2>(p.ragged, share);
-    if (!q.ok) {
-        if (i == 0 && p.error_word) atomicOr(p.error_word, 1u);
-        return;  // uniform, as below
-    }
+    if ((!q.ok || q.told) && i == 0 && p.error_word) atomicOr(p.error_word, 1u);
+    if (!q.ok) return;  // uniform, as below
     const int64_t end = static_cast<int64_t>(q.held) + q.count;
     const int64_t block = static_cast<int64_t>(q.held / static_cast<int>(kBlockTokens)) + q.share;
     if (q.count == 0 || block * kBlockTokens >= end) return;

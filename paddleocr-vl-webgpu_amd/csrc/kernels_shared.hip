@@ -37,10 +37,8 @@ __device__ inline bool find_set(const SharedRows &p, uint32_t u, SharedSet *set)
         groups.max_tokens = 0xFFFFFFFFu;
         const SeqRows q = find_share<2 * CT, 1>(groups, u);
         first = q.share * 2 * CT;
-        if (!q.ok || first >= q.count) {
-            if (!q.ok && threadIdx.x == 0) atomicOr(p.error_word, 1u);
-            return false;
-        }
+        if ((!q.ok || q.told) && threadIdx.x == 0) atomicOr(p.error_word, 1u);
+        if (!q.ok || first >= q.count) return false;
         begin = q.begin;
         count = q.count;
         least = q.held;

@@ -14,6 +14,7 @@ namespace pvlc {
 struct SeqRows {
     int seq, begin, count, held;
     bool ok;    // the offsets ascend within the call's rows, and the rows fit the sequence's pages
+    bool told;  // offsets of the call that the wave has seen do not: to be reported
     int share;  // the workgroup's number within the sequence
 };
 
@@ -21,7 +22,10 @@ struct SeqRows {
 // SPARE * s: a closed form that leaves a sequence of n rows at least n / UNIT +
 // SPARE - 1 shares, so that no workgroup has to add up the lengths before it.
 // Every wave looks 64 sequences at once: one round of loads up to 64 sequences, two
-// up to 4096.  Whatever the offsets hold, the sequence is one of the call's.
+// up to 4096.  Whatever the offsets hold, the sequence is one of the call's, and the
+// share's number is not negative (shares before the first sequence's have no
+// rows).  Of offsets that descend or leave the rows some wave is told: a window of
+// the search that no wave looks into starts behind one that passes it.
 // Without offsets every sequence has shares_of_each.
 template <int UNIT, int SPARE>
 __device__ inline SeqRows find_share(const RaggedRows &r, uint32_t u) {
@@ -33,16 +37,21 @@ __device__ inline SeqRows find_share(const RaggedRows &r, uint32_t u) {
         q.count = static_cast<int>(r.each);
         q.held = r.lens ? r.lens[s] : 0;
         q.share = static_cast<int>(u - s * per);
+        q.told = false;
         q.ok = q.held >= 0 && static_cast<int64_t>(q.held) + q.count <= static_cast<int64_t>(r.max_tokens);
         return q;
     }
     const uint32_t lane = threadIdx.x & 63u;
     auto offset = [&](uint32_t s) { return r.offsets[s]; };
     auto first = [&](int32_t at, uint32_t s) { return static_cast<uint32_t>(max(at, 0)) / UNIT + SPARE * s; };
+    auto inside = [&](int32_t at) { return at >= 0 && static_cast<uint32_t>(at) <= r.rows; };
     uint32_t lo = 0, n = r.num_seqs;
+    q.told = false;
     while (n > 64) {
         const uint32_t stride = (n + 63) / 64, at = lane * stride;
-        const uint64_t before = __ballot(at < n && first(offset(lo + min(at, n - 1)), lo + at) <= u);
+        const int32_t start = offset(lo + min(at, n - 1));
+        const uint64_t before = __ballot(at < n && first(start, lo + at) <= u);
+        q.told |= __any(!inside(start) || __shfl_down(start, 1) < start) != 0;  // (the last lane meets itself)
         const uint32_t k = before ? 63 - __builtin_clzll(before) : 0;
         lo += k * stride;
         n = min(stride, n - k * stride);
@@ -58,7 +67,9 @@ __device__ inline SeqRows find_share(const RaggedRows &r, uint32_t u) {
     q.ok = q.begin >= 0 && end >= q.begin && static_cast<uint32_t>(end) <= r.rows && q.held >= 0;
     q.count = q.ok ? end - q.begin : 0;
     q.ok = q.ok && static_cast<int64_t>(q.held) + q.count <= static_cast<int64_t>(r.max_tokens);
-    q.share = static_cast<int>(u - first(q.begin, static_cast<uint32_t>(q.seq)));
+    q.told |= __any(!inside(a) || !inside(b) || b < a) != 0;
+    if (!before) q.count = 0;
+    q.share = before ? static_cast<int>(u - first(q.begin, static_cast<uint32_t>(q.seq))) : 0;
     return q;
 }
 

@@ -139,3 +139,35 @@ def test_errors_are_reported_and_skipped():
         b.put()
         b.check_planes("offsets")
         assert int(b.error) == 1
+
+
+@CODES
+@pytest.mark.parametrize("n", [3, 100])
+def test_rows_before_the_first_sequence(code, n):
+    """The first sequence need not begin at row 0: rows before it are not used, as those behind the last one are not."""
+    log(f"case: append, rows before the first sequence, code={code} n={n}")
+    counts, held = [60] + [1 + i % 3 for i in range(n)], [0] + [40 + i % 7 for i in range(n)]
+    b = B.Batch(counts, held, code, False, seed=n, spare=2)
+    b.upload()
+    b.append(b.append_args(num_seqs=n, row_offsets=b.doffsets[1:], cache_lens=b.dlens[1:], block_tables=b.dtable[1:]))
+    b.counts[0] = 0
+    b.put()
+    b.check_planes("behind row 60")
+    assert int(b.error) == 0
+
+
+@CODES
+@pytest.mark.parametrize("n", [3, 100, 5000])
+def test_offsets_that_descend_are_reported(code, n):
+    """Wherever they descend; other sequences' rows may be skipped, but nothing else is written."""
+    import torch
+    log(f"case: append, offsets that descend, code={code} n={n}")
+    for at in sorted({1, n // 2, n - 1}):
+        b = B.Batch([4] * n, [2] * n, code, False, seed=n + at).upload()
+        bad = b.offsets.copy()
+        bad[at] = bad[at + 1] + 3 if at % 2 else bad[at - 1] - 3
+        b.append(b.append_args(row_offsets=torch.from_numpy(bad).cuda()))
+        torch.cuda.synchronize()
+        assert int(b.error) == 1, at
+        unused = np.setdiff1d(np.arange(b.blocks), b.table)
+        assert np.array_equal(b.planes[0].cpu().numpy().view(b.cache.key.dtype)[unused], b.cache.key[unused])

@@ -167,3 +167,23 @@ def test_graphs_that_share_a_workspace():
         torch.cuda.synchronize()
         assert torch.equal(one.out, want[0])
     assert pvlc.workspace_error(ws, max(sizes)) == 0
+
+
+@WIDTHS
+@pytest.mark.parametrize("n", [3, 1100])
+def test_rows_before_the_first_sequence(f32, n):
+    """The first sequence need not begin at row 0, among those that are planned and those that are not."""
+    import torch
+    log(f"case: packed prefill, rows before the first sequence, f32={f32} n={n}")
+    b = B.Batch([60] + [1 + i % 3 for i in range(n)], [0] + [40 + i % 7 for i in range(n)], f32=f32, seed=n, spare=3).upload()
+    ws = workspace(b, b.width * 16)
+    launch(b, args_of(b, ws, num_seqs=n, row_offsets=b.doffsets[1:], cache_lens=b.dlens[1:], block_tables=b.dtable[1:]))
+    torch.cuda.synchronize()
+    assert pvlc.workspace_error(*ws) == 0
+    assert (b.out[:60] == 9.0).all() and (b.out[int(b.offsets[-1]):] == 9.0).all()
+    b.counts[0] = 0
+    b.put()
+    b.check_planes("behind row 60")
+    some = np.arange(60, int(b.offsets[-1]))
+    want, limit = wanted(b, some)
+    B.check("behind row 60", b.out.float().cpu().numpy()[some], want, limit)

@@ -188,3 +188,36 @@ def test_far_blocks():
     for p, small in zip(planes, c.planes):
         small.copy_(p.view(blocks, 4096)[blocks - c.blocks:].view_as(small))
     c.check("far")
+
+
+@CODES
+def test_sequences_before_the_first_group_have_no_output(code):
+    import torch
+    log(f"case: shared decode, sequences before the first group, code={code}")
+    c = Groups([9, 3, 2], [48, 33, 16], tails_of(14, 30), code, False, seed=8).upload()
+    nbytes = pvlc.shared_decode_workspace_bytes(14, 2, c.width * 16)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda"), nbytes
+    pvlc.workspace_init(*ws)
+    c.launch(c.shared_args(ws, num_groups=2, group_offsets=torch.from_numpy(c.firsts[1:]).cuda(), shared_lens=torch.tensor([33, 16], dtype=torch.int32, device="cuda")))
+    torch.cuda.synchronize()
+    assert pvlc.workspace_error(*ws) == 0
+    assert (c.out[:9] == 9.0).all()
+    got = c.out.float().cpu().numpy()
+    for i in range(9, 14):
+        c.cache.put_rows(c.table[i], c.held[i], c.turned(c.k[i], i)[None], c.v[i].astype(np.float64)[None])
+        k, v = c.cache.rows(c.table[i], c.held[i] + 1)
+        out, big, most = B.attend(c.turned(c.q[i], i)[None], k, v, [c.held[i] + 1])
+        B.check(f"sequence {i}", got[i:i + 1], out, B.bound(out, big, most, c.held[i] + 1, False, code))
+
+
+@pytest.mark.parametrize("n", [4, 90])
+def test_group_offsets_that_descend_are_reported(n):
+    import torch
+    log(f"case: shared decode, group offsets that descend, n={n}")
+    for bad in (-1, 0, 10 ** 6):
+        c = Groups([2] * n, [16] * n, [1] * (2 * n), B.F16, False, seed=n).upload()
+        ws = c.workspace()
+        firsts = c.firsts.copy()
+        firsts[n // 2] = bad
+        c.launch(c.shared_args(ws, group_offsets=torch.from_numpy(firsts).cuda()))
+        assert pvlc.workspace_error(*ws) == 1
