@@ -41,14 +41,10 @@ COMMON = [
 DEVICE = [f"--offload-arch={ARCH}", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
           "-mllvm", "-amdgpu-kernarg-preload-count=16"]
 
-# The packed prompts' waves have 512 registers: results of matrix instructions
-# stay in the half that vector instructions read, in place of a copy for each.
-FILE_FLAGS = {}
-
 
 def _compile(src: str) -> str:
     obj = os.path.join(BUILD, os.path.basename(src) + ".o")
-    cmd = [HIPCC, *COMMON, *DEVICE, *FILE_FLAGS.get(os.path.basename(src), [])]
+    cmd = [HIPCC, *COMMON, *DEVICE]
     if src.endswith(".hip"):
         cmd += ["-x", "hip"]
     cmd += ["-c", src, "-o", obj]
