@@ -208,6 +208,7 @@ pvlc_hip_status prefill(const pvlc_hip_packed_prefill_args *args, const void *qu
     r.items = a.plan.items;
     r.joins = a.plan.joins;
     r.partials = reinterpret_cast<float *>(base + ws.partials_offset);
+    r.narrow = ws.narrow;
     r.max_items = ws.max_items;
     r.max_joins = ws.max_joins;
     if (const int e = launch_kv_append(a, stream)) return hip_status(e, "packed prefill append launch");

@@ -337,6 +337,100 @@ __global__ __launch_bounds__(kWideWaves * 64) void packed_join_kernel(PackedRows
     w.store(q, w.inverse_sum(), lds[w.wave]);
 }
 
+// Small calls: a workgroup takes 16 tokens and one head, its waves the pieces of
+// 32 keys in turn, keys and values from the pages into registers; no plan.  More
+// workgroups, and each has a quarter of the steps, but every head reads the keys
+// and values again.
+constexpr int kNarrowWaves = 4;
+template <bool F32>
+__global__ __launch_bounds__(kNarrowWaves * 64, 2) void packed_narrow_kernel(PackedRows p) {
+    constexpr int kF16 = PVLC_HIP_KV_F16, kThreads = kNarrowWaves * 64;
+    typedef typename AttendQuery<F32>::Element Element;
+    __shared__ float sm_m[kNarrowWaves][16], sm_l[kNarrowWaves][16];
+    __shared__ float4_t sm_o[kNarrowWaves][8 * 64];
+    const uint32_t g = blockIdx.x & 1u, head = g * kGroup + ((blockIdx.x >> 1) & (kGroup - 1));
+    const SeqRows q = find_share<kPackedTokens, 1>(p.ragged, blockIdx.x / kQueryHeads);
+    const int t0 = q.share * kPackedTokens;
+    if (!q.ok || t0 >= q.count) return;  // uniform (the append reports it)
+    const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int valid = q.held + q.count, keys = min(q.held + t0 + kPackedTokens, valid);
+    // Waves 0 and 1 rotate a pair of 32-dim slices each; all take the queries from LDS.
+    const int t = min(t0 + row, q.count - 1);  // (past the sequence: its last one again, not stored)
+    AttendQuery<F32> raw;
+    float4_t cs[2]{}, sn[2]{};
+    bool rope = false;
+    if (wave < 2) {
+        const int64_t at = q.begin + static_cast<int64_t>(t), pos = p.positions ? p.positions[at] : q.held + static_cast<int64_t>(t);
+        raw.load(static_cast<const Element *>(p.query) + at * p.query_stride + head * kHeadDim, attend_dim<kF16>(wave, kg));
+        rope = p.rope_cos != nullptr && pos >= 0 && pos < static_cast<int64_t>(p.rope_rows);
+        if (rope) {
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                cs[f] = *reinterpret_cast<const float4_t *>(p.rope_cos + pos * 64 + attend_dim<kF16>(wave, kg) + f * 4);
+                sn[f] = *reinterpret_cast<const float4_t *>(p.rope_sin + pos * 64 + attend_dim<kF16>(wave, kg) + f * 4);
+            }
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    AttendPages pages;
+    pages.keys = reinterpret_cast<const uint8_t *>(p.key_cache);
+    pages.values = reinterpret_cast<const uint8_t *>(p.value_cache);
+    pages.exponents = nullptr;
+    pages.table = p.ragged.tables ? p.ragged.tables + static_cast<size_t>(q.seq) * p.ragged.max_blocks : nullptr;
+    pages.first = static_cast<uint32_t>(q.seq) * p.ragged.max_blocks;
+    pages.num_blocks = p.ragged.num_blocks;
+    pages.head = g;
+    pages.last_tile = (keys - 1) >> 4;
+    Attend<kF16, F32, 1> loop;
+    loop.begin(pages, wave, (keys + kAttendStep - 1) / kAttendStep, kNarrowWaves);
+    half8_t *const sm_q = reinterpret_cast<half8_t *>(&sm_o[0][0]);  // [kb][lane], before the join
+    if (wave < 2) {
+        half8_t lo, hi;
+        raw.rotate(rope, cs, sn, &lo, &hi);
+        sm_q[wave * 64 + lane] = lo;
+        sm_q[(wave + 2) * 64 + lane] = hi;
+    }
+    // (fences of LDS alone: the keys and values stay in flight)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    half8_t qf[1][4];
+#pragma unroll
+    for (int kb = 0; kb < 4; ++kb) qf[0][kb] = sm_q[kb * 64 + lane];
+    const int limit[1] = {q.held + t + 1};
+    AttendState<1> st;
+    st.clear();
+    loop.run(qf, (q.held + t0 + 1) / kAttendStep, limit, valid, p.scale_log2, st);
+    const float l = column_sum(st.l[0]);
+    if (kg == 0) {
+        sm_m[wave][row] = st.m[0];
+        sm_l[wave][row] = l;
+    }
+    __syncthreads();
+    float m = sm_m[0][row], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < kNarrowWaves; ++w) m = fmaxf(m, sm_m[w][row]);
+#pragma unroll
+    for (int w = 0; w < kNarrowWaves; ++w) sum += sm_l[w][row] * (sm_m[w][row] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((sm_m[w][row] - m) * p.scale_log2));
+    const float a = st.m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[0] - m) * p.scale_log2), factor = a * (1.0f / sum);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) sm_o[wave][c * 64 + lane] = st.o[0][c] * factor;
+    __syncthreads();
+#pragma unroll
+    for (int i = static_cast<int>(threadIdx.x); i < 8 * 64; i += kThreads) {
+        const int token = t0 + (i & 15), d = (i >> 6) * 16 + ((i >> 4) & 3) * 4;
+        float4_t v = sm_o[0][i];
+#pragma unroll
+        for (int w = 1; w < kNarrowWaves; ++w) v += sm_o[w][i];
+        if (token < q.count) {
+            Element *dst = static_cast<Element *>(p.out) + ((q.begin + static_cast<int64_t>(token)) * kQueryHeads + head) * kHeadDim + d;
+            if constexpr (F32) *reinterpret_cast<float4_t *>(dst) = v;
+            else *reinterpret_cast<half4_t *>(dst) = half4_t{to_h(v[0]), to_h(v[1]), to_h(v[2]), to_h(v[3])};
+        }
+    }
+}
+
 }  // namespace
 
 int launch_packed_prefill(const PackedRows &rows, void *stream) {
@@ -344,6 +438,12 @@ int launch_packed_prefill(const PackedRows &rows, void *stream) {
     p.scale_log2 = kAttendLog2e / sqrtf(static_cast<float>(kHeadDim));
     const dim3 threads(kWideWaves * 64);
     const auto st = static_cast<hipStream_t>(stream);
+    if (p.narrow) {
+        const RaggedRows &r = p.ragged;
+        const uint32_t shares = r.offsets ? r.rows / kPackedTokens + r.num_seqs : r.num_seqs * shares_of_each<kPackedTokens, 1>(r.each);
+        hipLaunchKernelGGL(p.f32 ? packed_narrow_kernel<true> : packed_narrow_kernel<false>, dim3(kQueryHeads * shares), dim3(kNarrowWaves * 64), 0, st, p);
+        return static_cast<int>(hipGetLastError());
+    }
     hipLaunchKernelGGL(p.f32 ? packed_wide_kernel<true> : packed_wide_kernel<false>, dim3(2 * p.max_items), threads, 0, st, p);
     if (p.max_joins) hipLaunchKernelGGL(p.f32 ? packed_join_kernel<true> : packed_join_kernel<false>, dim3(2 * p.max_joins), threads, 0, st, p);
     return static_cast<int>(hipGetLastError());

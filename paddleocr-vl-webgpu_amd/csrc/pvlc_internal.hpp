@@ -276,24 +276,40 @@ struct PackedRows {
     const PackedItem *items, *joins;
     float *partials;  // [slot][kv head][kPackedPartFloats]
     uint32_t max_items, max_joins;
+    bool narrow;  // one head a workgroup, without a plan
 };
 int launch_packed_prefill(const PackedRows &rows, void *stream);
+// Calls of few tokens over short contexts give a workgroup one head, not eight:
+// eight times the workgroups and no plan, but every head reads its keys again.
+// Whole calls, us, one head against eight: a prompt of 16 tokens 7.7 against 12.4,
+// of 500 tokens 12.2 against 21.1; 16 tokens each on 500 held, 16 sequences 11.9
+// against 22.2, 32 sequences 18.5 against 23.1, 64 (128 shares) 27.4 against 25.1;
+// on 4000 held, 4 sequences 18.9 against 30.6, 16 (32 shares) 39.4 against 37.5;
+// 1000 tokens on 1000 held 34.9 against 44.8.
+constexpr uint32_t kNarrowShares = 72, kNarrowContext = 4096, kNarrowRows = 128000;
+inline bool packed_is_narrow(uint32_t num_seqs, uint32_t rows, uint32_t max_context) {
+    const uint64_t shares = static_cast<uint64_t>(rows / kPackedTokens) + num_seqs;
+    return shares <= kNarrowShares && max_context <= kNarrowContext && shares * max_context <= kNarrowRows;
+}
 // Its workspace: 256 bytes of words (0 the error word, 1 and 2 the plan's
-// counts), then the items, the joins and the parts.  Sequences beyond
-// kPackedPlanSeqs are not planned.  An item has at most kPackedLeastPart
-// pieces, or as many as an even share of the call's (512 workgroups are
-// resident); so a call's split items have at most kPackedMaxParts parts.
+// counts), then the items, the joins and the parts.  More sequences than
+// kPackedPlanSeqs (what the plan holds in LDS) are not planned.  Items are cut
+// from kPackedLeastPart pieces on, or from what lets the cut items of a call have
+// kPackedMaxParts parts at most: 2048 / 1024 / 768 / 512 / 256 of them made 20
+// prompts of 500 to 1157 tokens 117 / 106 / 95 / 90 / 85 us, and other calls no
+// more than 2% slower.
 constexpr uint32_t kPackedPlanSeqs = 1024, kPackedLeastPart = 16, kPackedMaxParts = 256;
 constexpr size_t kPackedPartFloats = 4 * 66 * 64;  // 4 waves x (64 outputs, reference, sum) x 64 lanes
 struct PackedWorkspace {
-    bool plan;
+    bool plan, narrow;
     uint32_t max_items, max_joins, max_parts;
     size_t items_offset, joins_offset, partials_offset, total;
 };
 inline PackedWorkspace packed_workspace_layout(uint32_t num_seqs, uint32_t rows, uint32_t max_context) {
     auto align = [](size_t v) { return (v + 255) / 256 * 256; };
     PackedWorkspace w{};
-    w.plan = num_seqs <= kPackedPlanSeqs;
+    w.narrow = packed_is_narrow(num_seqs, rows, max_context);
+    w.plan = !w.narrow && num_seqs <= kPackedPlanSeqs;
     w.max_items = rows / kPackedTokens + num_seqs;
     if (w.plan && max_context > 32 * kPackedLeastPart) w.max_parts = kPackedMaxParts;
     w.max_joins = w.max_parts / 2;

@@ -187,3 +187,45 @@ def test_rows_before_the_first_sequence(f32, n):
     some = np.arange(60, int(b.offsets[-1]))
     want, limit = wanted(b, some)
     B.check("behind row 60", b.out.float().cpu().numpy()[some], want, limit)
+
+
+@WIDTHS
+@pytest.mark.parametrize("name", list(BATCHES))
+def test_batches_in_wide_tables(f32, name):
+    """Small calls give a workgroup one head; with room for longer sequences the same ones give it eight."""
+    log(f"case: packed prefill {name} in wide tables f32={f32}")
+    counts, held = BATCHES[name]
+    b = B.Batch(counts, held, f32=f32, seed=len(name) + 40, fused=name in ("few", "chunk"), spare=3, positions=name == "behind", rope=name != "many")
+    b.width = 300
+    b.table = np.pad(b.table, ((0, 0), (0, 300 - b.table.shape[1])), constant_values=-1)
+    b.upload()
+    ws = workspace(b, 4800)
+    launch(b, args_of(b, ws))
+    check(b, name)
+    assert pvlc.workspace_error(*ws) == 0
+
+
+@WIDTHS
+@pytest.mark.parametrize("name", ["equal", "one_more", "tiles"])
+def test_small_calls(f32, name):
+    """Without offsets and tables, one token behind whole pieces of keys, and prompts that end at tiles."""
+    log(f"case: packed prefill, small calls, {name} f32={f32}")
+    counts, held = {"equal": ([16] * 5, [0] * 5), "one_more": ([1] * 6, [31, 32, 127, 128, 129, 1000]), "tiles": ([128, 127, 129], [0, 1, 0])}[name]
+    b = B.Batch(counts, held, f32=f32, seed=77, paged=name != "equal", spare=0 if name == "equal" else 5).upload()
+    ws = workspace(b, b.width * 16)
+    launch(b, args_of(b, ws, **(dict(row_offsets=None, cache_lens=None) if name == "equal" else {})))
+    check(b, name)
+    assert pvlc.workspace_error(*ws) == 0
+
+
+@WIDTHS
+def test_rising_scores_over_eight_heads(f32):
+    """As above, where a workgroup has eight heads, and parts of the keys to join."""
+    log(f"case: packed prefill, rising scores, eight heads f32={f32}")
+    b = B.Batch([100], [5000], f32=f32, seed=13, rope=False)
+    b.q[:] = 1.0
+    b.k[:, :, :] = (np.arange(b.rows)[:, None, None] * 0.05).astype(b.k.dtype)
+    b.upload()
+    ws = workspace(b, b.width * 16)
+    launch(b, args_of(b, ws))
+    check(b, "rising", np.arange(0, 100, 7))
