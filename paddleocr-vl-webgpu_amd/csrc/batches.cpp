@@ -286,7 +286,7 @@ pvlc_hip_status shared(const pvlc_hip_shared_decode_args *args, const void *quer
     if (pvlc_hip_status st = check_matrix(query, &query_stride, args->num_seqs, kQueryHeads * kHeadDim, size, "query", &queries)) return st;
     if (pvlc_hip_status st = check_matrix(out, &out_stride, args->num_seqs, kQueryHeads * kHeadDim, size, "out", &outs)) return st;
     const bool offsets = args->group_offsets != nullptr;
-    const bool small = shared_is_small(args->num_seqs, args->num_groups, args->max_context, offsets, args->code);
+    const bool small = shared_is_small(args->num_seqs, args->num_groups, args->max_context, offsets);
     const SharedWorkspace ws = shared_workspace_layout(args->num_seqs, args->num_groups, args->max_context, offsets);
     const size_t needed = small ? pvlc_hip_paged_decode_workspace_bytes(args->num_seqs, args->max_context, 0) : ws.total;
     if (pvlc_hip_status st = check_workspace(args, needed, "shared decode")) return st;
@@ -322,9 +322,6 @@ pvlc_hip_status shared(const pvlc_hip_shared_decode_args *args, const void *quer
     r.unit_columns = ws.unit_columns;
     r.part_o = reinterpret_cast<float *>(base + ws.part_o_offset);
     r.part_ml = reinterpret_cast<float *>(base + ws.part_ml_offset);
-    // (a row added to an 8-bit block may round the others of the block again: a launch before their readers)
-    if (args->code != PVLC_HIP_KV_F16)
-        if (const int e = launch_kv_append(a, stream)) return hip_status(e, "shared decode append launch");
     if (const int e = launch_shared_decode(r, stream)) return hip_status(e, "shared decode launch");
     return ok();
 }
@@ -361,7 +358,7 @@ size_t pvlc_hip_shared_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_gr
     const size_t with = shared_workspace_layout(num_seqs, num_groups, max_context, true).total;
     const size_t without = shared_workspace_layout(num_seqs, num_groups, max_context, false).total;
     size_t most = with > without ? with : without;
-    if (shared_is_small(num_seqs, num_groups, max_context, false, PVLC_HIP_KV_E4M3)) {
+    if (shared_is_small(num_seqs, num_groups, max_context, false)) {
         const size_t alone = pvlc_hip_paged_decode_workspace_bytes(num_seqs, max_context, 0);
         most = most > alone ? most : alone;
     }

@@ -217,26 +217,6 @@ __device__ inline void load_chunk(const DecodeParams &p, uint32_t g, uint32_t id
     for (int i = 0; i < 8; ++i) vr[i] = __builtin_nontemporal_load(reinterpret_cast<const q8x4_t *>(vp + i * 256));
 }
 
-// The rows before `slot` of a block and head rounded again in the cache, by one
-// wave, complete when this returns.  A loop over the block's dwords in memory: it
-// runs for a few of a sequence's rows, and in the registers of the main path its
-// code, unrolled, was a third of the kernel.
-template <int CODE>
-__device__ inline void requantise_block(uint8_t *keys, uint8_t *values, int lane, int slot, int grown_k, int grown_v) {
-#pragma unroll 1
-    for (int i = lane; i < static_cast<int>(kQ8SlabBytes) / 4; i += 64) {
-        // key dword i: token (i / 128) * 4 + (i / 4) % 4; value dword i: tokens (i % 4) * 4 .. +3
-        uint32_t *k = reinterpret_cast<uint32_t *>(keys) + i, *v = reinterpret_cast<uint32_t *>(values) + i;
-        if ((i >> 7) * 4 + ((i >> 2) & 3) < slot) *k = q8_requantise<CODE>(*k, grown_k);
-        const int rows = min(max(slot - (i & 3) * 4, 0), 4);
-        if (rows > 0) {
-            const uint32_t before = rows == 4 ? ~0u : (1u << (8 * rows)) - 1u, old = *v;
-            *v = (q8_requantise<CODE>(old, grown_v) & before) | (old & ~before);
-        }
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-}
-
 // One work item: partition `part` (P tokens) of kv head g of sequence s, as
 // decode_item of the fp16 cache.
 template <int WAVES, bool DEFER_MERGE, bool F32IO, int CODE>

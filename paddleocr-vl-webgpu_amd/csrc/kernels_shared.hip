@@ -156,6 +156,60 @@ __device__ inline void append_and_attend(const SharedRows &p, int seq, int len, 
         for (int r = 0; r < 4; ++r) st.o[0][c][r] = st.o[0][c][r] * a + w * static_cast<float>(half_value(c * 16 + kg * 4 + r));
 }
 
+// The new row of a sequence into its 8-bit block, by the one wave that reads this
+// block: two dims a lane, as the paged decode appends its own.  Complete, and seen by
+// the wave's loads, when this returns.
+template <int CODE, bool F32>
+__device__ inline void append_q8(const SharedRows &p, int seq, int len, uint32_t g) {
+    typedef std::conditional_t<F32, float, uint16_t> Element;
+    const int lane = threadIdx.x & 63, slot = len % static_cast<int>(kBlockTokens);
+    const size_t at = (static_cast<size_t>(seq) * kKvHeads + g) * kHeadDim + lane;
+    const Element *key = static_cast<const Element *>(p.new_key) + at, *value = static_cast<const Element *>(p.new_value) + at;
+    auto given = [](Element x) { return F32 ? static_cast<float>(x) : static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(x))); };
+    const Element kl = key[0], kh = key[64], vl = value[0], vh = value[64];
+    const int64_t pos = p.positions ? p.positions[seq] : len;
+    const bool rope = p.rope_cos != nullptr && pos >= 0 && pos < static_cast<int64_t>(p.rope_rows);
+    const float c = rope ? p.rope_cos[pos * 64 + lane] : 1.f, s = rope ? p.rope_sin[pos * 64 + lane] : 0.f;
+    bool ok;
+    const size_t slab = static_cast<size_t>(checked_block(p.ragged, p.ragged.tables[static_cast<size_t>(seq) * p.ragged.max_blocks + len / static_cast<int>(kBlockTokens)], &ok)) * kKvHeads + g;
+    const uint32_t old = *reinterpret_cast<const uint16_t *>(p.exponents + slab * 2);
+    if (lane == 0 && g == 0) {
+        if (!ok) atomicOr(p.error_word, 2u);
+        if (!rope && p.rope_cos != nullptr) atomicOr(p.error_word, 4u);
+    }
+    if (!ok) return;  // uniform
+    float k_lo = given(kl), k_hi = given(kh);
+    if (rope) {
+        const float x = k_lo;
+        k_lo = x * c + (-k_hi) * s;
+        k_hi = k_hi * c + x * s;
+    }
+    auto held = [](float x) { return q8_value(static_cast<float>(to_h(x))); };
+    k_lo = held(k_lo);
+    k_hi = held(k_hi);
+    const float v_lo = held(given(vl)), v_hi = held(given(vh));
+    const int old_k = static_cast<int>(old & 255) - kQ8Bias, old_v = static_cast<int>(old >> 8) - kQ8Bias;
+    int e_k = q8_exponent<CODE>(wave_max(q8_size(q8_size(0.f, k_lo), k_hi)));
+    int e_v = q8_exponent<CODE>(wave_max(q8_size(q8_size(0.f, v_lo), v_hi)));
+    if (slot > 0) {
+        e_k = max(e_k, old_k);
+        e_v = max(e_v, old_v);
+    }
+    const float pk = exp2_whole(-e_k), pv = exp2_whole(-e_v);
+    const uint32_t codes = q8_encode<CODE>(k_lo * pk, k_hi * pk, v_lo * pv, v_hi * pv);
+    uint8_t *ks = static_cast<uint8_t *>(p.key_cache) + slab * kQ8SlabBytes, *vs = static_cast<uint8_t *>(p.value_cache) + slab * kQ8SlabBytes;
+    const int grown = __builtin_amdgcn_readfirstlane(slot > 0 ? (e_k - old_k) | (e_v - old_v) << 16 : 0);
+    if (grown != 0) requantise_block<CODE>(ks, vs, lane, slot, grown & 0xFFFF, grown >> 16);
+    // key (slot, d) at (slot/4)*512 + (d/16)*64 + (slot%4)*16 + d%16, value at d*16 + slot
+    uint8_t *kd = ks + (slot >> 2) * 512 + (slot & 3) * 16 + (lane >> 4) * 64 + (lane & 15), *vd = vs + lane * 16 + slot;
+    kd[0] = static_cast<uint8_t>(codes);
+    kd[256] = static_cast<uint8_t>(codes >> 8);
+    vd[0] = static_cast<uint8_t>(codes >> 16);
+    vd[1024] = static_cast<uint8_t>(codes >> 24);
+    if (lane == 0) *reinterpret_cast<uint16_t *>(p.exponents + slab * 2) = static_cast<uint16_t>((e_k + kQ8Bias) | (e_v + kQ8Bias) << 8);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+}
+
 // Eight dims of a lane's column (the query of head row & 7 of sequence r of the
 // set) and their rotary partners: sent for, then rotated.
 template <int CODE, bool F32>
@@ -263,7 +317,8 @@ __device__ inline void attend_shared(const SharedRows &p, const SharedSet &set, 
 }
 
 // A part of a sequence's own rows, by one wave.  new_row: the sequence's length,
-// whose new row is one more key (fp16 pages), or -1.
+// whose new row the wave appends, or -1: one more key behind the part's (fp16
+// pages), or the last of the part's keys (8-bit pages).
 template <int CODE, bool F32>
 __device__ inline void attend_own(const SharedRows &p, const SharedSet &set, int r, uint32_t g, int keys, int first, int end, int new_row, float *part_o,
                                   float *part_ml) {
@@ -272,6 +327,9 @@ __device__ inline void attend_own(const SharedRows &p, const SharedSet &set, int
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) query[kb].send(p, set, r, g, kb);
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (CODE != PVLC_HIP_KV_F16) {
+        if (new_row >= 0) append_q8<CODE, F32>(p, set.first + r, new_row, g);  // uniform
+    }
     Attend<CODE, F32, 1> loop;
     loop.begin(pages_of(p, set.first + r, set.shared, keys, g), first, end, 1);
     half8_t qf[1][4];
@@ -300,7 +358,7 @@ __device__ inline void attend_own(const SharedRows &p, const SharedSet &set, int
 template <int CODE, bool F32, int CT>
 __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedRows p) {
     __shared__ SharedLds<CT> lds;
-    constexpr int kNewRow = CODE == PVLC_HIP_KV_F16;  // (8-bit pages hold the new rows already)
+    constexpr int kNewRow = CODE == PVLC_HIP_KV_F16;  // (not a key of the parts')
     const uint32_t g = blockIdx.x & 1u;
     uint32_t b = blockIdx.x >> 1;
     const bool common = b < p.shares * p.shared_parts;  // uniform, as all below
@@ -326,10 +384,11 @@ __global__ __launch_bounds__(kThreads, 2) void shared_attention_kernel(SharedRow
         if ((threadIdx.x & 63) == 0 && part == 0) atomicOr(p.error_word, 1u);
         return;
     }
-    if (part >= max(parts_of(keys, own_parts, kLeastOwn), kNewRow)) return;
+    const int parts = max(parts_of(keys, own_parts, kLeastOwn), kNewRow);
+    if (part >= parts) return;
     const int steps = part_steps(keys, own_parts, kLeastOwn), first = part * steps;
     const int column = shared_parts * CT * 16 + (r * own_parts + part) * static_cast<int>(kGroup);
-    attend_own<CODE, F32>(p, set, r, g, keys, first, min(first + steps, (keys + kAttendStep - 1) / kAttendStep), part == 0 ? len : -1,
+    attend_own<CODE, F32>(p, set, r, g, keys, first, min(first + steps, (keys + kAttendStep - 1) / kAttendStep), part == (kNewRow ? 0 : parts - 1) ? len : -1,
                           part_o + column * static_cast<int>(kHeadDim), part_ml + column * 2);
 }
 

@@ -322,7 +322,7 @@ inline PackedWorkspace packed_workspace_layout(uint32_t num_seqs, uint32_t rows,
 }
 
 // A decode step of groups with shared pages (kernels_shared.hip).  ragged: the
-// sequences, a row each (8-bit pages hold it already).
+// sequences, a row each.
 constexpr int kSharedWaves = 4;
 struct SharedRows {
     RaggedRows ragged;
@@ -336,7 +336,7 @@ struct SharedRows {
     const int32_t *positions;
     uint32_t rotate_query;
     void *key_cache, *value_cache;
-    const uint8_t *exponents;
+    uint8_t *exponents;
     float scale_log2;
     uint32_t *error_word;
     // sets of 2 * columns sequences, the parts that their shared rows and a
@@ -350,18 +350,16 @@ int launch_shared_decode(const SharedRows &rows, void *stream);
 // Calls that the paged decode answers sooner, each sequence reading all of its
 // rows: those of up to so many rows (num_seqs times max_context; what is shared,
 // and how many rows there are, the host does not know), and those without a
-// group of two.  Two launches (three over 8-bit pages) take 10-20 us of any
-// call, the paged decode's one 8-12 of these: 4 sequences of 1157 rows 12.1
-// against 8.3 us (fp16) and 15.3 against 7.9 (e4m3), 16 groups of 4 (80 thousand
-// rows) 16.6 against 16.4 and 18.8 against 12.3, 16 groups of 8 (160 thousand)
-// 17.8 against 24.1 and 20.7 against 19.5, 32 groups of 8 (320 thousand) 26.8
-// against 44.4 and 30.2 against 32.4, 64 sequences with none in common 30.3
-// against 28.6 and 25.3 against 19.0.
-constexpr uint32_t kSharedLeastRows = 80000, kSharedLeastRowsQ8 = 200000;
-inline bool shared_is_small(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context, bool offsets, uint32_t code) {
+// group of two.  Two launches take 11 us of any call, the paged decode's one 8:
+// 4 sequences of 1221 rows 11.7 against 7.7 us (fp16) and 10.9 against 7.8 (e4m3), 16
+// groups of 4 (80 thousand rows) 15.8 against 16.2 and 14.5 against 12.3, 12 groups
+// of 8 (120 thousand) 16.3 against 20.4 and 15.9 against 18.9, 32 groups of 8 (320
+// thousand) 26.8 against 44.4 and 25.5 against 31.7, 64 sequences with none in
+// common 30.3 against 28.6 and 20.1 against 19.3.
+constexpr uint32_t kSharedLeastRows = 90000;
+inline bool shared_is_small(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context, bool offsets) {
     if (num_seqs > kMaxRaggedSeqs || max_context > kMaxMergeParts * 4096) return false;
-    return (!offsets && num_seqs == num_groups) ||
-           static_cast<uint64_t>(num_seqs) * max_context <= (code == PVLC_HIP_KV_F16 ? kSharedLeastRows : kSharedLeastRowsQ8);
+    return (!offsets && num_seqs == num_groups) || static_cast<uint64_t>(num_seqs) * max_context <= kSharedLeastRows;
 }
 // Its workspace: the paged decode's words and counters (0 the error word), which
 // no call's parts lie on, then the parts' results.
