@@ -91,7 +91,7 @@ __device__ inline void make_packed_plan(const RaggedRows &r, const PackedPlan &p
         if (w.ok && n) atomicAdd(&sm_pieces, (n * (w.held + 47ull) + 8 * n * (n - 1)) / 32 + 1);
     }
     __syncthreads();
-    // An even share of both kv heads' pieces, in whole steps of two.  An item of
+    // A share of the pieces, in whole steps of two.  An item of
     // n > most pieces is cut into at most n / most + 1 <= 2 n / most parts, so all
     // of them into at most 2 pieces / most <= kPackedMaxParts.
     const unsigned long long share = (sm_pieces / (kPackedMaxParts / 2) + 3) / 2 * 2;

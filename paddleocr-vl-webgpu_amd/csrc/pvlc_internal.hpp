@@ -295,10 +295,13 @@ inline bool packed_is_narrow(uint32_t num_seqs, uint32_t rows, uint32_t max_cont
 // counts), then the items, the joins and the parts.  More sequences than
 // kPackedPlanSeqs (what the plan holds in LDS) are not planned.  Items are cut
 // from kPackedLeastPart pieces on, or from what lets the cut items of a call have
-// kPackedMaxParts parts at most: 2048 / 1024 / 768 / 512 / 256 of them made 20
-// prompts of 500 to 1157 tokens 117 / 106 / 95 / 90 / 85 us, and other calls no
-// more than 2% slower.
-constexpr uint32_t kPackedPlanSeqs = 1024, kPackedLeastPart = 16, kPackedMaxParts = 256;
+// kPackedMaxParts parts at most, 1.28 times what each of the 512 resident
+// workgroups would have of an even share.  256 / 400 / 512 / 640 / 768 / 1024 parts: 12
+// prompts of 211 to 2010 tokens 79 / 78 / 82 / 86 / 89 / 97 us, 6 chunks of 256 to 512
+// tokens on 16384 rows 221 / 197 / 213 / 201 / 214 / 216.  (All pieces laid end to end and
+// cut at even shares balance the workgroups better and took these chunks 222 us:
+// parts of one sequence that begin at different keys read 711 MB past L2, not 278.)
+constexpr uint32_t kPackedPlanSeqs = 1024, kPackedLeastPart = 16, kPackedMaxParts = 400;
 constexpr size_t kPackedPartFloats = 4 * 66 * 64;  // 4 waves x (64 outputs, reference, sum) x 64 lanes
 struct PackedWorkspace {
     bool plan, narrow;
