@@ -197,20 +197,18 @@ pvlc_hip_status prefill(const pvlc_hip_packed_prefill_args *args, const void *qu
     r.value_cache = args->value_cache;
     auto *base = static_cast<unsigned char *>(args->workspace);
     if (ws.plan) {
-        a.plan.counts = reinterpret_cast<int32_t *>(base) + 1;
+        a.plan.count = reinterpret_cast<int32_t *>(base) + 1;
         a.plan.items = reinterpret_cast<PackedItem *>(base + ws.items_offset);
-        a.plan.joins = reinterpret_cast<PackedItem *>(base + ws.joins_offset);
+        a.plan.arrived = reinterpret_cast<uint32_t *>(base + ws.arrived_offset);
         a.plan.max_items = ws.max_items;
-        a.plan.max_joins = ws.max_joins;
         a.plan.max_parts = ws.max_parts;
     }
-    r.counts = a.plan.counts;
+    r.count = a.plan.count;
     r.items = a.plan.items;
-    r.joins = a.plan.joins;
-    r.partials = reinterpret_cast<float *>(base + ws.partials_offset);
+    r.arrived = a.plan.arrived;
+    r.partials = reinterpret_cast<uint64_t *>(base + ws.partials_offset);
     r.narrow = ws.narrow;
     r.max_items = ws.max_items;
-    r.max_joins = ws.max_joins;
     if (const int e = launch_kv_append(a, stream)) return hip_status(e, "packed prefill append launch");
     if (const int e = launch_packed_prefill(r, stream)) return hip_status(e, "packed prefill launch");
     return ok();

@@ -17,7 +17,7 @@ typedef float float16_t __attribute__((ext_vector_type(16)));
 // A workgroup takes 16 tokens of a sequence and the 8 query heads of a kv head,
 // a wave two of the heads: 32 columns.
 constexpr int kWideWaves = 4, kWideStep = 64;
-constexpr size_t kPartFloats = kPackedPartFloats / kWideWaves;  // of a wave: outputs, references and sums
+constexpr size_t kPartPairs = kPackedPartPairs / kWideWaves;  // of a wave: (reference, sum) and outputs
 constexpr int kStepElems = kWideStep * kHeadDim;  // fp16 elements of a step's keys (or values) of a kv head
 
 template <bool F32>
@@ -137,6 +137,46 @@ struct Wide {
                 if constexpr (F32) o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, lo[b], o[dt], 0, 0, 0);
             }
     }
+    // A part of the keys, left as it is, and the parts of an item joined in their
+    // order: wave and lane hold there what they hold here.  Relaxed agent-scope
+    // accesses, coherent across the XCDs' L2s by themselves (a fence at that scope
+    // would write the whole L2 back).
+    __device__ uint64_t *part(int slot) const { return p.partials + ((static_cast<size_t>(slot) * 2 + g) * kWideWaves + wave) * kPartPairs + lane; }
+    static __device__ uint64_t pair(float a, float b) { return static_cast<uint64_t>(__float_as_uint(a)) | static_cast<uint64_t>(__float_as_uint(b)) << 32; }
+    __device__ void leave(int slot) const {
+        uint64_t *to = part(slot);
+        __hip_atomic_store(to, pair(m, l), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            __hip_atomic_store(to + (i + 1) * 64, pair(o[i >> 3][(i & 7) * 2], o[i >> 3][(i & 7) * 2 + 1]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __device__ void join(const PackedItem &q) {
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[dt][r] = 0.f;
+        for (int s = q.slots; s < q.slots + q.parts; ++s) {
+            const uint64_t *from = part(s);
+            uint64_t in[33];
+#pragma unroll
+            for (int i = 0; i < 33; ++i) in[i] = __hip_atomic_load(from + i * 64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            auto low = [&](int i) { return __uint_as_float(static_cast<uint32_t>(in[i])); };
+            auto high = [&](int i) { return __uint_as_float(static_cast<uint32_t>(in[i] >> 32)); };
+            const float n = low(0), top = fmaxf(m, n);
+            const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
+            const float c = n == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((n - top) * p.scale_log2);
+            l = l * a + high(0) * c;
+            m = top;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                float16_t &t = o[i >> 3];
+                t[(i & 7) * 2] = t[(i & 7) * 2] * a + low(i + 1) * c;
+                t[(i & 7) * 2 + 1] = t[(i & 7) * 2 + 1] * a + high(i + 1) * c;
+            }
+        }
+    }
     // 1 / the sum of the query's weights, over both halves of the wave.
     __device__ float inverse_sum() const {
         const attend_u32x2 v = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
@@ -188,10 +228,11 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedR
     // (distinct arrays, picked at compile time, so that the compiler sees that a
     // step's loads and its reads touch different ones)
     __shared__ __align__(16) uint16_t sk0[kStepElems], sk1[kStepElems], sv0[kStepElems], sv1[kStepElems];
+    __shared__ int sm_last;
     const uint32_t g = blockIdx.x & 1u, b = blockIdx.x >> 1;
     PackedItem q;
     if (p.items) {
-        const uint32_t items = load_const(p.counts, 0);
+        const uint32_t items = load_const(p.count, 0);
         q = load_item(p.items, b);  // (beside the count, in one round)
         if (b >= items) return;
     } else {
@@ -289,52 +330,19 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedR
     }
 
     if (q.slot >= 0) {
-        // A part of the keys: left as it is, for the join.
-        float *part = p.partials + ((static_cast<size_t>(q.slot) * 2 + g) * kWideWaves + wave) * kPartFloats;
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                *reinterpret_cast<float4_t *>(part + ((dt * 4 + r) * 64 + lane) * 4) =
-                    float4_t{w.o[dt][r * 4], w.o[dt][r * 4 + 1], w.o[dt][r * 4 + 2], w.o[dt][r * 4 + 3]};
-        part[64 * 64 + lane] = w.m;
-        part[65 * 64 + lane] = w.l;
-    } else {
-        // (every wave is past its last read of the buffers)
-        w.store(q, w.inverse_sum(), wave < 2 ? (wave == 0 ? sk0 : sk1) : (wave == 2 ? sv0 : sv1));
+        // A part of the keys.  The workgroup that leaves the last one of its item joins
+        // them (a launch of its own would take calls without parts 1 us, too).
+        w.leave(q.slot);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the wave's part is there
+        __syncthreads();
+        if (threadIdx.x == 0)
+            sm_last = __hip_atomic_fetch_add(p.arrived + q.slots * 2 + static_cast<int>(g), 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<uint32_t>(q.parts) - 1;
+        __syncthreads();
+        if (!sm_last) return;  // uniform
+        w.join(q);
     }
-}
-
-// The parts of a split item joined: wave and lane hold what they held there.
-template <bool F32>
-__global__ __launch_bounds__(kWideWaves * 64) void packed_join_kernel(PackedRows p) {
-    __shared__ __align__(16) float lds[kWideWaves][32 * 68];
-    const uint32_t g = blockIdx.x & 1u, b = blockIdx.x >> 1, joins = load_const(p.counts, 1);
-    const PackedItem q = load_item(p.joins, b);  // first, end: its slots
-    if (b >= joins) return;
-    Wide<F32> w(p, g);
-    w.m = -INFINITY;
-    w.l = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) w.o[dt][r] = 0.f;
-    for (int s = q.first; s < q.end; ++s) {
-        const float *part = p.partials + ((static_cast<size_t>(s) * 2 + g) * kWideWaves + w.wave) * kPartFloats;
-        float4_t o[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = *reinterpret_cast<const float4_t *>(part + (i * 64 + w.lane) * 4);
-        const float m = part[64 * 64 + w.lane], l = part[65 * 64 + w.lane], top = fmaxf(w.m, m);
-        const float a = w.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((w.m - top) * p.scale_log2);
-        const float c = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - top) * p.scale_log2);
-        w.l = w.l * a + l * c;
-        w.m = top;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w.o[i >> 2][(i & 3) * 4 + e] = w.o[i >> 2][(i & 3) * 4 + e] * a + o[i][e] * c;
-    }
-    w.store(q, w.inverse_sum(), lds[w.wave]);
+    // (every wave is past its last read of the buffers)
+    w.store(q, w.inverse_sum(), wave < 2 ? (wave == 0 ? sk0 : sk1) : (wave == 2 ? sv0 : sv1));
 }
 
 // Small calls: a workgroup takes 16 tokens and one head, its waves the pieces of
@@ -436,7 +444,6 @@ __global__ __launch_bounds__(kNarrowWaves * 64, 2) void packed_narrow_kernel(Pac
 int launch_packed_prefill(const PackedRows &rows, void *stream) {
     PackedRows p = rows;
     p.scale_log2 = kAttendLog2e / sqrtf(static_cast<float>(kHeadDim));
-    const dim3 threads(kWideWaves * 64);
     const auto st = static_cast<hipStream_t>(stream);
     if (p.narrow) {
         const RaggedRows &r = p.ragged;
@@ -444,8 +451,7 @@ int launch_packed_prefill(const PackedRows &rows, void *stream) {
         hipLaunchKernelGGL(p.f32 ? packed_narrow_kernel<true> : packed_narrow_kernel<false>, dim3(kQueryHeads * shares), dim3(kNarrowWaves * 64), 0, st, p);
         return static_cast<int>(hipGetLastError());
     }
-    hipLaunchKernelGGL(p.f32 ? packed_wide_kernel<true> : packed_wide_kernel<false>, dim3(2 * p.max_items), threads, 0, st, p);
-    if (p.max_joins) hipLaunchKernelGGL(p.f32 ? packed_join_kernel<true> : packed_join_kernel<false>, dim3(2 * p.max_joins), threads, 0, st, p);
+    hipLaunchKernelGGL(p.f32 ? packed_wide_kernel<true> : packed_wide_kernel<false>, dim3(2 * p.max_items), dim3(kWideWaves * 64), 0, st, p);
     return static_cast<int>(hipGetLastError());
 }
 

@@ -21,13 +21,15 @@ __device__ inline PackedItem load_item(const PackedItem *items, uint32_t i) {
     q.first = load_const(src, 5);
     q.end = load_const(src, 6);
     q.slot = load_const(src, 7);
+    q.slots = load_const(src, 8);
+    q.parts = load_const(src, 9);
     return q;
 }
 
 // A share of kPackedTokens as a whole item.
 __device__ inline PackedItem packed_item(const SeqRows &s) {
     const int t0 = s.share * kPackedTokens, keys = min(s.held + t0 + kPackedTokens, s.held + s.count);
-    return {s.begin, s.count, s.held, s.seq, t0, 0, (keys + 31) / 32, -1};
+    return {s.begin, s.count, s.held, s.seq, t0, 0, (keys + 31) / 32, -1, 0, 1};
 }
 
 // By one workgroup of 256 threads.  An item longer than `most` pieces is cut
@@ -39,7 +41,7 @@ __device__ inline void make_packed_plan(const RaggedRows &r, const PackedPlan &p
     constexpr int kThreads = 256, kLengths = 64;
     __shared__ int32_t sm_offset[kPackedPlanSeqs + 1], sm_held[kPackedPlanSeqs];
     __shared__ uint32_t sm_length[kLengths];
-    __shared__ uint32_t sm_parts, sm_joins;
+    __shared__ uint32_t sm_parts;
     __shared__ unsigned long long sm_pieces;
     const int i = threadIdx.x;
     for (uint32_t s = i; s <= r.num_seqs; s += kThreads) {
@@ -49,7 +51,7 @@ __device__ inline void make_packed_plan(const RaggedRows &r, const PackedPlan &p
     if (i < kLengths) sm_length[i] = 0;
     if (i == 0) {
         sm_pieces = 0;
-        sm_parts = sm_joins = 0;
+        sm_parts = 0;
     }
     __syncthreads();
     auto first_share = [&](uint32_t s) { return static_cast<uint32_t>(max(sm_offset[s], 0)) / kPackedTokens + s; };
@@ -109,14 +111,9 @@ __device__ inline void make_packed_plan(const RaggedRows &r, const PackedPlan &p
                 continue;
             }
             int slot = -1;
-            if (used > 1) {
-                slot = static_cast<int>(atomicAdd(&sm_parts, static_cast<uint32_t>(used)));
-                const uint32_t join = atomicAdd(&sm_joins, 1u);
-                PackedItem j = q;
-                j.first = slot;
-                j.end = slot + used;
-                if (join < plan.max_joins) plan.joins[join] = j;
-            }
+            if (used > 1) slot = static_cast<int>(atomicAdd(&sm_parts, static_cast<uint32_t>(used)));
+            q.slots = max(slot, 0);
+            q.parts = used;
             for (int k = 0; k < used; ++k) {
                 q.first = k * each;
                 q.end = min(q.first + each, end);
@@ -134,12 +131,12 @@ __device__ inline void make_packed_plan(const RaggedRows &r, const PackedPlan &p
                     sm_length[k] = sum;
                     sum += n;
                 }
-                plan.counts[0] = static_cast<int32_t>(min(sum, plan.max_items));
+                *plan.count = static_cast<int32_t>(min(sum, plan.max_items));
             }
             __syncthreads();
         }
     }
-    if (i == 0) plan.counts[1] = static_cast<int32_t>(min(sm_joins, plan.max_joins));
+    for (uint32_t s = i; s < 2 * plan.max_parts; s += kThreads) plan.arrived[s] = 0;
 }
 
 }  // namespace pvlc

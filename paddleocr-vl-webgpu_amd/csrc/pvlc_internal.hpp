@@ -230,17 +230,18 @@ constexpr uint32_t shares_of_each(uint32_t n) {
     return SPARE == 2 ? (n + UNIT - 2) / UNIT + 1 : (n + UNIT - 1) / UNIT;
 }
 // Packed prompts: 16 tokens t0 .. of a sequence (its rows begin at `begin`) and
-// the pieces of 32 keys that one workgroup takes; slot: where it leaves a part
-// of them, or -1.
+// the pieces of 32 keys that one workgroup takes; slot: where it leaves a part of
+// an item (-1: it has all of them), among the slots slots .. slots + parts - 1.
 constexpr int kPackedTokens = 16;
 struct PackedItem {
-    int32_t begin, count, held, seq, t0, first, end, slot;
+    int32_t begin, count, held, seq, t0, first, end, slot, slots, parts;
 };
 // Where an append's launch leaves a plan of items (items null: it makes none).
 struct PackedPlan {
-    int32_t *counts;
-    PackedItem *items, *joins;
-    uint32_t max_items, max_joins, max_parts;
+    int32_t *count;
+    PackedItem *items;
+    uint32_t *arrived;  // [slot][kv head], cleared: parts that have been left
+    uint32_t max_items, max_parts;
 };
 // Rows appended to their pages (kernels_append.hip); strides in elements.
 struct AppendRows {
@@ -270,12 +271,13 @@ struct PackedRows {
     const int32_t *positions;
     const uint16_t *key_cache, *value_cache;
     float scale_log2;
-    // The plan that the append's launch made (items null: none), and what
-    // bounds its items and joins.
-    const int32_t *counts;  // items, joins
-    const PackedItem *items, *joins;
-    float *partials;  // [slot][kv head][kPackedPartFloats]
-    uint32_t max_items, max_joins;
+    // The plan that the append's launch made (items null: none), and what bounds
+    // its items.
+    const int32_t *count;
+    const PackedItem *items;
+    uint32_t *arrived;
+    uint64_t *partials;  // [slot][kv head][kPackedPartPairs]
+    uint32_t max_items;
     bool narrow;  // one head a workgroup, without a plan
 };
 int launch_packed_prefill(const PackedRows &rows, void *stream);
@@ -291,8 +293,8 @@ inline bool packed_is_narrow(uint32_t num_seqs, uint32_t rows, uint32_t max_cont
     const uint64_t shares = static_cast<uint64_t>(rows / kPackedTokens) + num_seqs;
     return shares <= kNarrowShares && max_context <= kNarrowContext && shares * max_context <= kNarrowRows;
 }
-// Its workspace: 256 bytes of words (0 the error word, 1 and 2 the plan's
-// counts), then the items, the joins and the parts.  More sequences than
+// Its workspace: 256 bytes of words (0 the error word, 1 the plan's count), then
+// the items, the counts of parts that have been left, and the parts.  More sequences than
 // kPackedPlanSeqs (what the plan holds in LDS) are not planned.  Items are cut
 // from kPackedLeastPart pieces on, or from what lets the cut items of a call have
 // kPackedMaxParts parts at most, 1.28 times what each of the 512 resident
@@ -302,11 +304,11 @@ inline bool packed_is_narrow(uint32_t num_seqs, uint32_t rows, uint32_t max_cont
 // cut at even shares balance the workgroups better and took these chunks 222 us:
 // parts of one sequence that begin at different keys read 711 MB past L2, not 278.)
 constexpr uint32_t kPackedPlanSeqs = 1024, kPackedLeastPart = 16, kPackedMaxParts = 400;
-constexpr size_t kPackedPartFloats = 4 * 66 * 64;  // 4 waves x (64 outputs, reference, sum) x 64 lanes
+constexpr size_t kPackedPartPairs = 4 * 33 * 64;  // 4 waves x ((reference, sum), 64 outputs) x 64 lanes
 struct PackedWorkspace {
     bool plan, narrow;
-    uint32_t max_items, max_joins, max_parts;
-    size_t items_offset, joins_offset, partials_offset, total;
+    uint32_t max_items, max_parts;
+    size_t items_offset, arrived_offset, partials_offset, total;
 };
 inline PackedWorkspace packed_workspace_layout(uint32_t num_seqs, uint32_t rows, uint32_t max_context) {
     auto align = [](size_t v) { return (v + 255) / 256 * 256; };
@@ -315,12 +317,11 @@ inline PackedWorkspace packed_workspace_layout(uint32_t num_seqs, uint32_t rows,
     w.plan = !w.narrow && num_seqs <= kPackedPlanSeqs;
     w.max_items = rows / kPackedTokens + num_seqs;
     if (w.plan && max_context > 32 * kPackedLeastPart) w.max_parts = kPackedMaxParts;
-    w.max_joins = w.max_parts / 2;
     w.max_items += w.max_parts;
     w.items_offset = 256;
-    w.joins_offset = w.items_offset + align(w.plan ? w.max_items * sizeof(PackedItem) : 0);
-    w.partials_offset = w.joins_offset + align(w.max_joins * sizeof(PackedItem));
-    w.total = w.partials_offset + static_cast<size_t>(w.max_parts) * 2 * kPackedPartFloats * 4;
+    w.arrived_offset = w.items_offset + align(w.plan ? w.max_items * sizeof(PackedItem) : 0);
+    w.partials_offset = w.arrived_offset + align(w.max_parts * 2 * 4);
+    w.total = w.partials_offset + static_cast<size_t>(w.max_parts) * 2 * kPackedPartPairs * 8;
     return w;
 }
 
