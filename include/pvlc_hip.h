@@ -718,21 +718,22 @@ pvlc_hip_status pvlc_hip_kv_pages_copy(const pvlc_hip_kv_pool *from, const int32
  *
  * Rows are packed: sequence s has the rows row_offsets[s] .. row_offsets[s+1]-1
  * of the call's matrices (row_offsets NULL: rows / num_seqs each), any number of
- * them, none included.  They follow the cache_lens[s] rows that its pages hold
- * (cache_lens NULL: none), in the blocks that its table names; the tables,
- * lengths and offsets are device memory and are not changed.  A block that a
- * call writes to belongs to one sequence alone (see the fork of pages); what a
- * block holds behind a sequence's last row is neither used nor changed.
+ * them, none included; the first sequence need not begin at row 0.  They follow
+ * the cache_lens[s] rows that its pages hold (cache_lens NULL: none), in the
+ * blocks that its table names; the tables, lengths and offsets are device memory
+ * and are not changed.  A block that a call writes to belongs to one sequence
+ * alone (see the fork of pages); what a block holds behind a sequence's last row
+ * is neither used nor changed.
  * Matrices and planes are 16-byte aligned.  Everything runs on the caller's
  * stream, without allocation, synchronisation or a copy to the host, and may be
  * captured; calls on one workspace are stream-ordered.
  *
  * Device error bits (of error_word, or the first word of a workspace, which
  * pvlc_hip_workspace_error reads): 1 = offsets that descend or pass `rows`, a
- * negative length, or rows that pass a sequence's table (the sequence is skipped;
- * with such offsets others may be, too); 2 = a block id outside the planes (its
- * rows are not written, block 0 is read); 4 = a rotary position outside the
- * tables (no rotation).
+ * negative length, or rows that pass a sequence's table or max_context (the
+ * sequence is skipped; with such offsets others may be, too); 2 = a block id
+ * outside the planes (its rows are not written, block 0 is read); 4 = a rotary
+ * position outside the tables (no rotation).
  * ------------------------------------------------------------------------- */
 
 /* Rows rotated and written into pages. */
@@ -795,8 +796,9 @@ size_t pvlc_hip_packed_prefill_workspace_bytes(uint32_t num_seqs, uint32_t rows,
  * as the key is.  query: rows of [16][128]; out: [rows][16][128], compact, of
  * which only the sequences' rows are written.  Arithmetic as
  * pvlc_hip_paged_prefill_f16, and, with f32 operands, pvlc_hip_paged_prefill_f32io.
- * A sequence longer than max_context is skipped (error bit 1).  The output may
- * overlap no input and no plane. */
+ * A sequence longer than max_context is skipped (error bit 1).  Values are finite:
+ * one that is not may also reach rows up to 31 places before its own, whose weight
+ * for it is 0.  The output may overlap no input and no plane. */
 pvlc_hip_status pvlc_hip_packed_prefill_f16(const pvlc_hip_packed_prefill_args *args, const uint16_t *query,
                                             const uint16_t *key, const uint16_t *value, uint16_t *out, void *stream);
 pvlc_hip_status pvlc_hip_packed_prefill_f32io(const pvlc_hip_packed_prefill_args *args, const float *query,
@@ -835,9 +837,13 @@ size_t pvlc_hip_shared_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_gr
  * sequence's table, whose entries the others repeat: rows in whole blocks of 16,
  * and no more than the group's shortest sequence has (so a prompt's length may
  * stand there although its last block has been copied).  Any number of sequences
- * may share any number of rows, none included; every sequence is in one group
- * (others are appended to, and not attended).  query [num_seqs][16][128], new_key
- * and new_value [num_seqs][2][128], out [num_seqs][16][128], compact. */
+ * may share any number of rows, none included; every sequence is in one group.
+ * Calls of few rows (num_seqs times max_context up to 90000) and those without a
+ * group of two run as paged decodes, which are faster there; the offsets and shared
+ * lengths are not looked at then.  Otherwise offsets that descend or pass num_seqs
+ * and a negative shared length are error bit 1: their groups' sequences, and those of
+ * no group, have no output and no new row.  query [num_seqs][16][128], new_key and
+ * new_value [num_seqs][2][128], out [num_seqs][16][128], compact. */
 pvlc_hip_status pvlc_hip_shared_decode_f16(const pvlc_hip_shared_decode_args *args, const uint16_t *query,
                                            const uint16_t *new_key, const uint16_t *new_value, uint16_t *out,
                                            void *stream);

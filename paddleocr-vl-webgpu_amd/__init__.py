@@ -13,8 +13,12 @@ Python host mirror of the reference's operator surface, over the C ABI of
 * serving beside it -- the cache in 8 bits (:func:`paged_decode_q8_f16`,
   :func:`paged_decode_q8_f32io`, :func:`kv_pack_q8`, :func:`kv_unpack_q8`), its
   pages (:func:`kv_page_pool`, :func:`kv_pages_fork`, :func:`kv_pages_compact`,
-  :func:`kv_pages_copy`) and the selection of a beam search
-  (:func:`beam_select`).
+  :func:`kv_pages_copy`), the selection of a beam search
+  (:func:`beam_select`), and batches over either cache: rows of several sequences
+  in one call (:func:`kv_append_f16`, :func:`kv_append_f32`), packed prompts
+  (:func:`packed_prefill_f16`, :func:`packed_prefill_f32io`) and a decode step of
+  groups that share their first pages (:func:`shared_decode_f16`,
+  :func:`shared_decode_f32io`).
 
 Names, argument meaning and error behaviour follow the reference; failures
 raise :class:`PvlcHipError` carrying the reference's ``RuntimeErrorCode`` and,

@@ -1,5 +1,5 @@
 // Attention of a few columns of 16 queries over paged keys and values, by one
-// wave: the loop that the packed prompts and the shared decode have in common.
+// wave: the loop of the shared decode and of small packed prompts.
 //
 //   S^T[key][query] = K Q^T        v_mfma_f32_16x16x32_f16
 //   O^T[dim][query] += V^T P^T     the same (8-bit pages: ..._bf16)
@@ -8,7 +8,13 @@
 // keys such that lane (query, kg) receives keys kg * 8 + h * 4 + r: 8 consecutive
 // ones after both, which is its operand of the second product.  With the values
 // as the first operand a lane keeps one query's outputs, so the softmax's
-// factors never leave the lane.
+// factors never leave the lane.  Keys and values come from the pages into
+// registers, whole lines a load, a step ahead of their use: where few queries read
+// each key, LDS would only add a round.
+//
+// Sums and outputs are f32.  Scores are products of fp16 (8-bit codes are exact in
+// it).  Weights are fp16, with f32 operands pairs of it (22 bits); over 8-bit pages,
+// whose powers of two they carry, two or three bf16 terms (16 and 24 bits).
 #pragma once
 
 #include <hip/hip_runtime.h>

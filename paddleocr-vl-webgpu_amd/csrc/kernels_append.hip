@@ -47,7 +47,11 @@ __device__ inline uint32_t row_max(uint32_t x) {
 //
 // Short calls are bound by the chain of dependent rounds: the sequence; its
 // table entry, positions and rows; cos and sin; (8 bits: the old block with the
-// rows); the stores.
+// rows); the stores.  A few rows for each of 24 sequences 4.4 us a call, a page of 1157
+// f32 rows into e4m3 4.4.  Long calls: 16 prompts of 90 to 2010 fp16 rows (20 MB) 7.4
+// us, 2.8 TB/s with the launch; 8 documents of 4096 to 14336 rows into int8 (100 MB)
+// 25.1 us, 4.0 TB/s of a copy's 5.1: sizes and codes are 60% of their vector
+// instructions.
 template <bool F32, int CODE>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendRows p) {
     constexpr bool kQ8 = CODE != PVLC_HIP_KV_F16;
