@@ -13,6 +13,7 @@ namespace {
 
 constexpr uint64_t kMaxGroups = 1u << 24;  // workgroups of 256 threads that a launch may have (below 2^32 threads)
 constexpr uint64_t kMaxStride = 1ull << 31;
+constexpr uint32_t kMaxTokens = 0x7FFFFF00u;  // of a table's row: positions rounded up to a few blocks stay whole numbers of 32 bits
 
 bool aligned(const void *p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
 
@@ -55,8 +56,8 @@ pvlc_hip_status check_append(const pvlc_hip_kv_append_args *args, const void *ke
     if (pvlc_hip_status st = check_planes(args->code, args->key_cache, args->value_cache, args->exponents)) return st;
     if (args->num_seqs == 0 || args->rows == 0 || args->num_blocks == 0 || args->max_blocks_per_seq == 0)
         return invalid(PVLC_HIP_INV_ZERO_DIMENSION, "sequences, rows, blocks and table width must be nonzero");
-    if (args->rows > 0x7FFFFFFFu || args->num_blocks > 0x7FFFFFFFu || args->max_blocks_per_seq > 0x7FFFFFFFu / kBlockTokens)
-        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows, blocks and a table row's tokens must be below 2^31");
+    if (args->rows > 0x7FFFFFFFu || args->num_blocks > 0x7FFFFFFFu || args->max_blocks_per_seq > kMaxTokens / kBlockTokens)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows and blocks must be below 2^31, a table row's tokens up to 2^31 - 256");
     if (args->rows / kBlockTokens + 2ull * args->num_seqs >= kMaxGroups)
         return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows and sequences exceed the grid");
     if (!args->row_offsets && args->rows % args->num_seqs != 0)
@@ -180,6 +181,8 @@ pvlc_hip_status prefill(const pvlc_hip_packed_prefill_args *args, const void *qu
     if (pvlc_hip_status st = check_matrix(query, &query_stride, args->rows, kQueryHeads * kHeadDim, size, "query", &queries)) return st;
     if (pvlc_hip_status st = check_matrix(out, &out_stride, args->rows, kQueryHeads * kHeadDim, size, "out", &outs)) return st;
     const PackedWorkspace ws = packed_workspace_layout(args->num_seqs, args->rows, args->max_context);
+    if (2ull * ws.max_items >= kMaxGroups)
+        return invalid(PVLC_HIP_INV_INVALID_DECODER_GEOMETRY, "rows and sequences of a packed prefill exceed the grid");
     if (pvlc_hip_status st = check_workspace(args, ws.total, "packed prefill")) return st;
     if (pvlc_hip_status st = check_apart(rows, keys, values, {queries}, {{args->workspace, ws.total}, outs})) return st;
     a.ragged.max_tokens = args->max_context;

@@ -103,3 +103,17 @@ def test_workspace_sizes():
             message = refused(shared(dict(base, workspace_bytes=256, **more)), "LengthMismatch")
             assert int(message.rsplit(" ", 1)[1]) <= nbytes, (seqs, groups, context)
         pvlc.packed_prefill_workspace_bytes(seqs, seqs * 3, context)
+
+
+@CALLS
+def test_tables_of_nearly_2_31_tokens(call):
+    """Positions are whole numbers of 32 bits, and so is one rounded up to the next pieces of keys."""
+    refused(call(dict(max_blocks_per_seq=(1 << 27) - 15)), "InvalidDecoderGeometry")
+    refused(call(dict(max_blocks_per_seq=(1 << 27) - 16, key=None)), "LengthMismatch")  # (a later check)
+
+
+def test_prefill_grid():
+    """Two workgroups of 256 threads for every 16 rows and for every sequence: fewer than 2^32 threads."""
+    far = dict(query=1 << 44, key=2 << 44, value=3 << 44, out=4 << 44, workspace_bytes=1 << 40, row_offsets=5 << 44, cache_lens=6 << 44, block_tables=7 << 44)
+    refused(prefill(dict(far, num_seqs=1 << 22, rows=1 << 26)), "InvalidDecoderGeometry")
+    refused(prefill(dict(far, num_seqs=1 << 22, rows=1 << 25, workspace=None)), "LengthMismatch")  # (the next check)
