@@ -229,3 +229,46 @@ def test_rising_scores_over_eight_heads(f32):
     ws = workspace(b, b.width * 16)
     launch(b, args_of(b, ws))
     check(b, "rising", np.arange(0, 100, 7))
+
+
+@WIDTHS
+@pytest.mark.parametrize("wide", [False, True])
+def test_histories_on_the_same_pages(f32, wide):
+    """Three requests behind one instruction: the same blocks in every table, rows of their own behind them."""
+    log(f"case: packed prefill, one history, f32={f32} wide={wide}")
+    b = B.Batch([5, 40, 17], [64, 64, 64], f32=f32, seed=21, room=5000 if wide else 0)
+    for s in (1, 2):
+        b.table[s, :4] = b.table[0, :4]
+    b.upload()
+    ws = workspace(b, b.width * 16)
+    launch(b, args_of(b, ws))
+    check(b, "one history")
+    assert pvlc.workspace_error(*ws) == 0
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_replays_follow_the_lengths(wide):
+    """Offsets, lengths and tables are read by the launches: what lies there at a replay counts, not what lay there at the capture."""
+    import torch
+    log(f"case: packed prefill, replays with other lengths, wide={wide}")
+    b = B.Batch([30, 7, 50], [20, 0, 33], seed=22, room=5000 if wide else 64, spare=6).upload()
+    other = B.Batch([1, 80, 6], [0, 40, 17], seed=23, room=b.width * 16 - 120, spare=6)
+    assert other.width == b.width and other.rows == b.rows and other.blocks == b.blocks
+    ws = workspace(b, b.width * 16)
+    args = args_of(b, ws, rope_rows=min(b.table_rows, other.table_rows))
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        launch(b, args, stream)
+    graph.replay()
+    check(b, "as captured")
+    other.upload()
+    for name in ("planes", "dtable", "dlens", "doffsets", "dq", "dk", "dv"):
+        for to, of in zip(*([getattr(x, name)] if name != "planes" else x.planes for x in (b, other))):
+            to.copy_(of)
+    b.out.fill_(9.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    other.planes, other.out = b.planes, b.out
+    check(other, "with other lengths")
+    assert pvlc.workspace_error(*ws) == 0

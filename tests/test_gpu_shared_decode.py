@@ -221,3 +221,43 @@ def test_group_offsets_that_descend_are_reported(n):
         firsts[n // 2] = bad
         c.launch(c.shared_args(ws, group_offsets=torch.from_numpy(firsts).cuda()))
         assert pvlc.workspace_error(*ws) == 1
+
+
+@CODES
+def test_two_steps_at_once(code):
+    """On two streams, each with its workspace, and pools of their own."""
+    import torch
+    log(f"case: shared decode, two at once, code={code}")
+    pair = [Groups([5, 3], [900, 40], tails_of(8, 60, seed), code, seed == 1, seed=seed).upload() for seed in (1, 2)]
+    spaces = [c.workspace() for c in pair]
+    args = [c.shared_args(ws) if len(set(c.sizes)) == 1 else c.shared_args(ws, offsets=True) for c, ws in zip(pair, spaces)]
+    streams = [torch.cuda.Stream() for _ in pair]
+    torch.cuda.synchronize()
+    for c, a, s in zip(pair, args, streams):
+        c.launch(a, s)
+    for c, ws in zip(pair, spaces):
+        c.check("at once")
+        assert pvlc.workspace_error(*ws) == 0
+
+
+@CODES
+def test_replays_follow_the_lengths(code):
+    """A captured step replayed as its sequences grow: lengths, shared lengths and rows change in place."""
+    import torch
+    log(f"case: shared decode, replays of a growing batch, code={code}")
+    c = Groups([4, 4], [100, 31], tails_of(8, 40), code, True, seed=9, room=8).upload()
+    ws = c.workspace()
+    args = c.shared_args(ws)
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        c.launch(args, stream)
+    for step in range(4):
+        c.out.fill_(9.0)
+        graph.replay()
+        c.check(f"step {step}")
+        c.held = [t + 1 for t in c.held]
+        c.dlens.add_(1)
+        if step == 1:
+            c.dshared[1] = 0  # (shared as before, attended as rows of each one's own)
+    assert pvlc.workspace_error(*ws) == 0
