@@ -796,9 +796,9 @@ size_t pvlc_hip_packed_prefill_workspace_bytes(uint32_t num_seqs, uint32_t rows,
  * as the key is.  query: rows of [16][128]; out: [rows][16][128], compact, of
  * which only the sequences' rows are written.  Arithmetic as
  * pvlc_hip_paged_prefill_f16, and, with f32 operands, pvlc_hip_paged_prefill_f32io.
- * A sequence longer than max_context is skipped (error bit 1).  Values are finite:
- * one that is not may also reach rows up to 31 places before its own, whose weight
- * for it is 0.  The output may overlap no input and no plane. */
+ * A sequence longer than max_context is skipped (error bit 1).  A value that is not
+ * finite leaves the rows before its own as they are, and that dim of the others
+ * infinite or NaN.  The output may overlap no input and no plane. */
 pvlc_hip_status pvlc_hip_packed_prefill_f16(const pvlc_hip_packed_prefill_args *args, const uint16_t *query,
                                             const uint16_t *key, const uint16_t *value, uint16_t *out, void *stream);
 pvlc_hip_status pvlc_hip_packed_prefill_f32io(const pvlc_hip_packed_prefill_args *args, const float *query,

@@ -107,6 +107,19 @@ __device__ inline float column_sum(float c) {
     return __uint_as_float(v[0]) + __uint_as_float(v[1]);
 }
 
+// Infinities and NaN among values become 0.  (A weight of 0, for a key that a query
+// does not see, would make them NaN.)
+__device__ inline bool is_odd(uint16_t v) { return (v & 0x7C00) == 0x7C00; }
+__device__ inline void clean(half8_t &v) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const _Float16 x = v[e];  // (a bit cast of the element itself takes the first one's bits)
+        v[e] = is_odd(__builtin_bit_cast(uint16_t, x)) ? static_cast<_Float16>(0.0f) : x;
+    }
+}
+// Such a value, where the query sees its key; else 0.
+__device__ inline float odd_value(uint16_t v, bool seen) { return seen && is_odd(v) ? static_cast<float>(__builtin_bit_cast(_Float16, v)) : 0.f; }
+
 // Keys and values of a step as they lie in the pages.
 template <int CODE>
 struct AttendTile {
@@ -178,8 +191,11 @@ struct AttendTile {
 // query sees the keys below its limit; steps below `masked` lie below every
 // limit.  `valid` keys are the sequence's (see AttendTile::keep).  begin() sends
 // out the first step's loads, so that the queries can be made ready under them.
-template <int CODE, bool F32, int CT>
+// CLEAN: limits differ, and if `odd`, values that are not finite are left out of
+// the masked steps; add_odd adds them where they are seen.
+template <int CODE, bool F32, int CT, bool CLEAN = false>
 struct Attend {
+    bool odd = false;  // uniform
     AttendPages p;
     int first, end, stride;
     uint32_t ids;  // blocks, one per lane: lane 2 i + j holds tile j of step i0 + i (32 steps a load)
@@ -206,11 +222,32 @@ struct Attend {
     }
     __device__ __attribute__((always_inline)) void run(const half8_t (&qf)[CT][4], int masked, const int (&limit)[CT], int valid, float scale,
                                                        AttendState<CT> &st);
+    __device__ void add_odd(int masked, const int (&limit)[CT], int valid, AttendState<CT> &st) const {
+        const int kg = (threadIdx.x & 63) >> 4;
+#pragma unroll 1
+        for (int s = first; s < end; s += stride) {
+            if (s < masked) continue;
+#pragma unroll 1
+            for (int key = s * kAttendStep; key < min((s + 1) * kAttendStep, valid) && key / static_cast<int>(kBlockTokens) <= p.last_tile; ++key) {
+                const size_t slab = static_cast<size_t>(attend_block(p, key / static_cast<int>(kBlockTokens))) * kKvHeads + p.head;
+                const uint16_t *src = reinterpret_cast<const uint16_t *>(p.values) + slab * kBlockHeadElems + key % static_cast<int>(kBlockTokens);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        __builtin_amdgcn_sched_barrier(0);  // (few loads at once: this is seldom run, and must not cost the loop registers)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) st.o[ct][c][r] += odd_value(src[(c * 16 + kg * 4 + r) * static_cast<int>(kBlockTokens)], key < limit[ct]);
+                    }
+            }
+        }
+    }
 };
 
-template <int CODE, bool F32, int CT>
-__device__ __attribute__((always_inline)) inline void Attend<CODE, F32, CT>::run(const half8_t (&qf)[CT][4], int masked, const int (&limit)[CT],
-                                                                                  int valid, float scale, AttendState<CT> &st) {
+template <int CODE, bool F32, int CT, bool CLEAN>
+__device__ __attribute__((always_inline)) inline void Attend<CODE, F32, CT, CLEAN>::run(const half8_t (&qf)[CT][4], int masked, const int (&limit)[CT],
+                                                                                         int valid, float scale, AttendState<CT> &st) {
+    static_assert(!CLEAN || CODE == PVLC_HIP_KV_F16);
     constexpr bool kQ8 = CODE != PVLC_HIP_KV_F16;
     if (first >= end) return;  // uniform
     const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
@@ -257,6 +294,12 @@ __device__ __attribute__((always_inline)) inline void Attend<CODE, F32, CT>::run
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct) x[ct][e] = key + e < limit[ct] ? x[ct][e] : -INFINITY;
             if ((s + 1) * kAttendStep > valid) tile.keep(key, valid);  // uniform
+            if constexpr (CLEAN) {
+                if (odd) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) clean(tile.v[c]);
+                }
+            }
         }
         bool far = false;
         float m_new[CT];

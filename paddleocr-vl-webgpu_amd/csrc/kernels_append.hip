@@ -174,6 +174,12 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendRows p) {
         if (!rope && p.rope_cos != nullptr && c == 0 && hh == 0 && tt >= lo && tt < hi) atomicOr(p.error_word, 4u);
     }
     if constexpr (!kQ8) {
+        if (p.odd) {  // for the packed prompts: which blocks have values that are not finite (a byte for each wave)
+            const u16x8_t every = static_cast<uint16_t>(0x7FFF);
+            const u16x8_t size = __builtin_elementwise_max(__builtin_bit_cast(u16x8_t, v[0]) & every, __builtin_bit_cast(u16x8_t, v[1]) & every);
+            const bool odd = __any(largest(size) > kLargestHalf) != 0;
+            if ((i & 63) == 0) reinterpret_cast<uint8_t *>(p.odd + share)[i >> 6] = odd;
+        }
         if (ok && tt >= lo && tt < hi) {
             uint16_t *dst = static_cast<uint16_t *>(p.key_cache) + (static_cast<size_t>(id) * kKvHeads + hh) * kBlockHeadElems + c * 128 + key_slot(tt) * 8;
             *reinterpret_cast<half8_t *>(dst) = out[0];

@@ -24,6 +24,14 @@ namespace {
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
+// Whether the append met values that are not finite in the blocks of an item's rows.
+__device__ inline bool item_is_odd(const PackedRows &p, int seq, int begin, int held, int count, int t0) {
+    const int32_t *seen = p.odd + first_append_share(p.ragged, seq, begin);
+    constexpr int kTokens = kBlockTokens;
+    const int before = held / kTokens, a = (held + t0) / kTokens - before, b = (held + min(t0 + kPackedTokens, count) - 1) / kTokens - before;
+    return (load_const(seen, a) | load_const(seen, b)) != 0;
+}
+
 // A workgroup takes 16 tokens of a sequence and the 8 query heads of a kv head,
 // a wave two of the heads: 32 columns, in v_mfma_f32_32x32x16_f16.  Two workgroups
 // are on each compute unit, at 190 to 202 registers a wave: one waits or computes
@@ -124,6 +132,17 @@ struct Wide {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[dt][r] *= a;
         }
+    }
+    // The values that are not finite, of a key in `block`, where the query sees it.
+    __device__ __attribute__((always_inline)) void add_odd(const uint16_t *block, int key) {
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                if ((r & 3) == 0) __builtin_amdgcn_sched_barrier(0);  // (few loads at once: seldom run, and must not cost the loop registers)
+                const int d = dt * 32 + (r >> 2) * 8 + half * 4 + (r & 3);
+                o[dt][r] += odd_value(block[d * static_cast<int>(kBlockTokens) + key % static_cast<int>(kBlockTokens)], key < limit);
+            }
     }
     // The weights of 32 keys in fp16 (with f32 operands as hi + lo), their sum as
     // rounded, and O^T += V^T P^T.
@@ -261,6 +280,7 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedR
     const int lane = w.lane, wave = w.wave, t0 = q.t0, first = q.first, end = q.end;
     const int valid = q.held + q.count, last_tile = (min(q.held + t0 + kPackedTokens, valid) - 1) >> 4;
     const int masked = (q.held + t0 + 1) / 32;  // pieces from this one on reach past the first query's keys
+    const bool odd = item_is_odd(p, q.seq, q.begin, q.held, q.count, t0);
 
     const int32_t *table = p.ragged.tables ? p.ragged.tables + static_cast<size_t>(q.seq) * p.ragged.max_blocks : nullptr;
     const int64_t base = static_cast<int64_t>(q.seq) * p.ragged.max_blocks;
@@ -313,11 +333,12 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedR
     auto edge = [&](int n, const uint16_t *kc, uint16_t *kn, uint16_t *vc, uint16_t *vn) __attribute__((always_inline)) {
         fetch_k(n + 2, kn);
         fetch_v(n + 2, vn);
-        if ((n + 2) * 32 > valid) {
+        if ((n + 2) * 32 > valid || odd) {
             // Values behind the sequence's rows become 0: what the pages hold there may
-            // be NaN, and a weight of 0 would not remove it.
+            // be NaN, and a weight of 0 would not remove it.  And values of the
+            // item's own rows that are not finite: some of its queries do not see them.
             for (int i = static_cast<int>(threadIdx.x); i < kStepElems; i += kWideWaves * 64)
-                if (n * 32 + (i >> 11) * 16 + ((i >> 10) & 1) * 8 + (i & 7) >= valid) vc[i] = 0;
+                if (n * 32 + (i >> 11) * 16 + ((i >> 10) & 1) * 8 + (i & 7) >= valid || (odd && is_odd(vc[i]))) vc[i] = 0;
             __syncthreads();
         }
         if (n + 1 < end) {
@@ -341,9 +362,15 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedR
         plain(n, sk0, sk1, sv0, sv1);
         plain(n + 2, sk1, sk0, sv1, sv0);
     }
+    const int edges = n;
     for (; n < end; n += 4) {
         edge(n, sk0, sk1, sv0, sv1);
         if (n + 2 < end) edge(n + 2, sk1, sk0, sv1, sv0);
+    }
+    if (odd) {  // uniform
+#pragma unroll 1
+        for (int key = edges * 32; key < min(end * 32, valid) && key / static_cast<int>(kBlockTokens) <= last_tile; ++key)
+            w.add_odd(p.value_cache + slab(key / static_cast<int>(kBlockTokens)), key);
     }
 
     if (q.slot >= 0) {
@@ -407,8 +434,9 @@ __global__ __launch_bounds__(kNarrowWaves * 64, 2) void packed_narrow_kernel(Pac
     pages.num_blocks = p.ragged.num_blocks;
     pages.head = g;
     pages.last_tile = (keys - 1) >> 4;
-    Attend<kF16, F32, 1> loop;
+    Attend<kF16, F32, 1, true> loop;
     loop.begin(pages, wave, (keys + kAttendStep - 1) / kAttendStep, kNarrowWaves);
+    loop.odd = item_is_odd(p, q.seq, q.begin, q.held, q.count, t0);
     half8_t *const sm_q = reinterpret_cast<half8_t *>(&sm_o[0][0]);  // [kb][lane], before the join
     if (wave < 2) {
         half8_t lo, hi;
@@ -426,7 +454,9 @@ __global__ __launch_bounds__(kNarrowWaves * 64, 2) void packed_narrow_kernel(Pac
     const int limit[1] = {q.held + t + 1};
     AttendState<1> st;
     st.clear();
-    loop.run(qf, (q.held + t0 + 1) / kAttendStep, limit, valid, p.scale_log2, st);
+    const int masked = (q.held + t0 + 1) / kAttendStep;
+    loop.run(qf, masked, limit, valid, p.scale_log2, st);
+    if (loop.odd) loop.add_odd(masked, limit, valid, st);
     const float l = column_sum(st.l[0]);
     if (kg == 0) {
         sm_m[wave][row] = st.m[0];

@@ -257,6 +257,7 @@ struct AppendRows {
     uint8_t *exponents;
     uint32_t *error_word;
     PackedPlan plan;
+    uint32_t *odd;  // [workgroup] or null: not 0 where a block's values are not all finite
 };
 int launch_kv_append(const AppendRows &rows, void *stream);
 // Packed prompts over pages that hold their rows (kernels_packed.hip).
@@ -277,13 +278,14 @@ struct PackedRows {
     const PackedItem *items;
     uint32_t *arrived;
     uint64_t *partials;  // [slot][kv head][kPackedPartPairs]
+    const int32_t *odd;
     uint32_t max_items;
     bool narrow;  // one head a workgroup, without a plan
 };
 int launch_packed_prefill(const PackedRows &rows, void *stream);
 // Calls of few tokens over short contexts give a workgroup one head, not eight:
 // eight times the workgroups and no plan, but every head reads its keys again.
-// Whole calls, us, one head against eight: a prompt of 16 tokens 7.7 against 12.4,
+// Whole calls, us, one head against eight: a prompt of 16 tokens 7.9 against 12.4,
 // of 500 tokens 12.2 against 21.1; 16 tokens each on 500 held, 16 sequences 11.9
 // against 22.2, 32 sequences 18.5 against 23.1, 64 (128 shares) 27.4 against 25.1;
 // on 4000 held, 4 sequences 18.9 against 30.6, 16 (32 shares) 39.4 against 37.5;
@@ -293,9 +295,9 @@ inline bool packed_is_narrow(uint32_t num_seqs, uint32_t rows, uint32_t max_cont
     const uint64_t shares = static_cast<uint64_t>(rows / kPackedTokens) + num_seqs;
     return shares <= kNarrowShares && max_context <= kNarrowContext && shares * max_context <= kNarrowRows;
 }
-// Its workspace: 256 bytes of words (0 the error word, 1 the plan's count), then
-// the items, the counts of parts that have been left, and the parts.  More sequences than
-// kPackedPlanSeqs (what the plan holds in LDS) are not planned.  Items are cut
+// Its workspace: 256 bytes of words (0 the error word, 1 the plan's count), what the
+// append says of its blocks, the items, the counts of parts that have been left,
+// and the parts.  More sequences than kPackedPlanSeqs (what the plan holds in LDS) are not planned.  Items are cut
 // from kPackedLeastPart pieces on, or from what lets the cut items of a call have
 // kPackedMaxParts parts at most, 1.28 times what each of the 512 resident
 // workgroups would have of an even share.  256 / 400 / 512 / 640 / 768 / 1024 parts: 12
@@ -318,7 +320,7 @@ inline PackedWorkspace packed_workspace_layout(uint32_t num_seqs, uint32_t rows,
     w.max_items = rows / kPackedTokens + num_seqs;
     if (w.plan && max_context > 32 * kPackedLeastPart) w.max_parts = kPackedMaxParts;
     w.max_items += w.max_parts;
-    w.items_offset = 256;
+    w.items_offset = 256 + align((static_cast<size_t>(rows / kBlockTokens) + 2 * static_cast<size_t>(num_seqs)) * 4);
     w.arrived_offset = w.items_offset + align(w.plan ? w.max_items * sizeof(PackedItem) : 0);
     w.partials_offset = w.arrived_offset + align(w.max_parts * 2 * 4);
     w.total = w.partials_offset + static_cast<size_t>(w.max_parts) * 2 * kPackedPartPairs * 8;

@@ -73,6 +73,12 @@ __device__ inline SeqRows find_share(const RaggedRows &r, uint32_t u) {
     return q;
 }
 
+// The first workgroup of a sequence in an append (find_share<16, 2>).
+__device__ inline uint32_t first_append_share(const RaggedRows &r, int seq, int begin) {
+    constexpr int kTokens = kBlockTokens;
+    return r.offsets ? static_cast<uint32_t>(begin) / kTokens + 2 * seq : static_cast<uint32_t>(seq) * shares_of_each<kTokens, 2>(r.each);
+}
+
 // A block of a sequence as its table gives it; outside the planes: block 0 and
 // *ok false.
 __device__ inline uint32_t checked_block(const RaggedRows &r, int64_t id, bool *ok) {

@@ -272,3 +272,31 @@ def test_replays_follow_the_lengths(wide):
     other.planes, other.out = b.planes, b.out
     check(other, "with other lengths")
     assert pvlc.workspace_error(*ws) == 0
+
+
+@WIDTHS
+@pytest.mark.parametrize("held,wide", [(0, False), (21, False), (0, True), (21, True), (4500, True)])
+def test_values_that_are_not_finite(f32, held, wide):
+    """An infinity or NaN among the values reaches the rows that see it, in its head and dim, and no other."""
+    import torch
+    log(f"case: packed prefill, values that are not finite, held={held} f32={f32} wide={wide}")
+    b = B.Batch([70, 33], [held, held // 2], f32=f32, seed=held + 5, room=4600 - held if wide else 0)
+    for row, head, dim, value in ((3, 0, 5, np.inf), (37, 0, 5, -np.inf), (40, 1, 127, np.nan), (63, 1, 64, -np.inf), (69, 0, 0, np.nan), (70 + 32, 1, 9, np.inf)):
+        b.v[row, head, dim] = value
+    b.upload()
+    ws = workspace(b, b.width * 16)
+    launch(b, args_of(b, ws))
+    torch.cuda.synchronize()
+    got = b.out.float().cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        b.put()
+        seen = np.zeros((103, 16, 128), bool)
+        bad = ~np.isfinite(b.v.astype(np.float64))
+        for row, head, dim in np.argwhere(bad):
+            seen[row:70 if row < 70 else 103, head * 8:head * 8 + 8, dim] = True
+        for plane in (b.cache.value,):  # the finite values' attention: 0 in the places of the others
+            plane[(plane & 0x7C00) == 0x7C00] = 0
+        want, limit = wanted(b)
+    assert np.array_equal(~np.isfinite(got), seen)
+    B.check("finite ones", np.where(seen, 0, got), np.where(seen, 0, want), limit)
+    assert pvlc.workspace_error(*ws) == 0
