@@ -39,9 +39,12 @@ struct SharedSet {
     __device__ int len(int i) const { return __builtin_amdgcn_readlane(lens, i); }
 };
 
+__device__ inline bool fits(const SharedRows &p, int len) { return len >= 0 && static_cast<uint32_t>(len) < p.ragged.max_tokens; }
+
 // The rows that a group shares are no more than its shortest sequence has.
 // Sequences whose length does not fit the call are left out (they are reported
-// where their row would be appended).
+// where their row would be appended); a group of none else shares nothing, whatever
+// its shared length says: nothing would keep that within the table.
 template <int CT>
 __device__ inline bool find_set(const SharedRows &p, uint32_t u, SharedSet *set) {
     int begin, count, first, least;
@@ -70,9 +73,13 @@ __device__ inline bool find_set(const SharedRows &p, uint32_t u, SharedSet *set)
     set->first = begin + first;
     set->count = min(count - first, 2 * CT);
     set->lens = p.ragged.lens[set->first + min(lane, set->count - 1)];
+    bool some = false;
     for (int i = lane; i < count; i += 64) {
         const int len = p.ragged.lens[begin + i];
-        if (len >= 0 && static_cast<uint32_t>(len) < p.ragged.max_tokens) least = min(least, len);
+        if (fits(p, len)) {
+            least = min(least, len);
+            some = true;
+        }
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) least = min(least, __shfl_xor(least, d));
@@ -81,11 +88,9 @@ __device__ inline bool find_set(const SharedRows &p, uint32_t u, SharedSet *set)
         if (threadIdx.x == 0) atomicOr(p.error_word, 1u);
         return false;
     }
-    set->shared = least / static_cast<int>(kBlockTokens) * static_cast<int>(kBlockTokens);
+    set->shared = __any(some) ? least / static_cast<int>(kBlockTokens) * static_cast<int>(kBlockTokens) : 0;
     return true;
 }
-
-__device__ inline bool fits(const SharedRows &p, int len) { return len >= 0 && static_cast<uint32_t>(len) < p.ragged.max_tokens; }
 
 // Steps of a part: the keys are cut into `parts`, fewer for few keys (a part has
 // `least` steps: one for each wave of shared rows, two of own ones); and the

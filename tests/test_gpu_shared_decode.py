@@ -261,3 +261,21 @@ def test_replays_follow_the_lengths(code):
         if step == 1:
             c.dshared[1] = 0  # (shared as before, attended as rows of each one's own)
     assert pvlc.workspace_error(*ws) == 0
+
+
+@CODES
+@pytest.mark.parametrize("offsets", [False, True])
+def test_groups_of_sequences_that_do_not_fit(code, offsets):
+    """A group whose sequences are all left out shares nothing, however far beyond the tables its shared length is; the other
+    group, of the first sequences, is attended."""
+    import torch
+    log(f"case: shared decode, groups that do not fit, code={code} offsets={offsets}")
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    for length, beyond in ((-1, 4000), (None, 1 << 20), (-1, 0x7FFFFFFF)):
+        c = Groups([3, 3], [48, 32], [0, 5, 20, 3, 4, 17], code, False, seed=23).upload()
+        ws = c.workspace()
+        lens = c.held[:3] + [c.width * 16 if length is None else length] * 3
+        c.shared = [48, beyond]
+        c.launch(c.shared_args(ws, offsets=offsets, cache_lens=ints(lens)))
+        c.check("left out", skipped=(3, 4, 5))
+        assert pvlc.workspace_error(*ws) == 1
