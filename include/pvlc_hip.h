@@ -833,10 +833,11 @@ typedef struct pvlc_hip_shared_decode_args {
 size_t pvlc_hip_shared_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context);
 /* pvlc_hip_paged_decode_f16 / _q8_f16 of every sequence (rotation, append,
  * attention over cache_len + 1 rows, and their arithmetic), with the first
- * shared_lens[g] rows of a group read once for all of it, through its first
- * sequence's table, whose entries the others repeat: rows in whole blocks of 16,
- * and no more than the group's shortest sequence has (so a prompt's length may
- * stand there although its last block has been copied).  Any number of sequences
+ * shared_lens[g] rows of a group read once for all of it, through the table of
+ * one sequence, whose entries the others repeat: rows in whole blocks of 16, and
+ * no more than the group's shortest sequence has (so a prompt's length may stand
+ * there although its last block has been copied).  Sequences that are skipped
+ * (error bit 1) count for neither: their tables may hold anything.  Any number of sequences
  * may share any number of rows, none included; every sequence is in one group.
  * Calls of few rows (num_seqs times max_context up to 90000) and those without a
  * group of two run as paged decodes, which are faster there; the offsets and shared

@@ -34,7 +34,8 @@ constexpr int kWaves = kSharedWaves, kThreads = kWaves * 64;
 // Up to 2 CT sequences of a group: 16 columns are the 8 heads of a kv head of 2 sequences.
 struct SharedSet {
     int first, count;  // sequences
-    int shared;        // rows, in whole blocks
+    int shared;        // rows, in whole blocks (0 where no sequence of the set fits)
+    int through;       // of the set's sequences, the first that fits: its table has the shared blocks
     int lens;          // lane i: the length of sequence i
     __device__ int len(int i) const { return __builtin_amdgcn_readlane(lens, i); }
 };
@@ -43,8 +44,8 @@ __device__ inline bool fits(const SharedRows &p, int len) { return len >= 0 && s
 
 // The rows that a group shares are no more than its shortest sequence has.
 // Sequences whose length does not fit the call are left out (they are reported
-// where their row would be appended); a group of none else shares nothing, whatever
-// its shared length says: nothing would keep that within the table.
+// where their row would be appended); a set of none else shares nothing, whatever
+// the shared length says: nothing would keep that within the table.
 template <int CT>
 __device__ inline bool find_set(const SharedRows &p, uint32_t u, SharedSet *set) {
     int begin, count, first, least;
@@ -73,13 +74,9 @@ __device__ inline bool find_set(const SharedRows &p, uint32_t u, SharedSet *set)
     set->first = begin + first;
     set->count = min(count - first, 2 * CT);
     set->lens = p.ragged.lens[set->first + min(lane, set->count - 1)];
-    bool some = false;
     for (int i = lane; i < count; i += 64) {
         const int len = p.ragged.lens[begin + i];
-        if (fits(p, len)) {
-            least = min(least, len);
-            some = true;
-        }
+        if (fits(p, len)) least = min(least, len);
     }
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) least = min(least, __shfl_xor(least, d));
@@ -88,7 +85,9 @@ __device__ inline bool find_set(const SharedRows &p, uint32_t u, SharedSet *set)
         if (threadIdx.x == 0) atomicOr(p.error_word, 1u);
         return false;
     }
-    set->shared = __any(some) ? least / static_cast<int>(kBlockTokens) * static_cast<int>(kBlockTokens) : 0;
+    const uint64_t mine = __ballot(lane < set->count && fits(p, set->lens));
+    set->through = mine ? __builtin_ctzll(mine) : 0;
+    set->shared = mine ? least / static_cast<int>(kBlockTokens) * static_cast<int>(kBlockTokens) : 0;
     return true;
 }
 
@@ -276,7 +275,7 @@ __device__ inline void attend_shared(const SharedRows &p, const SharedSet &set, 
     if (wave < 2 * CT) query.send(p, set, min((wave >> 1) * 2 + (row >> 3), set.count - 1), g, wave & 1);
     __builtin_amdgcn_sched_barrier(0);
     Attend<CODE, F32, CT> loop;
-    loop.begin(pages_of(p, set.first, 0, keys, g), first + wave, end, kWaves);
+    loop.begin(pages_of(p, set.first + set.through, 0, keys, g), first + wave, end, kWaves);
     half8_t *const sm_q = reinterpret_cast<half8_t *>(&lds.o[0][0]);  // [column tile][kb][lane], before the join
     if (wave < 2 * CT) {
         half8_t lo, hi;

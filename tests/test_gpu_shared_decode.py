@@ -279,3 +279,21 @@ def test_groups_of_sequences_that_do_not_fit(code, offsets):
         c.launch(c.shared_args(ws, offsets=offsets, cache_lens=ints(lens)))
         c.check("left out", skipped=(3, 4, 5))
         assert pvlc.workspace_error(*ws) == 1
+
+
+@CODES
+@FAR
+@pytest.mark.parametrize("out", [(0,), (0, 1), (2, 5, 6), (0, 1, 2, 3)])
+def test_sequences_left_out_beside_others(code, far, out):
+    """Sequences that are done, with a negative length and a table of no blocks, and the others of their groups: the shared pages
+    are the others', too."""
+    import torch
+    log(f"case: shared decode, sequences left out, code={code} far={far} out={out}")
+    c = Groups([7], [64], [0, 5, 20, 3, 4, 17, 33], code, True, seed=24, far=far).upload()
+    ws = c.workspace()
+    lens, table = list(c.held), c.dtable.clone()
+    for i in out:
+        lens[i], table[i] = -1, -1
+    c.launch(c.shared_args(ws, cache_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"), block_tables=table))
+    c.check("beside others", skipped=out)
+    assert pvlc.workspace_error(*ws) == 1
