@@ -6,6 +6,9 @@
 // values over any part of a sequence's rows, parts join as
 //   m = max m_p,  out = sum_p exp(m_p - m) o_p / sum_p exp(m_p - m) l_p.
 //
+// A part whose scores are all NaN has the reference of one without keys, -infinity, and a
+// sum of NaN: parts join by products with a factor of 0, which keep it, and are never left out.
+//
 // Bytes are what a group's shared rows take once, so large calls are bound by
 // memory: 32 groups of eight sequences on 8192 to 32768 shared rows (fp16, 607 MB) 150
 // us, 4.0 TB/s of a copy's 5.1.  A group of more than four sequences is several sets,
@@ -168,7 +171,7 @@ __device__ inline void append_and_attend(const SharedRows &p, int seq, int len, 
     for (int kb = 0; kb < 4; ++kb) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(row == 0 ? k[kb] : half8_t{}, qf[kb], acc, 0, 0, 0);
     const float x = __shfl(acc[0], row), top = fmaxf(st.m[0], x);
     const float a = st.m[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((st.m[0] - top) * p.scale_log2);
-    const float w = __builtin_amdgcn_exp2f((x - top) * p.scale_log2);
+    const float w = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((x - top) * p.scale_log2);  // (it may be the only key so far)
     st.m[0] = top;
     st.l[0] = st.l[0] * a + (kg == 0 ? w : 0.f);
 #pragma unroll
@@ -322,7 +325,7 @@ __device__ inline void attend_shared(const SharedRows &p, const SharedSet &set, 
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) m = fmaxf(m, lds.m[w][c]);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) l += lds.m[w][c] == -INFINITY ? 0.f : lds.l[w][c] * __builtin_amdgcn_exp2f((lds.m[w][c] - m) * p.scale_log2);
+        for (int w = 0; w < kWaves; ++w) l += lds.l[w][c] * (lds.m[w][c] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((lds.m[w][c] - m) * p.scale_log2));
         part_ml[c * 2] = m * p.scale_log2;
         part_ml[c * 2 + 1] = l;
     }
@@ -457,8 +460,8 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedRows p) {
         m = top;
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            if (there(i) && ml[i][0] != -INFINITY) {
-                const float w = __builtin_amdgcn_exp2f(ml[i][0] - top);
+            if (there(i)) {
+                const float w = ml[i][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i][0] - top);
                 l += ml[i][1] * w;
                 o += v[i] * w;
             }

@@ -297,3 +297,67 @@ def test_sequences_left_out_beside_others(code, far, out):
     c.launch(c.shared_args(ws, cache_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"), block_tables=table))
     c.check("beside others", skipped=out)
     assert pvlc.workspace_error(*ws) == 1
+
+
+# (8-bit pages hold an infinity as the largest code, and int8 no NaN; a paged decode gives NaN, too, where all that a wave has
+# are scores of -infinity)
+ODD = [(code, far, kind) for code, kinds in ((B.F16, ("nan", "cancel", "plus", "minus", "value")), (R.E4M3, ("nan",))) for far in (False, True)
+       for kind in kinds if far or kind != "minus"]
+
+
+@WIDTHS
+@pytest.mark.parametrize("tail", [0, 1, 40])
+@pytest.mark.parametrize("code,far,kind", ODD)
+def test_new_rows_that_are_not_finite(code, f32, far, tail, kind):
+    """A new key with a NaN, or with infinities whose products cancel, makes its head's outputs NaN, and so does one whose score
+    is +infinity; a score of -infinity is a weight of 0.  An infinite value is infinite or NaN in its dim."""
+    import torch
+    log(f"case: shared decode, new row {kind} code={code} f32={f32} far={far} tail={tail}")
+    c = Groups([3, 3], [64, 32], [tail] * 6, code, f32, seed=25, far=far, rope=False)
+    c.q[:, :, :2] = np.abs(c.q[:, :, :2]) + np.asarray(0.5, c.q.dtype)
+    if kind == "value":
+        c.v[1, 1, 3] = np.inf
+    else:
+        c.k[1, 1, :2] = {"nan": (np.nan, 1), "cancel": (np.inf, -np.inf), "plus": (np.inf, 1), "minus": (-np.inf, 1)}[kind]
+    c.upload()
+    ws = c.workspace()
+    c.launch(c.shared_args(ws))
+    torch.cuda.synchronize()
+    got, odd = c.out.float().cpu().numpy(), np.zeros((6, 16, 128), bool)
+    if kind == "value":
+        odd[1, 8:, 3] = True
+    elif kind != "minus":
+        odd[1, 8:] = True
+    assert np.array_equal(~np.isfinite(got), odd)
+    with np.errstate(invalid="ignore"):
+        for i in range(6):
+            c.cache.put_rows(c.table[i], c.held[i], c.k[i].astype(np.float16).astype(np.float64)[None], c.v[i].astype(np.float16).astype(np.float64)[None])
+    c.check_planes(kind)
+    for i in range(6):
+        q = c.q[i].astype(np.float16).astype(np.float64)[None]
+        k, v = (np.where(np.isfinite(x), x, 0) for x in c.cache.rows(c.table[i], c.held[i] + 1))
+        out, big, most = B.attend(q, k, v, [c.held[i] + 1])
+        if i == 1 and kind == "minus":
+            out[:, 8:] = B.attend(q, k, v, [c.held[i]])[0][:, 8:]
+        mine = ~odd[i:i + 1]
+        B.check(f"{kind} sequence {i}", np.where(mine, got[i:i + 1], 0), np.where(mine, out, 0), B.bound(out, big, most, c.held[i] + 1, f32, code))
+
+
+@pytest.mark.parametrize("code", [B.F16, R.E4M3])
+@FAR
+def test_shared_rows_that_are_not_finite(code, far):
+    """Keys of NaN among the shared rows make every output of their head NaN, one or all of them."""
+    import torch
+    log(f"case: shared decode, shared rows that are not finite, code={code} far={far}")
+    for rows in ([5], range(64)):
+        c = Groups([3], [64], [0, 5, 20], code, True, seed=26, far=far, rope=False)
+        bad = 0x7F if code == R.E4M3 else 0x7E00
+        at = R.KEY_AT if code == R.E4M3 else B.KEY_AT
+        for r in rows:
+            c.cache.key[c.table[0, r // 16], 1, at[r % 16]] = bad
+        c.upload()
+        ws = c.workspace()
+        c.launch(c.shared_args(ws))
+        torch.cuda.synchronize()
+        got = c.out.cpu().numpy()
+        assert np.isnan(got[:, 8:]).all() and np.isfinite(got[:, :8]).all(), (len(rows))
