@@ -39,9 +39,12 @@ struct AttendPages {
     int last_tile;  // tiles behind it are read as it
 };
 
-__device__ inline uint32_t attend_block(const AttendPages &p, int tile) {
+// A block outside the planes is read as block 0, and `bad` set, for the wave.
+__device__ inline uint32_t attend_block(const AttendPages &p, int tile, bool *bad) {
     const int64_t id = p.table ? p.table[tile] : static_cast<int64_t>(p.first) + tile;
-    return id >= 0 && id < static_cast<int64_t>(p.num_blocks) ? static_cast<uint32_t>(id) : 0u;
+    const bool out = id < 0 || id >= static_cast<int64_t>(p.num_blocks);
+    *bad |= __any(out) != 0;
+    return out ? 0u : static_cast<uint32_t>(id);
 }
 
 // First dim of the 8 that a lane's operand kb of a score MFMA covers.  8-bit keys
@@ -196,6 +199,7 @@ struct AttendTile {
 template <int CODE, bool F32, int CT, bool CLEAN = false>
 struct Attend {
     bool odd = false;  // uniform
+    bool bad = false;  // uniform: a block of the steps, or of the next 32, lies outside the planes
     AttendPages p;
     int first, end, stride;
     uint32_t ids;  // blocks, one per lane: lane 2 i + j holds tile j of step i0 + i (32 steps a load)
@@ -215,7 +219,7 @@ struct Attend {
         stride = by;
         if (first >= end) return;  // uniform
         const int lane = threadIdx.x & 63, row = lane & 15, kg = lane >> 4;
-        ids = attend_block(p, tile_of(0));
+        ids = attend_block(p, tile_of(0), &bad);
         tile.load_k(p, id_of(0, 0), id_of(0, 1), row, kg);
         tile.load_v(p, id_of(0, 0), id_of(0, 1), row, kg);
         __builtin_amdgcn_sched_barrier(0);
@@ -229,7 +233,8 @@ struct Attend {
             if (s < masked) continue;
 #pragma unroll 1
             for (int key = s * kAttendStep; key < min((s + 1) * kAttendStep, valid) && key / static_cast<int>(kBlockTokens) <= p.last_tile; ++key) {
-                const size_t slab = static_cast<size_t>(attend_block(p, key / static_cast<int>(kBlockTokens))) * kKvHeads + p.head;
+                bool seen = false;  // (by the loop)
+                const size_t slab = static_cast<size_t>(attend_block(p, key / static_cast<int>(kBlockTokens), &seen)) * kKvHeads + p.head;
                 const uint16_t *src = reinterpret_cast<const uint16_t *>(p.values) + slab * kBlockHeadElems + key % static_cast<int>(kBlockTokens);
 #pragma unroll
                 for (int ct = 0; ct < CT; ++ct)
@@ -254,7 +259,7 @@ __device__ __attribute__((always_inline)) inline void Attend<CODE, F32, CT, CLEA
     uint32_t next_ids = 0;
 
     auto step = [&](auto mask, int s, int i) __attribute__((always_inline)) {
-        if ((i & 31) == 0 && s + 32 * stride < end) next_ids = attend_block(p, tile_of(i + 32));
+        if ((i & 31) == 0 && s + 32 * stride < end) next_ids = attend_block(p, tile_of(i + 32), &bad);
         float x[CT][8];
         {
             float4_t acc[CT][2];

@@ -301,6 +301,7 @@ __device__ inline void attend_shared(const SharedRows &p, const SharedSet &set, 
     AttendState<CT> st;
     st.clear();
     loop.run(qf, keys / kAttendStep, limit, keys, p.scale_log2, st);
+    if (loop.bad && lane == 0) atomicOr(p.error_word, 2u);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
         const float l = column_sum(st.l[ct]);
@@ -363,6 +364,7 @@ __device__ inline void attend_own(const SharedRows &p, const SharedSet &set, int
     AttendState<1> st;
     st.clear();
     loop.run(qf, keys / kAttendStep, limit, keys, p.scale_log2, st);
+    if (loop.bad && lane == 0) atomicOr(p.error_word, 2u);
     if constexpr (CODE == PVLC_HIP_KV_F16) {
         if (new_row >= 0) append_and_attend<F32>(p, set.first + r, new_row, g, qf[0], st);  // uniform
     }

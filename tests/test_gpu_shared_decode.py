@@ -361,3 +361,32 @@ def test_shared_rows_that_are_not_finite(code, far):
         torch.cuda.synchronize()
         got = c.out.cpu().numpy()
         assert np.isnan(got[:, 8:]).all() and np.isfinite(got[:, :8]).all(), (len(rows))
+
+
+@CODES
+@FAR
+@pytest.mark.parametrize("where", ["shared", "own"])
+def test_blocks_outside_the_planes(code, far, where):
+    """A block id outside the planes among the rows that are held is reported, block 0 read; others' outputs and all new rows are
+    as ever."""
+    import torch
+    log(f"case: shared decode, blocks outside the planes, code={code} far={far} where={where}")
+    for bad in (-1, None):
+        c = Groups([3, 2], [64, 160], [40, 33, 70, 20, 0], code, False, seed=27, far=far).upload()
+        ws = c.workspace()
+        table = c.dtable.clone()
+        if where == "shared":
+            table[0:3, 2] = c.blocks if bad is None else bad
+        else:
+            table[2, 5] = c.blocks if bad is None else bad
+        c.launch(c.shared_args(ws, offsets=True, block_tables=table))
+        torch.cuda.synchronize()
+        assert pvlc.workspace_error(*ws) == 2
+        got = c.out.float().cpu().numpy()
+        for i in range(5):
+            c.cache.put_rows(c.table[i], c.held[i], c.turned(c.k[i], i)[None], c.v[i].astype(np.float64)[None])
+        c.check_planes(where)
+        for i in (3, 4) if where == "shared" else (0, 1, 3, 4):
+            k, v = c.cache.rows(c.table[i], c.held[i] + 1)
+            out, big, most = B.attend(c.turned(c.q[i], i)[None], k, v, [c.held[i] + 1])
+            B.check(f"{where} sequence {i}", got[i:i + 1], out, B.bound(out, big, most, c.held[i] + 1, False, code))
