@@ -198,6 +198,7 @@ pvlc_hip_status prefill(const pvlc_hip_packed_prefill_args *args, const void *qu
     r.positions = args->positions;
     r.key_cache = args->key_cache;
     r.value_cache = args->value_cache;
+    r.error_word = a.error_word;
     auto *base = static_cast<unsigned char *>(args->workspace);
     if (ws.plan) {
         a.plan.count = reinterpret_cast<int32_t *>(base) + 1;

@@ -284,10 +284,12 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedR
 
     const int32_t *table = p.ragged.tables ? p.ragged.tables + static_cast<size_t>(q.seq) * p.ragged.max_blocks : nullptr;
     const int64_t base = static_cast<int64_t>(q.seq) * p.ragged.max_blocks;
+    bool bad = false;  // uniform over the wave: a block id outside the planes
     auto slab = [&](int tile) -> size_t {
         tile = min(tile, last_tile);  // (tiles behind the last are never used)
         const int64_t id = table ? load_const(table, tile) : base + tile;
         const bool ok = id >= 0 && id < static_cast<int64_t>(p.ragged.num_blocks);
+        bad |= !ok;
         return (static_cast<size_t>(ok ? id : 0) * kKvHeads + g) * kBlockHeadElems;
     };
     typedef __attribute__((address_space(3))) void *lds_ptr;
@@ -373,6 +375,8 @@ __global__ __launch_bounds__(kWideWaves * 64, 2) void packed_wide_kernel(PackedR
             w.add_odd(p.value_cache + slab(key / static_cast<int>(kBlockTokens)), key);
     }
 
+    if (bad && lane == 0) atomicOr(p.error_word, 2u);
+
     if (q.slot >= 0) {
         // A part of the keys.  The workgroup that leaves the last one of its item joins
         // them (a launch of its own would take calls without parts 1 us, too).
@@ -456,6 +460,7 @@ __global__ __launch_bounds__(kNarrowWaves * 64, 2) void packed_narrow_kernel(Pac
     st.clear();
     const int masked = (q.held + t0 + 1) / kAttendStep;
     loop.run(qf, masked, limit, valid, p.scale_log2, st);
+    if (loop.bad && lane == 0) atomicOr(p.error_word, 2u);
     if (loop.odd) loop.add_odd(masked, limit, valid, st);
     const float l = column_sum(st.l[0]);
     if (kg == 0) {

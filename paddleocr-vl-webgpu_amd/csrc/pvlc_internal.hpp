@@ -271,6 +271,7 @@ struct PackedRows {
     uint32_t rope_rows;
     const int32_t *positions;
     const uint16_t *key_cache, *value_cache;
+    uint32_t *error_word;
     float scale_log2;
     // The plan that the append's launch made (items null: none), and what bounds
     // its items.

@@ -300,3 +300,29 @@ def test_values_that_are_not_finite(f32, held, wide):
     assert np.array_equal(~np.isfinite(got), seen)
     B.check("finite ones", np.where(seen, 0, got), np.where(seen, 0, want), limit)
     assert pvlc.workspace_error(*ws) == 0
+
+
+@WIDTHS
+@pytest.mark.parametrize("counts,held,wide", [([40, 9, 17], [100, 64, 0], False), ([40, 9, 17], [100, 64, 0], True), ([50, 20], [6000, 700], True)])
+def test_blocks_outside_the_planes(f32, counts, held, wide):
+    """A block id outside the planes, among the rows that are held or the call's own, is reported and block 0 read; other
+    sequences are as ever, and the rows of a block that is not there are not written."""
+    import torch
+    log(f"case: packed prefill, blocks outside the planes, held={held} f32={f32} wide={wide}")
+    for bad, at in ((-1, 2), (None, 0), (-1, (held[0] + counts[0] - 1) // 16), (None, held[0] // 16 - 1)):
+        b = B.Batch(counts, held, f32=f32, seed=41, room=5000 if wide else 0)
+        b.upload()
+        ws = workspace(b, b.width * 16)
+        table = b.dtable.clone()
+        table[0, at] = b.blocks if bad is None else bad
+        launch(b, args_of(b, ws, block_tables=table))
+        torch.cuda.synchronize()
+        assert pvlc.workspace_error(*ws) == 2, at
+        kept = [x[b.table[0, at]].copy() for x in (b.cache.key, b.cache.value)]
+        b.put()
+        for x, k in zip((b.cache.key, b.cache.value), kept):
+            x[b.table[0, at]] = k
+        b.check_planes(f"block {at}")
+        some = np.arange(counts[0], int(b.offsets[-1]))
+        want, limit = wanted(b, some)
+        B.check("the others", b.out.float().cpu().numpy()[some], want, limit)
