@@ -830,6 +830,8 @@ typedef struct pvlc_hip_shared_decode_args {
     size_t workspace_bytes;
 } pvlc_hip_shared_decode_args;
 
+/* Enough for every call of up to so many sequences, groups and rows of context,
+ * with group offsets or without. */
 size_t pvlc_hip_shared_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context);
 /* pvlc_hip_paged_decode_f16 / _q8_f16 of every sequence (rotation, append,
  * attention over cache_len + 1 rows, and their arithmetic), with the first

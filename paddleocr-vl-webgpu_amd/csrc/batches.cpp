@@ -253,6 +253,30 @@ pvlc_hip_status decode_alone(const pvlc_hip_shared_decode_args *args, const void
     return ok();
 }
 
+// The most that a shared decode of up to so many sequences, groups and rows needs.
+// It is not what the largest one needs: fewer sets are cut into more parts, and
+// fewer sequences may run as paged decodes, whose parts are others.
+size_t most_shared_bytes(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context) {
+    size_t most = 0;
+    auto take = [&](size_t bytes) { most = bytes > most ? bytes : most; };
+    for (uint32_t columns = 1; columns <= 2; ++columns) {
+        const uint64_t sets = static_cast<uint64_t>(num_seqs) / (2 * columns) + num_groups;  // of a call of any offsets, or none, at most
+        const uint32_t shares = static_cast<uint32_t>(sets < kMaxSharedSets ? sets : kMaxSharedSets);
+        // (of more than 256 sets all have one part of either kind)
+        for (uint32_t n = 1; n <= shares && n <= 256; ++n) take(shared_workspace_of(columns, n, max_context).total);
+        take(shared_workspace_of(columns, shares, max_context).total);
+    }
+    for (uint32_t n = 1; n <= num_seqs && n <= kMaxRaggedSeqs; ++n) {
+        // The longest context that n sequences may run alone with; they are cut
+        // into balanced_parts, or from 512 rows on.
+        uint32_t rows = n <= num_groups ? max_context : kSharedLeastRows / n;
+        rows = rows < max_context ? rows : max_context;
+        const uint32_t cut = rows / 512 + 1, parts = balanced_parts(n), streamed = cut < kMaxMergeParts ? cut : kMaxMergeParts;
+        if (rows > 0) take(decode_workspace_layout(n, parts > streamed ? parts : streamed).total);
+    }
+    return most;
+}
+
 pvlc_hip_status shared(const pvlc_hip_shared_decode_args *args, const void *query, const void *key, const void *value, void *out, bool f32,
                        void *stream) {
     if (!args) return invalid(PVLC_HIP_INV_LENGTH_MISMATCH, "shared decode args are NULL");
@@ -359,14 +383,7 @@ pvlc_hip_status pvlc_hip_packed_prefill_f32io(const pvlc_hip_packed_prefill_args
 
 size_t pvlc_hip_shared_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context) {
     if (num_seqs == 0 || num_groups == 0 || max_context == 0) return 0;
-    const size_t with = shared_workspace_layout(num_seqs, num_groups, max_context, true).total;
-    const size_t without = shared_workspace_layout(num_seqs, num_groups, max_context, false).total;
-    size_t most = with > without ? with : without;
-    if (shared_is_small(num_seqs, num_groups, max_context, false)) {
-        const size_t alone = pvlc_hip_paged_decode_workspace_bytes(num_seqs, max_context, 0);
-        most = most > alone ? most : alone;
-    }
-    return most;
+    return most_shared_bytes(num_seqs, num_groups, max_context);
 }
 
 pvlc_hip_status pvlc_hip_shared_decode_f16(const pvlc_hip_shared_decode_args *args, const uint16_t *query, const uint16_t *new_key,

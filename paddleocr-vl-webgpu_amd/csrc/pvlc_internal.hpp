@@ -375,22 +375,25 @@ struct SharedWorkspace {
     uint32_t columns, shares, shared_parts, own_parts, unit_columns;
     size_t part_o_offset, part_ml_offset, total;
 };
-inline SharedWorkspace shared_workspace_layout(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context, bool offsets) {
+inline SharedWorkspace shared_workspace_of(uint32_t columns, uint32_t shares, uint32_t max_context) {
     auto align = [](size_t v) { return (v + 255) / 256 * 256; };
     auto clamp = [](uint32_t v, uint32_t hi) { return v < 1 ? 1u : v > hi ? hi : v; };
     SharedWorkspace w{};
-    const uint32_t each = (num_seqs + num_groups - 1) / num_groups;
-    w.columns = each <= 2 ? 1 : 2;
-    w.shares = offsets ? num_seqs / (2 * w.columns) + num_groups : num_groups * ((each + 2 * w.columns - 1) / (2 * w.columns));
+    w.columns = columns;
+    w.shares = shares;
     const uint32_t most = clamp((max_context + 32 * kSharedWaves - 1) / (32 * kSharedWaves), 64);
     w.shared_parts = clamp((256 / (2 * w.shares) + 3) / 4 * 4, most);
     w.own_parts = clamp(128 / (2 * w.shares), most);
     w.unit_columns = w.shared_parts * w.columns * 16 + 2 * w.columns * w.own_parts * kGroup;
-    const size_t columns = static_cast<size_t>(w.shares) * 2 * w.unit_columns;
+    const size_t all = static_cast<size_t>(w.shares) * 2 * w.unit_columns;
     w.part_o_offset = 256 + align(kMaxRaggedSeqs * kKvHeads * 4);
-    w.part_ml_offset = w.part_o_offset + align(columns * kHeadDim * 4);
-    w.total = w.part_ml_offset + align(columns * 8);
+    w.part_ml_offset = w.part_o_offset + align(all * kHeadDim * 4);
+    w.total = w.part_ml_offset + align(all * 8);
     return w;
+}
+inline SharedWorkspace shared_workspace_layout(uint32_t num_seqs, uint32_t num_groups, uint32_t max_context, bool offsets) {
+    const uint32_t each = (num_seqs + num_groups - 1) / num_groups, columns = each <= 2 ? 1 : 2, set = 2 * columns;
+    return shared_workspace_of(columns, offsets ? num_seqs / set + num_groups : num_groups * ((each + set - 1) / set), max_context);
 }
 
 // Prefill projection with fp16 weights: workspace of the exact hi/lo split

@@ -1,6 +1,7 @@
 """Refusals of the batches over paged caches, on the host: every one is an error with its code before any GPU effect (the
 pointers here are numbers)."""
 
+import numpy as np
 import pytest
 
 from pvlc_testlib import pvlc
@@ -117,3 +118,26 @@ def test_prefill_grid():
     far = dict(query=1 << 44, key=2 << 44, value=3 << 44, out=4 << 44, workspace_bytes=1 << 40, row_offsets=5 << 44, cache_lens=6 << 44, block_tables=7 << 44)
     refused(prefill(dict(far, num_seqs=1 << 22, rows=1 << 26)), "InvalidDecoderGeometry")
     refused(prefill(dict(far, num_seqs=1 << 22, rows=1 << 25, workspace=None)), "LengthMismatch")  # (the next check)
+
+
+def needed(call, change):
+    """What a call says that it needs, given too little."""
+    return int(refused(call(dict(change, workspace_bytes=256)), "LengthMismatch").rsplit(" ", 1)[1])
+
+
+def test_a_shared_workspace_serves_smaller_calls():
+    """A batch that shrinks, as its pages finish, keeps the workspace of its largest step."""
+    far = dict(zip(("query", "key", "value", "out"), (x << 44 for x in range(1, 5))))
+    g = np.random.default_rng(3)
+    largest = [(64, 16, 4096), (72, 9, 32768), (256, 32, 32768), (4, 1, 1300), (7, 7, 262144), (2000, 100, 500), (12000, 4000, 40), (300, 300, 5000),
+               (1, 1, 1)] + [tuple(int(np.exp(g.uniform(0, np.log(top)))) for top in (4096, 512, 1 << 18)) for _ in range(12)]
+    for seqs, groups, context in largest:
+        nbytes = pvlc.shared_decode_workspace_bytes(seqs, groups, context)
+        smaller = [(seqs * a // b, max(1, groups * a // b), max(1, context // c)) for a, b in ((1, 1), (9, 10), (3, 4), (1, 2), (1, 3), (1, 16), (1, 100)) for c in (1, 2, 5, 64)]
+        smaller += [tuple(int(g.integers(1, top + 1)) for top in (seqs, groups, context)) for _ in range(40)]
+        smaller += [(n, n, c) for n in range(1, min(seqs, groups) + 1, 7) for c in (context, max(1, context // 2))]
+        for n, m, c in smaller:
+            base = dict(far, num_seqs=n, num_groups=m, max_context=c, max_blocks_per_seq=-(-c // 16), num_blocks=64)
+            for more in (dict(), dict(group_offsets=11 * M)):
+                if n and (more or n % m == 0):
+                    assert needed(shared, dict(base, **more)) <= nbytes, (seqs, groups, context, n, m, c, more)
