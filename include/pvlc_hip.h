@@ -790,6 +790,7 @@ typedef struct pvlc_hip_packed_prefill_args {
     size_t workspace_bytes;
 } pvlc_hip_packed_prefill_args;
 
+/* Enough for every call of up to so many sequences, rows and rows of context. */
 size_t pvlc_hip_packed_prefill_workspace_bytes(uint32_t num_seqs, uint32_t rows, uint32_t max_context);
 /* Every sequence's rows appended (as pvlc_hip_kv_append_f16) and attended: row i
  * of sequence s to the cache_lens[s] + i + 1 rows up to itself, its query rotated

@@ -368,7 +368,10 @@ pvlc_hip_status pvlc_hip_kv_append_f32(const pvlc_hip_kv_append_args *args, cons
 
 size_t pvlc_hip_packed_prefill_workspace_bytes(uint32_t num_seqs, uint32_t rows, uint32_t max_context) {
     if (num_seqs == 0 || rows == 0 || max_context == 0) return 0;
-    return packed_workspace_layout(num_seqs, rows, max_context).total;
+    // (past kPackedPlanSeqs sequences a call has no plan, and no parts; a smaller one has both)
+    const size_t own = packed_workspace_layout(num_seqs, rows, max_context).total;
+    const size_t planned = packed_workspace_layout(num_seqs < kPackedPlanSeqs ? num_seqs : kPackedPlanSeqs, rows, max_context).total;
+    return own > planned ? own : planned;
 }
 
 pvlc_hip_status pvlc_hip_packed_prefill_f16(const pvlc_hip_packed_prefill_args *args, const uint16_t *query, const uint16_t *key,

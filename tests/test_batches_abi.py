@@ -141,3 +141,17 @@ def test_a_shared_workspace_serves_smaller_calls():
             for more in (dict(), dict(group_offsets=11 * M)):
                 if n and (more or n % m == 0):
                     assert needed(shared, dict(base, **more)) <= nbytes, (seqs, groups, context, n, m, c, more)
+
+
+def test_a_packed_workspace_serves_smaller_calls():
+    far = dict(zip(("query", "key", "value", "out"), (x << 44 for x in range(1, 5))))
+    g = np.random.default_rng(4)
+    largest = [(1025, 5000, 4096), (1024, 5000, 4096), (3000, 3000, 513), (72, 1152, 4096), (73, 73, 600), (4, 32768, 8192), (1, 1, 1), (40, 9000, 512)]
+    largest += [tuple(int(np.exp(g.uniform(0, np.log(top)))) for top in (4096, 1 << 16, 1 << 16)) for _ in range(12)]
+    for seqs, rows, context in largest:
+        nbytes = pvlc.packed_prefill_workspace_bytes(seqs, rows, context)
+        smaller = [(max(1, seqs * a // b), max(1, rows * d // b), max(1, context // c)) for a, b in ((1, 1), (99, 100), (1, 2), (1, 40)) for d in (a, b) for c in (1, 2, 9)]
+        smaller += [tuple(int(g.integers(1, top + 1)) for top in (seqs, rows, context)) for _ in range(40)]
+        for n, r, c in smaller:
+            base = dict(far, num_seqs=n, rows=r, max_context=c, max_blocks_per_seq=-(-c // 16), num_blocks=64)
+            assert needed(prefill, base) <= nbytes, (seqs, rows, context, n, r, c)
