@@ -726,7 +726,10 @@ pvlc_hip_status pvlc_hip_kv_pages_copy(const pvlc_hip_kv_pool *from, const int32
  * is neither used nor changed.
  * Matrices and planes are 16-byte aligned.  Everything runs on the caller's
  * stream, without allocation, synchronisation or a copy to the host, and may be
- * captured; calls on one workspace are stream-ordered.
+ * captured; calls on one workspace are stream-ordered.  One workspace that holds
+ * the largest of them may serve packed prefills, shared decodes and the paged
+ * decodes of either cache (of up to 2048 sequences) in any order; other calls'
+ * workspaces are their own.
  *
  * Device error bits (of error_word, or the first word of a workspace, which
  * pvlc_hip_workspace_error reads): 1 = offsets that descend or pass `rows`, a

@@ -207,7 +207,7 @@ pvlc_hip_status prefill(const pvlc_hip_packed_prefill_args *args, const void *qu
         a.plan.max_items = ws.max_items;
         a.plan.max_parts = ws.max_parts;
     }
-    a.odd = reinterpret_cast<uint32_t *>(base + 256);
+    a.odd = reinterpret_cast<uint32_t *>(base + ws.odd_offset);
     r.odd = reinterpret_cast<const int32_t *>(a.odd);
     r.count = a.plan.count;
     r.items = a.plan.items;

@@ -296,9 +296,10 @@ inline bool packed_is_narrow(uint32_t num_seqs, uint32_t rows, uint32_t max_cont
     const uint64_t shares = static_cast<uint64_t>(rows / kPackedTokens) + num_seqs;
     return shares <= kNarrowShares && max_context <= kNarrowContext && shares * max_context <= kNarrowRows;
 }
-// Its workspace: 256 bytes of words (0 the error word, 1 the plan's count), what the
-// append says of its blocks, the items, the counts of parts that have been left,
-// and the parts.  More sequences than kPackedPlanSeqs (what the plan holds in LDS) are not planned.  Items are cut
+// Its workspace: 256 bytes of words (0 the error word, 1 the plan's count), room for the
+// paged decodes' arrival counters, which are never cleared (a workspace may serve
+// both, and lies off them here), what the append says of its blocks, the items, the counts of
+// parts that have been left, and the parts.  More sequences than kPackedPlanSeqs (what the plan holds in LDS) are not planned.  Items are cut
 // from kPackedLeastPart pieces on, or from what lets the cut items of a call have
 // kPackedMaxParts parts at most, 1.28 times what each of the 512 resident
 // workgroups would have of an even share.  256 / 400 / 512 / 640 / 768 / 1024 parts: 12
@@ -306,12 +307,14 @@ inline bool packed_is_narrow(uint32_t num_seqs, uint32_t rows, uint32_t max_cont
 // tokens on 16384 rows 221 / 197 / 213 / 201 / 214 / 216.  (All pieces laid end to end and
 // cut at even shares balance the workgroups better and took these chunks 222 us:
 // parts of one sequence that begin at different keys read 711 MB past L2, not 278.)
+constexpr size_t kWorkspaceCounters = 256 + kMaxRaggedSeqs * kKvHeads * 4;  // bytes of the words and counters
+static_assert(kWorkspaceCounters % 256 == 0, "what lies behind is 256-byte aligned");
 constexpr uint32_t kPackedPlanSeqs = 1024, kPackedLeastPart = 16, kPackedMaxParts = 400;
 constexpr size_t kPackedPartPairs = 4 * 33 * 64;  // 4 waves x ((reference, sum), 64 outputs) x 64 lanes
 struct PackedWorkspace {
     bool plan, narrow;
     uint32_t max_items, max_parts;
-    size_t items_offset, arrived_offset, partials_offset, total;
+    size_t odd_offset, items_offset, arrived_offset, partials_offset, total;
 };
 inline PackedWorkspace packed_workspace_layout(uint32_t num_seqs, uint32_t rows, uint32_t max_context) {
     auto align = [](size_t v) { return (v + 255) / 256 * 256; };
@@ -321,7 +324,8 @@ inline PackedWorkspace packed_workspace_layout(uint32_t num_seqs, uint32_t rows,
     w.max_items = rows / kPackedTokens + num_seqs;
     if (w.plan && max_context > 32 * kPackedLeastPart) w.max_parts = kPackedMaxParts;
     w.max_items += w.max_parts;
-    w.items_offset = 256 + align((static_cast<size_t>(rows / kBlockTokens) + 2 * static_cast<size_t>(num_seqs)) * 4);
+    w.odd_offset = kWorkspaceCounters;
+    w.items_offset = w.odd_offset + align((static_cast<size_t>(rows / kBlockTokens) + 2 * static_cast<size_t>(num_seqs)) * 4);
     w.arrived_offset = w.items_offset + align(w.plan ? w.max_items * sizeof(PackedItem) : 0);
     w.partials_offset = w.arrived_offset + align(w.max_parts * 2 * 4);
     w.total = w.partials_offset + static_cast<size_t>(w.max_parts) * 2 * kPackedPartPairs * 8;
@@ -386,7 +390,7 @@ inline SharedWorkspace shared_workspace_of(uint32_t columns, uint32_t shares, ui
     w.own_parts = clamp(128 / (2 * w.shares), most);
     w.unit_columns = w.shared_parts * w.columns * 16 + 2 * w.columns * w.own_parts * kGroup;
     const size_t all = static_cast<size_t>(w.shares) * 2 * w.unit_columns;
-    w.part_o_offset = 256 + align(kMaxRaggedSeqs * kKvHeads * 4);
+    w.part_o_offset = kWorkspaceCounters;
     w.part_ml_offset = w.part_o_offset + align(all * kHeadDim * 4);
     w.total = w.part_ml_offset + align(all * 8);
     return w;

@@ -144,3 +144,50 @@ def prompt_table(pool, i):
     import torch
     first = sum(-(-t // 16) for t in PROMPTS[:i])
     return torch.arange(first, first + -(-PROMPTS[i] // 16), dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("code", [pvlc.KV_F16, R.E4M3])
+def test_one_workspace(code):
+    """Packed prompts (whose values are not all finite, whose items are many), groups' decodes of either route and paged decodes in
+    turn over one workspace."""
+    import torch
+
+    import batches_ref as B
+    from test_gpu_packed_prefill import args_of, launch, wanted
+    from test_gpu_shared_decode import Groups, tails_of
+    log(f"case: one workspace code={code}")
+
+    def prompts(seed, room):
+        b = B.Batch([70, 33] + [20] * 40, [9, 0] + [3] * 40, f32=True, seed=seed, room=room)
+        b.v[3, 0, 5] = np.inf
+        return b.upload()
+
+    def groups(seed):
+        return [Groups([4] * 10, [400 + 16 * i for i in range(10)], tails_of(40, 60), code, True, seed=seed, far=False).upload(),
+                Groups([2], [4000], [5, 90], code, False, seed=seed + 1, far=False).upload(),
+                Groups([5, 5], [700, 40], tails_of(10, 90), code, True, seed=seed + 2).upload()]
+
+    def needs(c):
+        if isinstance(c, Groups):
+            return pvlc.shared_decode_workspace_bytes(c.n, len(c.sizes), c.width * 16)
+        return pvlc.packed_prefill_workspace_bytes(c.n, c.rows, c.width * 16)
+    steps = [prompts(31, 5000)] + groups(32) + [prompts(36, 0)] + groups(37) + [prompts(41, 5000)] + groups(42)
+    nbytes = max(needs(c) for c in steps)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    pvlc.workspace_init(ws, nbytes)
+    for c in steps:
+        if isinstance(c, Groups):
+            c.launch(c.shared_args((ws, nbytes)))
+        else:
+            launch(c, args_of(c, (ws, nbytes)))
+    torch.cuda.synchronize()
+    for i, c in enumerate(steps):
+        if isinstance(c, Groups):
+            c.check(f"step {i}")
+            continue
+        with np.errstate(invalid="ignore"):
+            c.put()
+        some = np.arange(70, c.rows)
+        want, limit = wanted(c, some)
+        B.check(f"step {i}", c.out.cpu().numpy()[some], want, limit)
+    assert pvlc.workspace_error(ws, nbytes) == 0
