@@ -5,11 +5,13 @@
 //
 // 4 * 128 operations a (query, head, key), and with f32 operands 6 * 128, the weights
 // being pairs of fp16: large calls are bound by matrix instructions and the vector
-// ones between them.  The loop over whole pieces runs at 955 TFLOP/s, with f32
-// operands at 700 (1050 of products); a large library product reaches 1104 to 1331.
-// 4 prompts of 4096 to 8192 tokens 624 us (948 TFLOP/s), 12 of 211 to 2010 tokens 75
-// (575; items of 18 pieces on average, of which an item's start and end take the time
-// of six), 6 chunks of 256 to 512 tokens on 16384 rows 200 (578, f32 operands).
+// ones between them.  4096 tokens on 61440 rows, all but the loop over whole pieces a
+// hundredth of the call, run at 960 TFLOP/s, with f32 operands at 701 (1050 of products); a
+// large library product reaches 1090 to 1330.  4 prompts of 4096 to 8192 tokens 627 us (943
+// TFLOP/s), 12 of 211 to 2010 tokens 77 (563; items of 18 pieces on average, whose pieces
+// would take 47 at the loop's rate: the rest are items' starts and ends, the last round, and
+// the append), 6 chunks of 256 to 512 tokens on 16384 rows 201 (576, f32 operands); up to 5%
+// more from one card to another.
 
 #include <hip/hip_runtime.h>
 
@@ -34,13 +36,13 @@ __device__ inline bool item_is_odd(const PackedRows &p, int seq, int begin, int 
 
 // A workgroup takes 16 tokens of a sequence and the 8 query heads of a kv head,
 // a wave two of the heads: 32 columns, in v_mfma_f32_32x32x16_f16.  Two workgroups
-// are on each compute unit, at 190 to 202 registers a wave: one waits or computes
+// are on each compute unit, at 188 and 198 registers a wave: one waits or computes
 // weights while the other multiplies.  The longest prompts above took 936 us with 64 columns
 // a wave straight from the pages, 778 with them through LDS (one wave a SIMD), 749
 // with two workgroups of 32, 690 with the plan's order of items, 636 with outputs
 // stored through LDS.  The compiler's order of a step is the best one found:
 // orders forced by groups ran the loop at 922 to 949 TFLOP/s, other scheduling
-// strategies and wave priorities at 933 to 944.
+// strategies and wave priorities at 933 to 944, where it ran at 955.
 constexpr int kWideWaves = 4, kWideStep = 64;
 constexpr size_t kPartPairs = kPackedPartPairs / kWideWaves;  // of a wave: (reference, sum) and outputs
 constexpr int kStepElems = kWideStep * kHeadDim;  // fp16 elements of a step's keys (or values) of a kv head

@@ -16,7 +16,7 @@
 // which puts a part of every set of a group on one XCD), and converts 8-bit codes
 // again: 64 sequences on 16384 rows (int8, f32 operands) 41 us where the products
 // take 16.  Small calls are bound by two launches of dependent rounds: 16 groups of
-// eight on 300 to 2010 rows (e4m3) 17.3 us.  Measured and not kept: sets of eight
+// eight on 300 to 2010 rows (e4m3) 17.2 us.  Measured and not kept: sets of eight
 // sequences (512 registers, one workgroup a compute unit: those 16 groups 55 us against
 // 29 then), the join by the workgroup that comes last (33 against 29, one group of four
 // 15.9 against 13.2), parts for 384 / 512 / 1024 workgroups in place of 256 (the 64
