@@ -843,14 +843,17 @@ size_t pvlc_hip_shared_decode_workspace_bytes(uint32_t num_seqs, uint32_t num_gr
  * one sequence, whose entries the others repeat: rows in whole blocks of 16, and
  * no more than the group's shortest sequence has (so a prompt's length may stand
  * there although its last block has been copied).  Sequences that are skipped
- * (error bit 1) count for neither: their tables may hold anything.  Any number of sequences
- * may share any number of rows, none included; every sequence is in one group.
+ * (error bit 1) count for neither: their tables may hold anything.  Any number of
+ * sequences may share any number of rows, none included; every sequence is in one
+ * group.
  * Calls of few rows (num_seqs times max_context up to 90000) and those without a
  * group of two run as paged decodes, which are faster there; the offsets and shared
  * lengths are not looked at then.  Otherwise offsets that descend or pass num_seqs
  * and a negative shared length are error bit 1: their groups' sequences, and those of
- * no group, have no output and no new row.  query [num_seqs][16][128], new_key and
- * new_value [num_seqs][2][128], out [num_seqs][16][128], compact. */
+ * no group, have no output and no new row.  A score that is NaN or +infinity makes
+ * its head's output NaN; one of -infinity has no weight, except that a paged decode
+ * may give NaN for it.  query [num_seqs][16][128], new_key and new_value
+ * [num_seqs][2][128], out [num_seqs][16][128], compact. */
 pvlc_hip_status pvlc_hip_shared_decode_f16(const pvlc_hip_shared_decode_args *args, const uint16_t *query,
                                            const uint16_t *new_key, const uint16_t *new_value, uint16_t *out,
                                            void *stream);
